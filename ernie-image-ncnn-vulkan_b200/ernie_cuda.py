@@ -62,6 +62,16 @@ class Shape(ctypes.Structure):
     _fields_ = [("width", I), ("height", I), ("text_tokens", I), ("valid_text", I)]
 
 
+class PagedKvFields(ctypes.Structure):
+    _fields_ = [("k", P), ("v", P), ("precision", I), ("layers", I), ("pages", I), ("page_size", I), ("kv_heads", I),
+                ("head_dim", I)]
+
+
+class PagedBatchFields(ctypes.Structure):
+    _fields_ = [("sequences", I), ("queries", I), ("tables", P), ("max_pages", I), ("lens", P), ("counts", P),
+                ("groups", I), ("prefix_tables", P), ("max_prefix_pages", I), ("prefix_lens", P)]
+
+
 SIGNATURES = {
     "ernie_cuda_last_error": (ctypes.c_char_p, []),
     "ernie_cuda_device_count": (I, [ctypes.POINTER(I)]),
@@ -163,6 +173,12 @@ SIGNATURES = {
     "ernie_cuda_pe_session_position": (I, [P, ctypes.POINTER(I)]),
     "ernie_cuda_pe_session_append": (I, [P, P, P, P, I, P]),
     "ernie_cuda_pe_logits": (I, [P, P, P]),
+    "ernie_cuda_paged_append": (I, [P, P, I, P, P, I, I64, I, P, P, I, P]),
+    "ernie_cuda_prefix_attention_workspace": (I, [P, P, P, I, ctypes.POINTER(SZ)]),
+    "ernie_cuda_prefix_attention": (I, [P, P, I, P, P, I, P, P, SZ]),
+    "ernie_cuda_beam_select_workspace": (I, [P, I, I, I, ctypes.POINTER(SZ)]),
+    "ernie_cuda_beam_select": (I, [P, P, I, I64, I, I, I, I, P, P, P, P, P, P, P, SZ]),
+    "ernie_cuda_beam_reorder": (I, [P, P, I, I, P, P, I, P, P, P]),
 }
 
 
@@ -269,6 +285,35 @@ class Buffer:
         if self.ptr:
             lib().ernie_cuda_free(self.ctx.handle, self.c)
             self.ptr = None
+
+
+def device_pointer(a):
+    """Address of device memory: a Buffer, an address, None, or an array with data_ptr() (a torch tensor)."""
+    if a is None or isinstance(a, int):
+        return a
+    return a.ptr if isinstance(a, Buffer) else a.data_ptr()
+
+
+class PagedKv:
+    """Description of a paged K/V cache (ernie_cuda_paged_kv); keeps its device arrays alive."""
+
+    def __init__(self, k, v, layers, pages, page_size, kv_heads, head_dim, precision):
+        self.arrays = (k, v)
+        self.fields = PagedKvFields(device_pointer(k), device_pointer(v), precision, layers, pages, page_size, kv_heads,
+                                    head_dim)
+        self.c = ctypes.c_void_p(ctypes.addressof(self.fields))
+
+
+class PagedBatch:
+    """A batch over a paged cache (ernie_cuda_paged_batch): int32 device arrays, which it keeps alive."""
+
+    def __init__(self, sequences, queries, tables, max_pages, lens, counts=None, groups=1, prefix_tables=None,
+                 max_prefix_pages=0, prefix_lens=None):
+        self.arrays = (tables, lens, counts, prefix_tables, prefix_lens)
+        self.fields = PagedBatchFields(sequences, queries, device_pointer(tables), max_pages, device_pointer(lens),
+                                       device_pointer(counts), groups, device_pointer(prefix_tables), max_prefix_pages,
+                                       device_pointer(prefix_lens))
+        self.c = ctypes.c_void_p(ctypes.addressof(self.fields))
 
 
 class Context:
@@ -391,6 +436,38 @@ class Context:
             if x:
                 x.free()
         return res
+
+    # batched decoding: device arrays in and out (a Buffer, an address or a torch tensor), enqueued on the
+    # context's stream; arrays written on another stream have to be ready, and stay alive until the work is done
+    def paged_append(self, kv, layer, batch, qkv, precision, ld, heads, cos, sin, rope_rows, q_out):
+        check(lib().ernie_cuda_paged_append(self.handle, kv.c, layer, batch.c, device_pointer(qkv), precision, ld, heads,
+                                            device_pointer(cos), device_pointer(sin), rope_rows, device_pointer(q_out)))
+
+    def prefix_attention_workspace(self, kv, batch, heads):
+        n = SZ(0)
+        check(lib().ernie_cuda_prefix_attention_workspace(self.handle, kv.c, batch.c, heads, ctypes.byref(n)))
+        return n.value
+
+    def prefix_attention(self, kv, layer, batch, q, heads, out, workspace, workspace_bytes):
+        check(lib().ernie_cuda_prefix_attention(self.handle, kv.c, layer, batch.c, device_pointer(q), heads,
+                                                device_pointer(out), device_pointer(workspace), workspace_bytes))
+
+    def beam_select_workspace(self, groups, beams, vocab):
+        n = SZ(0)
+        check(lib().ernie_cuda_beam_select_workspace(self.handle, groups, beams, vocab, ctypes.byref(n)))
+        return n.value
+
+    def beam_select(self, logits, precision, ld, groups, beams, vocab, end_token, scores, finished, parents, tokens,
+                    new_scores, new_finished, workspace, workspace_bytes):
+        check(lib().ernie_cuda_beam_select(self.handle, device_pointer(logits), precision, ld, groups, beams, vocab,
+                                           end_token, device_pointer(scores), device_pointer(finished),
+                                           device_pointer(parents), device_pointer(tokens), device_pointer(new_scores),
+                                           device_pointer(new_finished), device_pointer(workspace), workspace_bytes))
+
+    def beam_reorder(self, kv, groups, beams, parents, tables, max_pages, lens, new_tables, new_lens):
+        check(lib().ernie_cuda_beam_reorder(self.handle, kv.c, groups, beams, device_pointer(parents),
+                                            device_pointer(tables), max_pages, device_pointer(lens),
+                                            device_pointer(new_tables), device_pointer(new_lens)))
 
     def euler_step(self, sample, prediction, delta):
         sample = np.ascontiguousarray(sample, np.float32)

@@ -369,6 +369,109 @@ int ernie_cuda_pe_session_append(ernie_cuda_pe_session *session, const float *em
 /* logits [131072] (host FP32) of one hidden row [3072] through the model's LM head. */
 int ernie_cuda_pe_logits(ernie_cuda_pe_session *session, const float *hidden, float *logits);
 
+/* ---- Batched decoding behind shared prefixes ------------------------------------------------------
+   Operators for decoding many sequences at once over a paged K/V cache (no counterpart in the reference,
+   whose PeSession runs one sequence over one dense cache): the beams of a prompt, or a batch behind one
+   chat template. All pointers are device memory on the context's device; every call enqueues on the
+   context's stream and returns. Lengths and tables are read on the device when the call runs, so the
+   caller may fill them by earlier work of the same stream.
+
+   The cache of one layer is K and V [pages][kv_heads][page_size][head_dim] each, `layers` of them one
+   after the other. A batch is `sequences` rows of `queries` new-token slots each. Sequence s holds
+   lens[s] tokens of its own in the pages tables[s][0], tables[s][1], ...; the last counts[s] of them are
+   this call's new tokens, which take the first counts[s] of its slots. The sequences form `groups`
+   equal, consecutive groups; the sequences of group g share a prefix of prefix_lens[g] tokens in the
+   pages prefix_tables[g][...], which precedes their own tokens: token i of a sequence stands at position
+   prefix_lens[g] + i, and its own tokens begin a page of their own whatever the prefix's length.
+
+   A length above its table's pages, a negative one, a count outside 0..queries or a page outside
+   0..pages-1 that a call has to touch is never followed: lengths and counts are clamped, a bad page's
+   keys count as zeros and nothing is stored there, and the next ernie_cuda_context_synchronize reports
+   status 41. Two sequences that store into the same page in one call race. */
+#define ERNIE_CUDA_STATUS_PAGED_RANGE 41
+
+typedef struct
+{
+    void *k, *v;    /* [layers][pages][kv_heads][page_size][head_dim], 16-byte aligned */
+    int precision;  /* element type: ERNIE_PRECISION_BF16 or ERNIE_PRECISION_FP32 */
+    int layers;
+    int pages;      /* pages * kv_heads * page_size below 2^31 */
+    int page_size;  /* 8, 16, 32, 64 or 128 tokens */
+    int kv_heads;
+    int head_dim;   /* 64 or 128 */
+} ernie_cuda_paged_kv;
+
+typedef struct
+{
+    int sequences, queries;
+    const int32_t *tables;        /* [sequences][max_pages] */
+    int max_pages;
+    const int32_t *lens;          /* [sequences], the new tokens included */
+    const int32_t *counts;        /* [sequences] new tokens, 0..queries; NULL: `queries` each */
+    int groups;                   /* divides sequences */
+    const int32_t *prefix_tables; /* [groups][max_prefix_pages]; NULL with max_prefix_pages 0: no prefix */
+    int max_prefix_pages;
+    const int32_t *prefix_lens;   /* [groups]; NULL without a prefix */
+} ernie_cuda_paged_batch;
+
+/* The new tokens' projections into the cache. qkv [sequences*queries][ld] holds in each row the heads'
+   queries, the keys and the values ((heads + 2*kv_heads)*head_dim numbers, then ld's padding) in
+   `precision`. Queries and keys are rotated as the text layers do it (out[:h] = x[:h]cos[:h] -
+   x[h:]sin[h:], out[h:] = x[h:]cos[h:] + x[:h]sin[h:], h = head_dim/2, FP32 without contraction) by row
+   `position` of cos/sin [rope_rows][head_dim] FP32 and rounded once to the cache's type; keys and
+   values go to the token's page, queries to q_out [sequences*queries][heads][head_dim]. Slots without a
+   token and everything else in the cache stay as they were. A position outside 0..rope_rows-1 stores
+   nothing and reports status 41. q_out may not overlap qkv. */
+int ernie_cuda_paged_append(ernie_cuda_context *ctx, const ernie_cuda_paged_kv *kv, int layer,
+                            const ernie_cuda_paged_batch *batch, const void *qkv, int precision, int64_t ld, int heads,
+                            const float *cos, const float *sin, int rope_rows, void *q_out);
+
+/* out = softmax(q k^T / sqrt(head_dim)) v for every slot that holds a token, over its group's prefix and
+   its own sequence's tokens up to and including itself; heads/kv_heads query heads share a K/V head. q
+   and out [sequences*queries][heads][head_dim] in the cache's type, 16-byte aligned, not overlapping.
+   The prefix is read once for all the rows of its group. Scores, softmax statistics and sums are FP32;
+   with a BF16 cache the weights are rounded to BF16 for the second product. Slots without a token stay
+   as they were; a row that sees no key at all (a token before its sequence's begin, lens < counts,
+   without a prefix) gives zeros. What lies past a sequence's last token is never used; a non-finite
+   value of an appended token may reach every row of its sequence in the same call.
+   The workspace is scratch of at least ..._workspace bytes (16-byte aligned); it holds nothing between
+   calls, and calls that may run at the same time need one each. */
+int ernie_cuda_prefix_attention_workspace(ernie_cuda_context *ctx, const ernie_cuda_paged_kv *kv,
+                                          const ernie_cuda_paged_batch *batch, int heads, size_t *bytes);
+int ernie_cuda_prefix_attention(ernie_cuda_context *ctx, const ernie_cuda_paged_kv *kv, int layer,
+                                const ernie_cuda_paged_batch *batch, const void *q, int heads, void *out,
+                                void *workspace, size_t workspace_bytes);
+
+/* One step of beam search: of each group's beams x vocab continuations the `beams` best (1..32).
+   logits [groups*beams][ld] in `precision`; a continuation's total is score + (logit - log sum exp
+   logits), in 64 bits from the row's 32-bit sum. An unfinished beam offers its tokens by descending
+   logit, equal logits by ascending token; a finished one (finished != 0) offers itself once, with
+   end_token and its score unchanged. Over the beams the larger total wins, equal totals the lower beam.
+   Not offered: logits of -inf, rows with a NaN, a +inf or no finite logit, beams whose score is not
+   finite (-inf is the usual start of all beams but the first).
+   Out, best first: parents (the beam within the group), tokens, new_scores (the total rounded to FP32),
+   new_finished (its parent was, or its token is end_token; a negative end_token ends none). Places
+   without a continuation left get parent -1, token -1, score -inf, finished 1. The outputs may be the
+   inputs of the same name. The workspace as for ernie_cuda_prefix_attention. */
+int ernie_cuda_beam_select_workspace(ernie_cuda_context *ctx, int groups, int beams, int vocab, size_t *bytes);
+int ernie_cuda_beam_select(ernie_cuda_context *ctx, const void *logits, int precision, int64_t ld, int groups, int beams,
+                           int vocab, int end_token, const float *scores, const int32_t *finished, int32_t *parents,
+                           int32_t *tokens, float *new_scores, int32_t *new_finished, void *workspace,
+                           size_t workspace_bytes);
+
+/* The cached state after a selection: place i of a group becomes the continuation of place parents[i]
+   (-1: of none, an empty sequence; other values outside 0..beams-1 count as -1 and report status 41).
+   Places are the cache's sequences, groups*beams rows of tables [..][max_pages] and lens. Each parent's
+   pages pass to one child, its heir (its own place if that is its child, else its first child); the
+   other children, in order, take the pages of the places without children, in order, and the parent's
+   tokens are copied there in every layer. So pages only change hands within a group, every page keeps
+   one owner, and only duplicated beams cost copies. Every row of a group needs as many good pages as its
+   group's longest sequence uses (a bad one is not written: status 41). new_tables and new_lens get the
+   new rows and may not overlap tables, lens or each other; the prefix pages take no part. */
+int ernie_cuda_beam_reorder(ernie_cuda_context *ctx, const ernie_cuda_paged_kv *kv, int groups, int beams,
+                            const int32_t *parents, const int32_t *tables, int max_pages, const int32_t *lens,
+                            int32_t *new_tables, int32_t *new_lens);
+
 /* ---- Ulysses sequence parallelism (one process per GPU, 2, 4 or 8 members, BF16) ---------------
    Tokens are split into contiguous shards of S = ceil(N / world) rows (rounded up to 16); every member
    holds the full weights. Per block, the QKV GEMM's epilogue stores each head of this GPU's rows straight
