@@ -3,6 +3,7 @@
 // in the sm_100a kernels of gemm.cu, attention.cu and elementwise.cu.
 #include "ernie_cuda.h"
 #include "ernie_synth.h"
+#include "decode.h"
 #include "kernels.h"
 #include "capi_internal.h"
 #include <algorithm>
@@ -248,6 +249,7 @@ extern "C" int ernie_cuda_context_create(int device, ernie_cuda_context **out)
     if (e == cudaSuccess) e = static_cast<cudaError_t>(prepare_flash_kernels());
     if (e == cudaSuccess) e = static_cast<cudaError_t>(prepare_flash_f32_kernels());
     if (e == cudaSuccess) e = static_cast<cudaError_t>(prepare_conv_kernels());
+    if (e == cudaSuccess) e = static_cast<cudaError_t>(prepare_prefix_attention_kernels());
     if (e != cudaSuccess)
     {
         ernie_cuda_context_destroy(ctx);

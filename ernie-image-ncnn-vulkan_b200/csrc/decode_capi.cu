@@ -88,6 +88,13 @@ int check_heads(int heads, const PagedLayer &kv)
     return ERNIE_CUDA_OK;
 }
 
+int check_rows(const PagedBatch &b, int heads)
+{
+    if (static_cast<long long>(b.sequences) * b.queries * heads > INT32_MAX)
+        return fail(ERNIE_CUDA_ERROR, "More than 2^31 query rows in one call");
+    return ERNIE_CUDA_OK;
+}
+
 // A position or length past 2^31 - 1 tokens cannot be addressed by the 32-bit lengths.
 int check_tokens(const PagedBatch &b, const PagedLayer &kv)
 {
@@ -151,6 +158,7 @@ extern "C" int ernie_cuda_prefix_attention_workspace(ernie_cuda_context *ctx, co
     ERNIE_TRY(check_batch(batch, b));
     ERNIE_TRY(check_tokens(b, layer));
     ERNIE_TRY(check_heads(heads, layer));
+    ERNIE_TRY(check_rows(b, heads));
     if (!ctx) return fail(ERNIE_CUDA_ERROR, "null context");
     *bytes = prefix_attention_workspace(layer, b, heads, ctx->num_sms);
     return ERNIE_CUDA_OK;
@@ -165,6 +173,7 @@ extern "C" int ernie_cuda_prefix_attention(ernie_cuda_context *ctx, const ernie_
     ERNIE_TRY(check_batch(batch, a.batch));
     ERNIE_TRY(check_tokens(a.batch, a.kv));
     ERNIE_TRY(check_heads(heads, a.kv));
+    ERNIE_TRY(check_rows(a.batch, heads));
     if (!q || !out || !workspace) return fail(ERNIE_CUDA_ERROR, "null argument");
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16))
         return fail(ERNIE_CUDA_ERROR, "Queries, output and workspace must be 16-byte aligned");

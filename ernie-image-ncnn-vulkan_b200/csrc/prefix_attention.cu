@@ -1,98 +1,1331 @@
-// Attention of a batch whose sequences share a prefix, over the paged K/V cache.
+// Attention of a batch whose sequences share prefixes, over the paged K/V cache:
+//   out = softmax(q k^T / sqrt(D)) v over [the group's prefix | the sequence's own tokens up to the row's place].
+//
+// The softmax over both stretches is joined from partial results: a stretch of keys leaves, per row, its
+// maximum m, l = sum 2^(s - m) and o = sum 2^(s - m) v (scores s in units of log2), and the join weighs them by
+// 2^(m - max m). Two lists of items are worked on at the same time by one grid, one CTA per SM:
+//   prefix  (group, block of rows, K/V head): every row of the group against the group's prefix, which is
+//           read once per block of rows however many sequences share it;
+//   own     (sequence, block of rows, K/V head): a sequence's rows against its own tokens.
+// A row is a query head of a slot: the heads/kv_heads query heads that share a K/V head are rows of one item.
+// An item's keys are cut into units of 128. Each list's units are dealt out evenly, in order, to that list's
+// CTAs, so that an item may span several CTAs and a CTA several items; an item's share of a CTA is a part.
+// Along the order both the item and the CTA only ever step up, so item + CTA numbers the parts without gaps
+// or clashes, and an item's parts lie side by side. The lists share the CTAs by their estimated cost. All of
+// this is worked out on the device, by every CTA for itself, from the lengths of this very call.
+//
+// A CTA works on its units in one of two ways, chosen per list on the host by the rows of a block:
+//   stream  few rows, or an FP32 cache: eight warps with mma.sync m16n8 tiles, 16 rows x 16 keys at a time,
+//           fed by a six-slot TMA ring. The bound is the K/V traffic: a unit of BF16 K and V is 64 KB;
+//           FP32 operands are split into two TF32 parts and multiplied in three products.
+//   tile    many rows of a BF16 cache: 256 rows (two tiles of 128) share each K/V tile on the tensor cores
+//           (tcgen05.mma, accumulators in TMEM), one row per softmax thread.
+// A second kernel joins the parts of each row.
 #include "decode.h"
+#include "ptx.cuh"
+#include <cudaTypedefs.h>
 
 namespace ernie_b200
 {
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
+
 namespace
 {
-constexpr int kWarps = 4;
+constexpr int kThreads = 384; // three warpgroups: control, and twice four working warps
+constexpr int kUnit = 128;    // keys of a unit
+// As for the block attention: 128 x 88 + 256 x 208 registers are the launch's 384 x 168.
+constexpr int kRegsControl = 88, kRegsWork = 208, kMinLaunchRegs = 168;
+static_assert(128 * kRegsControl + 256 * kRegsWork <= kThreads * kMinLaunchRegs, "register split");
+constexpr int kSlots = 6;
+constexpr int kErrAttendTimeout = 42;
 
-__device__ __forceinline__ float warp_total(float v)
+// One of the two lists, as the host lays it out.
+struct List
 {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    int owners;    // groups or sequences
+    int rows;      // of an owner and K/V head
+    int block;     // rows of an item
+    int blocks;    // items of an owner and K/V head
+    int part_rows; // rows that a part stores
+    int tile;      // 1: on the tensor cores' tiles, 0: streamed
+    int row_tiles; // streamed: 16-row tiles of an item (1, 2, 4 or 8)
+    int cost;      // of a unit, relative
+    float *o;      // [items + CTAs][part_rows][D]
+    float2 *ml;    // [items + CTAs][part_rows]
+    int2 *meta;    // [items]: first part's CTA, number of parts
+};
+
+struct AttendArgs
+{
+    PrefixAttentionArgs a;
+    List list[2]; // prefix, own
+    int ctas;
+    int share;    // query heads of a K/V head
+    float scale;  // log2(e) / sqrt(D)
+    int granule;  // keys of a TMA box
+};
+
+template <class T> struct Kind;
+template <> struct Kind<__nv_bfloat16>
+{
+    static constexpr int kSlotKeys = 64;
+};
+template <> struct Kind<float>
+{
+    static constexpr int kSlotKeys = 32;
+};
+
+template <class T, int D> struct Layout
+{
+    static constexpr int kSlotKeys = Kind<T>::kSlotKeys;
+    static constexpr int kColumns = D * static_cast<int>(sizeof(T)) / 128; // 128-byte column blocks of a row
+    static constexpr int kSlotHalf = kSlotKeys * D * static_cast<int>(sizeof(T)); // K or V of a slot
+    static constexpr int kUnitSlots = kUnit / kSlotKeys;
+    static constexpr int kScratch = kSlots * 2 * kSlotHalf; // the warps' merge area behind the ring
+    static constexpr int kStreamBytes = kScratch + 4 * 16 * D * 4;
+    static constexpr int kTileBytes = kUnit * D * 2;       // a Q, K or V tile
+    static constexpr int kWeightBytes = kUnit * kUnit * 2; // a P tile
+    static constexpr int kTileModeBytes = 5 * kTileBytes + 2 * kWeightBytes;
+    static constexpr int kBody = kStreamBytes > kTileModeBytes ? kStreamBytes : kTileModeBytes;
+    static constexpr int kSmemBytes = kBody + 1024 + 2048; // alignment; barriers, the plan and the merge statistics
+};
+
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d)
+{
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ float ld_shared(uint32_t addr)
+{
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void store(float *p, float v) { *p = v; }
-__device__ __forceinline__ void store(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
 
-// One CTA per slot and query head; its warps take the keys in turn, lanes the dimensions, and each warp
-// keeps its running maximum, sum and weighted values, joined at the end.
-template <class T, int D> __global__ void __launch_bounds__(kWarps * 32) attend_kernel(PrefixAttentionArgs a)
+__device__ __forceinline__ void ldmatrix(uint32_t addr, uint32_t (&r)[4])
 {
-    constexpr int N = D / 32;
-    __shared__ float wm[kWarps], wl[kWarps], wo[kWarps][D];
-    const int slot = blockIdx.x, head = blockIdx.y, s = slot / a.batch.queries, i = slot - s * a.batch.queries;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const SequenceView view = sequence_view(a.batch, a.kv.page_shift, s);
-    if (i >= view.count) return;
-    const int own = max(0, view.len - view.count + i + 1), kv_head = head / (a.heads / a.kv.kv_heads);
-    const int *own_table = a.batch.tables + static_cast<size_t>(s) * a.batch.max_pages;
-    const int *prefix_table = a.batch.max_prefix_pages ? a.batch.prefix_tables + static_cast<size_t>(s / (a.batch.sequences / a.batch.groups)) * a.batch.max_prefix_pages : nullptr;
-    const T *q = static_cast<const T *>(a.q) + (static_cast<size_t>(slot) * a.heads + head) * D;
-    float x[N], o[N] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int n = 0; n < N; ++n) x[n] = to_float(q[lane + 32 * n]) * rsqrtf(static_cast<float>(D));
-    for (int key = warp; key < view.prefix_len + own; key += kWarps)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix_trans(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x = high + low up to 2^-22 |x|, both in TF32.
+__device__ __forceinline__ void split_tf32(float x, uint32_t &high, uint32_t &low)
+{
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(high) : "f"(x));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(low) : "f"(x - __uint_as_float(high)));
+}
+
+// A whole warp's bounded wait, with one answer for all its lanes.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity)
+{
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
+// The eight working warps meet (bounded, like every wait).
+__device__ __forceinline__ bool meet(uint32_t bar, unsigned &round)
+{
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+    return warp_wait(bar, round++ & 1u);
+}
+
+// ---------------------------------------------------------------- the plan
+// Keys that the rows of an item see at most, and with it the item's units.
+__device__ __forceinline__ int item_keys(const AttendArgs &p, int which, int owner, int block)
+{
+    const PagedBatch &b = p.a.batch;
+    if (which == 0) return clamped_length(b.prefix_lens[owner], b.max_prefix_pages, p.a.kv.page_shift, b.error_flag);
+    const SequenceView v = sequence_view(b, p.a.kv.page_shift, owner);
+    const int first = block * p.list[1].block, rows = min(first + p.list[1].block, v.count * p.share);
+    if (rows <= first) return 0;
+    return max(0, v.len - v.count + (rows - 1) / p.share + 1);
+}
+
+__device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
+
+// The CTA of a list of `units` dealt out to `ctas` that holds unit u (the inverse of first_unit).
+__device__ __forceinline__ int cta_of_unit(long long u, long long units, int ctas)
+{
+    return static_cast<int>(((u + 1) * ctas - 1) / units);
+}
+__device__ __forceinline__ long long first_unit(int cta, long long units, int ctas) { return cta * units / ctas; }
+
+struct PlanShared
+{
+    long long warp_sum[2][kThreads / 32];
+    int owner, block, head, unit; // where the CTA begins
+};
+
+// A CTA's walk over its units.
+struct Walk
+{
+    int which;           // list
+    int cta, ctas;       // within the list
+    long long at, end, units;
+    int owner, block, head, unit; // the next unit's item and its number within the item
+};
+
+struct Part
+{
+    int owner, block, head;
+    int keys;               // of the item
+    int first_unit, units;  // of the part
+    long long place;        // of its results
+};
+
+// The next part of the walk; false at its end. Every warp of the CTA takes the same steps.
+__device__ __forceinline__ bool next_part(const AttendArgs &p, Walk &w, Part &part)
+{
+    if (w.at >= w.end) return false;
+    const List &l = p.list[w.which];
+    int keys, units;
+    if (w.owner >= l.owners) return false;
+    for (;;)
     {
-        const bool shared = key < view.prefix_len;
-        const int at = shared ? key : key - view.prefix_len;
-        const int page = (shared ? prefix_table : own_table)[at >> a.kv.page_shift];
-        const bool good = page >= 0 && page < a.kv.pages;
-        if (!good) report_range(a.batch.error_flag);
-        const size_t row = ((static_cast<size_t>(good ? page : 0) * a.kv.kv_heads + kv_head) << a.kv.page_shift) + (at & ((1 << a.kv.page_shift) - 1));
-        const T *k = static_cast<const T *>(a.kv.k) + row * D, *v = static_cast<const T *>(a.kv.v) + row * D;
-        float d = 0.f;
-#pragma unroll
-        for (int n = 0; n < N; ++n) d = fmaf(x[n], good ? to_float(k[lane + 32 * n]) : 0.f, d);
-        d = warp_total(d);
-        const float m_new = fmaxf(m, d);
-        if (m_new == -INFINITY) continue;
-        const float alpha = __expf(m - m_new), p = __expf(d - m_new);
-        l = l * alpha + p;
-#pragma unroll
-        for (int n = 0; n < N; ++n) o[n] = fmaf(p, good ? to_float(v[lane + 32 * n]) : 0.f, o[n] * alpha);
-        m = m_new;
+        keys = item_keys(p, w.which, w.owner, w.block);
+        units = units_of(keys);
+        if (w.unit < units) break;
+        w.unit = 0;
+        w.head = 0;
+        if (++w.block == l.blocks) w.block = 0, ++w.owner;
+        if (w.owner >= l.owners) return false; // the lengths have changed under the call
     }
-    if (lane == 0)
+    part.owner = w.owner;
+    part.block = w.block;
+    part.head = w.head;
+    part.keys = keys;
+    part.first_unit = w.unit;
+    part.units = static_cast<int>(min(static_cast<long long>(units - w.unit), w.end - w.at));
+    part.place = (static_cast<long long>(w.owner) * l.blocks + w.block) * p.a.kv.kv_heads + w.head + w.cta;
+    w.at += part.units;
+    w.unit += part.units;
+    if (w.unit == units)
     {
-        wm[warp] = m;
-        wl[warp] = l;
-    }
-#pragma unroll
-    for (int n = 0; n < N; ++n) wo[warp][lane + 32 * n] = o[n];
-    __syncthreads();
-    for (int d = threadIdx.x; d < D; d += kWarps * 32)
-    {
-        float top = -INFINITY, sum = 0.f, acc = 0.f;
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, wm[w]);
-        for (int w = 0; w < kWarps; ++w)
+        w.unit = 0;
+        if (++w.head == p.a.kv.kv_heads)
         {
-            if (wm[w] == -INFINITY) continue;
-            const float f = __expf(wm[w] - top);
-            sum += wl[w] * f;
-            acc += wo[w][d] * f;
+            w.head = 0;
+            if (++w.block == l.blocks) w.block = 0, ++w.owner;
         }
-        store(static_cast<T *>(a.out) + (static_cast<size_t>(slot) * a.heads + head) * D + d, sum > 0.f ? acc / sum : 0.f);
     }
+    return true;
+}
+
+// Written by the part that holds the item's first unit (`begin`: that unit's number in the list).
+__device__ __forceinline__ void write_meta(const AttendArgs &p, const Walk &w, const Part &part, long long begin)
+{
+    const int last = cta_of_unit(begin + units_of(part.keys) - 1, w.units, w.ctas);
+    p.list[w.which].meta[part.place - w.cta] = make_int2(w.cta, last - w.cta + 1);
+}
+
+// All threads: the lists' units, the CTA's list and its share. False: nothing to do.
+__device__ bool make_plan(const AttendArgs &p, PlanShared &s, Walk &w)
+{
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    long long mine[2], before[2];
+    int chunk[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+    {
+        const List &l = p.list[i];
+        chunk[i] = (l.owners + kThreads - 1) / kThreads;
+        long long sum = 0;
+        for (int o = tid * chunk[i]; o < min(l.owners, (tid + 1) * chunk[i]); ++o)
+            for (int b = 0; b < l.blocks; ++b) sum += units_of(item_keys(p, i, o, b));
+        mine[i] = sum * p.a.kv.kv_heads;
+        long long scan = mine[i];
+#pragma unroll
+        for (int step = 1; step < 32; step *= 2)
+        {
+            const long long other = __shfl_up_sync(0xffffffffu, scan, step);
+            if (lane >= step) scan += other;
+        }
+        before[i] = scan - mine[i];
+        if (lane == 31) s.warp_sum[i][warp] = scan;
+    }
+    __syncthreads();
+    long long total[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kThreads / 32; ++j)
+        {
+            if (j < warp) before[i] += s.warp_sum[i][j];
+            total[i] += s.warp_sum[i][j];
+        }
+    if (total[0] + total[1] == 0) return false;
+    // the lists' CTAs: by cost, at least one for a list with work, no more than it has units
+    const double cost0 = static_cast<double>(total[0]) * p.list[0].cost, cost1 = static_cast<double>(total[1]) * p.list[1].cost;
+    int n0 = static_cast<int>(p.ctas * (cost0 / (cost0 + cost1)) + 0.5);
+    n0 = total[0] == 0 ? 0 : max(1, total[1] == 0 ? p.ctas : min(p.ctas - 1, n0));
+    int n1 = p.ctas - n0;
+    if (n0 > total[0]) n0 = static_cast<int>(total[0]), n1 = total[1] ? p.ctas - n0 : 0;
+    if (n1 > total[1]) n1 = static_cast<int>(total[1]);
+    if (total[0] && n0 + n1 < p.ctas) n0 = static_cast<int>(min(total[0], static_cast<long long>(p.ctas - n1)));
+    const int cta = blockIdx.x;
+    if (cta >= n0 + n1) return false;
+    w.which = cta < n0 ? 0 : 1;
+    w.cta = cta - (w.which ? n0 : 0);
+    w.ctas = w.which ? n1 : n0;
+    w.units = w.which ? total[1] : total[0];
+    w.at = first_unit(w.cta, w.units, w.ctas);
+    w.end = first_unit(w.cta + 1, w.units, w.ctas);
+    const long long ahead = w.which ? before[1] : before[0], held = w.which ? mine[1] : mine[0];
+    if (w.at >= ahead && w.at < ahead + held)
+    {
+        const List &l = p.list[w.which];
+        long long left = w.at - ahead;
+        int o = tid * (w.which ? chunk[1] : chunk[0]), b = 0, units;
+        for (;;)
+        {
+            units = units_of(item_keys(p, w.which, o, b));
+            const long long item = static_cast<long long>(units) * p.a.kv.kv_heads;
+            if (left < item) break;
+            left -= item;
+            if (++b == l.blocks) b = 0, ++o;
+        }
+        s.owner = o;
+        s.block = b;
+        s.head = static_cast<int>(left / units);
+        s.unit = static_cast<int>(left % units);
+    }
+    __syncthreads();
+    w.owner = s.owner;
+    w.block = s.block;
+    w.head = s.head;
+    w.unit = s.unit;
+    return true;
+}
+
+// ---------------------------------------------------------------- rows
+struct Row
+{
+    long long offset; // of the query in q, in elements
+    int keys;         // that the row sees of the item's; 0 without a token
+};
+
+__device__ __forceinline__ Row row_of(const AttendArgs &p, int which, const Part &part, int row, int dim)
+{
+    const PagedBatch &b = p.a.batch;
+    const List &l = p.list[which];
+    const int r = part.block * l.block + row;
+    Row out = {0, 0};
+    if (row >= l.block || r >= l.rows) return out;
+    const int at = r / p.share, head = part.head * p.share + r - at * p.share;
+    long long slot;
+    if (which == 0)
+    {
+        const int per = b.sequences / b.groups, s = part.owner * per + at / b.queries, i = at % b.queries;
+        const int count = b.counts ? b.counts[s] : b.queries;
+        if (i >= count) return out;
+        slot = static_cast<long long>(s) * b.queries + i;
+        out.keys = part.keys;
+    }
+    else
+    {
+        const SequenceView v = sequence_view(b, p.a.kv.page_shift, part.owner);
+        if (at >= v.count) return out;
+        slot = static_cast<long long>(part.owner) * b.queries + at;
+        out.keys = max(0, v.len - v.count + at + 1);
+    }
+    out.offset = (slot * p.a.heads + head) * dim;
+    return out;
+}
+
+// First row of the pool that holds key `key` of the part's item, or the row past the end (TMA reads zeros
+// there) for a key past the item's or a bad page.
+__device__ __forceinline__ int pool_row(const AttendArgs &p, int which, const Part &part, int key)
+{
+    const PagedLayer &kv = p.a.kv;
+    const int outside = (kv.pages * kv.kv_heads) << kv.page_shift;
+    if (key >= part.keys) return outside;
+    const PagedBatch &b = p.a.batch;
+    const int *table = which == 0 ? b.prefix_tables + static_cast<long long>(part.owner) * b.max_prefix_pages
+                                  : b.tables + static_cast<long long>(part.owner) * b.max_pages;
+    const int page = table[key >> kv.page_shift];
+    if (page < 0 || page >= kv.pages)
+    {
+        report_range(b.error_flag);
+        return outside;
+    }
+    return ((page * kv.kv_heads + part.head) << kv.page_shift) + (key & ((1 << kv.page_shift) - 1));
+}
+
+// ---------------------------------------------------------------- stream
+// A warp's 16 rows: queries, running maximum, sum and weighted values, in mma.sync fragments (rows lane/4
+// and lane/4 + 8; a lane's columns 2 (lane % 4) and the next of every eight).
+template <class T, int D> struct Rows16;
+
+template <int D> struct Rows16<__nv_bfloat16, D>
+{
+    uint32_t q[D / 16][4];
+    __device__ __forceinline__ void load(const AttendArgs &p, const Row &r0, const Row &r1, int lane)
+    {
+        const __nv_bfloat16 *base = static_cast<const __nv_bfloat16 *>(p.a.q) + 2 * (lane & 3);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+        {
+            q[s][0] = r0.keys ? *reinterpret_cast<const uint32_t *>(base + r0.offset + 16 * s) : 0u;
+            q[s][1] = r1.keys ? *reinterpret_cast<const uint32_t *>(base + r1.offset + 16 * s) : 0u;
+            q[s][2] = r0.keys ? *reinterpret_cast<const uint32_t *>(base + r0.offset + 16 * s + 8) : 0u;
+            q[s][3] = r1.keys ? *reinterpret_cast<const uint32_t *>(base + r1.offset + 16 * s + 8) : 0u;
+        }
+    }
+    // scores of 16 keys: two tiles of eight
+    __device__ __forceinline__ void scores(uint32_t k, int lane, float (&s)[2][4]) const
+    {
+        const int key = (lane >> 4) * 8 + (lane & 7), half = (lane >> 3) & 1;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+        {
+            uint32_t b[4];
+            const int chunk = 2 * i + half;
+            ldmatrix(k + (chunk >> 3) * (64 * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), b);
+            mma_bf16(s[0], q[i], b[0], b[1]);
+            mma_bf16(s[1], q[i], b[2], b[3]);
+        }
+    }
+    // o += p v over 16 keys, of which the first `valid` count
+    __device__ __forceinline__ void weigh(uint32_t v, int lane, const float (&s)[2][4], int valid, float (&o)[D / 8][4]) const
+    {
+        const uint32_t a[4] = {pack2(s[0][0], s[0][1]), pack2(s[0][2], s[0][3]), pack2(s[1][0], s[1][1]), pack2(s[1][2], s[1][3])};
+        const int key = ((lane >> 3) & 1) * 8 + (lane & 7), half = lane >> 4;
+        uint32_t keep[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+        {
+            const int first = 8 * h + 2 * (lane & 3);
+            keep[h] = (first < valid ? 0xffffu : 0u) | (first + 1 < valid ? 0xffff0000u : 0u);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+        {
+            uint32_t b[4];
+            const int chunk = 2 * i + half;
+            ldmatrix_trans(v + (chunk >> 3) * (64 * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), b);
+            if (valid < 16) // what lies past the last key may be anything, NaN too
+            {
+                b[0] &= keep[0], b[1] &= keep[1], b[2] &= keep[0], b[3] &= keep[1];
+            }
+            mma_bf16(o[2 * i], a, b[0], b[1]);
+            mma_bf16(o[2 * i + 1], a, b[2], b[3]);
+        }
+    }
+};
+
+template <int D> struct Rows16<float, D>
+{
+    float q[D / 8][4];
+    __device__ __forceinline__ void load(const AttendArgs &p, const Row &r0, const Row &r1, int lane)
+    {
+        const float *base = static_cast<const float *>(p.a.q) + (lane & 3);
+#pragma unroll
+        for (int s = 0; s < D / 8; ++s)
+        {
+            q[s][0] = r0.keys ? base[r0.offset + 8 * s] : 0.f;
+            q[s][1] = r1.keys ? base[r1.offset + 8 * s] : 0.f;
+            q[s][2] = r0.keys ? base[r0.offset + 8 * s + 4] : 0.f;
+            q[s][3] = r1.keys ? base[r1.offset + 8 * s + 4] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void scores(uint32_t k, int lane, float (&s)[2][4]) const
+    {
+        const int key = (lane >> 4) * 8 + (lane & 7), half = (lane >> 3) & 1;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+        {
+            uint32_t raw[4], high[4], low[4], qh[4], ql[4];
+            const int chunk = 2 * i + half;
+            ldmatrix(k + (chunk >> 3) * (32 * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), raw);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+            {
+                split_tf32(__uint_as_float(raw[j]), high[j], low[j]);
+                split_tf32(q[i][j], qh[j], ql[j]);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+            {
+                mma_tf32(s[t], ql, high[2 * t], high[2 * t + 1]);
+                mma_tf32(s[t], qh, low[2 * t], low[2 * t + 1]);
+                mma_tf32(s[t], qh, high[2 * t], high[2 * t + 1]);
+            }
+        }
+    }
+    // The weights' fragment of key columns 2t and 2t + 1 serves as one whose columns are t and t + 4, with
+    // the value rows taken in that order.
+    __device__ __forceinline__ void weigh(uint32_t v, int lane, const float (&s)[2][4], int valid, float (&o)[D / 8][4]) const
+    {
+        uint32_t ph[2][4], pl[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+        {
+            split_tf32(s[t][0], ph[t][0], pl[t][0]);
+            split_tf32(s[t][2], ph[t][1], pl[t][1]);
+            split_tf32(s[t][1], ph[t][2], pl[t][2]);
+            split_tf32(s[t][3], ph[t][3], pl[t][3]);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+        {
+            const int d = (i & 3) * 8 + (lane >> 2);
+            const uint32_t column = v + (i >> 2) * (32 * 128) + (d & 3) * 4;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+            {
+                uint32_t high[2], low[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                {
+                    const int key = 8 * t + 2 * (lane & 3) + e;
+                    float x = ld_shared(column + key * 128 + (((d >> 2) ^ (key & 7)) << 4));
+                    if (valid < 16 && key >= valid) x = 0.f;
+                    split_tf32(x, high[e], low[e]);
+                }
+                mma_tf32(o[i], pl[t], high[0], high[1]);
+                mma_tf32(o[i], ph[t], low[0], low[1]);
+                mma_tf32(o[i], ph[t], high[0], high[1]);
+            }
+        }
+    }
+};
+
+template <class T, int D>
+__device__ __forceinline__ void stream_produce(const AttendArgs &p, Walk w, const CUtensorMap *map_k, const CUtensorMap *map_v,
+                                               uint32_t ring, uint32_t bars)
+{
+    using L = Layout<T, D>;
+    const int lane = threadIdx.x & 31;
+    const int granules = L::kSlotKeys / p.granule, boxes = granules * L::kColumns * 2;
+    // a lane's box of every slot: granule, column block, K or V
+    const int granule = lane % granules, column = (lane / granules) % L::kColumns, value = lane / (granules * L::kColumns);
+    const uint32_t box_bytes = p.granule * 128;
+    const uint32_t into = (value ? L::kSlotHalf : 0) + column * (L::kSlotKeys * 128) + granule * box_bytes;
+    unsigned n = 0; // slots so far
+    Part part;
+    while (next_part(p, w, part))
+    {
+        int key = part.first_unit * kUnit + granule * p.granule;
+        int row = lane < boxes ? pool_row(p, w.which, part, key) : 0;
+        for (int u = 0; u < part.units * L::kUnitSlots; ++u, ++n)
+        {
+            const unsigned slot = n % kSlots, round = n / kSlots;
+            const bool wanted = lane < boxes && key < part.keys;
+            const int next = lane < boxes ? pool_row(p, w.which, part, key + L::kSlotKeys) : 0;
+            const unsigned count = __popc(__ballot_sync(0xffffffffu, wanted));
+            const uint32_t full = bars + 8 * slot, empty = bars + 8 * (kSlots + slot);
+            if (!warp_wait(empty, (round & 1u) ^ 1u))
+            {
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                return;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(full, count * box_bytes);
+            __syncwarp();
+            if (wanted)
+                tma_load_2d(ring + slot * (2 * L::kSlotHalf) + into, value ? map_v : map_k, full,
+                            column * (128 / static_cast<int>(sizeof(T))), row);
+            key += L::kSlotKeys;
+            row = next;
+        }
+    }
+}
+
+template <class T, int D>
+__device__ __forceinline__ void stream_work(const AttendArgs &p, Walk w, uint32_t ring, uint32_t bars, float *scratch, float2 *stats)
+{
+    using L = Layout<T, D>;
+    const List &l = p.list[w.which];
+    const int warp = threadIdx.x / 32 - 4, lane = threadIdx.x & 31;
+    const int tiles = l.row_tiles, tile = warp % tiles, subset = warp / tiles, subsets = 8 / tiles;
+    const int r0 = tile * 16 + (lane >> 2), r1 = r0 + 8;
+    bool ok = true;
+    unsigned n = 0, met = 0; // units so far; meetings
+    Part part;
+    for (long long begin = w.at; next_part(p, w, part); begin = w.at)
+    {
+        if (warp == 0 && lane == 0 && part.first_unit == 0) write_meta(p, w, part, begin);
+        const int rows = min(l.block, l.rows - part.block * l.block); // of the item
+        const Row first = row_of(p, w.which, part, r0, D), second = row_of(p, w.which, part, r1, D);
+        Rows16<T, D> x;
+        x.load(p, first, second, lane);
+        // below this key every row with a token sees every key
+        const int all_see = __reduce_min_sync(0xffffffffu, min(first.keys ? first.keys : INT_MAX, second.keys ? second.keys : INT_MAX));
+        float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+        for (int u = 0; u < part.units; ++u, ++n)
+        {
+            int held = -1; // the unit's slot that the warp has waited for
+            for (int g = 0; g < tiles; ++g)
+            {
+                const int off = (subset * tiles + g) * 16, slot_of_unit = off / L::kSlotKeys;
+                const unsigned index = n * L::kUnitSlots + slot_of_unit, slot = index % kSlots;
+                if (slot_of_unit != held)
+                {
+                    if (held >= 0)
+                    {
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bars + 8 * (kSlots + (n * L::kUnitSlots + held) % kSlots));
+                    }
+                    held = slot_of_unit;
+                    if (ok) ok = warp_wait(bars + 8 * slot, (index / kSlots) & 1u);
+                }
+                const int key0 = (part.first_unit + u) * kUnit + off, valid = part.keys - key0;
+                if (!ok || valid <= 0) continue;
+                const uint32_t k = ring + slot * (2 * L::kSlotHalf) + (off % L::kSlotKeys) * 128, v = k + L::kSlotHalf;
+                float s[2][4] = {};
+                x.scores(k, lane, s);
+                if (key0 + 16 > all_see)
+                {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (key0 + 8 * t + 2 * (lane & 3) + (j & 1) >= (j < 2 ? first.keys : second.keys)) s[t][j] = -INFINITY;
+                }
+                float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
+                float t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+                t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
+                t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
+                t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
+                t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
+                if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1))
+                {
+                    const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+                    const float f0 = n0 == m0 ? 1.f : exp2_fast((m0 - n0) * p.scale), f1 = n1 == m1 ? 1.f : exp2_fast((m1 - n1) * p.scale);
+                    m0 = n0;
+                    m1 = n1;
+                    l0 *= f0;
+                    l1 *= f1;
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i)
+                    {
+                        o[i][0] *= f0;
+                        o[i][1] *= f0;
+                        o[i][2] *= f1;
+                        o[i][3] *= f1;
+                    }
+                }
+                const float c0 = m0 == -INFINITY ? 0.f : -m0 * p.scale, c1 = m1 == -INFINITY ? 0.f : -m1 * p.scale;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+                {
+                    s[t][0] = exp2_fast(fmaf(s[t][0], p.scale, c0));
+                    s[t][1] = exp2_fast(fmaf(s[t][1], p.scale, c0));
+                    s[t][2] = exp2_fast(fmaf(s[t][2], p.scale, c1));
+                    s[t][3] = exp2_fast(fmaf(s[t][3], p.scale, c1));
+                    l0 += s[t][0] + s[t][1];
+                    l1 += s[t][2] + s[t][3];
+                }
+                x.weigh(v, lane, s, valid, o);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + 8 * (kSlots + (n * L::kUnitSlots + held) % kSlots));
+        }
+        // a lane's sums cover its columns only
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        // the subsets of keys, the upper half into the lower, until one is left
+        for (int half = subsets / 2; half > 0; half /= 2)
+        {
+            if (subset >= half && subset < 2 * half)
+            {
+                const int place = (subset - half) * tiles + tile;
+                float *dst = scratch + place * (16 * D) + 2 * (lane & 3);
+                if ((lane & 3) == 0)
+                {
+                    stats[place * 16 + (lane >> 2)] = make_float2(m0, l0);
+                    stats[place * 16 + (lane >> 2) + 8] = make_float2(m1, l1);
+                }
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                {
+                    if (r0 < rows) *reinterpret_cast<float2 *>(dst + (lane >> 2) * D + 8 * i) = make_float2(o[i][0], o[i][1]);
+                    if (r1 < rows) *reinterpret_cast<float2 *>(dst + ((lane >> 2) + 8) * D + 8 * i) = make_float2(o[i][2], o[i][3]);
+                }
+            }
+            ok &= meet(bars + 8 * (2 * kSlots), met);
+            if (subset < half)
+            {
+                const int place = subset * tiles + tile;
+                const float *src = scratch + place * (16 * D) + 2 * (lane & 3);
+                const float2 s0 = stats[place * 16 + (lane >> 2)], s1 = stats[place * 16 + (lane >> 2) + 8];
+                const float n0 = fmaxf(m0, s0.x), n1 = fmaxf(m1, s1.x);
+                const float a0 = n0 == m0 ? 1.f : exp2_fast((m0 - n0) * p.scale), b0 = n0 == s0.x ? 1.f : exp2_fast((s0.x - n0) * p.scale);
+                const float a1 = n1 == m1 ? 1.f : exp2_fast((m1 - n1) * p.scale), b1 = n1 == s1.x ? 1.f : exp2_fast((s1.x - n1) * p.scale);
+                m0 = n0;
+                m1 = n1;
+                l0 = l0 * a0 + s0.y * b0;
+                l1 = l1 * a1 + s1.y * b1;
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                {
+                    if (r0 < rows)
+                    {
+                        const float2 v = *reinterpret_cast<const float2 *>(src + (lane >> 2) * D + 8 * i);
+                        o[i][0] = o[i][0] * a0 + v.x * b0;
+                        o[i][1] = o[i][1] * a0 + v.y * b0;
+                    }
+                    if (r1 < rows)
+                    {
+                        const float2 v = *reinterpret_cast<const float2 *>(src + ((lane >> 2) + 8) * D + 8 * i);
+                        o[i][2] = o[i][2] * a1 + v.x * b1;
+                        o[i][3] = o[i][3] * a1 + v.y * b1;
+                    }
+                }
+            }
+            ok &= meet(bars + 8 * (2 * kSlots), met);
+        }
+        if (!ok && lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+        if (subset == 0)
+        {
+            float *dst = l.o + part.place * l.part_rows * D + 2 * (lane & 3);
+            float2 *ml = l.ml + part.place * l.part_rows;
+            if ((lane & 3) == 0)
+            {
+                if (r0 < rows) ml[r0] = make_float2(m0 * p.scale, l0);
+                if (r1 < rows) ml[r1] = make_float2(m1 * p.scale, l1);
+            }
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+            {
+                if (r0 < rows) *reinterpret_cast<float2 *>(dst + static_cast<size_t>(r0) * D + 8 * i) = make_float2(o[i][0], o[i][1]);
+                if (r1 < rows) *reinterpret_cast<float2 *>(dst + static_cast<size_t>(r1) * D + 8 * i) = make_float2(o[i][2], o[i][3]);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- tile (BF16)
+// Shared memory: Q_A, Q_B, P_A, P_B, K (two buffers), V. TMEM: S_A 0, S_B 128, O_A 256, O_B 384.
+// As in the block attention, softmax copies S_g to registers and frees it, so that S_g of the next tile is
+// computed meanwhile, and rescales O_g only when a row's maximum has grown by more than 2^8.
+template <int D> struct TileSmem
+{
+    using L = Layout<__nv_bfloat16, D>;
+    uint32_t base, bars;
+    __device__ uint32_t q(int g) const { return base + g * L::kTileBytes; }
+    __device__ uint32_t k(int s) const { return base + (2 + s) * L::kTileBytes; }
+    __device__ uint32_t v() const { return base + 4 * L::kTileBytes; }
+    __device__ uint32_t p(int g) const { return base + 5 * L::kTileBytes + g * L::kWeightBytes; }
+    __device__ uint32_t q_full(int g) const { return bars + 8u * g; }
+    __device__ uint32_t k_full(int s) const { return bars + 8u * (2 + s); }
+    __device__ uint32_t k_empty(int s) const { return bars + 8u * (4 + s); }
+    __device__ uint32_t v_full() const { return bars + 8u * 6; }
+    __device__ uint32_t v_empty() const { return bars + 8u * 7; }
+    __device__ uint32_t s_full(int g) const { return bars + 8u * (8 + g); }
+    __device__ uint32_t s_free(int g) const { return bars + 8u * (10 + g); }
+    __device__ uint32_t p_full(int g) const { return bars + 8u * (12 + g); }
+    __device__ uint32_t pv_done(int g) const { return bars + 8u * (14 + g); }
+    __device__ uint32_t done() const { return bars + 8u * 16; }
+    __device__ uint32_t tmem_slot() const { return bars + 8u * 17; }
+};
+
+// Descriptor of V [key][dim] as the second operand (dims x keys, dims contiguous): 128-byte rows of 64 dims,
+// 8-key groups 1024 bytes apart, the other 64 dims a column block of 128 keys further on.
+__device__ __forceinline__ uint64_t value_desc(uint32_t addr)
+{
+    uint64_t desc = 0;
+    desc |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+    desc |= static_cast<uint64_t>((kUnit * 128) >> 4) << 16;
+    desc |= static_cast<uint64_t>(1024u >> 4) << 32;
+    desc |= static_cast<uint64_t>(1u) << 46;
+    desc |= static_cast<uint64_t>(2u) << 61;
+    return desc;
+}
+
+// One of K (value 0) and V (value 1) of the CTA's units; a lane per box.
+template <int D>
+__device__ __forceinline__ void tile_produce(const AttendArgs &p, Walk w, const CUtensorMap *map, const TileSmem<D> &sm, int value)
+{
+    using L = Layout<__nv_bfloat16, D>;
+    const int lane = threadIdx.x & 31, granules = kUnit / p.granule;
+    const int granule = lane % 16, column = lane / 16;
+    const bool active = granule < granules && column < L::kColumns;
+    const uint32_t into = column * (kUnit * 128) + granule * p.granule * 128;
+    unsigned n = 0;
+    Part part;
+    while (next_part(p, w, part))
+    {
+        int key = part.first_unit * kUnit + granule * p.granule;
+        int row = active ? pool_row(p, w.which, part, key) : 0;
+        for (int u = 0; u < part.units; ++u, ++n)
+        {
+            key += kUnit;
+            const int next = active ? pool_row(p, w.which, part, key) : 0;
+            const uint32_t full = value ? sm.v_full() : sm.k_full(n & 1), empty = value ? sm.v_empty() : sm.k_empty(n & 1);
+            const unsigned round = value ? n : n >> 1;
+            if (!warp_wait(empty, (round & 1u) ^ 1u))
+            {
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                return;
+            }
+            if (lane == 0) mbar_arrive_expect_tx(full, L::kTileBytes);
+            __syncwarp();
+            if (active) tma_load_2d((value ? sm.v() : sm.k(n & 1)) + into, map, full, column * 64, row);
+            row = next;
+        }
+    }
+}
+
+template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs &p, Walk w, const TileSmem<D> &sm, uint32_t tmem)
+{
+    const List &l = p.list[w.which];
+    constexpr uint32_t score_desc = idesc_bf16(128, 128);
+    constexpr uint32_t value_idesc = idesc_bf16(128, D) | (1u << 16); // second operand with contiguous dims
+    unsigned n = 0, seen[2] = {0, 0}, parts[2] = {0, 0}; // units; units and parts of each tile of rows
+    bool ok = true;
+    auto issue_s = [&](int g, unsigned unit) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+        {
+            const uint64_t ad = smem_desc_sw128(sm.q(g) + (i >> 2) * (kUnit * 128)) + 2u * (i & 3);
+            const uint64_t bd = smem_desc_sw128(sm.k(unit & 1) + (i >> 2) * (kUnit * 128)) + 2u * (i & 3);
+            umma_bf16(tmem + g * 128, ad, bd, score_desc, i > 0 ? 1u : 0u);
+        }
+        umma_commit(sm.s_full(g));
+    };
+    Part part;
+    while (ok && next_part(p, w, part))
+    {
+        const int groups = min(l.block, l.rows - part.block * l.block) > kUnit ? 2 : 1;
+        for (int g = 0; g < groups && ok; ++g) ok = mbar_wait(sm.q_full(g), parts[g]++ & 1u);
+        if (ok) ok = mbar_wait(sm.k_full(n & 1), (n >> 1) & 1u);
+        if (!ok) break;
+        tc_fence_after();
+        for (int g = 0; g < groups; ++g) issue_s(g, n);
+        umma_commit(sm.k_empty(n & 1));
+        for (int u = 0; u < part.units && ok; ++u, ++n)
+        {
+            if (u + 1 < part.units)
+            {
+                if (!(ok = mbar_wait(sm.k_full((n + 1) & 1), ((n + 1) >> 1) & 1u))) break;
+                for (int g = 0; g < groups; ++g)
+                {
+                    if (!(ok = mbar_wait(sm.s_free(g), seen[g] & 1u))) break;
+                    tc_fence_after();
+                    issue_s(g, n + 1);
+                }
+                if (!ok) break;
+                umma_commit(sm.k_empty((n + 1) & 1));
+            }
+            if (!(ok = mbar_wait(sm.v_full(), n & 1u))) break;
+            for (int g = 0; g < groups; ++g)
+            {
+                if (!(ok = mbar_wait(sm.p_full(g), seen[g]++ & 1u))) break;
+                tc_fence_after();
+#pragma unroll
+                for (int i = 0; i < kUnit / 16; ++i)
+                {
+                    const uint64_t ad = smem_desc_sw128(sm.p(g) + (i >> 2) * (kUnit * 128)) + 2u * (i & 3);
+                    umma_bf16(tmem + 256 + g * 128, ad, value_desc(sm.v() + i * 2048), value_idesc, (u > 0 || i > 0) ? 1u : 0u);
+                }
+                umma_commit(sm.pv_done(g));
+            }
+            if (ok) umma_commit(sm.v_empty());
+        }
+    }
+    if (!ok) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+}
+
+template <int D>
+__device__ __forceinline__ void tile_softmax(const AttendArgs &p, Walk w, const TileSmem<D> &sm, uint32_t tmem)
+{
+    const List &l = p.list[w.which];
+    const int warp = threadIdx.x / 32 - 4, lane = threadIdx.x & 31, g = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16), s_at = lanes + g * 128, o_at = lanes + 256 + g * 128;
+    const float c = p.scale;
+    unsigned seen = 0; // units of this tile of rows
+    bool ok = true;
+    unsigned n = 0; // units of the CTA
+    Part part;
+    for (long long begin = w.at; next_part(p, w, part); begin = w.at)
+    {
+        if (warp == 0 && lane == 0 && part.first_unit == 0) write_meta(p, w, part, begin);
+        const int rows = min(l.block, l.rows - part.block * l.block);
+        if (g * kUnit >= rows)
+        {
+            n += part.units;
+            continue;
+        }
+        const Row row = row_of(p, w.which, part, g * kUnit + r, D);
+        // the tile of queries: the warp's 32 rows, 16 bytes per lane, D/8 lanes per row
+        {
+            constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
+#pragma unroll 8
+            for (int i = 0; i < 32; i += kRowsAtOnce)
+            {
+                const int from = i + lane / kLanes, chunk = lane % kLanes, at = quarter * 32 + from;
+                const long long offset = __shfl_sync(0xffffffffu, row.offset, from);
+                const int keys = __shfl_sync(0xffffffffu, row.keys, from);
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (keys) x = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.a.q) + offset + chunk * 8);
+                st_shared_v4(sm.q(g) + (chunk >> 3) * (kUnit * 128) + at * 128 + (((chunk & 7) ^ (at & 7)) << 4), x.x, x.y, x.z, x.w);
+            }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sm.q_full(g));
+        float m = -INFINITY, sum = 0.f;
+        for (int u = 0; u < part.units && ok; ++u, ++seen)
+        {
+            if (!(ok = warp_wait(sm.s_full(g), seen & 1u))) break;
+            tc_fence_after();
+            float x[128];
+            tmem_load_128(s_at, x);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sm.s_free(g));
+            const int key0 = (part.first_unit + u) * kUnit, visible = row.keys - key0;
+            if (visible < kUnit)
+            {
+#pragma unroll
+                for (int k = 0; k < 128; ++k)
+                    if (k >= visible) x[k] = -INFINITY;
+            }
+            float mx[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mx[k] = x[k];
+#pragma unroll
+            for (int k = 8; k < 128; k += 2) mx[(k >> 1) & 7] = max3(mx[(k >> 1) & 7], x[k], x[k + 1]);
+            const float top = fmaxf(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], max3(mx[5], mx[6], mx[7])));
+            if (u > 0)
+            {
+                if (!(ok = warp_wait(sm.pv_done(g), (seen - 1) & 1u))) break;
+                tc_fence_after();
+            }
+            if (u == 0) m = top;
+            else if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) // NaN while neither is finite: no
+            {
+                const float raised = fmaxf(m, top), alpha = raised == m ? 1.f : exp2_fast((m - raised) * c);
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+                {
+                    float o[32];
+                    tmem_load_32(o_at + i * 32, o);
+#pragma unroll
+                    for (int t = 0; t < 32; ++t) o[t] *= alpha;
+                    tmem_store_32(o_at + i * 32, o);
+                }
+                tmem_store_wait();
+                sum *= alpha;
+                m = raised;
+            }
+            const float offset = m == -INFINITY ? 0.f : -m * c;
+            const float2 scale2 = make_float2(c, c), offset2 = make_float2(offset, offset);
+            float2 part_sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+            for (int k8 = 0; k8 < 128; k8 += 8)
+            {
+                uint32_t packed[4];
+#pragma unroll
+                for (int t = 0; t < 8; t += 2)
+                {
+                    const float2 arg = __ffma2_rn(make_float2(x[k8 + t], x[k8 + t + 1]), scale2, offset2);
+                    const float e0 = exp2_fast(arg.x), e1 = exp2_fast(arg.y);
+                    part_sum[t >> 1] = __fadd2_rn(part_sum[t >> 1], make_float2(e0, e1));
+                    packed[t >> 1] = pack2(e0, e1);
+                }
+                const int chunk = (k8 & 63) >> 3;
+                st_shared_v4(sm.p(g) + (k8 >> 6) * (kUnit * 128) + r * 128 + ((chunk ^ (r & 7)) << 4), packed[0], packed[1], packed[2], packed[3]);
+            }
+            const float2 s4 = __fadd2_rn(__fadd2_rn(part_sum[0], part_sum[1]), __fadd2_rn(part_sum[2], part_sum[3]));
+            sum += s4.x + s4.y;
+            // values past the item's last key may be anything, NaN too: zeros, by both tiles' threads alike
+            if (key0 + kUnit > part.keys)
+            {
+                if (!(ok = warp_wait(sm.v_full(), (n + u) & 1u))) break;
+                if (key0 + r >= part.keys)
+                {
+#pragma unroll
+                    for (int i = 0; i < D / 8; ++i) st_shared_v4(sm.v() + (i >> 3) * (kUnit * 128) + r * 128 + (i & 7) * 16, 0, 0, 0, 0);
+                }
+            }
+            fence_async_smem();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sm.p_full(g));
+        }
+        n += part.units;
+        if (ok) ok = warp_wait(sm.pv_done(g), (seen - 1) & 1u);
+        if (!ok)
+        {
+            if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+            break;
+        }
+        tc_fence_after();
+        const int at = g * kUnit + r;
+        if (at < rows) l.ml[part.place * l.part_rows + at] = make_float2(m * c, sum);
+        float *dst = l.o + (part.place * l.part_rows + at) * D;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+        {
+            float o[32];
+            tmem_load_32(o_at + i * 32, o);
+            if (at < rows)
+            {
+#pragma unroll
+                for (int t = 0; t < 32; t += 4) *reinterpret_cast<float4 *>(dst + i * 32 + t) = make_float4(o[t], o[t + 1], o[t + 2], o[t + 3]);
+            }
+        }
+        tc_fence_before();
+    }
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(sm.done());
+}
+
+// ---------------------------------------------------------------- the kernel
+template <class T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttendArgs p)
+{
+    using L = Layout<T, D>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t *base_ptr = smem_raw + (base - raw);
+    const uint32_t bars = base + L::kBody;
+    PlanShared &plan = *reinterpret_cast<PlanShared *>(base_ptr + L::kBody + 256);
+    float2 *stats = reinterpret_cast<float2 *>(base_ptr + L::kBody + 1024); // 4 x 16 of them
+    const int warp = threadIdx.x / 32;
+    if (threadIdx.x == 0)
+    {
+        prefetch_tensormap(&map_k);
+        prefetch_tensormap(&map_v);
+    }
+    grid_dependency_wait(); // the lengths, tables, queries and the cache are written from here on
+    grid_dependents_launch();
+    Walk w;
+    if (!make_plan(p, plan, w)) return;
+    const List &l = p.list[w.which];
+    TileSmem<D> sm{base, bars};
+    if (threadIdx.x == 0)
+    {
+        if (l.tile)
+        {
+            for (int g = 0; g < 2; ++g)
+            {
+                mbar_init(sm.q_full(g), 4);
+                mbar_init(sm.k_full(g), 1);
+                mbar_init(sm.k_empty(g), 1);
+                mbar_init(sm.s_full(g), 1);
+                mbar_init(sm.s_free(g), 4);
+                mbar_init(sm.p_full(g), 4);
+                mbar_init(sm.pv_done(g), 1);
+            }
+            mbar_init(sm.v_full(), 1);
+            mbar_init(sm.v_empty(), 1);
+            mbar_init(sm.done(), 8);
+        }
+        else
+        {
+            // the warps that read a slot: those of its keys' subsets, or all of them
+            const int readers = max(8 * L::kSlotKeys / kUnit, l.row_tiles);
+            for (int i = 0; i < kSlots; ++i)
+            {
+                mbar_init(bars + 8 * i, 1);
+                mbar_init(bars + 8 * (kSlots + i), readers);
+            }
+            mbar_init(bars + 8 * (2 * kSlots), 8);
+        }
+        fence_barrier_init();
+    }
+    if (l.tile && warp == 1)
+    {
+        tmem_alloc(sm.tmem_slot(), 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem = 0;
+    if (l.tile) tmem = *reinterpret_cast<volatile uint32_t *>(base_ptr + (sm.tmem_slot() - base));
+    if (warp < 4)
+    {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
+        if constexpr (sizeof(T) == 2)
+        {
+            if (l.tile)
+            {
+                if (warp == 0) tile_produce<D>(p, w, &map_k, sm, 0);
+                else if (warp == 2) tile_produce<D>(p, w, &map_v, sm, 1);
+                else if (warp == 1)
+                {
+                    if ((threadIdx.x & 31) == 0) tile_multiply<D>(p, w, sm, tmem);
+                    __syncwarp();
+                    if (!warp_wait(sm.done(), 0) && (threadIdx.x & 31) == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                    tc_fence_after();
+                    tmem_dealloc(tmem, 512);
+                }
+                return;
+            }
+        }
+        if (warp == 0) stream_produce<T, D>(p, w, &map_k, &map_v, base, bars);
+    }
+    else
+    {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsWork));
+        if constexpr (sizeof(T) == 2)
+        {
+            if (l.tile)
+            {
+                tile_softmax<D>(p, w, sm, tmem);
+                return;
+            }
+        }
+        stream_work<T, D>(p, w, base, bars, reinterpret_cast<float *>(base_ptr + L::kScratch), stats);
+    }
+}
+
+// ---------------------------------------------------------------- the join
+// A warp per row: the weights of its parts (a lane each), then the weighted sum of their values.
+constexpr int kJoinWarps = 8;
+
+template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ AttendArgs p)
+{
+    constexpr int N = D / 32; // values of a lane
+    const unsigned full = 0xffffffffu;
+    const int lane = threadIdx.x & 31;
+    const PagedBatch &b = p.a.batch;
+    const long long at = static_cast<long long>(blockIdx.x) * kJoinWarps + threadIdx.x / 32;
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const long long slots = static_cast<long long>(b.sequences) * b.queries;
+    if (at >= slots * p.a.heads) return;
+    const int slot = static_cast<int>(at / p.a.heads), head = static_cast<int>(at % p.a.heads);
+    const int s = slot / b.queries, i = slot % b.queries, kv_head = head / p.share;
+    const SequenceView view = sequence_view(b, p.a.kv.page_shift, s);
+    if (i >= view.count) return;
+    int parts[2] = {0, 0};
+    long long first[2] = {0, 0}; // row of the first part's statistics
+    const int per = b.sequences / b.groups, group = s / per;
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+    {
+        const List &l = p.list[which];
+        if (which == 0 ? view.prefix_len == 0 : view.len - view.count + i + 1 <= 0) continue;
+        const int owner = which == 0 ? group : s;
+        const int r = (which == 0 ? slot - group * per * b.queries : i) * p.share + head % p.share;
+        const long long item = (static_cast<long long>(owner) * l.blocks + r / l.block) * p.a.kv.kv_heads + kv_head;
+        const int2 meta = l.meta[item];
+        parts[which] = meta.y;
+        first[which] = (item + meta.x) * l.part_rows + r % l.block;
+    }
+    const int total = parts[0] + parts[1];
+    float top = -INFINITY, sum = 0.f, o[N] = {};
+    for (int base = 0; base < total; base += 32)
+    {
+        const int j = base + lane;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (j < parts[0]) ml = p.list[0].ml[first[0] + static_cast<long long>(j) * p.list[0].part_rows];
+        else if (j < total) ml = p.list[1].ml[first[1] + static_cast<long long>(j - parts[0]) * p.list[1].part_rows];
+        float most = ml.x;
+#pragma unroll
+        for (int step = 16; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor_sync(full, most, step));
+        most = fmaxf(most, top);
+        const float before = top == most ? 1.f : exp2_fast(top - most);
+        const float weight = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - most);
+        float l = weight * ml.y;
+#pragma unroll
+        for (int step = 16; step > 0; step >>= 1) l += __shfl_xor_sync(full, l, step);
+        sum = sum * before + l;
+        top = most;
+#pragma unroll
+        for (int d = 0; d < N; ++d) o[d] *= before;
+        const int here = min(32, total - base);
+#pragma unroll 4
+        for (int k = 0; k < here; ++k)
+        {
+            const float f = __shfl_sync(full, weight, k);
+            const int jj = base + k;
+            const float *src = jj < parts[0] ? p.list[0].o + (first[0] + static_cast<long long>(jj) * p.list[0].part_rows) * D
+                                             : p.list[1].o + (first[1] + static_cast<long long>(jj - parts[0]) * p.list[1].part_rows) * D;
+            float x[N];
+            if constexpr (N == 4)
+            {
+                const float4 t = *reinterpret_cast<const float4 *>(src + lane * 4);
+                x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+            }
+            else
+            {
+                const float2 t = *reinterpret_cast<const float2 *>(src + lane * 2);
+                x[0] = t.x, x[1] = t.y;
+            }
+#pragma unroll
+            for (int d = 0; d < N; ++d) o[d] = fmaf(f, x[d], o[d]);
+        }
+    }
+    const float inverse = sum > 0.f ? 1.f / sum : 0.f;
+    T *dst = static_cast<T *>(p.a.out) + at * D + lane * N;
+    if constexpr (sizeof(T) == 4)
+    {
+        if constexpr (N == 4) *reinterpret_cast<float4 *>(dst) = make_float4(o[0] * inverse, o[1] * inverse, o[2] * inverse, o[3] * inverse);
+        else *reinterpret_cast<float2 *>(dst) = make_float2(o[0] * inverse, o[1] * inverse);
+    }
+    else if constexpr (N == 4)
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0] * inverse, o[1] * inverse), pack2(o[2] * inverse, o[3] * inverse));
+    else
+        *reinterpret_cast<uint32_t *>(dst) = pack2(o[0] * inverse, o[1] * inverse);
+}
+
+// ---------------------------------------------------------------- host
+constexpr int kTileRows = 32; // more rows than this go to the tensor cores' tiles
+
+size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// Lays out the lists and the workspace; returns its size.
+size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, void *workspace, AttendArgs &p)
+{
+    p.ctas = ctas;
+    p.share = heads / kv.kv_heads;
+    char *base = static_cast<char *>(workspace);
+    size_t at = 0;
+    for (int i = 0; i < 2; ++i)
+    {
+        List &l = p.list[i];
+        l.owners = i == 0 ? (b.max_prefix_pages ? b.groups : 0) : b.sequences;
+        l.rows = (i == 0 ? b.sequences / b.groups : 1) * b.queries * p.share;
+        l.tile = kv.bf16 && l.rows > kTileRows;
+        l.row_tiles = 1;
+        while (l.row_tiles < 8 && 16 * l.row_tiles < l.rows) l.row_tiles *= 2;
+        l.block = l.tile ? 2 * kUnit : 16 * l.row_tiles;
+        l.blocks = (l.rows + l.block - 1) / l.block;
+        l.part_rows = l.rows < l.block ? l.rows : l.block;
+        l.cost = l.tile ? (l.rows > kUnit ? 14 : 9) : kv.bf16 ? 12 : (l.row_tiles < 4 ? 24 : 14 * l.row_tiles);
+        const size_t items = static_cast<size_t>(l.owners) * l.blocks * kv.kv_heads, parts = l.owners ? items + ctas : 0;
+        l.o = reinterpret_cast<float *>(base + at);
+        at += rounded(parts * l.part_rows * kv.dim * sizeof(float));
+        l.ml = reinterpret_cast<float2 *>(base + at);
+        at += rounded(parts * l.part_rows * sizeof(float2));
+        l.meta = reinterpret_cast<int2 *>(base + at);
+        at += rounded(items * sizeof(int2));
+    }
+    return at;
+}
+
+bool map_pool(CUtensorMap *map, const void *pool, const PagedLayer &kv, int granule)
+{
+    const auto encode = tensor_map_encoder();
+    if (!encode) return false;
+    const cuuint64_t element = kv.bf16 ? 2 : 4;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(kv.dim), (static_cast<cuuint64_t>(kv.pages) * kv.kv_heads) << kv.page_shift};
+    const cuuint64_t strides[1] = {kv.dim * element};
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(128 / element), static_cast<cuuint32_t>(granule)};
+    const cuuint32_t element_strides[2] = {1, 1};
+    return encode(map, kv.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void *>(pool), dims,
+                  strides, box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <class T, int D> int launch(const PrefixAttentionArgs &a, int sms, cudaStream_t stream)
+{
+    AttendArgs p;
+    p.a = a;
+    lay_out(a.kv, a.batch, a.heads, sms, a.workspace, p);
+    p.scale = 1.4426950408889634f / sqrtf(static_cast<float>(D));
+    p.granule = 1 << a.kv.page_shift;
+    if (p.granule > Kind<T>::kSlotKeys) p.granule = Kind<T>::kSlotKeys;
+    CUtensorMap map_k, map_v;
+    if (!map_pool(&map_k, a.kv.k, a.kv, p.granule) || !map_pool(&map_v, a.kv.v, a.kv, p.granule)) return cudaErrorInvalidValue;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3(sms);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Layout<T, D>::kSmemBytes;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, attend_kernel<T, D>, map_k, map_v, p);
+    if (e != cudaSuccess) return e;
+    const long long rows = static_cast<long long>(a.batch.sequences) * a.batch.queries * a.heads;
+    cfg.gridDim = dim3(static_cast<unsigned>((rows + kJoinWarps - 1) / kJoinWarps));
+    cfg.blockDim = dim3(kJoinWarps * 32);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p);
+}
+
+template <class T, int D> cudaError_t prepare()
+{
+    cudaFuncAttributes attr;
+    const cudaError_t e = cudaFuncGetAttributes(&attr, attend_kernel<T, D>);
+    if (e != cudaSuccess) return e;
+    // the register split needs this many registers per thread at launch
+    if (attr.numRegs < kMinLaunchRegs) return cudaErrorInvalidConfiguration;
+    static_assert(Layout<T, D>::kSmemBytes <= 232448, "shared memory of a CTA");
+    return cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<T, D>::kSmemBytes);
 }
 } // namespace
 
-size_t prefix_attention_workspace(const PagedLayer &, const PagedBatch &, int, int) { return 16; }
-int prepare_prefix_attention_kernels() { return cudaSuccess; }
-
-int launch_prefix_attention(const PrefixAttentionArgs &a, int, cudaStream_t stream)
+size_t prefix_attention_workspace(const PagedLayer &kv, const PagedBatch &batch, int heads, int sms)
 {
-    const dim3 grid(a.batch.sequences * a.batch.queries, a.heads);
-    if (a.kv.bf16)
-    {
-        if (a.kv.dim == 64) attend_kernel<__nv_bfloat16, 64><<<grid, kWarps * 32, 0, stream>>>(a);
-        else attend_kernel<__nv_bfloat16, 128><<<grid, kWarps * 32, 0, stream>>>(a);
-    }
-    else if (a.kv.dim == 64) attend_kernel<float, 64><<<grid, kWarps * 32, 0, stream>>>(a);
-    else attend_kernel<float, 128><<<grid, kWarps * 32, 0, stream>>>(a);
-    return cudaGetLastError();
+    AttendArgs p;
+    return lay_out(kv, batch, heads, sms, nullptr, p);
+}
+
+int prepare_prefix_attention_kernels()
+{
+    cudaError_t e = prepare<__nv_bfloat16, 128>();
+    if (e == cudaSuccess) e = prepare<__nv_bfloat16, 64>();
+    if (e == cudaSuccess) e = prepare<float, 128>();
+    if (e == cudaSuccess) e = prepare<float, 64>();
+    return e;
+}
+
+int launch_prefix_attention(const PrefixAttentionArgs &a, int sms, cudaStream_t stream)
+{
+    if (a.kv.bf16) return a.kv.dim == 64 ? launch<__nv_bfloat16, 64>(a, sms, stream) : launch<__nv_bfloat16, 128>(a, sms, stream);
+    return a.kv.dim == 64 ? launch<float, 64>(a, sms, stream) : launch<float, 128>(a, sms, stream);
 }
 } // namespace ernie_b200
