@@ -39,16 +39,15 @@ __device__ __forceinline__ int clamped_length(int len, int max_pages, int page_s
     return len < 0 ? 0 : static_cast<int>(most);
 }
 
-struct SequenceView
+struct OwnView
 {
     int len;   // own tokens
     int count; // of them new
-    int prefix_len;
 };
 
-__device__ __forceinline__ SequenceView sequence_view(const PagedBatch &b, int page_shift, int s)
+__device__ __forceinline__ OwnView own_view(const PagedBatch &b, int page_shift, int s)
 {
-    SequenceView v;
+    OwnView v;
     v.len = clamped_length(b.lens[s], b.max_pages, page_shift, b.error_flag);
     v.count = b.counts ? b.counts[s] : b.queries;
     if (v.count < 0 || v.count > b.queries)
@@ -56,6 +55,18 @@ __device__ __forceinline__ SequenceView sequence_view(const PagedBatch &b, int p
         report_range(b.error_flag);
         v.count = v.count < 0 ? 0 : b.queries;
     }
+    return v;
+}
+
+struct SequenceView : OwnView
+{
+    int prefix_len;
+};
+
+__device__ __forceinline__ SequenceView sequence_view(const PagedBatch &b, int page_shift, int s)
+{
+    SequenceView v;
+    static_cast<OwnView &>(v) = own_view(b, page_shift, s);
     v.prefix_len = 0;
     if (b.max_prefix_pages)
         v.prefix_len = clamped_length(b.prefix_lens[s / (b.sequences / b.groups)], b.max_prefix_pages, page_shift, b.error_flag);

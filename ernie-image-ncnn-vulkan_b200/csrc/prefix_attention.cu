@@ -8,18 +8,20 @@
 //           read once per block of rows however many sequences share it;
 //   own     (sequence, block of rows, K/V head): a sequence's rows against its own tokens.
 // A row is a query head of a slot: the heads/kv_heads query heads that share a K/V head are rows of one item.
-// An item's keys are cut into units of 128. Each list's units are dealt out evenly, in order, to that list's
-// CTAs, so that an item may span several CTAs and a CTA several items; an item's share of a CTA is a part.
-// Along the order both the item and the CTA only ever step up, so item + CTA numbers the parts without gaps
-// or clashes, and an item's parts lie side by side. The lists share the CTAs by their estimated cost. All of
-// this is worked out on the device, by every CTA for itself, from the lengths of this very call.
+// An item's keys are cut into units, and each list's units are dealt out evenly, in order, to that list's
+// workers, so that an item may span several workers and a worker several items; an item's share of a worker
+// is a part. Along the order both the item and the worker only ever step up, so item + worker numbers the
+// parts without gaps or clashes, and an item's parts lie side by side. The lists share the CTAs by their
+// estimated cost. All of this is worked out on the device, by every CTA for itself, from the lengths of this
+// very call.
 //
-// A CTA works on its units in one of two ways, chosen per list on the host by the rows of a block:
-//   stream  few rows, or an FP32 cache: eight warps with mma.sync m16n8 tiles, 16 rows x 16 keys at a time,
-//           fed by a six-slot TMA ring. The bound is the K/V traffic: a unit of BF16 K and V is 64 KB;
-//           FP32 operands are split into two TF32 parts and multiplied in three products.
-//   tile    many rows of a BF16 cache: 256 rows (two tiles of 128) share each K/V tile on the tensor cores
-//           (tcgen05.mma, accumulators in TMEM), one row per softmax thread.
+// A list is worked on in one of two ways, chosen on the host by the rows of an item:
+//   stream  few rows, or an FP32 cache. A worker is a warp: 16 rows, its own TMA ring of K/V slots, mma.sync
+//           m16n8 tiles. The bound is the K/V traffic, and eight independent warps per SM hide each other's
+//           latencies without ever meeting. FP32 operands are split into two TF32 parts and multiplied in
+//           three products.
+//   tile    many rows of a BF16 cache. A worker is a CTA: 256 rows (two tiles of 128) share each K/V tile on
+//           the tensor cores (tcgen05.mma, accumulators in TMEM), one row per softmax thread.
 // A second kernel joins the parts of each row.
 #include "decode.h"
 #include "ptx.cuh"
@@ -32,27 +34,27 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 namespace
 {
 constexpr int kThreads = 384; // three warpgroups: control, and twice four working warps
-constexpr int kUnit = 128;    // keys of a unit
+constexpr int kWorkers = 8;   // streaming warps of a CTA
+constexpr int kTile = 128;    // rows and keys of a tile
 // As for the block attention: 128 x 88 + 256 x 208 registers are the launch's 384 x 168.
 constexpr int kRegsControl = 88, kRegsWork = 208, kMinLaunchRegs = 168;
 static_assert(128 * kRegsControl + 256 * kRegsWork <= kThreads * kMinLaunchRegs, "register split");
-constexpr int kSlots = 6;
 constexpr int kErrAttendTimeout = 42;
 
 // One of the two lists, as the host lays it out.
 struct List
 {
-    int owners;    // groups or sequences
-    int rows;      // of an owner and K/V head
-    int block;     // rows of an item
-    int blocks;    // items of an owner and K/V head
-    int part_rows; // rows that a part stores
-    int tile;      // 1: on the tensor cores' tiles, 0: streamed
-    int row_tiles; // streamed: 16-row tiles of an item (1, 2, 4 or 8)
-    int cost;      // of a unit, relative
-    float *o;      // [items + CTAs][part_rows][D]
-    float2 *ml;    // [items + CTAs][part_rows]
-    int2 *meta;    // [items]: first part's CTA, number of parts
+    int owners;     // groups or sequences
+    int rows;       // of an owner and K/V head
+    int block;      // rows of an item
+    int blocks;     // items of an owner and K/V head
+    int part_rows;  // rows that a part stores
+    int tile;       // 1: on the tensor cores' tiles, 0: streamed
+    int unit_shift; // log2 of a unit's keys
+    int cost;       // of a unit on an SM, relative
+    float *o;       // [items + workers][part_rows][D]
+    float2 *ml;     // [items + workers][part_rows]
+    int2 *meta;     // [items]: first part's worker, number of parts
 };
 
 struct AttendArgs
@@ -65,29 +67,18 @@ struct AttendArgs
     int granule;  // keys of a TMA box
 };
 
-template <class T> struct Kind;
-template <> struct Kind<__nv_bfloat16>
-{
-    static constexpr int kSlotKeys = 64;
-};
-template <> struct Kind<float>
-{
-    static constexpr int kSlotKeys = 32;
-};
-
 template <class T, int D> struct Layout
 {
-    static constexpr int kSlotKeys = Kind<T>::kSlotKeys;
-    static constexpr int kColumns = D * static_cast<int>(sizeof(T)) / 128; // 128-byte column blocks of a row
+    static constexpr int kSlotKeys = sizeof(T) == 2 ? 16 : 8;                     // a K/V slot: one step of a streaming warp
+    static constexpr int kColumns = D * static_cast<int>(sizeof(T)) / 128;        // 128-byte column blocks of a row
     static constexpr int kSlotHalf = kSlotKeys * D * static_cast<int>(sizeof(T)); // K or V of a slot
-    static constexpr int kUnitSlots = kUnit / kSlotKeys;
-    static constexpr int kScratch = kSlots * 2 * kSlotHalf; // the warps' merge area behind the ring
-    static constexpr int kStreamBytes = kScratch + 4 * 16 * D * 4;
-    static constexpr int kTileBytes = kUnit * D * 2;       // a Q, K or V tile
-    static constexpr int kWeightBytes = kUnit * kUnit * 2; // a P tile
+    static constexpr int kRing = D == 128 ? 3 : 7;                                // slots of a warp
+    static constexpr int kStreamBytes = kWorkers * kRing * 2 * kSlotHalf;
+    static constexpr int kTileBytes = kTile * D * 2;       // a Q, K or V tile
+    static constexpr int kWeightBytes = kTile * kTile * 2; // a P tile
     static constexpr int kTileModeBytes = 5 * kTileBytes + 2 * kWeightBytes;
     static constexpr int kBody = kStreamBytes > kTileModeBytes ? kStreamBytes : kTileModeBytes;
-    static constexpr int kSmemBytes = kBody + 1024 + 2048; // alignment; barriers, the plan and the merge statistics
+    static constexpr int kSmemBytes = kBody + 1024 + 2048; // alignment; barriers and the plan
 };
 
 __device__ __forceinline__ float exp2_fast(float x)
@@ -121,6 +112,13 @@ __device__ __forceinline__ float ld_shared(uint32_t addr)
 {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float4 ld_shared_v4(uint32_t addr)
+{
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
 
@@ -161,88 +159,93 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t &high, uint32_t &lo
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(low) : "f"(x - __uint_as_float(high)));
 }
 
+// The same, worked out anew where it stands: hoisted out of the key loop the queries' parts would spill.
+__device__ __forceinline__ void split_tf32_here(float x, uint32_t &high, uint32_t &low)
+{
+    asm volatile("cvt.rna.tf32.f32 %0, %1;" : "=r"(high) : "f"(x));
+    asm volatile("cvt.rna.tf32.f32 %0, %1;" : "=r"(low) : "f"(x - __uint_as_float(high)));
+}
+
 // A whole warp's bounded wait, with one answer for all its lanes.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity)
 {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity));
 }
 
-// The eight working warps meet (bounded, like every wait).
-__device__ __forceinline__ bool meet(uint32_t bar, unsigned &round)
-{
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-    return warp_wait(bar, round++ & 1u);
-}
-
 // ---------------------------------------------------------------- the plan
-// Keys that the rows of an item see at most, and with it the item's units.
+// Keys that the rows of an item see at most.
 __device__ __forceinline__ int item_keys(const AttendArgs &p, int which, int owner, int block)
 {
     const PagedBatch &b = p.a.batch;
     if (which == 0) return clamped_length(b.prefix_lens[owner], b.max_prefix_pages, p.a.kv.page_shift, b.error_flag);
-    const SequenceView v = sequence_view(b, p.a.kv.page_shift, owner);
+    const OwnView v = own_view(b, p.a.kv.page_shift, owner);
     const int first = block * p.list[1].block, rows = min(first + p.list[1].block, v.count * p.share);
     if (rows <= first) return 0;
     return max(0, v.len - v.count + (rows - 1) / p.share + 1);
 }
 
-__device__ __forceinline__ int units_of(int keys) { return (keys + kUnit - 1) / kUnit; }
-
-// The CTA of a list of `units` dealt out to `ctas` that holds unit u (the inverse of first_unit).
-__device__ __forceinline__ int cta_of_unit(long long u, long long units, int ctas)
+__device__ __forceinline__ int units_of(const List &l, int keys)
 {
-    return static_cast<int>(((u + 1) * ctas - 1) / units);
+    return (keys >> l.unit_shift) + ((keys & ((1 << l.unit_shift) - 1)) != 0);
 }
-__device__ __forceinline__ long long first_unit(int cta, long long units, int ctas) { return cta * units / ctas; }
+
+// `units` dealt out to `workers`: the first units % workers of them take one more.
+__device__ __forceinline__ int first_unit(int worker, int units, int workers)
+{
+    const int each = units / workers;
+    return worker * each + min(worker, units - each * workers);
+}
+__device__ __forceinline__ int worker_of_unit(int u, int units, int workers)
+{
+    const int each = units / workers, more = units - each * workers, ahead = more * (each + 1);
+    return u < ahead ? u / (each + 1) : more + (u - ahead) / each;
+}
+
+// A worker's walk over its units.
+struct Walk
+{
+    int worker, workers; // within the list
+    int at, end, units;  // next unit, the worker's last and the list's number of them
+    int owner, block, head, unit; // the next unit's item and its number within the item
+};
 
 struct PlanShared
 {
-    long long warp_sum[2][kThreads / 32];
-    int owner, block, head, unit; // where the CTA begins
-};
-
-// A CTA's walk over its units.
-struct Walk
-{
-    int which;           // list
-    int cta, ctas;       // within the list
-    long long at, end, units;
-    int owner, block, head, unit; // the next unit's item and its number within the item
+    int warp_sum[2][kThreads / 32];
+    int4 begin[kWorkers]; // owner, block, head, unit where a worker begins
 };
 
 struct Part
 {
     int owner, block, head;
-    int keys;               // of the item
-    int first_unit, units;  // of the part
-    long long place;        // of its results
+    int keys;              // of the item
+    int first_unit, units; // of the part
+    int place;             // of its results
 };
 
-// The next part of the walk; false at its end. Every warp of the CTA takes the same steps.
-__device__ __forceinline__ bool next_part(const AttendArgs &p, Walk &w, Part &part)
+// The next part of the walk; false at its end. All threads of a worker take the same steps.
+__device__ __forceinline__ bool next_part(const AttendArgs &p, int which, Walk &w, Part &part)
 {
     if (w.at >= w.end) return false;
-    const List &l = p.list[w.which];
+    const List &l = p.list[which];
     int keys, units;
-    if (w.owner >= l.owners) return false;
     for (;;)
     {
-        keys = item_keys(p, w.which, w.owner, w.block);
-        units = units_of(keys);
+        if (w.owner >= l.owners) return false; // only if the lengths change under the call
+        keys = item_keys(p, which, w.owner, w.block);
+        units = units_of(l, keys);
         if (w.unit < units) break;
         w.unit = 0;
         w.head = 0;
         if (++w.block == l.blocks) w.block = 0, ++w.owner;
-        if (w.owner >= l.owners) return false; // the lengths have changed under the call
     }
     part.owner = w.owner;
     part.block = w.block;
     part.head = w.head;
     part.keys = keys;
     part.first_unit = w.unit;
-    part.units = static_cast<int>(min(static_cast<long long>(units - w.unit), w.end - w.at));
-    part.place = (static_cast<long long>(w.owner) * l.blocks + w.block) * p.a.kv.kv_heads + w.head + w.cta;
+    part.units = min(units - w.unit, w.end - w.at);
+    part.place = (w.owner * l.blocks + w.block) * p.a.kv.kv_heads + w.head + w.worker;
     w.at += part.units;
     w.unit += part.units;
     if (w.unit == units)
@@ -257,100 +260,122 @@ __device__ __forceinline__ bool next_part(const AttendArgs &p, Walk &w, Part &pa
     return true;
 }
 
-// Written by the part that holds the item's first unit (`begin`: that unit's number in the list).
-__device__ __forceinline__ void write_meta(const AttendArgs &p, const Walk &w, const Part &part, long long begin)
+// Written by the part that holds the item's first unit; `w` has just stepped over the part.
+__device__ __forceinline__ void write_meta(const AttendArgs &p, int which, const Walk &w, const Part &part)
 {
-    const int last = cta_of_unit(begin + units_of(part.keys) - 1, w.units, w.ctas);
-    p.list[w.which].meta[part.place - w.cta] = make_int2(w.cta, last - w.cta + 1);
+    const List &l = p.list[which];
+    const int last = worker_of_unit(w.at - part.units + units_of(l, part.keys) - 1, w.units, w.workers);
+    l.meta[part.place - w.worker] = make_int2(w.worker, last - w.worker + 1);
 }
 
-// All threads: the lists' units, the CTA's list and its share. False: nothing to do.
-__device__ bool make_plan(const AttendArgs &p, PlanShared &s, Walk &w)
+// All threads: the lists' units, the CTA's list (-1: nothing to do) and its workers' shares. `mine` is the
+// walk of worker `warp` of the CTA (streamed) or of the CTA (tile: worker 0).
+struct Plan
 {
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    long long mine[2], before[2];
-    int chunk[2];
+    int which, cta, ctas, units, workers;
+};
+
+__device__ __forceinline__ Walk walk_of(const AttendArgs &p, const Plan &plan, const PlanShared &s, int local)
+{
+    Walk w;
+    w.worker = local * plan.ctas + plan.cta; // neighbours in the order go to different SMs
+    w.workers = plan.workers;
+    w.units = plan.units;
+    const bool any = w.worker < plan.workers;
+    w.at = any ? first_unit(w.worker, plan.units, plan.workers) : 0;
+    w.end = any ? first_unit(w.worker + 1, plan.units, plan.workers) : 0;
+    const int4 b = s.begin[local];
+    w.owner = b.x;
+    w.block = b.y;
+    w.head = b.z;
+    w.unit = b.w;
+    return w;
+}
+
+__device__ __forceinline__ Plan make_plan(const AttendArgs &p, PlanShared &s)
+{
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, heads = p.a.kv.kv_heads;
+    int mine[2], before[2], chunk[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
     {
         const List &l = p.list[i];
-        chunk[i] = (l.owners + kThreads - 1) / kThreads;
-        long long sum = 0;
+        chunk[i] = l.owners <= kThreads ? 1 : (l.owners + kThreads - 1) / kThreads;
+        int sum = 0;
         for (int o = tid * chunk[i]; o < min(l.owners, (tid + 1) * chunk[i]); ++o)
-            for (int b = 0; b < l.blocks; ++b) sum += units_of(item_keys(p, i, o, b));
-        mine[i] = sum * p.a.kv.kv_heads;
-        long long scan = mine[i];
+            for (int b = 0; b < l.blocks; ++b) sum += units_of(l, item_keys(p, i, o, b));
+        mine[i] = sum * heads;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+    {
+        int scan = mine[i];
 #pragma unroll
         for (int step = 1; step < 32; step *= 2)
         {
-            const long long other = __shfl_up_sync(0xffffffffu, scan, step);
+            const int other = __shfl_up_sync(0xffffffffu, scan, step);
             if (lane >= step) scan += other;
         }
         before[i] = scan - mine[i];
         if (lane == 31) s.warp_sum[i][warp] = scan;
     }
     __syncthreads();
-    long long total[2] = {0, 0};
+    int total[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < kThreads / 32; ++j)
         {
-            if (j < warp) before[i] += s.warp_sum[i][j];
-            total[i] += s.warp_sum[i][j];
+            const int sum = s.warp_sum[i][j];
+            if (j < warp) before[i] += sum;
+            total[i] += sum;
         }
-    if (total[0] + total[1] == 0) return false;
+    Plan plan = {-1, 0, 0, 0, 0};
+    if (total[0] + total[1] == 0) return plan;
     // the lists' CTAs: by cost, at least one for a list with work, no more than it has units
-    const double cost0 = static_cast<double>(total[0]) * p.list[0].cost, cost1 = static_cast<double>(total[1]) * p.list[1].cost;
-    int n0 = static_cast<int>(p.ctas * (cost0 / (cost0 + cost1)) + 0.5);
-    n0 = total[0] == 0 ? 0 : max(1, total[1] == 0 ? p.ctas : min(p.ctas - 1, n0));
-    int n1 = p.ctas - n0;
-    if (n0 > total[0]) n0 = static_cast<int>(total[0]), n1 = total[1] ? p.ctas - n0 : 0;
-    if (n1 > total[1]) n1 = static_cast<int>(total[1]);
-    if (total[0] && n0 + n1 < p.ctas) n0 = static_cast<int>(min(total[0], static_cast<long long>(p.ctas - n1)));
+    const float cost0 = static_cast<float>(total[0]) * p.list[0].cost, cost1 = static_cast<float>(total[1]) * p.list[1].cost;
+    int n0 = static_cast<int>(p.ctas * __fdividef(cost0, cost0 + cost1) + 0.5f);
+    n0 = total[0] == 0 ? 0 : total[1] == 0 ? p.ctas : max(1, min(p.ctas - 1, n0));
+    if (n0 > total[0]) n0 = total[0];
+    const int n1 = min(total[1], p.ctas - n0);
+    if (n0 + n1 < p.ctas) n0 = min(total[0], p.ctas - n1);
     const int cta = blockIdx.x;
-    if (cta >= n0 + n1) return false;
-    w.which = cta < n0 ? 0 : 1;
-    w.cta = cta - (w.which ? n0 : 0);
-    w.ctas = w.which ? n1 : n0;
-    w.units = w.which ? total[1] : total[0];
-    w.at = first_unit(w.cta, w.units, w.ctas);
-    w.end = first_unit(w.cta + 1, w.units, w.ctas);
-    const long long ahead = w.which ? before[1] : before[0], held = w.which ? mine[1] : mine[0];
-    if (w.at >= ahead && w.at < ahead + held)
+    if (cta >= n0 + n1) return plan;
+    plan.which = cta < n0 ? 0 : 1;
+    plan.cta = plan.which ? cta - n0 : cta;
+    plan.ctas = plan.which ? n1 : n0;
+    plan.units = plan.which ? total[1] : total[0];
+    const List &l = p.list[plan.which];
+    plan.workers = l.tile ? plan.ctas : min(plan.units, plan.ctas * kWorkers);
+    const int ahead = plan.which ? before[1] : before[0], held = plan.which ? mine[1] : mine[0];
+    for (int local = 0; local < (l.tile ? 1 : kWorkers); ++local)
     {
-        const List &l = p.list[w.which];
-        long long left = w.at - ahead;
-        int o = tid * (w.which ? chunk[1] : chunk[0]), b = 0, units;
+        const int worker = local * plan.ctas + plan.cta;
+        if (worker >= plan.workers) break;
+        int left = first_unit(worker, plan.units, plan.workers) - ahead;
+        if (left < 0 || left >= held) continue;
+        int o = tid * (plan.which ? chunk[1] : chunk[0]), b = 0, units;
         for (;;)
         {
-            units = units_of(item_keys(p, w.which, o, b));
-            const long long item = static_cast<long long>(units) * p.a.kv.kv_heads;
-            if (left < item) break;
-            left -= item;
+            units = units_of(l, item_keys(p, plan.which, o, b));
+            if (left < units * heads) break;
+            left -= units * heads;
             if (++b == l.blocks) b = 0, ++o;
         }
-        s.owner = o;
-        s.block = b;
-        s.head = static_cast<int>(left / units);
-        s.unit = static_cast<int>(left % units);
+        s.begin[local] = make_int4(o, b, left / units, left % units);
     }
     __syncthreads();
-    w.owner = s.owner;
-    w.block = s.block;
-    w.head = s.head;
-    w.unit = s.unit;
-    return true;
+    return plan;
 }
 
 // ---------------------------------------------------------------- rows
 struct Row
 {
-    long long offset; // of the query in q, in elements
-    int keys;         // that the row sees of the item's; 0 without a token
+    int query; // row of q and out
+    int keys;  // that the row sees of the item's; 0 without a token
 };
 
-__device__ __forceinline__ Row row_of(const AttendArgs &p, int which, const Part &part, int row, int dim)
+__device__ __forceinline__ Row row_of(const AttendArgs &p, int which, const Part &part, int row)
 {
     const PagedBatch &b = p.a.batch;
     const List &l = p.list[which];
@@ -358,23 +383,23 @@ __device__ __forceinline__ Row row_of(const AttendArgs &p, int which, const Part
     Row out = {0, 0};
     if (row >= l.block || r >= l.rows) return out;
     const int at = r / p.share, head = part.head * p.share + r - at * p.share;
-    long long slot;
+    int slot;
     if (which == 0)
     {
-        const int per = b.sequences / b.groups, s = part.owner * per + at / b.queries, i = at % b.queries;
-        const int count = b.counts ? b.counts[s] : b.queries;
-        if (i >= count) return out;
-        slot = static_cast<long long>(s) * b.queries + i;
+        const int per = l.rows / p.share; // slots of the group
+        slot = part.owner * per + at;
+        const int s = slot / b.queries, i = slot - s * b.queries;
+        if (b.counts && i >= b.counts[s]) return out;
         out.keys = part.keys;
     }
     else
     {
-        const SequenceView v = sequence_view(b, p.a.kv.page_shift, part.owner);
+        const OwnView v = own_view(b, p.a.kv.page_shift, part.owner);
         if (at >= v.count) return out;
-        slot = static_cast<long long>(part.owner) * b.queries + at;
+        slot = part.owner * b.queries + at;
         out.keys = max(0, v.len - v.count + at + 1);
     }
-    out.offset = (slot * p.a.heads + head) * dim;
+    out.query = slot * p.a.heads + head;
     return out;
 }
 
@@ -398,41 +423,48 @@ __device__ __forceinline__ int pool_row(const AttendArgs &p, int which, const Pa
 }
 
 // ---------------------------------------------------------------- stream
-// A warp's 16 rows: queries, running maximum, sum and weighted values, in mma.sync fragments (rows lane/4
-// and lane/4 + 8; a lane's columns 2 (lane % 4) and the next of every eight).
+// A warp's 16 rows in mma.sync fragments: rows lane/4 and lane/4 + 8; a lane's columns are 2 (lane % 4) and
+// the next of every eight. A slot holds K and V of kSlotKeys keys, 128-byte rows in swizzled column blocks.
 template <class T, int D> struct Rows16;
 
 template <int D> struct Rows16<__nv_bfloat16, D>
 {
+    static constexpr int kKeys = 16, kTiles = 2; // of a step; score tiles of eight keys
     uint32_t q[D / 16][4];
     __device__ __forceinline__ void load(const AttendArgs &p, const Row &r0, const Row &r1, int lane)
     {
         const __nv_bfloat16 *base = static_cast<const __nv_bfloat16 *>(p.a.q) + 2 * (lane & 3);
+        const __nv_bfloat16 *x0 = base + static_cast<size_t>(r0.query) * D, *x1 = base + static_cast<size_t>(r1.query) * D;
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
         {
-            q[s][0] = r0.keys ? *reinterpret_cast<const uint32_t *>(base + r0.offset + 16 * s) : 0u;
-            q[s][1] = r1.keys ? *reinterpret_cast<const uint32_t *>(base + r1.offset + 16 * s) : 0u;
-            q[s][2] = r0.keys ? *reinterpret_cast<const uint32_t *>(base + r0.offset + 16 * s + 8) : 0u;
-            q[s][3] = r1.keys ? *reinterpret_cast<const uint32_t *>(base + r1.offset + 16 * s + 8) : 0u;
+            q[s][0] = r0.keys ? *reinterpret_cast<const uint32_t *>(x0 + 16 * s) : 0u;
+            q[s][1] = r1.keys ? *reinterpret_cast<const uint32_t *>(x1 + 16 * s) : 0u;
+            q[s][2] = r0.keys ? *reinterpret_cast<const uint32_t *>(x0 + 16 * s + 8) : 0u;
+            q[s][3] = r1.keys ? *reinterpret_cast<const uint32_t *>(x1 + 16 * s + 8) : 0u;
         }
     }
-    // scores of 16 keys: two tiles of eight
-    __device__ __forceinline__ void scores(uint32_t k, int lane, float (&s)[2][4]) const
+    // two chains per score tile, so that a step waits for half as many products in a row
+    __device__ __forceinline__ void scores(uint32_t k, int lane, float (&s)[kTiles][4]) const
     {
         const int key = (lane >> 4) * 8 + (lane & 7), half = (lane >> 3) & 1;
+        float odd[kTiles][4] = {};
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
         {
             uint32_t b[4];
             const int chunk = 2 * i + half;
-            ldmatrix(k + (chunk >> 3) * (64 * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), b);
-            mma_bf16(s[0], q[i], b[0], b[1]);
-            mma_bf16(s[1], q[i], b[2], b[3]);
+            ldmatrix(k + (chunk >> 3) * (kKeys * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), b);
+            mma_bf16((i & 1 ? odd : s)[0], q[i], b[0], b[1]);
+            mma_bf16((i & 1 ? odd : s)[1], q[i], b[2], b[3]);
         }
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[t][j] += odd[t][j];
     }
-    // o += p v over 16 keys, of which the first `valid` count
-    __device__ __forceinline__ void weigh(uint32_t v, int lane, const float (&s)[2][4], int valid, float (&o)[D / 8][4]) const
+    // o += p v, of the step's keys the first `valid`
+    __device__ __forceinline__ void weigh(uint32_t v, int lane, const float (&s)[kTiles][4], int valid, float (&o)[D / 8][4]) const
     {
         const uint32_t a[4] = {pack2(s[0][0], s[0][1]), pack2(s[0][2], s[0][3]), pack2(s[1][0], s[1][1]), pack2(s[1][2], s[1][3])};
         const int key = ((lane >> 3) & 1) * 8 + (lane & 7), half = lane >> 4;
@@ -448,8 +480,8 @@ template <int D> struct Rows16<__nv_bfloat16, D>
         {
             uint32_t b[4];
             const int chunk = 2 * i + half;
-            ldmatrix_trans(v + (chunk >> 3) * (64 * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), b);
-            if (valid < 16) // what lies past the last key may be anything, NaN too
+            ldmatrix_trans(v + (chunk >> 3) * (kKeys * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), b);
+            if (valid < kKeys) // what lies past the last key may be anything, NaN too
             {
                 b[0] &= keep[0], b[1] &= keep[1], b[2] &= keep[0], b[3] &= keep[1];
             }
@@ -459,289 +491,272 @@ template <int D> struct Rows16<__nv_bfloat16, D>
     }
 };
 
+// FP32 sums: the tensor cores drop low bits at every step of a chain, so chains are kept short and added up
+// with rounding (one chain of 48 products left 3.4e-6 against 1e-6 of the result).
 template <int D> struct Rows16<float, D>
 {
+    static constexpr int kKeys = 8, kTiles = 1;
     float q[D / 8][4];
     __device__ __forceinline__ void load(const AttendArgs &p, const Row &r0, const Row &r1, int lane)
     {
         const float *base = static_cast<const float *>(p.a.q) + (lane & 3);
+        const float *x0 = base + static_cast<size_t>(r0.query) * D, *x1 = base + static_cast<size_t>(r1.query) * D;
 #pragma unroll
         for (int s = 0; s < D / 8; ++s)
         {
-            q[s][0] = r0.keys ? base[r0.offset + 8 * s] : 0.f;
-            q[s][1] = r1.keys ? base[r1.offset + 8 * s] : 0.f;
-            q[s][2] = r0.keys ? base[r0.offset + 8 * s + 4] : 0.f;
-            q[s][3] = r1.keys ? base[r1.offset + 8 * s + 4] : 0.f;
+            q[s][0] = r0.keys ? x0[8 * s] : 0.f;
+            q[s][1] = r1.keys ? x1[8 * s] : 0.f;
+            q[s][2] = r0.keys ? x0[8 * s + 4] : 0.f;
+            q[s][3] = r1.keys ? x1[8 * s + 4] : 0.f;
         }
     }
-    __device__ __forceinline__ void scores(uint32_t k, int lane, float (&s)[2][4]) const
+    __device__ __forceinline__ void scores(uint32_t k, int lane, float (&s)[kTiles][4]) const
     {
-        const int key = (lane >> 4) * 8 + (lane & 7), half = (lane >> 3) & 1;
+        // a load brings the key fragments of two steps of eight dims
+        const int key = lane & 7, quarter = lane >> 3;
+        float chain[4][4] = {}, cross[2][4] = {};
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i)
+        for (int i = 0; i < D / 16; ++i)
         {
-            uint32_t raw[4], high[4], low[4], qh[4], ql[4];
-            const int chunk = 2 * i + half;
-            ldmatrix(k + (chunk >> 3) * (32 * 128) + key * 128 + (((chunk & 7) ^ (key & 7)) << 4), raw);
+            uint32_t raw[4], high[4], low[4];
+            const int chunk = 4 * i + quarter;
+            ldmatrix(k + (chunk >> 3) * (kKeys * 128) + key * 128 + (((chunk & 7) ^ key) << 4), raw);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-            {
-                split_tf32(__uint_as_float(raw[j]), high[j], low[j]);
-                split_tf32(q[i][j], qh[j], ql[j]);
-            }
+            for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(raw[j]), high[j], low[j]);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int h = 0; h < 2; ++h)
             {
-                mma_tf32(s[t], ql, high[2 * t], high[2 * t + 1]);
-                mma_tf32(s[t], qh, low[2 * t], low[2 * t + 1]);
-                mma_tf32(s[t], qh, high[2 * t], high[2 * t + 1]);
+                uint32_t qh[4], ql[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split_tf32_here(q[2 * i + h][j], qh[j], ql[j]);
+                mma_tf32(cross[0], ql, high[2 * h], high[2 * h + 1]);
+                mma_tf32(cross[1], qh, low[2 * h], low[2 * h + 1]);
+                mma_tf32(chain[(2 * i + h) & 3], qh, high[2 * h], high[2 * h + 1]);
             }
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            s[0][j] = ((chain[0][j] + chain[1][j]) + (chain[2][j] + chain[3][j])) + (cross[0][j] + cross[1][j]);
     }
     // The weights' fragment of key columns 2t and 2t + 1 serves as one whose columns are t and t + 4, with
     // the value rows taken in that order.
-    __device__ __forceinline__ void weigh(uint32_t v, int lane, const float (&s)[2][4], int valid, float (&o)[D / 8][4]) const
+    __device__ __forceinline__ void weigh(uint32_t v, int lane, const float (&s)[kTiles][4], int valid, float (&o)[D / 8][4]) const
     {
-        uint32_t ph[2][4], pl[2][4];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-        {
-            split_tf32(s[t][0], ph[t][0], pl[t][0]);
-            split_tf32(s[t][2], ph[t][1], pl[t][1]);
-            split_tf32(s[t][1], ph[t][2], pl[t][2]);
-            split_tf32(s[t][3], ph[t][3], pl[t][3]);
-        }
+        uint32_t ph[4], pl[4];
+        split_tf32(s[0][0], ph[0], pl[0]);
+        split_tf32(s[0][2], ph[1], pl[1]);
+        split_tf32(s[0][1], ph[2], pl[2]);
+        split_tf32(s[0][3], ph[3], pl[3]);
+        const int key = 2 * (lane & 3);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
         {
             const int d = (i & 3) * 8 + (lane >> 2);
-            const uint32_t column = v + (i >> 2) * (32 * 128) + (d & 3) * 4;
+            const uint32_t column = v + (i >> 2) * (kKeys * 128) + (d & 3) * 4;
+            uint32_t high[2], low[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int e = 0; e < 2; ++e)
             {
-                uint32_t high[2], low[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                {
-                    const int key = 8 * t + 2 * (lane & 3) + e;
-                    float x = ld_shared(column + key * 128 + (((d >> 2) ^ (key & 7)) << 4));
-                    if (valid < 16 && key >= valid) x = 0.f;
-                    split_tf32(x, high[e], low[e]);
-                }
-                mma_tf32(o[i], pl[t], high[0], high[1]);
-                mma_tf32(o[i], ph[t], low[0], low[1]);
-                mma_tf32(o[i], ph[t], high[0], high[1]);
+                float x = ld_shared(column + (key + e) * 128 + (((d >> 2) ^ (key + e)) << 4));
+                if (key + e >= valid) x = 0.f;
+                split_tf32(x, high[e], low[e]);
             }
+            float sum[4] = {};
+            mma_tf32(sum, pl, high[0], high[1]);
+            mma_tf32(sum, ph, low[0], low[1]);
+            mma_tf32(sum, ph, high[0], high[1]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] += sum[j];
         }
     }
 };
 
-template <class T, int D>
-__device__ __forceinline__ void stream_produce(const AttendArgs &p, Walk w, const CUtensorMap *map_k, const CUtensorMap *map_v,
-                                               uint32_t ring, uint32_t bars)
+template <class T, int D> struct Ring
 {
     using L = Layout<T, D>;
-    const int lane = threadIdx.x & 31;
-    const int granules = L::kSlotKeys / p.granule, boxes = granules * L::kColumns * 2;
-    // a lane's box of every slot: granule, column block, K or V
-    const int granule = lane % granules, column = (lane / granules) % L::kColumns, value = lane / (granules * L::kColumns);
+    uint32_t slots, bars; // of the CTA
+    __device__ uint32_t slot(int worker, unsigned n) const { return slots + (worker * L::kRing + n % L::kRing) * (2 * L::kSlotHalf); }
+    __device__ uint32_t full(int worker, unsigned n) const { return bars + 8 * (worker * L::kRing + n % L::kRing); }
+    __device__ uint32_t empty(int worker, unsigned n) const { return full(worker, n) + 8 * kWorkers * L::kRing; }
+    static __device__ uint32_t round(unsigned n) { return (n / L::kRing) & 1u; }
+};
+
+// Slots of a part.
+template <class T, int D> __device__ __forceinline__ int slots_of(const Part &part, int unit_shift)
+{
+    constexpr int keys = Layout<T, D>::kSlotKeys;
+    const int end = min(static_cast<long long>(part.keys), static_cast<long long>(part.first_unit + part.units) << unit_shift);
+    return (end - (part.first_unit << unit_shift) + keys - 1) / keys;
+}
+
+// Four producer warps, each feeding two workers with 16 lanes: a lane issues one box of every slot.
+template <class T, int D>
+__device__ __forceinline__ void stream_produce(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const CUtensorMap *map_k,
+                                               const CUtensorMap *map_v, const Ring<T, D> &ring)
+{
+    using L = Layout<T, D>;
+    const int lane = threadIdx.x & 31, sub = lane & 15, worker = (threadIdx.x / 32) * 2 + (lane >> 4), shift = p.list[plan.which].unit_shift;
+    const unsigned half_mask = 0xffffu << (lane & 16);
+    Walk w = walk_of(p, plan, shared, worker);
+    const int granules = L::kSlotKeys / p.granule;
+    const int granule = sub % granules, column = (sub / granules) % L::kColumns, value = sub / (granules * L::kColumns);
+    const bool has_box = value < 2;
     const uint32_t box_bytes = p.granule * 128;
     const uint32_t into = (value ? L::kSlotHalf : 0) + column * (L::kSlotKeys * 128) + granule * box_bytes;
+    const CUtensorMap *map = value ? map_v : map_k;
     unsigned n = 0; // slots so far
+    int left = 0, key = 0, row = 0;
     Part part;
-    while (next_part(p, w, part))
+    bool more = next_part(p, plan.which, w, part);
+    if (more)
     {
-        int key = part.first_unit * kUnit + granule * p.granule;
-        int row = lane < boxes ? pool_row(p, w.which, part, key) : 0;
-        for (int u = 0; u < part.units * L::kUnitSlots; ++u, ++n)
+        left = slots_of<T, D>(part, shift);
+        key = part.first_unit << shift;
+        row = has_box ? pool_row(p, plan.which, part, key + granule * p.granule) : 0;
+    }
+    long long since = clock64();
+    while (__any_sync(0xffffffffu, more))
+    {
+        const bool free = __shfl_sync(0xffffffffu, static_cast<int>(mbar_try_wait(ring.empty(worker, n), ring.round(n) ^ 1u)), lane & 16);
+        if (more && free)
         {
-            const unsigned slot = n % kSlots, round = n / kSlots;
-            const bool wanted = lane < boxes && key < part.keys;
-            const int next = lane < boxes ? pool_row(p, w.which, part, key + L::kSlotKeys) : 0;
-            const unsigned count = __popc(__ballot_sync(0xffffffffu, wanted));
-            const uint32_t full = bars + 8 * slot, empty = bars + 8 * (kSlots + slot);
-            if (!warp_wait(empty, (round & 1u) ^ 1u))
-            {
-                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
-                return;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(full, count * box_bytes);
-            __syncwarp();
-            if (wanted)
-                tma_load_2d(ring + slot * (2 * L::kSlotHalf) + into, value ? map_v : map_k, full,
-                            column * (128 / static_cast<int>(sizeof(T))), row);
+            const int kept = min(granules, (part.keys - key + p.granule - 1) / p.granule); // granules with keys
+            if (sub == 0) mbar_arrive_expect_tx(ring.full(worker, n), kept * L::kColumns * 2 * box_bytes);
+            __syncwarp(half_mask);
+            if (has_box && granule < kept)
+                tma_load_2d(ring.slot(worker, n) + into, map, ring.full(worker, n), column * (128 / static_cast<int>(sizeof(T))), row);
+            ++n;
             key += L::kSlotKeys;
-            row = next;
+            if (--left == 0)
+            {
+                more = next_part(p, plan.which, w, part);
+                if (more)
+                {
+                    left = slots_of<T, D>(part, shift);
+                    key = part.first_unit << shift;
+                }
+            }
+            if (more && has_box) row = pool_row(p, plan.which, part, key + granule * p.granule);
+            since = clock64();
         }
+        else if (more && clock64() - since > kWaitLimitCycles)
+        {
+            if (sub == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+            more = false;
+        }
+        __syncwarp();
+        more = __shfl_sync(0xffffffffu, static_cast<int>(more), lane & 16);
     }
 }
 
 template <class T, int D>
-__device__ __forceinline__ void stream_work(const AttendArgs &p, Walk w, uint32_t ring, uint32_t bars, float *scratch, float2 *stats)
+__device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const Ring<T, D> &ring)
 {
     using L = Layout<T, D>;
-    const List &l = p.list[w.which];
-    const int warp = threadIdx.x / 32 - 4, lane = threadIdx.x & 31;
-    const int tiles = l.row_tiles, tile = warp % tiles, subset = warp / tiles, subsets = 8 / tiles;
-    const int r0 = tile * 16 + (lane >> 2), r1 = r0 + 8;
-    bool ok = true;
-    unsigned n = 0, met = 0; // units so far; meetings
+    using R = Rows16<T, D>;
+    const List &l = p.list[plan.which];
+    const int worker = threadIdx.x / 32 - 4, lane = threadIdx.x & 31, r0 = lane >> 2, r1 = r0 + 8;
+    Walk w = walk_of(p, plan, shared, worker);
+    unsigned n = 0; // slots so far
     Part part;
-    for (long long begin = w.at; next_part(p, w, part); begin = w.at)
+    while (next_part(p, plan.which, w, part))
     {
-        if (warp == 0 && lane == 0 && part.first_unit == 0) write_meta(p, w, part, begin);
-        const int rows = min(l.block, l.rows - part.block * l.block); // of the item
-        const Row first = row_of(p, w.which, part, r0, D), second = row_of(p, w.which, part, r1, D);
-        Rows16<T, D> x;
+        if (lane == 0 && part.first_unit == 0) write_meta(p, plan.which, w, part);
+        const Row first = row_of(p, plan.which, part, r0), second = row_of(p, plan.which, part, r1);
+        R x;
         x.load(p, first, second, lane);
         // below this key every row with a token sees every key
         const int all_see = __reduce_min_sync(0xffffffffu, min(first.keys ? first.keys : INT_MAX, second.keys ? second.keys : INT_MAX));
-        float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        float o[D / 8][4], m0 = -INFINITY, m1 = -INFINITY, c0 = 0.f, c1 = 0.f, l0 = 0.f, l1 = 0.f;
 #pragma unroll
         for (int i = 0; i < D / 8; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-        for (int u = 0; u < part.units; ++u, ++n)
+        const int slots = slots_of<T, D>(part, l.unit_shift);
+        int key0 = part.first_unit << l.unit_shift;
+        for (int u = 0; u < slots; ++u, ++n, key0 += L::kSlotKeys)
         {
-            int held = -1; // the unit's slot that the warp has waited for
-            for (int g = 0; g < tiles; ++g)
+            if (!warp_wait(ring.full(worker, n), ring.round(n)))
             {
-                const int off = (subset * tiles + g) * 16, slot_of_unit = off / L::kSlotKeys;
-                const unsigned index = n * L::kUnitSlots + slot_of_unit, slot = index % kSlots;
-                if (slot_of_unit != held)
-                {
-                    if (held >= 0)
-                    {
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(bars + 8 * (kSlots + (n * L::kUnitSlots + held) % kSlots));
-                    }
-                    held = slot_of_unit;
-                    if (ok) ok = warp_wait(bars + 8 * slot, (index / kSlots) & 1u);
-                }
-                const int key0 = (part.first_unit + u) * kUnit + off, valid = part.keys - key0;
-                if (!ok || valid <= 0) continue;
-                const uint32_t k = ring + slot * (2 * L::kSlotHalf) + (off % L::kSlotKeys) * 128, v = k + L::kSlotHalf;
-                float s[2][4] = {};
-                x.scores(k, lane, s);
-                if (key0 + 16 > all_see)
-                {
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                return;
+            }
+            const uint32_t k = ring.slot(worker, n);
+            float s[R::kTiles][4] = {};
+            x.scores(k, lane, s);
+            if (key0 + L::kSlotKeys > all_see)
+            {
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < R::kTiles; ++t)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (key0 + 8 * t + 2 * (lane & 3) + (j & 1) >= (j < 2 ? first.keys : second.keys)) s[t][j] = -INFINITY;
-                }
-                float t0 = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
-                float t1 = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
+                    for (int j = 0; j < 4; ++j)
+                        if (key0 + 8 * t + 2 * (lane & 3) + (j & 1) >= (j < 2 ? first.keys : second.keys)) s[t][j] = -INFINITY;
+            }
+            float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < R::kTiles; ++t)
+            {
+                t0 = max3(t0, s[t][0], s[t][1]);
+                t1 = max3(t1, s[t][2], s[t][3]);
+            }
+            // the maximum is raised only when a score passes it by 2^8: until then sums and values share the
+            // old one. (Nothing compares above while both are -inf: the difference is NaN.)
+            if (__any_sync(0xffffffffu, (t0 - m0) * p.scale > 8.f || (t1 - m1) * p.scale > 8.f))
+            {
                 t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 1));
                 t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 1));
                 t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, 2));
                 t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, 2));
-                if (__any_sync(0xffffffffu, t0 > m0 || t1 > m1))
-                {
-                    const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
-                    const float f0 = n0 == m0 ? 1.f : exp2_fast((m0 - n0) * p.scale), f1 = n1 == m1 ? 1.f : exp2_fast((m1 - n1) * p.scale);
-                    m0 = n0;
-                    m1 = n1;
-                    l0 *= f0;
-                    l1 *= f1;
+                const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+                const float f0 = n0 == m0 ? 1.f : exp2_fast((m0 - n0) * p.scale), f1 = n1 == m1 ? 1.f : exp2_fast((m1 - n1) * p.scale);
+                m0 = n0;
+                m1 = n1;
+                c0 = m0 == -INFINITY ? 0.f : -m0 * p.scale;
+                c1 = m1 == -INFINITY ? 0.f : -m1 * p.scale;
+                l0 *= f0;
+                l1 *= f1;
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i)
-                    {
-                        o[i][0] *= f0;
-                        o[i][1] *= f0;
-                        o[i][2] *= f1;
-                        o[i][3] *= f1;
-                    }
-                }
-                const float c0 = m0 == -INFINITY ? 0.f : -m0 * p.scale, c1 = m1 == -INFINITY ? 0.f : -m1 * p.scale;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int i = 0; i < D / 8; ++i)
                 {
-                    s[t][0] = exp2_fast(fmaf(s[t][0], p.scale, c0));
-                    s[t][1] = exp2_fast(fmaf(s[t][1], p.scale, c0));
-                    s[t][2] = exp2_fast(fmaf(s[t][2], p.scale, c1));
-                    s[t][3] = exp2_fast(fmaf(s[t][3], p.scale, c1));
-                    l0 += s[t][0] + s[t][1];
-                    l1 += s[t][2] + s[t][3];
+                    o[i][0] *= f0;
+                    o[i][1] *= f0;
+                    o[i][2] *= f1;
+                    o[i][3] *= f1;
                 }
-                x.weigh(v, lane, s, valid, o);
             }
+#pragma unroll
+            for (int t = 0; t < R::kTiles; ++t)
+            {
+                s[t][0] = exp2_fast(fmaf(s[t][0], p.scale, c0));
+                s[t][1] = exp2_fast(fmaf(s[t][1], p.scale, c0));
+                s[t][2] = exp2_fast(fmaf(s[t][2], p.scale, c1));
+                s[t][3] = exp2_fast(fmaf(s[t][3], p.scale, c1));
+                l0 += s[t][0] + s[t][1];
+                l1 += s[t][2] + s[t][3];
+            }
+            x.weigh(k + L::kSlotHalf, lane, s, part.keys - key0, o);
             __syncwarp();
-            if (lane == 0) mbar_arrive(bars + 8 * (kSlots + (n * L::kUnitSlots + held) % kSlots));
+            if (lane == 0) mbar_arrive(ring.empty(worker, n));
         }
         // a lane's sums cover its columns only
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        // the subsets of keys, the upper half into the lower, until one is left
-        for (int half = subsets / 2; half > 0; half /= 2)
+        const int rows = min(l.block, l.rows - part.block * l.block); // of the item
+        const size_t place = static_cast<size_t>(part.place) * l.part_rows;
+        float *dst = l.o + place * D + 2 * (lane & 3);
+        float2 *ml = l.ml + place;
+        if ((lane & 3) == 0)
         {
-            if (subset >= half && subset < 2 * half)
-            {
-                const int place = (subset - half) * tiles + tile;
-                float *dst = scratch + place * (16 * D) + 2 * (lane & 3);
-                if ((lane & 3) == 0)
-                {
-                    stats[place * 16 + (lane >> 2)] = make_float2(m0, l0);
-                    stats[place * 16 + (lane >> 2) + 8] = make_float2(m1, l1);
-                }
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                {
-                    if (r0 < rows) *reinterpret_cast<float2 *>(dst + (lane >> 2) * D + 8 * i) = make_float2(o[i][0], o[i][1]);
-                    if (r1 < rows) *reinterpret_cast<float2 *>(dst + ((lane >> 2) + 8) * D + 8 * i) = make_float2(o[i][2], o[i][3]);
-                }
-            }
-            ok &= meet(bars + 8 * (2 * kSlots), met);
-            if (subset < half)
-            {
-                const int place = subset * tiles + tile;
-                const float *src = scratch + place * (16 * D) + 2 * (lane & 3);
-                const float2 s0 = stats[place * 16 + (lane >> 2)], s1 = stats[place * 16 + (lane >> 2) + 8];
-                const float n0 = fmaxf(m0, s0.x), n1 = fmaxf(m1, s1.x);
-                const float a0 = n0 == m0 ? 1.f : exp2_fast((m0 - n0) * p.scale), b0 = n0 == s0.x ? 1.f : exp2_fast((s0.x - n0) * p.scale);
-                const float a1 = n1 == m1 ? 1.f : exp2_fast((m1 - n1) * p.scale), b1 = n1 == s1.x ? 1.f : exp2_fast((s1.x - n1) * p.scale);
-                m0 = n0;
-                m1 = n1;
-                l0 = l0 * a0 + s0.y * b0;
-                l1 = l1 * a1 + s1.y * b1;
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i)
-                {
-                    if (r0 < rows)
-                    {
-                        const float2 v = *reinterpret_cast<const float2 *>(src + (lane >> 2) * D + 8 * i);
-                        o[i][0] = o[i][0] * a0 + v.x * b0;
-                        o[i][1] = o[i][1] * a0 + v.y * b0;
-                    }
-                    if (r1 < rows)
-                    {
-                        const float2 v = *reinterpret_cast<const float2 *>(src + ((lane >> 2) + 8) * D + 8 * i);
-                        o[i][2] = o[i][2] * a1 + v.x * b1;
-                        o[i][3] = o[i][3] * a1 + v.y * b1;
-                    }
-                }
-            }
-            ok &= meet(bars + 8 * (2 * kSlots), met);
+            if (r0 < rows) ml[r0] = make_float2(m0 * p.scale, l0);
+            if (r1 < rows) ml[r1] = make_float2(m1 * p.scale, l1);
         }
-        if (!ok && lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
-        if (subset == 0)
-        {
-            float *dst = l.o + part.place * l.part_rows * D + 2 * (lane & 3);
-            float2 *ml = l.ml + part.place * l.part_rows;
-            if ((lane & 3) == 0)
-            {
-                if (r0 < rows) ml[r0] = make_float2(m0 * p.scale, l0);
-                if (r1 < rows) ml[r1] = make_float2(m1 * p.scale, l1);
-            }
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-            {
-                if (r0 < rows) *reinterpret_cast<float2 *>(dst + static_cast<size_t>(r0) * D + 8 * i) = make_float2(o[i][0], o[i][1]);
-                if (r1 < rows) *reinterpret_cast<float2 *>(dst + static_cast<size_t>(r1) * D + 8 * i) = make_float2(o[i][2], o[i][3]);
-            }
+        for (int i = 0; i < D / 8; ++i)
+        {
+            if (r0 < rows) *reinterpret_cast<float2 *>(dst + r0 * D + 8 * i) = make_float2(o[i][0], o[i][1]);
+            if (r1 < rows) *reinterpret_cast<float2 *>(dst + r1 * D + 8 * i) = make_float2(o[i][2], o[i][3]);
         }
     }
 }
@@ -777,7 +792,7 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t addr)
 {
     uint64_t desc = 0;
     desc |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
-    desc |= static_cast<uint64_t>((kUnit * 128) >> 4) << 16;
+    desc |= static_cast<uint64_t>((kTile * 128) >> 4) << 16;
     desc |= static_cast<uint64_t>(1024u >> 4) << 32;
     desc |= static_cast<uint64_t>(1u) << 46;
     desc |= static_cast<uint64_t>(2u) << 61;
@@ -786,23 +801,23 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t addr)
 
 // One of K (value 0) and V (value 1) of the CTA's units; a lane per box.
 template <int D>
-__device__ __forceinline__ void tile_produce(const AttendArgs &p, Walk w, const CUtensorMap *map, const TileSmem<D> &sm, int value)
+__device__ __forceinline__ void tile_produce(const AttendArgs &p, int which, Walk w, const CUtensorMap *map, const TileSmem<D> &sm, int value)
 {
     using L = Layout<__nv_bfloat16, D>;
-    const int lane = threadIdx.x & 31, granules = kUnit / p.granule;
+    const int lane = threadIdx.x & 31, granules = kTile / p.granule;
     const int granule = lane % 16, column = lane / 16;
     const bool active = granule < granules && column < L::kColumns;
-    const uint32_t into = column * (kUnit * 128) + granule * p.granule * 128;
+    const uint32_t into = column * (kTile * 128) + granule * p.granule * 128;
     unsigned n = 0;
     Part part;
-    while (next_part(p, w, part))
+    while (next_part(p, which, w, part))
     {
-        int key = part.first_unit * kUnit + granule * p.granule;
-        int row = active ? pool_row(p, w.which, part, key) : 0;
+        int key = part.first_unit * kTile + granule * p.granule;
+        int row = active ? pool_row(p, which, part, key) : 0;
         for (int u = 0; u < part.units; ++u, ++n)
         {
-            key += kUnit;
-            const int next = active ? pool_row(p, w.which, part, key) : 0;
+            key += kTile;
+            const int next = active ? pool_row(p, which, part, key) : 0;
             const uint32_t full = value ? sm.v_full() : sm.k_full(n & 1), empty = value ? sm.v_empty() : sm.k_empty(n & 1);
             const unsigned round = value ? n : n >> 1;
             if (!warp_wait(empty, (round & 1u) ^ 1u))
@@ -818,9 +833,9 @@ __device__ __forceinline__ void tile_produce(const AttendArgs &p, Walk w, const 
     }
 }
 
-template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs &p, Walk w, const TileSmem<D> &sm, uint32_t tmem)
+template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs &p, int which, Walk w, const TileSmem<D> &sm, uint32_t tmem)
 {
-    const List &l = p.list[w.which];
+    const List &l = p.list[which];
     constexpr uint32_t score_desc = idesc_bf16(128, 128);
     constexpr uint32_t value_idesc = idesc_bf16(128, D) | (1u << 16); // second operand with contiguous dims
     unsigned n = 0, seen[2] = {0, 0}, parts[2] = {0, 0}; // units; units and parts of each tile of rows
@@ -829,16 +844,16 @@ template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs 
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
         {
-            const uint64_t ad = smem_desc_sw128(sm.q(g) + (i >> 2) * (kUnit * 128)) + 2u * (i & 3);
-            const uint64_t bd = smem_desc_sw128(sm.k(unit & 1) + (i >> 2) * (kUnit * 128)) + 2u * (i & 3);
+            const uint64_t ad = smem_desc_sw128(sm.q(g) + (i >> 2) * (kTile * 128)) + 2u * (i & 3);
+            const uint64_t bd = smem_desc_sw128(sm.k(unit & 1) + (i >> 2) * (kTile * 128)) + 2u * (i & 3);
             umma_bf16(tmem + g * 128, ad, bd, score_desc, i > 0 ? 1u : 0u);
         }
         umma_commit(sm.s_full(g));
     };
     Part part;
-    while (ok && next_part(p, w, part))
+    while (ok && next_part(p, which, w, part))
     {
-        const int groups = min(l.block, l.rows - part.block * l.block) > kUnit ? 2 : 1;
+        const int groups = min(l.block, l.rows - part.block * l.block) > kTile ? 2 : 1;
         for (int g = 0; g < groups && ok; ++g) ok = mbar_wait(sm.q_full(g), parts[g]++ & 1u);
         if (ok) ok = mbar_wait(sm.k_full(n & 1), (n >> 1) & 1u);
         if (!ok) break;
@@ -865,9 +880,9 @@ template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs 
                 if (!(ok = mbar_wait(sm.p_full(g), seen[g]++ & 1u))) break;
                 tc_fence_after();
 #pragma unroll
-                for (int i = 0; i < kUnit / 16; ++i)
+                for (int i = 0; i < kTile / 16; ++i)
                 {
-                    const uint64_t ad = smem_desc_sw128(sm.p(g) + (i >> 2) * (kUnit * 128)) + 2u * (i & 3);
+                    const uint64_t ad = smem_desc_sw128(sm.p(g) + (i >> 2) * (kTile * 128)) + 2u * (i & 3);
                     umma_bf16(tmem + 256 + g * 128, ad, value_desc(sm.v() + i * 2048), value_idesc, (u > 0 || i > 0) ? 1u : 0u);
                 }
                 umma_commit(sm.pv_done(g));
@@ -879,9 +894,9 @@ template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs 
 }
 
 template <int D>
-__device__ __forceinline__ void tile_softmax(const AttendArgs &p, Walk w, const TileSmem<D> &sm, uint32_t tmem)
+__device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Walk w, const TileSmem<D> &sm, uint32_t tmem)
 {
-    const List &l = p.list[w.which];
+    const List &l = p.list[which];
     const int warp = threadIdx.x / 32 - 4, lane = threadIdx.x & 31, g = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16), s_at = lanes + g * 128, o_at = lanes + 256 + g * 128;
     const float c = p.scale;
@@ -889,28 +904,31 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, Walk w, const 
     bool ok = true;
     unsigned n = 0; // units of the CTA
     Part part;
-    for (long long begin = w.at; next_part(p, w, part); begin = w.at)
+    while (next_part(p, which, w, part))
     {
-        if (warp == 0 && lane == 0 && part.first_unit == 0) write_meta(p, w, part, begin);
+        if (warp == 0 && lane == 0 && part.first_unit == 0) write_meta(p, which, w, part);
         const int rows = min(l.block, l.rows - part.block * l.block);
-        if (g * kUnit >= rows)
+        if (g * kTile >= rows)
         {
             n += part.units;
             continue;
         }
-        const Row row = row_of(p, w.which, part, g * kUnit + r, D);
+        const Row row = row_of(p, which, part, g * kTile + r);
         // the tile of queries: the warp's 32 rows, 16 bytes per lane, D/8 lanes per row
         {
             constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
-#pragma unroll 8
-            for (int i = 0; i < 32; i += kRowsAtOnce)
+            const int chunk = lane % kLanes;
+            const uint4 *q = static_cast<const uint4 *>(p.a.q) + chunk;
+            uint4 x[32 / kRowsAtOnce];
+#pragma unroll
+            for (int i = 0; i < 32 / kRowsAtOnce; ++i)
+                x[i] = q[static_cast<size_t>(__shfl_sync(0xffffffffu, row.query, i * kRowsAtOnce + lane / kLanes)) * kLanes];
+#pragma unroll
+            for (int i = 0; i < 32 / kRowsAtOnce; ++i)
             {
-                const int from = i + lane / kLanes, chunk = lane % kLanes, at = quarter * 32 + from;
-                const long long offset = __shfl_sync(0xffffffffu, row.offset, from);
-                const int keys = __shfl_sync(0xffffffffu, row.keys, from);
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (keys) x = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.a.q) + offset + chunk * 8);
-                st_shared_v4(sm.q(g) + (chunk >> 3) * (kUnit * 128) + at * 128 + (((chunk & 7) ^ (at & 7)) << 4), x.x, x.y, x.z, x.w);
+                const int from = i * kRowsAtOnce + lane / kLanes, at = quarter * 32 + from;
+                if (!__shfl_sync(0xffffffffu, row.keys, from)) x[i] = make_uint4(0, 0, 0, 0);
+                st_shared_v4(sm.q(g) + (chunk >> 3) * (kTile * 128) + at * 128 + (((chunk & 7) ^ (at & 7)) << 4), x[i].x, x[i].y, x[i].z, x[i].w);
             }
         }
         fence_async_smem();
@@ -926,8 +944,8 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, Walk w, const 
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(sm.s_free(g));
-            const int key0 = (part.first_unit + u) * kUnit, visible = row.keys - key0;
-            if (visible < kUnit)
+            const int key0 = (part.first_unit + u) * kTile, visible = row.keys - key0;
+            if (visible < kTile)
             {
 #pragma unroll
                 for (int k = 0; k < 128; ++k)
@@ -977,18 +995,18 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, Walk w, const 
                     packed[t >> 1] = pack2(e0, e1);
                 }
                 const int chunk = (k8 & 63) >> 3;
-                st_shared_v4(sm.p(g) + (k8 >> 6) * (kUnit * 128) + r * 128 + ((chunk ^ (r & 7)) << 4), packed[0], packed[1], packed[2], packed[3]);
+                st_shared_v4(sm.p(g) + (k8 >> 6) * (kTile * 128) + r * 128 + ((chunk ^ (r & 7)) << 4), packed[0], packed[1], packed[2], packed[3]);
             }
             const float2 s4 = __fadd2_rn(__fadd2_rn(part_sum[0], part_sum[1]), __fadd2_rn(part_sum[2], part_sum[3]));
             sum += s4.x + s4.y;
             // values past the item's last key may be anything, NaN too: zeros, by both tiles' threads alike
-            if (key0 + kUnit > part.keys)
+            if (key0 + kTile > part.keys)
             {
                 if (!(ok = warp_wait(sm.v_full(), (n + u) & 1u))) break;
                 if (key0 + r >= part.keys)
                 {
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) st_shared_v4(sm.v() + (i >> 3) * (kUnit * 128) + r * 128 + (i & 7) * 16, 0, 0, 0, 0);
+                    for (int i = 0; i < D / 8; ++i) st_shared_v4(sm.v() + (i >> 3) * (kTile * 128) + r * 128 + (i & 7) * 16, 0, 0, 0, 0);
                 }
             }
             fence_async_smem();
@@ -1004,19 +1022,35 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, Walk w, const 
             break;
         }
         tc_fence_after();
-        const int at = g * kUnit + r;
-        if (at < rows) l.ml[part.place * l.part_rows + at] = make_float2(m * c, sum);
-        float *dst = l.o + (part.place * l.part_rows + at) * D;
+        const int at = g * kTile + r;
+        const size_t place = static_cast<size_t>(part.place) * l.part_rows;
+        if (at < rows) l.ml[place + at] = make_float2(m * c, sum);
+        // a warp's 32 rows through its quarter of the P tile, 64 columns at a time, so that a store is whole
+        // rows: 16-byte chunk j of row i sits at chunk j ^ (i & 15)
+        const uint32_t stage = sm.p(g) + quarter * 8192;
+        float *dst = l.o + (place + g * kTile + quarter * 32) * D;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
+        for (int h = 0; h < D / 64; ++h)
         {
-            float o[32];
-            tmem_load_32(o_at + i * 32, o);
-            if (at < rows)
-            {
 #pragma unroll
-                for (int t = 0; t < 32; t += 4) *reinterpret_cast<float4 *>(dst + i * 32 + t) = make_float4(o[t], o[t + 1], o[t + 2], o[t + 3]);
+            for (int i = 0; i < 2; ++i)
+            {
+                float o[32];
+                tmem_load_32(o_at + h * 64 + i * 32, o);
+#pragma unroll
+                for (int t = 0; t < 8; ++t)
+                    st_shared_v4(stage + lane * 256 + (((i * 8 + t) ^ (lane & 15)) << 4), __float_as_uint(o[4 * t]), __float_as_uint(o[4 * t + 1]),
+                                 __float_as_uint(o[4 * t + 2]), __float_as_uint(o[4 * t + 3]));
             }
+            __syncwarp();
+#pragma unroll 8
+            for (int i = 0; i < 32; i += 2)
+            {
+                const int from = i + (lane >> 4);
+                const float4 v = ld_shared_v4(stage + from * 256 + (((lane & 15) ^ (from & 15)) << 4));
+                if (g * kTile + quarter * 32 + from < rows) *reinterpret_cast<float4 *>(dst + from * D + h * 64 + (lane & 15) * 4) = v;
+            }
+            __syncwarp();
         }
         tc_fence_before();
     }
@@ -1035,8 +1069,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *base_ptr = smem_raw + (base - raw);
     const uint32_t bars = base + L::kBody;
-    PlanShared &plan = *reinterpret_cast<PlanShared *>(base_ptr + L::kBody + 256);
-    float2 *stats = reinterpret_cast<float2 *>(base_ptr + L::kBody + 1024); // 4 x 16 of them
+    PlanShared &shared = *reinterpret_cast<PlanShared *>(base_ptr + L::kBody + 1024);
+    static_assert(2 * kWorkers * L::kRing * 8 <= 1024 && sizeof(PlanShared) <= 1024, "barriers and plan");
     const int warp = threadIdx.x / 32;
     if (threadIdx.x == 0)
     {
@@ -1045,13 +1079,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     grid_dependency_wait(); // the lengths, tables, queries and the cache are written from here on
     grid_dependents_launch();
-    Walk w;
-    if (!make_plan(p, plan, w)) return;
-    const List &l = p.list[w.which];
-    TileSmem<D> sm{base, bars};
+    const Plan plan = make_plan(p, shared);
+    if (plan.which < 0) return;
+    const bool tile = p.list[plan.which].tile != 0;
+    const TileSmem<D> sm{base, bars};
+    const Ring<T, D> ring{base, bars};
     if (threadIdx.x == 0)
     {
-        if (l.tile)
+        if (tile)
         {
             for (int g = 0; g < 2; ++g)
             {
@@ -1068,19 +1103,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(sm.done(), 8);
         }
         else
-        {
-            // the warps that read a slot: those of its keys' subsets, or all of them
-            const int readers = max(8 * L::kSlotKeys / kUnit, l.row_tiles);
-            for (int i = 0; i < kSlots; ++i)
-            {
-                mbar_init(bars + 8 * i, 1);
-                mbar_init(bars + 8 * (kSlots + i), readers);
-            }
-            mbar_init(bars + 8 * (2 * kSlots), 8);
-        }
+            for (int i = 0; i < 2 * kWorkers * L::kRing; ++i) mbar_init(bars + 8 * i, 1);
         fence_barrier_init();
     }
-    if (l.tile && warp == 1)
+    if (tile && warp == 1)
     {
         tmem_alloc(sm.tmem_slot(), 512);
         tmem_relinquish();
@@ -1088,20 +1114,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    uint32_t tmem = 0;
-    if (l.tile) tmem = *reinterpret_cast<volatile uint32_t *>(base_ptr + (sm.tmem_slot() - base));
     if (warp < 4)
     {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsControl));
         if constexpr (sizeof(T) == 2)
         {
-            if (l.tile)
+            if (tile)
             {
-                if (warp == 0) tile_produce<D>(p, w, &map_k, sm, 0);
-                else if (warp == 2) tile_produce<D>(p, w, &map_v, sm, 1);
+                const Walk w = walk_of(p, plan, shared, 0);
+                if (warp == 0) tile_produce<D>(p, plan.which, w, &map_k, sm, 0);
+                else if (warp == 2) tile_produce<D>(p, plan.which, w, &map_v, sm, 1);
                 else if (warp == 1)
                 {
-                    if ((threadIdx.x & 31) == 0) tile_multiply<D>(p, w, sm, tmem);
+                    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base_ptr + (sm.tmem_slot() - base));
+                    if ((threadIdx.x & 31) == 0) tile_multiply<D>(p, plan.which, w, sm, tmem);
                     __syncwarp();
                     if (!warp_wait(sm.done(), 0) && (threadIdx.x & 31) == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
                     tc_fence_after();
@@ -1110,20 +1136,21 @@ __global__ void __launch_bounds__(kThreads, 1)
                 return;
             }
         }
-        if (warp == 0) stream_produce<T, D>(p, w, &map_k, &map_v, base, bars);
+        stream_produce<T, D>(p, plan, shared, &map_k, &map_v, ring);
     }
     else
     {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsWork));
         if constexpr (sizeof(T) == 2)
         {
-            if (l.tile)
+            if (tile)
             {
-                tile_softmax<D>(p, w, sm, tmem);
+                const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base_ptr + (sm.tmem_slot() - base));
+                tile_softmax<D>(p, plan.which, walk_of(p, plan, shared, 0), sm, tmem);
                 return;
             }
         }
-        stream_work<T, D>(p, w, base, bars, reinterpret_cast<float *>(base_ptr + L::kScratch), stats);
+        stream_work<T, D>(p, plan, shared, ring);
     }
 }
 
@@ -1137,29 +1164,36 @@ template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) joi
     const unsigned full = 0xffffffffu;
     const int lane = threadIdx.x & 31;
     const PagedBatch &b = p.a.batch;
-    const long long at = static_cast<long long>(blockIdx.x) * kJoinWarps + threadIdx.x / 32;
-    grid_dependency_wait();
-    grid_dependents_launch();
-    const long long slots = static_cast<long long>(b.sequences) * b.queries;
-    if (at >= slots * p.a.heads) return;
-    const int slot = static_cast<int>(at / p.a.heads), head = static_cast<int>(at % p.a.heads);
-    const int s = slot / b.queries, i = slot % b.queries, kv_head = head / p.share;
+    const int at = blockIdx.x * kJoinWarps + threadIdx.x / 32; // row of q and out
+    // The lengths are older than the kernel before this one, which waited for them before it let this one start.
+    bool row = at < b.sequences * b.queries * p.a.heads;
+    const int slot = row ? at / p.a.heads : 0, head = at - slot * p.a.heads, s = slot / b.queries, i = slot - s * b.queries;
     const SequenceView view = sequence_view(b, p.a.kv.page_shift, s);
-    if (i >= view.count) return;
-    int parts[2] = {0, 0};
-    long long first[2] = {0, 0}; // row of the first part's statistics
-    const int per = b.sequences / b.groups, group = s / per;
+    row = row && i < view.count;
+    int item[2] = {-1, -1}, within[2] = {0, 0};
 #pragma unroll
     for (int which = 0; which < 2; ++which)
     {
         const List &l = p.list[which];
         if (which == 0 ? view.prefix_len == 0 : view.len - view.count + i + 1 <= 0) continue;
-        const int owner = which == 0 ? group : s;
-        const int r = (which == 0 ? slot - group * per * b.queries : i) * p.share + head % p.share;
-        const long long item = (static_cast<long long>(owner) * l.blocks + r / l.block) * p.a.kv.kv_heads + kv_head;
-        const int2 meta = l.meta[item];
+        const int per = p.list[0].owners ? p.list[0].rows / p.share : 1; // slots of a group
+        const int owner = which == 0 ? slot / per : s;
+        const int r = (which == 0 ? slot - owner * per : i) * p.share + head % p.share, block = r / l.block;
+        item[which] = (owner * l.blocks + block) * p.a.kv.kv_heads + head / p.share;
+        within[which] = r - block * l.block;
+    }
+    grid_dependency_wait();
+    grid_dependents_launch();
+    if (!row) return;
+    int parts[2] = {0, 0};
+    size_t first[2] = {0, 0}; // row of the first part's statistics
+#pragma unroll
+    for (int which = 0; which < 2; ++which)
+    {
+        if (item[which] < 0) continue;
+        const int2 meta = p.list[which].meta[item[which]];
         parts[which] = meta.y;
-        first[which] = (item + meta.x) * l.part_rows + r % l.block;
+        first[which] = static_cast<size_t>(item[which] + meta.x) * p.list[which].part_rows + within[which];
     }
     const int total = parts[0] + parts[1];
     float top = -INFINITY, sum = 0.f, o[N] = {};
@@ -1167,8 +1201,8 @@ template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) joi
     {
         const int j = base + lane;
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (j < parts[0]) ml = p.list[0].ml[first[0] + static_cast<long long>(j) * p.list[0].part_rows];
-        else if (j < total) ml = p.list[1].ml[first[1] + static_cast<long long>(j - parts[0]) * p.list[1].part_rows];
+        if (j < parts[0]) ml = p.list[0].ml[first[0] + static_cast<size_t>(j) * p.list[0].part_rows];
+        else if (j < total) ml = p.list[1].ml[first[1] + static_cast<size_t>(j - parts[0]) * p.list[1].part_rows];
         float most = ml.x;
 #pragma unroll
         for (int step = 16; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor_sync(full, most, step));
@@ -1188,8 +1222,8 @@ template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) joi
         {
             const float f = __shfl_sync(full, weight, k);
             const int jj = base + k;
-            const float *src = jj < parts[0] ? p.list[0].o + (first[0] + static_cast<long long>(jj) * p.list[0].part_rows) * D
-                                             : p.list[1].o + (first[1] + static_cast<long long>(jj - parts[0]) * p.list[1].part_rows) * D;
+            const float *src = jj < parts[0] ? p.list[0].o + (first[0] + static_cast<size_t>(jj) * p.list[0].part_rows) * D
+                                             : p.list[1].o + (first[1] + static_cast<size_t>(jj - parts[0]) * p.list[1].part_rows) * D;
             float x[N];
             if constexpr (N == 4)
             {
@@ -1206,7 +1240,7 @@ template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) joi
         }
     }
     const float inverse = sum > 0.f ? 1.f / sum : 0.f;
-    T *dst = static_cast<T *>(p.a.out) + at * D + lane * N;
+    T *dst = static_cast<T *>(p.a.out) + static_cast<size_t>(at) * D + lane * N;
     if constexpr (sizeof(T) == 4)
     {
         if constexpr (N == 4) *reinterpret_cast<float4 *>(dst) = make_float4(o[0] * inverse, o[1] * inverse, o[2] * inverse, o[3] * inverse);
@@ -1236,13 +1270,15 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
         l.owners = i == 0 ? (b.max_prefix_pages ? b.groups : 0) : b.sequences;
         l.rows = (i == 0 ? b.sequences / b.groups : 1) * b.queries * p.share;
         l.tile = kv.bf16 && l.rows > kTileRows;
-        l.row_tiles = 1;
-        while (l.row_tiles < 8 && 16 * l.row_tiles < l.rows) l.row_tiles *= 2;
-        l.block = l.tile ? 2 * kUnit : 16 * l.row_tiles;
+        l.block = l.tile ? 2 * kTile : 16;
         l.blocks = (l.rows + l.block - 1) / l.block;
         l.part_rows = l.rows < l.block ? l.rows : l.block;
-        l.cost = l.tile ? (l.rows > kUnit ? 14 : 9) : kv.bf16 ? 12 : (l.row_tiles < 4 ? 24 : 14 * l.row_tiles);
-        const size_t items = static_cast<size_t>(l.owners) * l.blocks * kv.kv_heads, parts = l.owners ? items + ctas : 0;
+        l.unit_shift = l.tile ? 7 : 5;
+        // nanoseconds of an SM: a tile's step with one and with two tiles of rows; a streamed unit at its share
+        // of the memory's rate (BF16) or at the rate of the split products (FP32)
+        l.cost = l.tile ? (l.rows > kTile ? 1600 : 900) : kv.bf16 ? 370 * kv.dim / 128 : 800 * kv.dim / 128;
+        const size_t items = static_cast<size_t>(l.owners) * l.blocks * kv.kv_heads;
+        const size_t parts = l.owners ? items + ctas * (l.tile ? 1 : kWorkers) : 0;
         l.o = reinterpret_cast<float *>(base + at);
         at += rounded(parts * l.part_rows * kv.dim * sizeof(float));
         l.ml = reinterpret_cast<float2 *>(base + at);
@@ -1251,6 +1287,19 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
         at += rounded(items * sizeof(int2));
     }
     return at;
+}
+
+// The plan counts units in 32 bits.
+bool countable(const PagedLayer &kv, const AttendArgs &p, const PagedBatch &b)
+{
+    double units = 0;
+    for (int i = 0; i < 2; ++i)
+    {
+        const List &l = p.list[i];
+        const double keys = static_cast<double>(i == 0 ? b.max_prefix_pages : b.max_pages) * (1 << kv.page_shift);
+        units += (keys / (1 << l.unit_shift) + 1) * l.owners * l.blocks * kv.kv_heads;
+    }
+    return units < 1e9;
 }
 
 bool map_pool(CUtensorMap *map, const void *pool, const PagedLayer &kv, int granule)
@@ -1272,9 +1321,10 @@ template <class T, int D> int launch(const PrefixAttentionArgs &a, int sms, cuda
     AttendArgs p;
     p.a = a;
     lay_out(a.kv, a.batch, a.heads, sms, a.workspace, p);
+    if (!countable(a.kv, p, a.batch)) return cudaErrorInvalidValue;
     p.scale = 1.4426950408889634f / sqrtf(static_cast<float>(D));
     p.granule = 1 << a.kv.page_shift;
-    if (p.granule > Kind<T>::kSlotKeys) p.granule = Kind<T>::kSlotKeys;
+    if (p.granule > Layout<T, D>::kSlotKeys) p.granule = Layout<T, D>::kSlotKeys;
     CUtensorMap map_k, map_v;
     if (!map_pool(&map_k, a.kv.k, a.kv, p.granule) || !map_pool(&map_v, a.kv.v, a.kv, p.granule)) return cudaErrorInvalidValue;
     cudaLaunchAttribute attr;
