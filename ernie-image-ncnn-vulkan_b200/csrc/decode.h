@@ -45,11 +45,13 @@ struct OwnView
     int count; // of them new
 };
 
+// All loads come before the first check, so that they wait for one another once.
 __device__ __forceinline__ OwnView own_view(const PagedBatch &b, int page_shift, int s)
 {
     OwnView v;
-    v.len = clamped_length(b.lens[s], b.max_pages, page_shift, b.error_flag);
+    v.len = b.lens[s];
     v.count = b.counts ? b.counts[s] : b.queries;
+    v.len = clamped_length(v.len, b.max_pages, page_shift, b.error_flag);
     if (v.count < 0 || v.count > b.queries)
     {
         report_range(b.error_flag);
@@ -66,10 +68,9 @@ struct SequenceView : OwnView
 __device__ __forceinline__ SequenceView sequence_view(const PagedBatch &b, int page_shift, int s)
 {
     SequenceView v;
+    v.prefix_len = b.max_prefix_pages ? b.prefix_lens[s / (b.sequences / b.groups)] : 0;
     static_cast<OwnView &>(v) = own_view(b, page_shift, s);
-    v.prefix_len = 0;
-    if (b.max_prefix_pages)
-        v.prefix_len = clamped_length(b.prefix_lens[s / (b.sequences / b.groups)], b.max_prefix_pages, page_shift, b.error_flag);
+    if (b.max_prefix_pages) v.prefix_len = clamped_length(v.prefix_len, b.max_prefix_pages, page_shift, b.error_flag);
     return v;
 }
 #endif

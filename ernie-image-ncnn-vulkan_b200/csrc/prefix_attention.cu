@@ -404,22 +404,20 @@ __device__ __forceinline__ Row row_of(const AttendArgs &p, int which, const Part
 }
 
 // First row of the pool that holds key `key` of the part's item, or the row past the end (TMA reads zeros
-// there) for a key past the item's or a bad page.
-__device__ __forceinline__ int pool_row(const AttendArgs &p, int which, const Part &part, int key)
+// there) for a key past the item's or a bad page, which `bad` remembers: nothing here waits for the table.
+__device__ __forceinline__ int pool_row(const AttendArgs &p, int which, const Part &part, int key, bool &bad)
 {
     const PagedLayer &kv = p.a.kv;
     const int outside = (kv.pages * kv.kv_heads) << kv.page_shift;
     if (key >= part.keys) return outside;
     const PagedBatch &b = p.a.batch;
-    const int *table = which == 0 ? b.prefix_tables + static_cast<long long>(part.owner) * b.max_prefix_pages
-                                  : b.tables + static_cast<long long>(part.owner) * b.max_pages;
+    const int *table = which == 0 ? b.prefix_tables + static_cast<size_t>(part.owner) * b.max_prefix_pages
+                                  : b.tables + static_cast<size_t>(part.owner) * b.max_pages;
     const int page = table[key >> kv.page_shift];
-    if (page < 0 || page >= kv.pages)
-    {
-        report_range(b.error_flag);
-        return outside;
-    }
-    return ((page * kv.kv_heads + part.head) << kv.page_shift) + (key & ((1 << kv.page_shift) - 1));
+    const bool good = static_cast<unsigned>(page) < static_cast<unsigned>(kv.pages);
+    bad |= !good;
+    const int row = ((page * kv.kv_heads + part.head) << kv.page_shift) + (key & ((1 << kv.page_shift) - 1));
+    return good ? row : outside;
 }
 
 // ---------------------------------------------------------------- stream
@@ -606,13 +604,14 @@ __device__ __forceinline__ void stream_produce(const AttendArgs &p, const Plan &
     const CUtensorMap *map = value ? map_v : map_k;
     unsigned n = 0; // slots so far
     int left = 0, key = 0, row = 0;
+    bool bad = false;
     Part part;
     bool more = next_part(p, plan.which, w, part);
     if (more)
     {
         left = slots_of<T, D>(part, shift);
         key = part.first_unit << shift;
-        row = has_box ? pool_row(p, plan.which, part, key + granule * p.granule) : 0;
+        row = has_box ? pool_row(p, plan.which, part, key + granule * p.granule, bad) : 0;
     }
     long long since = clock64();
     while (__any_sync(0xffffffffu, more))
@@ -636,7 +635,7 @@ __device__ __forceinline__ void stream_produce(const AttendArgs &p, const Plan &
                     key = part.first_unit << shift;
                 }
             }
-            if (more && has_box) row = pool_row(p, plan.which, part, key + granule * p.granule);
+            if (more && has_box) row = pool_row(p, plan.which, part, key + granule * p.granule, bad);
             since = clock64();
         }
         else if (more && clock64() - since > kWaitLimitCycles)
@@ -647,6 +646,7 @@ __device__ __forceinline__ void stream_produce(const AttendArgs &p, const Plan &
         __syncwarp();
         more = __shfl_sync(0xffffffffu, static_cast<int>(more), lane & 16);
     }
+    if (bad) report_range(p.a.batch.error_flag);
 }
 
 template <class T, int D>
@@ -762,28 +762,32 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
 }
 
 // ---------------------------------------------------------------- tile (BF16)
-// Shared memory: Q_A, Q_B, P_A, P_B, K (two buffers), V. TMEM: S_A 0, S_B 128, O_A 256, O_B 384.
-// As in the block attention, softmax copies S_g to registers and frees it, so that S_g of the next tile is
-// computed meanwhile, and rescales O_g only when a row's maximum has grown by more than 2^8.
+// Shared memory: Q_A, Q_B, three tiles that K and V pass through, P_A, P_B. TMEM: S_A 0, S_B 128, O_A 256,
+// O_B 384. As in the block attention, softmax copies S_g to registers and frees it, so that S_g of the next
+// unit is computed meanwhile, and rescales O_g only when a row's maximum has grown by more than 2^8.
+// K and V tiles are loaded in the order K0 K1 V0 K2 V1 K3 V2 ..., in which they are also used: load i goes to
+// tile i % 3 once load i - 3 has been used, which is a whole unit ahead of its own use for K and V alike
+// (with two buffers for K and one for V, V came 0.6 us late in every unit).
 template <int D> struct TileSmem
 {
     using L = Layout<__nv_bfloat16, D>;
     uint32_t base, bars;
     __device__ uint32_t q(int g) const { return base + g * L::kTileBytes; }
-    __device__ uint32_t k(int s) const { return base + (2 + s) * L::kTileBytes; }
-    __device__ uint32_t v() const { return base + 4 * L::kTileBytes; }
+    __device__ uint32_t kv(unsigned load) const { return base + (2 + load % 3) * L::kTileBytes; }
     __device__ uint32_t p(int g) const { return base + 5 * L::kTileBytes + g * L::kWeightBytes; }
-    __device__ uint32_t q_full(int g) const { return bars + 8u * g; }
-    __device__ uint32_t k_full(int s) const { return bars + 8u * (2 + s); }
-    __device__ uint32_t k_empty(int s) const { return bars + 8u * (4 + s); }
-    __device__ uint32_t v_full() const { return bars + 8u * 6; }
-    __device__ uint32_t v_empty() const { return bars + 8u * 7; }
+    __device__ uint32_t full(unsigned load) const { return bars + 8u * (load % 3); }
+    __device__ uint32_t empty(unsigned load) const { return bars + 8u * (3 + load % 3); }
+    static __device__ uint32_t round(unsigned load) { return (load / 3) & 1u; }
+    static __device__ unsigned k_load(unsigned unit) { return unit ? 2 * unit - 1 : 0; }
+    static __device__ unsigned v_load(unsigned unit) { return 2 * unit + 2; }
+    __device__ uint32_t q_full(int g) const { return bars + 8u * (6 + g); }
     __device__ uint32_t s_full(int g) const { return bars + 8u * (8 + g); }
     __device__ uint32_t s_free(int g) const { return bars + 8u * (10 + g); }
     __device__ uint32_t p_full(int g) const { return bars + 8u * (12 + g); }
     __device__ uint32_t pv_done(int g) const { return bars + 8u * (14 + g); }
     __device__ uint32_t done() const { return bars + 8u * 16; }
     __device__ uint32_t tmem_slot() const { return bars + 8u * 17; }
+    static constexpr int kBarriers = 17;
 };
 
 // Descriptor of V [key][dim] as the second operand (dims x keys, dims contiguous): 128-byte rows of 64 dims,
@@ -799,38 +803,54 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t addr)
     return desc;
 }
 
-// One of K (value 0) and V (value 1) of the CTA's units; a lane per box.
+// The K and V tiles of the CTA's units; a lane per box.
 template <int D>
-__device__ __forceinline__ void tile_produce(const AttendArgs &p, int which, Walk w, const CUtensorMap *map, const TileSmem<D> &sm, int value)
+__device__ __forceinline__ void tile_produce(const AttendArgs &p, int which, Walk w, const CUtensorMap *map_k, const CUtensorMap *map_v,
+                                             const TileSmem<D> &sm)
 {
     using L = Layout<__nv_bfloat16, D>;
-    const int lane = threadIdx.x & 31, granules = kTile / p.granule;
-    const int granule = lane % 16, column = lane / 16;
+    const int lane = threadIdx.x & 31, granules = kTile / p.granule, granule = lane % 16, column = lane / 16;
     const bool active = granule < granules && column < L::kColumns;
     const uint32_t into = column * (kTile * 128) + granule * p.granule * 128;
-    unsigned n = 0;
     Part part;
-    while (next_part(p, which, w, part))
-    {
-        int key = part.first_unit * kTile + granule * p.granule;
-        int row = active ? pool_row(p, which, part, key) : 0;
-        for (int u = 0; u < part.units; ++u, ++n)
+    int u = 0, key = 0;
+    bool bad = false, ok = true;
+    part.units = 0;
+    // the pool's row of the lane's box of the next unit
+    auto fetch = [&](int &row) {
+        if (u == part.units)
         {
-            key += kTile;
-            const int next = active ? pool_row(p, which, part, key) : 0;
-            const uint32_t full = value ? sm.v_full() : sm.k_full(n & 1), empty = value ? sm.v_empty() : sm.k_empty(n & 1);
-            const unsigned round = value ? n : n >> 1;
-            if (!warp_wait(empty, (round & 1u) ^ 1u))
-            {
-                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
-                return;
-            }
-            if (lane == 0) mbar_arrive_expect_tx(full, L::kTileBytes);
-            __syncwarp();
-            if (active) tma_load_2d((value ? sm.v() : sm.k(n & 1)) + into, map, full, column * 64, row);
-            row = next;
+            if (!next_part(p, which, w, part)) return false;
+            u = 0;
+            key = part.first_unit * kTile + granule * p.granule;
         }
+        row = active ? pool_row(p, which, part, key, bad) : 0;
+        key += kTile;
+        ++u;
+        return true;
+    };
+    auto load = [&](unsigned i, const CUtensorMap *map, int row) {
+        if (ok) ok = warp_wait(sm.empty(i), TileSmem<D>::round(i) ^ 1u);
+        if (!ok) return;
+        if (lane == 0) mbar_arrive_expect_tx(sm.full(i), L::kTileBytes);
+        __syncwarp();
+        if (active) tma_load_2d(sm.kv(i) + into, map, sm.full(i), column * 64, row);
+    };
+    int row = 0, next = 0, after = 0; // of units n, n + 1 and n + 2
+    bool have = fetch(row), have_next = have && fetch(next);
+    if (have) load(0, map_k, row);
+    for (unsigned n = 0; have && ok; ++n)
+    {
+        const bool have_after = have_next && fetch(after);
+        if (have_next) load(sm.k_load(n + 1), map_k, next);
+        load(sm.v_load(n), map_v, row);
+        row = next;
+        next = after;
+        have = have_next;
+        have_next = have_after;
     }
+    if (bad) report_range(p.a.batch.error_flag);
+    if (!ok && lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
 }
 
 template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs &p, int which, Walk w, const TileSmem<D> &sm, uint32_t tmem)
@@ -845,7 +865,7 @@ template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs 
         for (int i = 0; i < D / 16; ++i)
         {
             const uint64_t ad = smem_desc_sw128(sm.q(g) + (i >> 2) * (kTile * 128)) + 2u * (i & 3);
-            const uint64_t bd = smem_desc_sw128(sm.k(unit & 1) + (i >> 2) * (kTile * 128)) + 2u * (i & 3);
+            const uint64_t bd = smem_desc_sw128(sm.kv(sm.k_load(unit)) + (i >> 2) * (kTile * 128)) + 2u * (i & 3);
             umma_bf16(tmem + g * 128, ad, bd, score_desc, i > 0 ? 1u : 0u);
         }
         umma_commit(sm.s_full(g));
@@ -855,16 +875,16 @@ template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs 
     {
         const int groups = min(l.block, l.rows - part.block * l.block) > kTile ? 2 : 1;
         for (int g = 0; g < groups && ok; ++g) ok = mbar_wait(sm.q_full(g), parts[g]++ & 1u);
-        if (ok) ok = mbar_wait(sm.k_full(n & 1), (n >> 1) & 1u);
+        if (ok) ok = mbar_wait(sm.full(sm.k_load(n)), sm.round(sm.k_load(n)));
         if (!ok) break;
         tc_fence_after();
         for (int g = 0; g < groups; ++g) issue_s(g, n);
-        umma_commit(sm.k_empty(n & 1));
+        umma_commit(sm.empty(sm.k_load(n)));
         for (int u = 0; u < part.units && ok; ++u, ++n)
         {
             if (u + 1 < part.units)
             {
-                if (!(ok = mbar_wait(sm.k_full((n + 1) & 1), ((n + 1) >> 1) & 1u))) break;
+                if (!(ok = mbar_wait(sm.full(sm.k_load(n + 1)), sm.round(sm.k_load(n + 1))))) break;
                 for (int g = 0; g < groups; ++g)
                 {
                     if (!(ok = mbar_wait(sm.s_free(g), seen[g] & 1u))) break;
@@ -872,9 +892,9 @@ template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs 
                     issue_s(g, n + 1);
                 }
                 if (!ok) break;
-                umma_commit(sm.k_empty((n + 1) & 1));
+                umma_commit(sm.empty(sm.k_load(n + 1)));
             }
-            if (!(ok = mbar_wait(sm.v_full(), n & 1u))) break;
+            if (!(ok = mbar_wait(sm.full(sm.v_load(n)), sm.round(sm.v_load(n))))) break;
             for (int g = 0; g < groups; ++g)
             {
                 if (!(ok = mbar_wait(sm.p_full(g), seen[g]++ & 1u))) break;
@@ -883,11 +903,11 @@ template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs 
                 for (int i = 0; i < kTile / 16; ++i)
                 {
                     const uint64_t ad = smem_desc_sw128(sm.p(g) + (i >> 2) * (kTile * 128)) + 2u * (i & 3);
-                    umma_bf16(tmem + 256 + g * 128, ad, value_desc(sm.v() + i * 2048), value_idesc, (u > 0 || i > 0) ? 1u : 0u);
+                    umma_bf16(tmem + 256 + g * 128, ad, value_desc(sm.kv(sm.v_load(n)) + i * 2048), value_idesc, (u > 0 || i > 0) ? 1u : 0u);
                 }
                 umma_commit(sm.pv_done(g));
             }
-            if (ok) umma_commit(sm.v_empty());
+            if (ok) umma_commit(sm.empty(sm.v_load(n)));
         }
     }
     if (!ok) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
@@ -1002,11 +1022,12 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Wal
             // values past the item's last key may be anything, NaN too: zeros, by both tiles' threads alike
             if (key0 + kTile > part.keys)
             {
-                if (!(ok = warp_wait(sm.v_full(), (n + u) & 1u))) break;
+                const unsigned load = sm.v_load(n + u);
+                if (!(ok = warp_wait(sm.full(load), sm.round(load)))) break;
                 if (key0 + r >= part.keys)
                 {
 #pragma unroll
-                    for (int i = 0; i < D / 8; ++i) st_shared_v4(sm.v() + (i >> 3) * (kTile * 128) + r * 128 + (i & 7) * 16, 0, 0, 0, 0);
+                    for (int i = 0; i < D / 8; ++i) st_shared_v4(sm.kv(load) + (i >> 3) * (kTile * 128) + r * 128 + (i & 7) * 16, 0, 0, 0, 0);
                 }
             }
             fence_async_smem();
@@ -1069,43 +1090,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *base_ptr = smem_raw + (base - raw);
     const uint32_t bars = base + L::kBody;
-    PlanShared &shared = *reinterpret_cast<PlanShared *>(base_ptr + L::kBody + 1024);
-    static_assert(2 * kWorkers * L::kRing * 8 <= 1024 && sizeof(PlanShared) <= 1024, "barriers and plan");
+    PlanShared &shared = *reinterpret_cast<PlanShared *>(base_ptr + L::kBody + 1152);
+    static_assert(sizeof(PlanShared) <= 2048 - 1152, "plan");
     const int warp = threadIdx.x / 32;
-    if (threadIdx.x == 0)
+    const TileSmem<D> sm{base, bars + 2 * kWorkers * L::kRing * 8};
+    const Ring<T, D> ring{base, bars};
+    static_assert(2 * kWorkers * L::kRing + TileSmem<D>::kBarriers <= kThreads, "a thread per barrier");
+    static_assert(2 * kWorkers * L::kRing * 8 + TileSmem<D>::kBarriers * 8 + 8 <= 1152, "barriers");
     {
-        prefetch_tensormap(&map_k);
-        prefetch_tensormap(&map_v);
+        // both ways' barriers: the softmax warps of a tile of rows arrive on three kinds, all of them on the last
+        const int t = threadIdx.x - 2 * kWorkers * L::kRing;
+        if (t < 0) mbar_init(bars + 8 * threadIdx.x, 1);
+        else if (t < TileSmem<D>::kBarriers)
+            mbar_init(sm.bars + 8 * t, t == 16 ? 8 : (t >= 6 && t < 8) || (t >= 10 && t < 14) ? 4 : 1);
+        fence_barrier_init();
+        if (threadIdx.x == kThreads - 1)
+        {
+            prefetch_tensormap(&map_k);
+            prefetch_tensormap(&map_v);
+        }
     }
     grid_dependency_wait(); // the lengths, tables, queries and the cache are written from here on
     grid_dependents_launch();
     const Plan plan = make_plan(p, shared);
     if (plan.which < 0) return;
     const bool tile = p.list[plan.which].tile != 0;
-    const TileSmem<D> sm{base, bars};
-    const Ring<T, D> ring{base, bars};
-    if (threadIdx.x == 0)
-    {
-        if (tile)
-        {
-            for (int g = 0; g < 2; ++g)
-            {
-                mbar_init(sm.q_full(g), 4);
-                mbar_init(sm.k_full(g), 1);
-                mbar_init(sm.k_empty(g), 1);
-                mbar_init(sm.s_full(g), 1);
-                mbar_init(sm.s_free(g), 4);
-                mbar_init(sm.p_full(g), 4);
-                mbar_init(sm.pv_done(g), 1);
-            }
-            mbar_init(sm.v_full(), 1);
-            mbar_init(sm.v_empty(), 1);
-            mbar_init(sm.done(), 8);
-        }
-        else
-            for (int i = 0; i < 2 * kWorkers * L::kRing; ++i) mbar_init(bars + 8 * i, 1);
-        fence_barrier_init();
-    }
     if (tile && warp == 1)
     {
         tmem_alloc(sm.tmem_slot(), 512);
@@ -1122,8 +1131,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (tile)
             {
                 const Walk w = walk_of(p, plan, shared, 0);
-                if (warp == 0) tile_produce<D>(p, plan.which, w, &map_k, sm, 0);
-                else if (warp == 2) tile_produce<D>(p, plan.which, w, &map_v, sm, 1);
+                if (warp == 0) tile_produce<D>(p, plan.which, w, &map_k, &map_v, sm);
                 else if (warp == 1)
                 {
                     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base_ptr + (sm.tmem_slot() - base));
@@ -1196,47 +1204,61 @@ template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) joi
         first[which] = static_cast<size_t>(item[which] + meta.x) * p.list[which].part_rows + within[which];
     }
     const int total = parts[0] + parts[1];
+    auto row_at = [&](int j, const List *&l) {
+        const bool shared = j < parts[0];
+        l = &p.list[shared ? 0 : 1];
+        return (shared ? first[0] : first[1]) + static_cast<size_t>(shared ? j : j - parts[0]) * l->part_rows;
+    };
+    constexpr int kAhead = 8; // parts whose values are fetched together, before their weights are known
     float top = -INFINITY, sum = 0.f, o[N] = {};
-    for (int base = 0; base < total; base += 32)
+    for (int base = 0; base < total; base += kAhead)
     {
-        const int j = base + lane;
+        const int here = min(kAhead, total - base);
+        const List *l;
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (j < parts[0]) ml = p.list[0].ml[first[0] + static_cast<size_t>(j) * p.list[0].part_rows];
-        else if (j < total) ml = p.list[1].ml[first[1] + static_cast<size_t>(j - parts[0]) * p.list[1].part_rows];
-        float most = ml.x;
-#pragma unroll
-        for (int step = 16; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor_sync(full, most, step));
-        most = fmaxf(most, top);
-        const float before = top == most ? 1.f : exp2_fast(top - most);
-        const float weight = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - most);
-        float l = weight * ml.y;
-#pragma unroll
-        for (int step = 16; step > 0; step >>= 1) l += __shfl_xor_sync(full, l, step);
-        sum = sum * before + l;
-        top = most;
-#pragma unroll
-        for (int d = 0; d < N; ++d) o[d] *= before;
-        const int here = min(32, total - base);
-#pragma unroll 4
-        for (int k = 0; k < here; ++k)
+        if (lane < here)
         {
-            const float f = __shfl_sync(full, weight, k);
-            const int jj = base + k;
-            const float *src = jj < parts[0] ? p.list[0].o + (first[0] + static_cast<size_t>(jj) * p.list[0].part_rows) * D
-                                             : p.list[1].o + (first[1] + static_cast<size_t>(jj - parts[0]) * p.list[1].part_rows) * D;
-            float x[N];
+            const size_t r = row_at(base + lane, l);
+            ml = l->ml[r];
+        }
+        float x[kAhead][N];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+        {
+            if (k >= here) break;
+            const size_t r = row_at(base + k, l);
+            const float *src = l->o + r * D + lane * N;
             if constexpr (N == 4)
             {
-                const float4 t = *reinterpret_cast<const float4 *>(src + lane * 4);
-                x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+                const float4 t = *reinterpret_cast<const float4 *>(src);
+                x[k][0] = t.x, x[k][1] = t.y, x[k][2] = t.z, x[k][3] = t.w;
             }
             else
             {
-                const float2 t = *reinterpret_cast<const float2 *>(src + lane * 2);
-                x[0] = t.x, x[1] = t.y;
+                const float2 t = *reinterpret_cast<const float2 *>(src);
+                x[k][0] = t.x, x[k][1] = t.y;
             }
+        }
+        float most = ml.x;
 #pragma unroll
-            for (int d = 0; d < N; ++d) o[d] = fmaf(f, x[d], o[d]);
+        for (int step = kAhead / 2; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor_sync(full, most, step));
+        most = fmaxf(__shfl_sync(full, most, 0), top);
+        const float before = top == most ? 1.f : exp2_fast(top - most);
+        const float weight = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - most);
+        float part_sum = weight * ml.y;
+#pragma unroll
+        for (int step = kAhead / 2; step > 0; step >>= 1) part_sum += __shfl_xor_sync(full, part_sum, step);
+        sum = sum * before + __shfl_sync(full, part_sum, 0);
+        top = most;
+#pragma unroll
+        for (int d = 0; d < N; ++d) o[d] *= before;
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+        {
+            const float f = __shfl_sync(full, weight, k);
+            if (k >= here) break;
+#pragma unroll
+            for (int d = 0; d < N; ++d) o[d] = fmaf(f, x[k][d], o[d]);
         }
     }
     const float inverse = sum > 0.f ? 1.f / sum : 0.f;
@@ -1354,6 +1376,10 @@ template <class T, int D> cudaError_t prepare()
     // the register split needs this many registers per thread at launch
     if (attr.numRegs < kMinLaunchRegs) return cudaErrorInvalidConfiguration;
     static_assert(Layout<T, D>::kSmemBytes <= 232448, "shared memory of a CTA");
+    // the join keeps the SMs' split between shared memory and L1: changing it between the two kernels of every
+    // call drains the SMs
+    const cudaError_t c = cudaFuncSetAttribute(join_kernel<T, D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (c != cudaSuccess) return c;
     return cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<T, D>::kSmemBytes);
 }
 } // namespace
