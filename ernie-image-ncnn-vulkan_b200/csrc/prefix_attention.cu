@@ -41,12 +41,28 @@ constexpr int kRegsControl = 88, kRegsWork = 208, kMinLaunchRegs = 168;
 static_assert(128 * kRegsControl + 256 * kRegsWork <= kThreads * kMinLaunchRegs, "register split");
 constexpr int kErrAttendTimeout = 42;
 
+// Division of numbers below 2^31 by a divisor that the host knows: n / d = (hi32(n m) + n) >> shift.
+struct Divisor
+{
+    unsigned m, shift;
+};
+Divisor divisor(unsigned d)
+{
+    Divisor r = {0, 0};
+    while ((1ull << r.shift) < d) ++r.shift;
+    r.m = static_cast<unsigned>(((1ull << 32) * ((1ull << r.shift) - d)) / d + 1);
+    return r;
+}
+__device__ __forceinline__ int divide(int n, Divisor d) { return static_cast<int>((__umulhi(n, d.m) + n) >> d.shift); }
+
 // One of the two lists, as the host lays it out.
 struct List
 {
     int owners;     // groups or sequences
     int rows;       // of an owner and K/V head
-    int block;      // rows of an item
+    int slots;      // of an owner
+    int block;      // rows of an item, and its log2
+    int block_shift;
     int blocks;     // items of an owner and K/V head
     int part_rows;  // rows that a part stores
     int tile;       // 1: on the tensor cores' tiles, 0: streamed
@@ -54,7 +70,7 @@ struct List
     int cost;       // of a unit on an SM, relative
     float *o;       // [items + workers][part_rows][D]
     float2 *ml;     // [items + workers][part_rows]
-    int2 *meta;     // [items]: first part's worker, number of parts
+    int2 *meta;     // [items]: the workers of the first and the last part
 };
 
 struct AttendArgs
@@ -63,6 +79,7 @@ struct AttendArgs
     List list[2]; // prefix, own
     int ctas;
     int share;    // query heads of a K/V head
+    Divisor by_share, by_queries, by_heads, by_group; // query heads of a K/V head, slots of a sequence, query heads, slots of a group
     float scale;  // log2(e) / sqrt(D)
     int granule;  // keys of a TMA box
 };
@@ -173,15 +190,25 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity)
 }
 
 // ---------------------------------------------------------------- the plan
-// Keys that the rows of an item see at most.
-__device__ __forceinline__ int item_keys(const AttendArgs &p, int which, int owner, int block)
+struct Keys
+{
+    int keys; // that the rows of an item see at most
+    OwnView own;
+};
+
+__device__ __forceinline__ Keys item_keys(const AttendArgs &p, int which, int owner, int block)
 {
     const PagedBatch &b = p.a.batch;
-    if (which == 0) return clamped_length(b.prefix_lens[owner], b.max_prefix_pages, p.a.kv.page_shift, b.error_flag);
-    const OwnView v = own_view(b, p.a.kv.page_shift, owner);
-    const int first = block * p.list[1].block, rows = min(first + p.list[1].block, v.count * p.share);
-    if (rows <= first) return 0;
-    return max(0, v.len - v.count + (rows - 1) / p.share + 1);
+    Keys k = {0, {0, 0}};
+    if (which == 0)
+    {
+        k.keys = clamped_length(b.prefix_lens[owner], b.max_prefix_pages, p.a.kv.page_shift, b.error_flag);
+        return k;
+    }
+    k.own = own_view(b, p.a.kv.page_shift, owner);
+    const int first = block << p.list[1].block_shift, rows = min(first + p.list[1].block, k.own.count * p.share);
+    if (rows > first) k.keys = max(0, k.own.len - k.own.count + divide(rows - 1, p.by_share) + 1);
+    return k;
 }
 
 __device__ __forceinline__ int units_of(const List &l, int keys)
@@ -189,37 +216,34 @@ __device__ __forceinline__ int units_of(const List &l, int keys)
     return (keys >> l.unit_shift) + ((keys & ((1 << l.unit_shift) - 1)) != 0);
 }
 
-// `units` dealt out to `workers`: the first units % workers of them take one more.
-__device__ __forceinline__ int first_unit(int worker, int units, int workers)
+// The CTA's list (-1: nothing to do) and how it is dealt out: `each` units to a worker, one more to the first
+// `more` of them.
+struct Plan
 {
-    const int each = units / workers;
-    return worker * each + min(worker, units - each * workers);
-}
-__device__ __forceinline__ int worker_of_unit(int u, int units, int workers)
+    int which, cta, ctas, workers, each, more;
+    __device__ int first_unit(int worker) const { return worker * each + min(worker, more); }
+};
+
+// Where a worker begins: so many units after the first one of the owners that a thread has summed up.
+struct PlanShared
 {
-    const int each = units / workers, more = units - each * workers, ahead = more * (each + 1);
-    return u < ahead ? u / (each + 1) : more + (u - ahead) / each;
-}
+    int warp_sum[2][kThreads / 32];
+    int2 begin[kWorkers]; // that thread's first owner, units
+};
 
 // A worker's walk over its units.
 struct Walk
 {
-    int worker, workers; // within the list
-    int at, end, units;  // next unit, the worker's last and the list's number of them
+    int worker, at, end;          // next unit and the worker's end
     int owner, block, head, unit; // the next unit's item and its number within the item
-};
-
-struct PlanShared
-{
-    int warp_sum[2][kThreads / 32];
-    int4 begin[kWorkers]; // owner, block, head, unit where a worker begins
 };
 
 struct Part
 {
     int owner, block, head;
-    int keys;              // of the item
+    Keys item;
     int first_unit, units; // of the part
+    bool last;             // the item's last part
     int place;             // of its results
 };
 
@@ -228,12 +252,12 @@ __device__ __forceinline__ bool next_part(const AttendArgs &p, int which, Walk &
 {
     if (w.at >= w.end) return false;
     const List &l = p.list[which];
-    int keys, units;
+    int units;
     for (;;)
     {
         if (w.owner >= l.owners) return false; // only if the lengths change under the call
-        keys = item_keys(p, which, w.owner, w.block);
-        units = units_of(l, keys);
+        part.item = item_keys(p, which, w.owner, w.block);
+        units = units_of(l, part.item.keys);
         if (w.unit < units) break;
         w.unit = 0;
         w.head = 0;
@@ -242,13 +266,13 @@ __device__ __forceinline__ bool next_part(const AttendArgs &p, int which, Walk &
     part.owner = w.owner;
     part.block = w.block;
     part.head = w.head;
-    part.keys = keys;
     part.first_unit = w.unit;
     part.units = min(units - w.unit, w.end - w.at);
     part.place = (w.owner * l.blocks + w.block) * p.a.kv.kv_heads + w.head + w.worker;
     w.at += part.units;
     w.unit += part.units;
-    if (w.unit == units)
+    part.last = w.unit == units;
+    if (part.last)
     {
         w.unit = 0;
         if (++w.head == p.a.kv.kv_heads)
@@ -260,38 +284,40 @@ __device__ __forceinline__ bool next_part(const AttendArgs &p, int which, Walk &
     return true;
 }
 
-// Written by the part that holds the item's first unit; `w` has just stepped over the part.
-__device__ __forceinline__ void write_meta(const AttendArgs &p, int which, const Walk &w, const Part &part)
+__device__ __forceinline__ void write_meta(const List &l, const Walk &w, const Part &part)
 {
-    const List &l = p.list[which];
-    const int last = worker_of_unit(w.at - part.units + units_of(l, part.keys) - 1, w.units, w.workers);
-    l.meta[part.place - w.worker] = make_int2(w.worker, last - w.worker + 1);
+    int *meta = reinterpret_cast<int *>(l.meta + (part.place - w.worker));
+    if (part.first_unit == 0) meta[0] = w.worker;
+    if (part.last) meta[1] = w.worker;
 }
 
-// All threads: the lists' units, the CTA's list (-1: nothing to do) and its workers' shares. `mine` is the
-// walk of worker `warp` of the CTA (streamed) or of the CTA (tile: worker 0).
-struct Plan
-{
-    int which, cta, ctas, units, workers;
-};
-
+// The walk of worker `local` of the CTA (tile: 0, the CTA itself).
 __device__ __forceinline__ Walk walk_of(const AttendArgs &p, const Plan &plan, const PlanShared &s, int local)
 {
-    Walk w;
-    w.worker = local * plan.ctas + plan.cta; // neighbours in the order go to different SMs
-    w.workers = plan.workers;
-    w.units = plan.units;
-    const bool any = w.worker < plan.workers;
-    w.at = any ? first_unit(w.worker, plan.units, plan.workers) : 0;
-    w.end = any ? first_unit(w.worker + 1, plan.units, plan.workers) : 0;
-    const int4 b = s.begin[local];
-    w.owner = b.x;
-    w.block = b.y;
-    w.head = b.z;
-    w.unit = b.w;
+    const List &l = p.list[plan.which];
+    Walk w = {local * plan.ctas + plan.cta, 0, 0, 0, 0, 0, 0}; // neighbours in the order go to different SMs
+    if (w.worker >= plan.workers) return w;
+    w.at = plan.first_unit(w.worker);
+    w.end = plan.first_unit(w.worker + 1);
+    const int2 begin = s.begin[local];
+    w.owner = begin.x;
+    int left = begin.y;
+    while (w.owner < l.owners)
+    {
+        const int units = units_of(l, item_keys(p, plan.which, w.owner, w.block).keys);
+        if (left < units * p.a.kv.kv_heads)
+        {
+            for (; left >= units; left -= units) ++w.head;
+            w.unit = left;
+            break;
+        }
+        left -= units * p.a.kv.kv_heads;
+        if (++w.block == l.blocks) w.block = 0, ++w.owner;
+    }
     return w;
 }
 
+// All threads: the lists' units, dealt out.
 __device__ __forceinline__ Plan make_plan(const AttendArgs &p, PlanShared &s)
 {
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, heads = p.a.kv.kv_heads;
@@ -303,7 +329,7 @@ __device__ __forceinline__ Plan make_plan(const AttendArgs &p, PlanShared &s)
         chunk[i] = l.owners <= kThreads ? 1 : (l.owners + kThreads - 1) / kThreads;
         int sum = 0;
         for (int o = tid * chunk[i]; o < min(l.owners, (tid + 1) * chunk[i]); ++o)
-            for (int b = 0; b < l.blocks; ++b) sum += units_of(l, item_keys(p, i, o, b));
+            for (int b = 0; b < l.blocks; ++b) sum += units_of(l, item_keys(p, i, o, b).keys);
         mine[i] = sum * heads;
     }
 #pragma unroll
@@ -330,7 +356,7 @@ __device__ __forceinline__ Plan make_plan(const AttendArgs &p, PlanShared &s)
             if (j < warp) before[i] += sum;
             total[i] += sum;
         }
-    Plan plan = {-1, 0, 0, 0, 0};
+    Plan plan = {-1, 0, 0, 0, 0, 0};
     if (total[0] + total[1] == 0) return plan;
     // the lists' CTAs: by cost, at least one for a list with work, no more than it has units
     const float cost0 = static_cast<float>(total[0]) * p.list[0].cost, cost1 = static_cast<float>(total[1]) * p.list[1].cost;
@@ -344,25 +370,18 @@ __device__ __forceinline__ Plan make_plan(const AttendArgs &p, PlanShared &s)
     plan.which = cta < n0 ? 0 : 1;
     plan.cta = plan.which ? cta - n0 : cta;
     plan.ctas = plan.which ? n1 : n0;
-    plan.units = plan.which ? total[1] : total[0];
     const List &l = p.list[plan.which];
-    plan.workers = l.tile ? plan.ctas : min(plan.units, plan.ctas * kWorkers);
+    const int units = plan.which ? total[1] : total[0];
+    plan.workers = l.tile ? plan.ctas : min(units, plan.ctas * kWorkers);
+    plan.each = units / plan.workers;
+    plan.more = units - plan.each * plan.workers;
     const int ahead = plan.which ? before[1] : before[0], held = plan.which ? mine[1] : mine[0];
-    for (int local = 0; local < (l.tile ? 1 : kWorkers); ++local)
+    const int owner = tid * (plan.which ? chunk[1] : chunk[0]);
+#pragma unroll
+    for (int local = 0; local < kWorkers; ++local)
     {
-        const int worker = local * plan.ctas + plan.cta;
-        if (worker >= plan.workers) break;
-        int left = first_unit(worker, plan.units, plan.workers) - ahead;
-        if (left < 0 || left >= held) continue;
-        int o = tid * (plan.which ? chunk[1] : chunk[0]), b = 0, units;
-        for (;;)
-        {
-            units = units_of(l, item_keys(p, plan.which, o, b));
-            if (left < units * heads) break;
-            left -= units * heads;
-            if (++b == l.blocks) b = 0, ++o;
-        }
-        s.begin[local] = make_int4(o, b, left / units, left % units);
+        const int worker = local * plan.ctas + plan.cta, left = plan.first_unit(worker) - ahead;
+        if (worker < plan.workers && left >= 0 && left < held) s.begin[local] = make_int2(owner, left);
     }
     __syncthreads();
     return plan;
@@ -379,25 +398,20 @@ __device__ __forceinline__ Row row_of(const AttendArgs &p, int which, const Part
 {
     const PagedBatch &b = p.a.batch;
     const List &l = p.list[which];
-    const int r = part.block * l.block + row;
+    const int r = (part.block << l.block_shift) + row;
     Row out = {0, 0};
     if (row >= l.block || r >= l.rows) return out;
-    const int at = r / p.share, head = part.head * p.share + r - at * p.share;
-    int slot;
+    const int at = divide(r, p.by_share), head = part.head * p.share + r - at * p.share, slot = part.owner * l.slots + at;
     if (which == 0)
     {
-        const int per = l.rows / p.share; // slots of the group
-        slot = part.owner * per + at;
-        const int s = slot / b.queries, i = slot - s * b.queries;
-        if (b.counts && i >= b.counts[s]) return out;
-        out.keys = part.keys;
+        const int s = divide(slot, p.by_queries);
+        if (b.counts && slot - s * b.queries >= b.counts[s]) return out;
+        out.keys = part.item.keys;
     }
     else
     {
-        const OwnView v = own_view(b, p.a.kv.page_shift, part.owner);
-        if (at >= v.count) return out;
-        slot = part.owner * b.queries + at;
-        out.keys = max(0, v.len - v.count + at + 1);
+        if (at >= part.item.own.count) return out;
+        out.keys = max(0, part.item.own.len - part.item.own.count + at + 1);
     }
     out.query = slot * p.a.heads + head;
     return out;
@@ -409,7 +423,7 @@ __device__ __forceinline__ int pool_row(const AttendArgs &p, int which, const Pa
 {
     const PagedLayer &kv = p.a.kv;
     const int outside = (kv.pages * kv.kv_heads) << kv.page_shift;
-    if (key >= part.keys) return outside;
+    if (key >= part.item.keys) return outside;
     const PagedBatch &b = p.a.batch;
     const int *table = which == 0 ? b.prefix_tables + static_cast<size_t>(part.owner) * b.max_prefix_pages
                                   : b.tables + static_cast<size_t>(part.owner) * b.max_pages;
@@ -583,7 +597,7 @@ template <class T, int D> struct Ring
 template <class T, int D> __device__ __forceinline__ int slots_of(const Part &part, int unit_shift)
 {
     constexpr int keys = Layout<T, D>::kSlotKeys;
-    const int end = min(static_cast<long long>(part.keys), static_cast<long long>(part.first_unit + part.units) << unit_shift);
+    const int end = min(static_cast<long long>(part.item.keys), static_cast<long long>(part.first_unit + part.units) << unit_shift);
     return (end - (part.first_unit << unit_shift) + keys - 1) / keys;
 }
 
@@ -619,7 +633,7 @@ __device__ __forceinline__ void stream_produce(const AttendArgs &p, const Plan &
         const bool free = __shfl_sync(0xffffffffu, static_cast<int>(mbar_try_wait(ring.empty(worker, n), ring.round(n) ^ 1u)), lane & 16);
         if (more && free)
         {
-            const int kept = min(granules, (part.keys - key + p.granule - 1) / p.granule); // granules with keys
+            const int kept = min(granules, (part.item.keys - key + p.granule - 1) / p.granule); // granules with keys
             if (sub == 0) mbar_arrive_expect_tx(ring.full(worker, n), kept * L::kColumns * 2 * box_bytes);
             __syncwarp(half_mask);
             if (has_box && granule < kept)
@@ -661,7 +675,7 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
     Part part;
     while (next_part(p, plan.which, w, part))
     {
-        if (lane == 0 && part.first_unit == 0) write_meta(p, plan.which, w, part);
+        if (lane == 0) write_meta(l, w, part);
         const Row first = row_of(p, plan.which, part, r0), second = row_of(p, plan.which, part, r1);
         R x;
         x.load(p, first, second, lane);
@@ -734,7 +748,7 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
                 l0 += s[t][0] + s[t][1];
                 l1 += s[t][2] + s[t][3];
             }
-            x.weigh(k + L::kSlotHalf, lane, s, part.keys - key0, o);
+            x.weigh(k + L::kSlotHalf, lane, s, part.item.keys - key0, o);
             __syncwarp();
             if (lane == 0) mbar_arrive(ring.empty(worker, n));
         }
@@ -926,7 +940,7 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Wal
     Part part;
     while (next_part(p, which, w, part))
     {
-        if (warp == 0 && lane == 0 && part.first_unit == 0) write_meta(p, which, w, part);
+        if (warp == 0 && lane == 0) write_meta(l, w, part);
         const int rows = min(l.block, l.rows - part.block * l.block);
         if (g * kTile >= rows)
         {
@@ -1020,11 +1034,11 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Wal
             const float2 s4 = __fadd2_rn(__fadd2_rn(part_sum[0], part_sum[1]), __fadd2_rn(part_sum[2], part_sum[3]));
             sum += s4.x + s4.y;
             // values past the item's last key may be anything, NaN too: zeros, by both tiles' threads alike
-            if (key0 + kTile > part.keys)
+            if (key0 + kTile > part.item.keys)
             {
                 const unsigned load = sm.v_load(n + u);
                 if (!(ok = warp_wait(sm.full(load), sm.round(load)))) break;
-                if (key0 + r >= part.keys)
+                if (key0 + r >= part.item.keys)
                 {
 #pragma unroll
                     for (int i = 0; i < D / 8; ++i) st_shared_v4(sm.kv(load) + (i >> 3) * (kTile * 128) + r * 128 + (i & 7) * 16, 0, 0, 0, 0);
@@ -1175,8 +1189,12 @@ template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) joi
     const int at = blockIdx.x * kJoinWarps + threadIdx.x / 32; // row of q and out
     // The lengths are older than the kernel before this one, which waited for them before it let this one start.
     bool row = at < b.sequences * b.queries * p.a.heads;
-    const int slot = row ? at / p.a.heads : 0, head = at - slot * p.a.heads, s = slot / b.queries, i = slot - s * b.queries;
-    const SequenceView view = sequence_view(b, p.a.kv.page_shift, s);
+    const int slot = row ? divide(at, p.by_heads) : 0, head = at - slot * p.a.heads, s = divide(slot, p.by_queries), i = slot - s * b.queries;
+    const int kv_head = divide(head, p.by_share), group = divide(slot, p.by_group);
+    SequenceView view;
+    view.prefix_len = b.max_prefix_pages ? b.prefix_lens[group] : 0;
+    static_cast<OwnView &>(view) = own_view(b, p.a.kv.page_shift, s);
+    if (b.max_prefix_pages) view.prefix_len = clamped_length(view.prefix_len, b.max_prefix_pages, p.a.kv.page_shift, b.error_flag);
     row = row && i < view.count;
     int item[2] = {-1, -1}, within[2] = {0, 0};
 #pragma unroll
@@ -1184,10 +1202,9 @@ template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) joi
     {
         const List &l = p.list[which];
         if (which == 0 ? view.prefix_len == 0 : view.len - view.count + i + 1 <= 0) continue;
-        const int per = p.list[0].owners ? p.list[0].rows / p.share : 1; // slots of a group
-        const int owner = which == 0 ? slot / per : s;
-        const int r = (which == 0 ? slot - owner * per : i) * p.share + head % p.share, block = r / l.block;
-        item[which] = (owner * l.blocks + block) * p.a.kv.kv_heads + head / p.share;
+        const int owner = which == 0 ? group : s;
+        const int r = (which == 0 ? slot - owner * l.slots : i) * p.share + head - kv_head * p.share, block = r >> l.block_shift;
+        item[which] = (owner * l.blocks + block) * p.a.kv.kv_heads + kv_head;
         within[which] = r - block * l.block;
     }
     grid_dependency_wait();
@@ -1200,7 +1217,7 @@ template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) joi
     {
         if (item[which] < 0) continue;
         const int2 meta = p.list[which].meta[item[which]];
-        parts[which] = meta.y;
+        parts[which] = meta.y - meta.x + 1;
         first[which] = static_cast<size_t>(item[which] + meta.x) * p.list[which].part_rows + within[which];
     }
     const int total = parts[0] + parts[1];
@@ -1284,15 +1301,21 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
 {
     p.ctas = ctas;
     p.share = heads / kv.kv_heads;
+    p.by_share = divisor(p.share);
+    p.by_queries = divisor(b.queries);
+    p.by_heads = divisor(heads);
+    p.by_group = divisor(b.sequences / b.groups * b.queries);
     char *base = static_cast<char *>(workspace);
     size_t at = 0;
     for (int i = 0; i < 2; ++i)
     {
         List &l = p.list[i];
         l.owners = i == 0 ? (b.max_prefix_pages ? b.groups : 0) : b.sequences;
-        l.rows = (i == 0 ? b.sequences / b.groups : 1) * b.queries * p.share;
+        l.slots = (i == 0 ? b.sequences / b.groups : 1) * b.queries;
+        l.rows = l.slots * p.share;
         l.tile = kv.bf16 && l.rows > kTileRows;
-        l.block = l.tile ? 2 * kTile : 16;
+        l.block_shift = l.tile ? 8 : 4;
+        l.block = 1 << l.block_shift;
         l.blocks = (l.rows + l.block - 1) / l.block;
         l.part_rows = l.rows < l.block ? l.rows : l.block;
         l.unit_shift = l.tile ? 7 : 5;
