@@ -9,7 +9,7 @@
 //   own     (sequence, block of rows, K/V head): a sequence's rows against its own tokens.
 // A row is a query head of a slot: the heads/kv_heads query heads that share a K/V head are rows of one item.
 // An item's keys are cut into units, and each list's units are dealt out evenly, in order, to that list's
-// workers, so that an item may span several workers and a worker several items; an item's share of a worker
+// workers (a fixed cost of every item counted in), so that an item may span several workers and a worker several items; an item's share of a worker
 // is a part. Along the order both the item and the worker only ever step up, so item + worker numbers the
 // parts without gaps or clashes, and an item's parts lie side by side. The lists share the CTAs by their
 // estimated cost. All of this is worked out on the device, by every CTA for itself, from the lengths of this
@@ -67,6 +67,7 @@ struct List
     int part_rows;  // rows that a part stores
     int tile;       // 1: on the tensor cores' tiles, 0: streamed
     int unit_shift; // log2 of a unit's keys
+    int lead;       // an item's fixed cost, in units
     int cost;       // of a unit on an SM, relative
     float *o;       // [items + workers][part_rows][D]
     float2 *ml;     // [items + workers][part_rows]
@@ -216,26 +217,34 @@ __device__ __forceinline__ int units_of(const List &l, int keys)
     return (keys >> l.unit_shift) + ((keys & ((1 << l.unit_shift) - 1)) != 0);
 }
 
-// The CTA's list (-1: nothing to do) and how it is dealt out: `each` units to a worker, one more to the first
+// An item takes so many steps of the order: its fixed cost first, during which nothing is computed, so that
+// many short items weigh what they take, then its units.
+__device__ __forceinline__ int steps_of(const List &l, int keys)
+{
+    const int units = units_of(l, keys);
+    return units ? units + l.lead : 0;
+}
+
+// The CTA's list (-1: nothing to do) and how it is dealt out: `each` steps to a worker, one more to the first
 // `more` of them.
 struct Plan
 {
     int which, cta, ctas, workers, each, more;
-    __device__ int first_unit(int worker) const { return worker * each + min(worker, more); }
+    __device__ int first_step(int worker) const { return worker * each + min(worker, more); }
 };
 
-// Where a worker begins: so many units after the first one of the owners that a thread has summed up.
+// Where a worker begins: so many steps after the first one of the owners that a thread has summed up.
 struct PlanShared
 {
     int warp_sum[2][kThreads / 32];
-    int2 begin[kWorkers]; // that thread's first owner, units
+    int2 begin[kWorkers]; // that thread's first owner, steps
 };
 
-// A worker's walk over its units.
+// A worker's walk over its steps.
 struct Walk
 {
-    int worker, at, end;          // next unit and the worker's end
-    int owner, block, head, unit; // the next unit's item and its number within the item
+    int worker, at, end;          // next step and the worker's end
+    int owner, block, head, step; // the next step's item and its number within the item
 };
 
 struct Part
@@ -250,38 +259,40 @@ struct Part
 // The next part of the walk; false at its end. All threads of a worker take the same steps.
 __device__ __forceinline__ bool next_part(const AttendArgs &p, int which, Walk &w, Part &part)
 {
-    if (w.at >= w.end) return false;
     const List &l = p.list[which];
-    int units;
-    for (;;)
+    while (w.at < w.end && w.owner < l.owners) // (the owners run out first only if the lengths change under the call)
     {
-        if (w.owner >= l.owners) return false; // only if the lengths change under the call
         part.item = item_keys(p, which, w.owner, w.block);
-        units = units_of(l, part.item.keys);
-        if (w.unit < units) break;
-        w.unit = 0;
-        w.head = 0;
-        if (++w.block == l.blocks) w.block = 0, ++w.owner;
-    }
-    part.owner = w.owner;
-    part.block = w.block;
-    part.head = w.head;
-    part.first_unit = w.unit;
-    part.units = min(units - w.unit, w.end - w.at);
-    part.place = (w.owner * l.blocks + w.block) * p.a.kv.kv_heads + w.head + w.worker;
-    w.at += part.units;
-    w.unit += part.units;
-    part.last = w.unit == units;
-    if (part.last)
-    {
-        w.unit = 0;
-        if (++w.head == p.a.kv.kv_heads)
+        const int steps = steps_of(l, part.item.keys);
+        if (w.step >= steps) // nothing here
         {
+            w.step = 0;
             w.head = 0;
             if (++w.block == l.blocks) w.block = 0, ++w.owner;
+            continue;
         }
+        const int end = min(steps, w.step + (w.end - w.at));
+        part.owner = w.owner;
+        part.block = w.block;
+        part.head = w.head;
+        part.first_unit = max(0, w.step - l.lead);
+        part.units = max(0, end - l.lead) - part.first_unit;
+        part.last = end == steps;
+        part.place = (w.owner * l.blocks + w.block) * p.a.kv.kv_heads + w.head + w.worker;
+        w.at += end - w.step;
+        w.step = end;
+        if (part.last)
+        {
+            w.step = 0;
+            if (++w.head == p.a.kv.kv_heads)
+            {
+                w.head = 0;
+                if (++w.block == l.blocks) w.block = 0, ++w.owner;
+            }
+        }
+        if (part.units) return true;
     }
-    return true;
+    return false;
 }
 
 __device__ __forceinline__ void write_meta(const List &l, const Walk &w, const Part &part)
@@ -297,27 +308,27 @@ __device__ __forceinline__ Walk walk_of(const AttendArgs &p, const Plan &plan, c
     const List &l = p.list[plan.which];
     Walk w = {local * plan.ctas + plan.cta, 0, 0, 0, 0, 0, 0}; // neighbours in the order go to different SMs
     if (w.worker >= plan.workers) return w;
-    w.at = plan.first_unit(w.worker);
-    w.end = plan.first_unit(w.worker + 1);
+    w.at = plan.first_step(w.worker);
+    w.end = plan.first_step(w.worker + 1);
     const int2 begin = s.begin[local];
     w.owner = begin.x;
     int left = begin.y;
     while (w.owner < l.owners)
     {
-        const int units = units_of(l, item_keys(p, plan.which, w.owner, w.block).keys);
-        if (left < units * p.a.kv.kv_heads)
+        const int steps = steps_of(l, item_keys(p, plan.which, w.owner, w.block).keys);
+        if (left < steps * p.a.kv.kv_heads)
         {
-            for (; left >= units; left -= units) ++w.head;
-            w.unit = left;
+            for (; left >= steps; left -= steps) ++w.head;
+            w.step = left;
             break;
         }
-        left -= units * p.a.kv.kv_heads;
+        left -= steps * p.a.kv.kv_heads;
         if (++w.block == l.blocks) w.block = 0, ++w.owner;
     }
     return w;
 }
 
-// All threads: the lists' units, dealt out.
+// All threads: the lists' steps, dealt out.
 __device__ __forceinline__ Plan make_plan(const AttendArgs &p, PlanShared &s)
 {
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, heads = p.a.kv.kv_heads;
@@ -329,7 +340,7 @@ __device__ __forceinline__ Plan make_plan(const AttendArgs &p, PlanShared &s)
         chunk[i] = l.owners <= kThreads ? 1 : (l.owners + kThreads - 1) / kThreads;
         int sum = 0;
         for (int o = tid * chunk[i]; o < min(l.owners, (tid + 1) * chunk[i]); ++o)
-            for (int b = 0; b < l.blocks; ++b) sum += units_of(l, item_keys(p, i, o, b).keys);
+            for (int b = 0; b < l.blocks; ++b) sum += steps_of(l, item_keys(p, i, o, b).keys);
         mine[i] = sum * heads;
     }
 #pragma unroll
@@ -358,7 +369,7 @@ __device__ __forceinline__ Plan make_plan(const AttendArgs &p, PlanShared &s)
         }
     Plan plan = {-1, 0, 0, 0, 0, 0};
     if (total[0] + total[1] == 0) return plan;
-    // the lists' CTAs: by cost, at least one for a list with work, no more than it has units
+    // the lists' CTAs: by cost, at least one for a list with work, no more than it has steps
     const float cost0 = static_cast<float>(total[0]) * p.list[0].cost, cost1 = static_cast<float>(total[1]) * p.list[1].cost;
     int n0 = static_cast<int>(p.ctas * __fdividef(cost0, cost0 + cost1) + 0.5f);
     n0 = total[0] == 0 ? 0 : total[1] == 0 ? p.ctas : max(1, min(p.ctas - 1, n0));
@@ -371,16 +382,16 @@ __device__ __forceinline__ Plan make_plan(const AttendArgs &p, PlanShared &s)
     plan.cta = plan.which ? cta - n0 : cta;
     plan.ctas = plan.which ? n1 : n0;
     const List &l = p.list[plan.which];
-    const int units = plan.which ? total[1] : total[0];
-    plan.workers = l.tile ? plan.ctas : min(units, plan.ctas * kWorkers);
-    plan.each = units / plan.workers;
-    plan.more = units - plan.each * plan.workers;
+    const int steps = plan.which ? total[1] : total[0];
+    plan.workers = l.tile ? plan.ctas : min(steps, plan.ctas * kWorkers);
+    plan.each = steps / plan.workers;
+    plan.more = steps - plan.each * plan.workers;
     const int ahead = plan.which ? before[1] : before[0], held = plan.which ? mine[1] : mine[0];
     const int owner = tid * (plan.which ? chunk[1] : chunk[0]);
 #pragma unroll
     for (int local = 0; local < kWorkers; ++local)
     {
-        const int worker = local * plan.ctas + plan.cta, left = plan.first_unit(worker) - ahead;
+        const int worker = local * plan.ctas + plan.cta, left = plan.first_step(worker) - ahead;
         if (worker < plan.workers && left >= 0 && left < held) s.begin[local] = make_int2(owner, left);
     }
     __syncthreads();
@@ -1319,9 +1330,10 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
         l.blocks = (l.rows + l.block - 1) / l.block;
         l.part_rows = l.rows < l.block ? l.rows : l.block;
         l.unit_shift = l.tile ? 7 : 5;
-        // nanoseconds of an SM: a tile's step with one and with two tiles of rows; a streamed unit at its share
-        // of the memory's rate (BF16) or at the rate of the split products (FP32)
-        l.cost = l.tile ? (l.rows > kTile ? 1600 : 900) : kv.bf16 ? 370 * kv.dim / 128 : 800 * kv.dim / 128;
+        // nanoseconds of an SM: a tile's unit with one and with two tiles of rows; a streamed unit as fast as an SM
+        // takes them when the memory is not the limit
+        l.cost = l.tile ? (l.rows > kTile ? 1900 : 1100) : kv.bf16 ? 180 * kv.dim / 128 : 800 * kv.dim / 128;
+        l.lead = l.tile ? (l.rows > kTile ? 4 : 6) : 3;
         const size_t items = static_cast<size_t>(l.owners) * l.blocks * kv.kv_heads;
         const size_t parts = l.owners ? items + ctas * (l.tile ? 1 : kWorkers) : 0;
         l.o = reinterpret_cast<float *>(base + at);
@@ -1334,7 +1346,7 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
     return at;
 }
 
-// The plan counts units in 32 bits.
+// The plan counts steps in 32 bits.
 bool countable(const PagedLayer &kv, const AttendArgs &p, const PagedBatch &b)
 {
     double units = 0;
@@ -1342,7 +1354,7 @@ bool countable(const PagedLayer &kv, const AttendArgs &p, const PagedBatch &b)
     {
         const List &l = p.list[i];
         const double keys = static_cast<double>(i == 0 ? b.max_prefix_pages : b.max_pages) * (1 << kv.page_shift);
-        units += (keys / (1 << l.unit_shift) + 1) * l.owners * l.blocks * kv.kv_heads;
+        units += (keys / (1 << l.unit_shift) + 1 + l.lead) * l.owners * l.blocks * kv.kv_heads;
     }
     return units < 1e9;
 }
