@@ -16,10 +16,10 @@
 // very call.
 //
 // A list is worked on in one of two ways, chosen on the host by the rows of an item:
-//   stream  few rows, or an FP32 cache. A worker is a warp: 16 rows, its own TMA ring of K/V slots, mma.sync
-//           m16n8 tiles. The bound is the K/V traffic, and eight independent warps per SM hide each other's
-//           latencies without ever meeting. FP32 operands are split into two TF32 parts and multiplied in
-//           three products.
+//   stream  few rows, or an FP32 cache. A worker is a warp: 16 rows and its own TMA ring of K/V slots. The
+//           bound is the K/V traffic, and eight independent warps per SM hide each other's latencies without
+//           ever meeting. BF16 uses mma.sync m16n8 tiles, FP32 packed FMAs (three products of TF32 parts on
+//           the tensor cores took 2.4 times as long and lost two bits).
 //   tile    many rows of a BF16 cache. A worker is a CTA: 256 rows (two tiles of 128) share each K/V tile on
 //           the tensor cores (tcgen05.mma, accumulators in TMEM), one row per softmax thread.
 // A second kernel joins the parts of each row.
@@ -126,13 +126,6 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-__device__ __forceinline__ float ld_shared(uint32_t addr)
-{
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-
 __device__ __forceinline__ float4 ld_shared_v4(uint32_t addr)
 {
     float4 v;
@@ -161,27 +154,6 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
-{
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// x = high + low up to 2^-22 |x|, both in TF32.
-__device__ __forceinline__ void split_tf32(float x, uint32_t &high, uint32_t &low)
-{
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(high) : "f"(x));
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(low) : "f"(x - __uint_as_float(high)));
-}
-
-// The same, worked out anew where it stands: hoisted out of the key loop the queries' parts would spill.
-__device__ __forceinline__ void split_tf32_here(float x, uint32_t &high, uint32_t &low)
-{
-    asm volatile("cvt.rna.tf32.f32 %0, %1;" : "=r"(high) : "f"(x));
-    asm volatile("cvt.rna.tf32.f32 %0, %1;" : "=r"(low) : "f"(x - __uint_as_float(high)));
 }
 
 // A whole warp's bounded wait, with one answer for all its lanes.
@@ -446,11 +418,11 @@ __device__ __forceinline__ int pool_row(const AttendArgs &p, int which, const Pa
 }
 
 // ---------------------------------------------------------------- stream
-// A warp's 16 rows in mma.sync fragments: rows lane/4 and lane/4 + 8; a lane's columns are 2 (lane % 4) and
-// the next of every eight. A slot holds K and V of kSlotKeys keys, 128-byte rows in swizzled column blocks.
-template <class T, int D> struct Rows16;
+// A slot holds K and V of kSlotKeys keys, 128-byte rows in swizzled column blocks.
 
-template <int D> struct Rows16<__nv_bfloat16, D>
+// BF16: a warp's 16 rows in mma.sync fragments: rows lane/4 and lane/4 + 8; a lane's columns are
+// 2 (lane % 4) and the next of every eight.
+template <int D> struct Rows16
 {
     static constexpr int kKeys = 16, kTiles = 2; // of a step; score tiles of eight keys
     uint32_t q[D / 16][4];
@@ -514,86 +486,6 @@ template <int D> struct Rows16<__nv_bfloat16, D>
     }
 };
 
-// FP32 sums: the tensor cores drop low bits at every step of a chain, so chains are kept short and added up
-// with rounding (one chain of 48 products left 3.4e-6 against 1e-6 of the result).
-template <int D> struct Rows16<float, D>
-{
-    static constexpr int kKeys = 8, kTiles = 1;
-    float q[D / 8][4];
-    __device__ __forceinline__ void load(const AttendArgs &p, const Row &r0, const Row &r1, int lane)
-    {
-        const float *base = static_cast<const float *>(p.a.q) + (lane & 3);
-        const float *x0 = base + static_cast<size_t>(r0.query) * D, *x1 = base + static_cast<size_t>(r1.query) * D;
-#pragma unroll
-        for (int s = 0; s < D / 8; ++s)
-        {
-            q[s][0] = r0.keys ? x0[8 * s] : 0.f;
-            q[s][1] = r1.keys ? x1[8 * s] : 0.f;
-            q[s][2] = r0.keys ? x0[8 * s + 4] : 0.f;
-            q[s][3] = r1.keys ? x1[8 * s + 4] : 0.f;
-        }
-    }
-    __device__ __forceinline__ void scores(uint32_t k, int lane, float (&s)[kTiles][4]) const
-    {
-        // a load brings the key fragments of two steps of eight dims
-        const int key = lane & 7, quarter = lane >> 3;
-        float chain[4][4] = {}, cross[2][4] = {};
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-        {
-            uint32_t raw[4], high[4], low[4];
-            const int chunk = 4 * i + quarter;
-            ldmatrix(k + (chunk >> 3) * (kKeys * 128) + key * 128 + (((chunk & 7) ^ key) << 4), raw);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) split_tf32(__uint_as_float(raw[j]), high[j], low[j]);
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-            {
-                uint32_t qh[4], ql[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) split_tf32_here(q[2 * i + h][j], qh[j], ql[j]);
-                mma_tf32(cross[0], ql, high[2 * h], high[2 * h + 1]);
-                mma_tf32(cross[1], qh, low[2 * h], low[2 * h + 1]);
-                mma_tf32(chain[(2 * i + h) & 3], qh, high[2 * h], high[2 * h + 1]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            s[0][j] = ((chain[0][j] + chain[1][j]) + (chain[2][j] + chain[3][j])) + (cross[0][j] + cross[1][j]);
-    }
-    // The weights' fragment of key columns 2t and 2t + 1 serves as one whose columns are t and t + 4, with
-    // the value rows taken in that order.
-    __device__ __forceinline__ void weigh(uint32_t v, int lane, const float (&s)[kTiles][4], int valid, float (&o)[D / 8][4]) const
-    {
-        uint32_t ph[4], pl[4];
-        split_tf32(s[0][0], ph[0], pl[0]);
-        split_tf32(s[0][2], ph[1], pl[1]);
-        split_tf32(s[0][1], ph[2], pl[2]);
-        split_tf32(s[0][3], ph[3], pl[3]);
-        const int key = 2 * (lane & 3);
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-        {
-            const int d = (i & 3) * 8 + (lane >> 2);
-            const uint32_t column = v + (i >> 2) * (kKeys * 128) + (d & 3) * 4;
-            uint32_t high[2], low[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-            {
-                float x = ld_shared(column + (key + e) * 128 + (((d >> 2) ^ (key + e)) << 4));
-                if (key + e >= valid) x = 0.f;
-                split_tf32(x, high[e], low[e]);
-            }
-            float sum[4] = {};
-            mma_tf32(sum, pl, high[0], high[1]);
-            mma_tf32(sum, ph, low[0], low[1]);
-            mma_tf32(sum, ph, high[0], high[1]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[i][j] += sum[j];
-        }
-    }
-};
-
 template <class T, int D> struct Ring
 {
     using L = Layout<T, D>;
@@ -642,6 +534,8 @@ __device__ __forceinline__ void stream_produce(const AttendArgs &p, const Plan &
     while (__any_sync(0xffffffffu, more))
     {
         const bool free = __shfl_sync(0xffffffffu, static_cast<int>(mbar_try_wait(ring.empty(worker, n), ring.round(n) ^ 1u)), lane & 16);
+        // neither ring has room: out of the workers' issue slots for a while (a slot lasts several times as long)
+        if (!__any_sync(0xffffffffu, more && free)) __nanosleep(64);
         if (more && free)
         {
             const int kept = min(granules, (part.item.keys - key + p.granule - 1) / p.granule); // granules with keys
@@ -674,11 +568,12 @@ __device__ __forceinline__ void stream_produce(const AttendArgs &p, const Plan &
     if (bad) report_range(p.a.batch.error_flag);
 }
 
-template <class T, int D>
-__device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const Ring<T, D> &ring)
+template <int D>
+__device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const Ring<__nv_bfloat16, D> &ring)
 {
+    using T = __nv_bfloat16;
     using L = Layout<T, D>;
-    using R = Rows16<T, D>;
+    using R = Rows16<D>;
     const List &l = p.list[plan.which];
     const int worker = threadIdx.x / 32 - 4, lane = threadIdx.x & 31, r0 = lane >> 2, r1 = r0 + 8;
     Walk w = walk_of(p, plan, shared, worker);
@@ -782,6 +677,215 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
         {
             if (r0 < rows) *reinterpret_cast<float2 *>(dst + r0 * D + 8 * i) = make_float2(o[i][0], o[i][1]);
             if (r1 < rows) *reinterpret_cast<float2 *>(dst + r1 * D + 8 * i) = make_float2(o[i][2], o[i][3]);
+        }
+    }
+}
+
+// FP32: R rows of a warp, in two halves of 16 lanes; a lane holds every sixteenth group of four dims of the
+// queries and values of its half's rows, two rows to a packed FMA. A step takes four keys: partial scores of
+// all rows, then a scatter of their sums over the 16 lanes (key lane/4 % 4 and a quarter of the rows each),
+// the weights there, and their way back by shuffles. Shared memory and shuffles deliver a value per lane and
+// cycle, so a value of K or V has to serve many rows: with eight rows to a lane a slot of eight keys takes
+// about 250 of those cycles, below its 350 cycles of the memory's rate (one row to a lane: 1024).
+template <int D, int R>
+__device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const Ring<float, D> &ring)
+{
+    using L = Layout<float, D>;
+    constexpr int kSlotKeys = L::kSlotKeys, kKeys = 4, kRows = R / 2, kPairs = kRows / 2, kGroups = D / 64, kDims = 4 * kGroups;
+    constexpr int kHeld = kRows >= 4 ? kRows / 4 : 1; // rows whose weights a lane works out
+    const List &l = p.list[plan.which];
+    const int worker = threadIdx.x / 32 - 4, lane = threadIdx.x & 31, half = lane & 16, share = lane & 15, first_row = half ? kRows : 0;
+    const int my_key = share >> 2, my_row = kRows >= 4 ? (share & 3) * kHeld : (share >> 1) & 1;
+    // the lane of key 0 that holds a row
+    auto holder = [&](int row) { return half + (kRows >= 4 ? row / kHeld : row * 2); };
+    Walk w = walk_of(p, plan, shared, worker);
+    unsigned n = 0; // slots so far
+    Part part;
+    while (next_part(p, plan.which, w, part))
+    {
+        if (lane == 0) write_meta(l, w, part);
+        float2 q[kPairs][kDims], o[kPairs][kDims];
+        int all_see = INT_MAX;
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+        {
+            const Row row = row_of(p, plan.which, part, first_row + i);
+            const float4 *query = reinterpret_cast<const float4 *>(static_cast<const float *>(p.a.q) + static_cast<size_t>(row.query) * D) + share;
+            if (row.keys) all_see = min(all_see, row.keys);
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j)
+            {
+                const float4 x = row.keys ? query[j * 16] : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) (i & 1 ? q[i / 2][4 * j + e].y : q[i / 2][4 * j + e].x) = y[e];
+            }
+        }
+        all_see = __reduce_min_sync(0xffffffffu, all_see);
+        int seen[kHeld];
+        float m[kHeld], c[kHeld], sum[kHeld];
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+        {
+            seen[i] = row_of(p, plan.which, part, first_row + my_row + i).keys;
+            m[i] = -INFINITY;
+            c[i] = sum[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i)
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) o[i][d] = make_float2(0.f, 0.f);
+        const int slots = slots_of<float, D>(part, l.unit_shift);
+        int key0 = part.first_unit << l.unit_shift;
+        for (int u = 0; u < slots; ++u, ++n)
+        {
+            if (!warp_wait(ring.full(worker, n), ring.round(n)))
+            {
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                return;
+            }
+            for (int first = 0; first < kSlotKeys; first += kKeys, key0 += kKeys)
+            {
+                const int valid = part.item.keys - key0; // what lies past the last key may be anything, NaN too
+                if (valid <= 0) continue;
+                const uint32_t k = ring.slot(worker, n), v = k + L::kSlotHalf;
+                // dims 64 j + 4 share .. + 3 of the step's key i: column block, then the key's row, swizzled
+                auto at = [&](int j, int i) {
+                    const int chunk = 16 * j + share, key = first + i;
+                    return (chunk >> 3) * (kSlotKeys * 128) + key * 128 + (((chunk & 7) ^ key) << 4);
+                };
+                float2 s2[kKeys][kPairs];
+#pragma unroll
+                for (int i = 0; i < kKeys; ++i)
+                {
+#pragma unroll
+                    for (int r = 0; r < kPairs; ++r) s2[i][r] = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int j = 0; j < kGroups; ++j)
+                    {
+                        const float4 x = ld_shared_v4(k + at(j, i));
+                        const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int r = 0; r < kPairs; ++r) s2[i][r] = __ffma2_rn(q[r][4 * j + e], make_float2(y[e], y[e]), s2[i][r]);
+                    }
+                }
+                // sums over the half's lanes, scattered: value i * kRows + row
+                float s[kKeys * kRows];
+#pragma unroll
+                for (int i = 0; i < kKeys; ++i)
+#pragma unroll
+                    for (int r = 0; r < kPairs; ++r)
+                    {
+                        s[i * kRows + 2 * r] = s2[i][r].x;
+                        s[i * kRows + 2 * r + 1] = s2[i][r].y;
+                    }
+                int values = kKeys * kRows;
+#pragma unroll
+                for (int step = 8; step > 0; step /= 2)
+                {
+                    if (values > 1)
+                    {
+                        values /= 2;
+#pragma unroll
+                        for (int i = 0; i < kKeys * kRows / 2; ++i)
+                        {
+                            if (i >= values) break;
+                            const float low = s[i], high = s[i + values];
+                            const bool upper = (share & step) != 0;
+                            s[i] = (upper ? high : low) + __shfl_xor_sync(0xffffffffu, upper ? low : high, step);
+                        }
+                    }
+                    else
+                        s[0] += __shfl_xor_sync(0xffffffffu, s[0], step);
+                }
+                if (key0 + kKeys > all_see)
+                {
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i)
+                        if (key0 + my_key >= seen[i]) s[i] = -INFINITY;
+                }
+                bool raise = false;
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) raise |= (s[i] - m[i]) * p.scale > 8.f;
+                // the maximum is raised only when a score passes it by 2^8, as for BF16
+                if (__any_sync(0xffffffffu, raise))
+                {
+                    float f[kHeld];
+#pragma unroll
+                    for (int i = 0; i < kHeld; ++i)
+                    {
+                        float top = fmaxf(s[i], __shfl_xor_sync(0xffffffffu, s[i], 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, m[i]);
+                        f[i] = top == m[i] ? 1.f : exp2_fast((m[i] - top) * p.scale);
+                        m[i] = top;
+                        c[i] = top == -INFINITY ? 0.f : -top * p.scale;
+                        sum[i] *= f[i];
+                    }
+#pragma unroll
+                    for (int r = 0; r < kPairs; ++r)
+                    {
+                        const float f0 = __shfl_sync(0xffffffffu, f[2 * r % kHeld], holder(2 * r));
+                        const float f1 = __shfl_sync(0xffffffffu, f[(2 * r + 1) % kHeld], holder(2 * r + 1));
+#pragma unroll
+                        for (int d = 0; d < kDims; ++d) o[r][d] = make_float2(o[r][d].x * f0, o[r][d].y * f1);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i)
+                {
+                    s[i] = exp2_fast(fmaf(s[i], p.scale, c[i]));
+                    sum[i] += s[i];
+                }
+#pragma unroll
+                for (int i = 0; i < kKeys; ++i)
+                {
+                    float2 weight[kPairs];
+#pragma unroll
+                    for (int r = 0; r < kPairs; ++r)
+                    {
+                        weight[r].x = __shfl_sync(0xffffffffu, s[2 * r % kHeld], holder(2 * r) + 4 * i);
+                        weight[r].y = __shfl_sync(0xffffffffu, s[(2 * r + 1) % kHeld], holder(2 * r + 1) + 4 * i);
+                    }
+                    if (i >= valid) break;
+#pragma unroll
+                    for (int j = 0; j < kGroups; ++j)
+                    {
+                        const float4 x = ld_shared_v4(v + at(j, i));
+                        const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+#pragma unroll
+                            for (int r = 0; r < kPairs; ++r) o[r][4 * j + e] = __ffma2_rn(weight[r], make_float2(y[e], y[e]), o[r][4 * j + e]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ring.empty(worker, n));
+        }
+        const int rows = min(l.block, l.rows - part.block * l.block); // of the item
+        const size_t place = static_cast<size_t>(part.place) * l.part_rows;
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+        {
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 4);
+            sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 8);
+            const int row = first_row + my_row + i;
+            if (my_key == 0 && lane == holder(my_row) && row < rows) l.ml[place + row] = make_float2(m[i] * p.scale, sum[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+        {
+            if (first_row + i >= rows) break;
+            float4 *dst = reinterpret_cast<float4 *>(l.o + (place + first_row + i) * D) + share;
+#pragma unroll
+            for (int j = 0; j < kGroups; ++j)
+            {
+                const float2 *x = &o[i / 2][4 * j];
+                dst[j * 16] = i & 1 ? make_float4(x[0].y, x[1].y, x[2].y, x[3].y) : make_float4(x[0].x, x[1].x, x[2].x, x[3].x);
+            }
         }
     }
 }
@@ -1183,7 +1287,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 return;
             }
         }
-        stream_work<T, D>(p, plan, shared, ring);
+        if constexpr (sizeof(T) == 2) stream_work<D>(p, plan, shared, ring);
+        else
+        {
+            const int rows = p.list[plan.which].part_rows;
+            if (rows > 8) stream_work_f32<D, 16>(p, plan, shared, ring);
+            else if (rows > 4) stream_work_f32<D, 8>(p, plan, shared, ring);
+            else stream_work_f32<D, 4>(p, plan, shared, ring);
+        }
     }
 }
 
@@ -1332,7 +1443,7 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
         l.unit_shift = l.tile ? 7 : 5;
         // nanoseconds of an SM: a tile's unit with one and with two tiles of rows; a streamed unit as fast as an SM
         // takes them when the memory is not the limit
-        l.cost = l.tile ? (l.rows > kTile ? 1900 : 1100) : kv.bf16 ? 180 * kv.dim / 128 : 800 * kv.dim / 128;
+        l.cost = l.tile ? (l.rows > kTile ? 1900 : 1100) : (kv.bf16 ? 180 : l.rows > 8 ? 850 : l.rows > 4 ? 500 : 350) * kv.dim / 128;
         l.lead = l.tile ? (l.rows > kTile ? 4 : 6) : 3;
         const size_t items = static_cast<size_t>(l.owners) * l.blocks * kv.kv_heads;
         const size_t parts = l.owners ? items + ctas * (l.tile ? 1 : kWorkers) : 0;
