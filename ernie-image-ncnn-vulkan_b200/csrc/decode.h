@@ -3,6 +3,7 @@
 // its bound before it is followed; a bad one records kErrPagedRange in the context's status word.
 #pragma once
 #include "kernels.h"
+#include <utility>
 
 namespace ernie_b200
 {
@@ -25,6 +26,23 @@ struct PagedBatch
 };
 
 #ifdef __CUDACC__
+// A kernel that waits for the one before it by itself (griddepcontrol.wait), so that its launch and set-up
+// overlap that one's end.
+template <class... Params, class... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, Args &&...args)
+{
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 __device__ __forceinline__ void report_range(int *flag)
 {
     if (flag) atomicExch(flag, kErrPagedRange);
@@ -87,7 +105,7 @@ struct AppendArgs
     int rope_rows = 0;
     void *q_out = nullptr;
 };
-int launch_paged_append(const AppendArgs &args, cudaStream_t stream);
+int launch_paged_append(const AppendArgs &args, int sms, cudaStream_t stream);
 
 struct ReorderArgs
 {

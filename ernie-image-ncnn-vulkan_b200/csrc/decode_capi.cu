@@ -37,7 +37,7 @@ int check_kv(const ernie_cuda_paged_kv *kv, int layer, PagedLayer &out)
     if (shift < 3 || kv->page_size != 1 << shift)
         return fail(ERNIE_CUDA_ERROR, "Page size must be 8, 16, 32, 64 or 128");
     if (kv->head_dim != 64 && kv->head_dim != 128) return fail(ERNIE_CUDA_ERROR, "Head dimension must be 64 or 128");
-    if (kv->layers < 1 || kv->pages < 1 || kv->kv_heads < 1 || kv->kv_heads > kMaxHeads ||
+    if (kv->layers < 1 || kv->layers > 65536 || kv->pages < 1 || kv->kv_heads < 1 || kv->kv_heads > kMaxHeads ||
         ((static_cast<long long>(kv->pages) * kv->kv_heads) << shift) > INT32_MAX)
         return fail(ERNIE_CUDA_ERROR, "Invalid paged cache shape");
     if (layer < 0 || layer >= kv->layers) return fail(ERNIE_CUDA_ERROR, "Layer outside the paged cache");
@@ -144,7 +144,7 @@ extern "C" int ernie_cuda_paged_append(ernie_cuda_context *ctx, const ernie_cuda
     a.q_out = q_out;
     a.batch.error_flag = ctx->error_flag;
     DeviceGuard guard(ctx->device);
-    return from_launch(launch_paged_append(a, ctx->stream), "Paged append");
+    return from_launch(launch_paged_append(a, ctx->num_sms, ctx->stream), "Paged append");
 }
 
 extern "C" int ernie_cuda_prefix_attention_workspace(ernie_cuda_context *ctx, const ernie_cuda_paged_kv *kv,

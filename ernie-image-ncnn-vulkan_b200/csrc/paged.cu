@@ -1,6 +1,7 @@
 // The paged K/V cache of batched decoding: new tokens' keys and values rotated into their pages, and the
 // cached state of beams rearranged after a selection.
 #include "decode.h"
+#include "ptx.cuh"
 
 namespace ernie_b200
 {
@@ -9,60 +10,139 @@ namespace
 template <class T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <class T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// One CTA per slot (a token, or nothing), one thread per pair (d, d + dim/2) of a head.
-template <class In, class Out> __global__ void append_kernel(AppendArgs a)
+// Four or eight consecutive values in FP32.
+template <class T, int N> __device__ __forceinline__ void load_values(const T *p, bool vectors, float (&v)[N])
 {
+    if (!vectors)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = to_float(p[i]);
+    }
+    else if constexpr (sizeof(T) == 4)
+    {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+        {
+            const float4 x = __ldcs(reinterpret_cast<const float4 *>(p + i));
+            v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+        }
+    }
+    else
+    {
+        static_assert(sizeof(T) == 4 || N == 8, "a 16-byte vector");
+        const uint4 x = __ldcs(reinterpret_cast<const uint4 *>(p));
+        const unsigned w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i)
+        {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+}
+
+template <int N> __device__ __forceinline__ void store_values(float *p, const float (&v)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+}
+template <int N> __device__ __forceinline__ void store_values(__nv_bfloat16 *p, const float (&v)[N])
+{
+    unsigned w[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+    {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const unsigned *>(&x);
+    }
+    if constexpr (N == 8) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    else *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+}
+
+constexpr int kAppendThreads = 256;
+
+// A CTA per slot (a token, or nothing) and share of its heads. A thread holds N dims of a head's lower half
+// and their partners in the upper one (16 bytes of the projection each) of every head of its row of threads,
+// with one read of their cos and sin; the first heads' loads are issued before the token's place is known.
+// The bound is the traffic: projection in, queries, keys and values out.
+template <class In, class Out, int D> __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a, int vectors)
+{
+    constexpr int N = sizeof(In) == 2 ? 8 : 4, kHalf = D / 2, kLanes = kHalf / N, kHeads = kAppendThreads / kLanes;
+    constexpr int kAhead = 3; // heads of a thread whose loads are in flight together
+    grid_dependency_wait();
+    grid_dependents_launch();
     const int slot = blockIdx.x, s = slot / a.batch.queries, i = slot - s * a.batch.queries;
+    const int d = (threadIdx.x % kLanes) * N, first = blockIdx.y * kHeads + threadIdx.x / kLanes, step = gridDim.y * kHeads;
+    const int rotated = a.heads + a.kv.kv_heads, width = rotated + a.kv.kv_heads;
+    const In *x = static_cast<const In *>(a.qkv) + static_cast<size_t>(slot) * a.ld + d;
+    float lo[kAhead][N], hi[kAhead][N];
+    auto fetch = [&](int head) {
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t)
+        {
+            if (head + t * step >= width) break;
+            load_values<In, N>(x + (head + t * step) * D, vectors, lo[t]);
+            load_values<In, N>(x + (head + t * step) * D + kHalf, vectors, hi[t]);
+        }
+    };
+    if (first < width) fetch(first);
     const SequenceView view = sequence_view(a.batch, a.kv.page_shift, s);
     if (i >= view.count) return;
     const int place = view.len - view.count + i; // in the sequence's own pages
-    const long long position = static_cast<long long>(view.prefix_len) + place;
+    const int position = view.prefix_len + place;
     if (position < 0 || position >= a.rope_rows)
     {
         report_range(a.batch.error_flag);
         return;
     }
-    const int dim = a.kv.dim, half = dim / 2;
-    int page = -1;
-    if (place >= 0)
+    int page = place >= 0 ? a.batch.tables[static_cast<size_t>(s) * a.batch.max_pages + (place >> a.kv.page_shift)] : -1;
+    float cos_lo[N], cos_hi[N], sin_lo[N], sin_hi[N];
+    const size_t angle = static_cast<size_t>(position) * D + d;
+#pragma unroll
+    for (int e = 0; e < N; e += 4)
     {
-        page = a.batch.tables[static_cast<size_t>(s) * a.batch.max_pages + (place >> a.kv.page_shift)];
-        if (page < 0 || page >= a.kv.pages)
-        {
-            report_range(a.batch.error_flag);
-            page = -1;
-        }
+        *reinterpret_cast<float4 *>(cos_lo + e) = *reinterpret_cast<const float4 *>(a.cos + angle + e);
+        *reinterpret_cast<float4 *>(cos_hi + e) = *reinterpret_cast<const float4 *>(a.cos + angle + kHalf + e);
+        *reinterpret_cast<float4 *>(sin_lo + e) = *reinterpret_cast<const float4 *>(a.sin + angle + e);
+        *reinterpret_cast<float4 *>(sin_hi + e) = *reinterpret_cast<const float4 *>(a.sin + angle + kHalf + e);
     }
-    const In *x = static_cast<const In *>(a.qkv) + static_cast<size_t>(slot) * a.ld;
-    const float *c = a.cos + position * dim, *sn = a.sin + position * dim;
-    const int width = a.heads + 2 * a.kv.kv_heads;
-    for (int t = threadIdx.x; t < width * half; t += blockDim.x)
+    if (place >= 0 && (page < 0 || page >= a.kv.pages))
     {
-        const int head = t / half, d = t - head * half;
-        float lo = to_float(x[head * dim + d]), hi = to_float(x[head * dim + d + half]);
-        if (head < a.heads + a.kv.kv_heads)
+        report_range(a.batch.error_flag);
+        page = -1;
+    }
+    for (int head = first; head < width; head += kAhead * step)
+    {
+        if (head != first) fetch(head);
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t)
         {
-            const float first = lo, second = hi;
-            lo = __fsub_rn(__fmul_rn(first, c[d]), __fmul_rn(second, sn[d]));
-            hi = __fadd_rn(__fmul_rn(second, c[d + half]), __fmul_rn(first, sn[d + half]));
+            const int h = head + t * step;
+            if (h >= width) break;
+            if (h < rotated)
+            {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                {
+                    const float low = lo[t][e], high = hi[t][e];
+                    lo[t][e] = __fsub_rn(__fmul_rn(low, cos_lo[e]), __fmul_rn(high, sin_lo[e]));
+                    hi[t][e] = __fadd_rn(__fmul_rn(high, cos_hi[e]), __fmul_rn(low, sin_hi[e]));
+                }
+            }
+            Out *dst;
+            if (h < a.heads) dst = static_cast<Out *>(a.q_out) + (static_cast<size_t>(slot) * a.heads + h) * D;
+            else
+            {
+                if (page < 0) continue;
+                const int kv_head = h - (h < rotated ? a.heads : rotated);
+                const size_t row = ((static_cast<size_t>(page) * a.kv.kv_heads + kv_head) << a.kv.page_shift) +
+                                   (place & ((1 << a.kv.page_shift) - 1));
+                dst = static_cast<Out *>(h < rotated ? a.kv.k : a.kv.v) + row * D;
+            }
+            store_values<N>(dst + d, lo[t]);
+            store_values<N>(dst + d + kHalf, hi[t]);
         }
-        Out *dst;
-        if (head < a.heads) dst = static_cast<Out *>(a.q_out) + (static_cast<size_t>(slot) * a.heads + head) * dim;
-        else
-        {
-            if (page < 0) continue;
-            const bool key = head < a.heads + a.kv.kv_heads;
-            const int kv_head = head - a.heads - (key ? 0 : a.kv.kv_heads);
-            const size_t row = ((static_cast<size_t>(page) * a.kv.kv_heads + kv_head) << a.kv.page_shift) +
-                               (place & ((1 << a.kv.page_shift) - 1));
-            dst = static_cast<Out *>(key ? a.kv.k : a.kv.v) + row * dim;
-        }
-        dst[d] = from_float<Out>(lo);
-        dst[d + half] = from_float<Out>(hi);
     }
 }
 
@@ -107,72 +187,124 @@ __device__ __forceinline__ void group_moves(const int *parents, int beams, int *
     }
 }
 
-// grid (groups, y): the CTAs of a group share its copies; each works out the moves for itself.
-__global__ void reorder_kernel(ReorderArgs a, int element_bytes)
+constexpr int kCopyWarps = 8, kCopyAhead = 8; // 16-byte loads of a lane in flight
+
+// A warp's copy of `vectors` 16-byte vectors of K and V.
+__device__ __forceinline__ void copy_rows(const uint4 *k_from, uint4 *k_into, const uint4 *v_from, uint4 *v_into, int vectors, int lane)
+{
+    for (int at = lane; at < vectors; at += 32 * kCopyAhead / 2)
+    {
+        uint4 k[kCopyAhead / 2], v[kCopyAhead / 2];
+#pragma unroll
+        for (int i = 0; i < kCopyAhead / 2; ++i)
+            if (at + 32 * i < vectors)
+            {
+                k[i] = __ldcs(k_from + at + 32 * i);
+                v[i] = __ldcs(v_from + at + 32 * i);
+            }
+#pragma unroll
+        for (int i = 0; i < kCopyAhead / 2; ++i)
+            if (at + 32 * i < vectors)
+            {
+                __stcs(k_into + at + 32 * i, k[i]);
+                __stcs(v_into + at + 32 * i, v[i]);
+            }
+    }
+}
+
+// grid (groups, y): the warps of a group's CTAs share its copies, a layer's head of a page at a time; each CTA
+// works out the moves for itself, the first one writes the new rows. Sources are pages that pass to an heir,
+// targets those of childless places, so no page is both and the copies need no order.
+__global__ void __launch_bounds__(kCopyWarps * 32) reorder_kernel(const __grid_constant__ ReorderArgs a, int element_shift)
 {
     __shared__ GroupMoves m;
-    const int group = blockIdx.x;
+    __shared__ int lens[kMaxBeams], first_page[kMaxBeams + 1]; // of the copied places' pages, one after the other
+    grid_dependency_wait();
+    grid_dependents_launch();
+    const int group = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const size_t base = static_cast<size_t>(group) * a.beams;
-    if (threadIdx.x < 32) group_moves(a.parents + base, a.beams, a.error_flag, m);
-    __syncthreads();
-    const size_t layer_bytes = a.kv.layer_elements() * element_bytes;
-    const size_t row_bytes = static_cast<size_t>(a.kv.dim) * element_bytes;
-    const size_t head_bytes = row_bytes << a.kv.page_shift;
     const int page_size = 1 << a.kv.page_shift;
-    for (int i = 0; i < a.beams; ++i)
+    if (warp == 0)
     {
-        const int p = m.parent[i];
-        const int len = p < 0 ? 0 : clamped_length(a.lens[base + p], a.max_pages, a.kv.page_shift, a.error_flag);
-        if (blockIdx.y == 0)
+        group_moves(a.parents + base, a.beams, a.error_flag, m);
+        __syncwarp();
+        int len = 0, pages = 0;
+        if (lane < a.beams)
         {
-            const int *row = a.tables + (base + m.takes[i]) * a.max_pages;
-            for (int t = threadIdx.x; t < a.max_pages; t += blockDim.x) a.new_tables[(base + i) * a.max_pages + t] = row[t];
-            if (threadIdx.x == 0) a.new_lens[base + i] = len;
+            const int p = m.parent[lane];
+            if (p >= 0) len = clamped_length(a.lens[base + p], a.max_pages, a.kv.page_shift, a.error_flag);
+            if (m.copies[lane]) pages = (len + page_size - 1) >> a.kv.page_shift;
         }
-        if (!m.copies[i]) continue;
-        const int *from = a.tables + (base + p) * a.max_pages, *into = a.tables + (base + m.takes[i]) * a.max_pages;
-        const int pages = (len + page_size - 1) >> a.kv.page_shift;
-        for (int u = blockIdx.y; u < pages * a.layers; u += gridDim.y)
+        lens[lane] = len;
+        int scan = pages;
+#pragma unroll
+        for (int step = 1; step < 32; step *= 2)
         {
-            const int layer = u / pages, t = u - layer * pages;
-            const int source = from[t], target = into[t];
-            if (source < 0 || source >= a.kv.pages || target < 0 || target >= a.kv.pages)
-            {
-                report_range(a.error_flag);
-                continue;
-            }
-            const int tokens = min(page_size, len - (t << a.kv.page_shift));
-            const int vectors = static_cast<int>(tokens * row_bytes / 16);
-            for (int w = threadIdx.x; w < vectors * a.kv.kv_heads; w += blockDim.x)
-            {
-                const int head = w / vectors, at = w - head * vectors;
-                const size_t src = layer * layer_bytes + (static_cast<size_t>(source) * a.kv.kv_heads + head) * head_bytes + at * 16;
-                const size_t dst = layer * layer_bytes + (static_cast<size_t>(target) * a.kv.kv_heads + head) * head_bytes + at * 16;
-                *reinterpret_cast<uint4 *>(static_cast<char *>(a.kv.k) + dst) = *reinterpret_cast<const uint4 *>(static_cast<const char *>(a.kv.k) + src);
-                *reinterpret_cast<uint4 *>(static_cast<char *>(a.kv.v) + dst) = *reinterpret_cast<const uint4 *>(static_cast<const char *>(a.kv.v) + src);
-            }
+            const int other = __shfl_up_sync(0xffffffffu, scan, step);
+            if (lane >= step) scan += other;
         }
+        first_page[lane + 1] = scan;
+        if (lane == 0) first_page[0] = 0;
     }
+    __syncthreads();
+    if (blockIdx.y == 0)
+    {
+        for (int t = threadIdx.x; t < a.beams * a.max_pages; t += blockDim.x)
+        {
+            const int i = t / a.max_pages;
+            a.new_tables[base * a.max_pages + t] = a.tables[(base + m.takes[i]) * a.max_pages + t - i * a.max_pages];
+        }
+        if (threadIdx.x < a.beams) a.new_lens[base + threadIdx.x] = lens[threadIdx.x];
+    }
+    const int pages = first_page[kMaxBeams], stride = gridDim.y * kCopyWarps;
+    const size_t row_vectors = (static_cast<size_t>(a.kv.dim) << element_shift) / 16, head_vectors = row_vectors << a.kv.page_shift;
+    const size_t layer_vectors = head_vectors * a.kv.kv_heads * a.kv.pages;
+    // a step copies page t of the copies for head h of all the layers' heads
+    if (pages == 0) return;
+    const int heads = a.kv.kv_heads * a.layers, begin = blockIdx.y * kCopyWarps + warp, more_h = stride / pages, more_t = stride - more_h * pages;
+    for (int h = begin / pages, t = begin - h * pages; h < heads; h += more_h + (t + more_t >= pages), t += more_t - (t + more_t >= pages ? pages : 0))
+    {
+        const int layer = h / a.kv.kv_heads, head = h - layer * a.kv.kv_heads;
+        const int i = __popc(__ballot_sync(0xffffffffu, first_page[lane + 1] <= t)); // the place that page belongs to
+        const int page = t - first_page[i];
+        const int source = a.tables[(base + m.parent[i]) * a.max_pages + page], target = a.tables[(base + m.takes[i]) * a.max_pages + page];
+        if (source < 0 || source >= a.kv.pages || target < 0 || target >= a.kv.pages)
+        {
+            if (lane == 0) report_range(a.error_flag);
+            continue;
+        }
+        const int vectors = min(page_size, lens[i] - (page << a.kv.page_shift)) * static_cast<int>(row_vectors);
+        const size_t from = layer * layer_vectors + (static_cast<size_t>(source) * a.kv.kv_heads + head) * head_vectors;
+        const size_t into = layer * layer_vectors + (static_cast<size_t>(target) * a.kv.kv_heads + head) * head_vectors;
+        copy_rows(static_cast<const uint4 *>(a.kv.k) + from, static_cast<uint4 *>(a.kv.k) + into, static_cast<const uint4 *>(a.kv.v) + from,
+                  static_cast<uint4 *>(a.kv.v) + into, vectors, lane);
+    }
+}
+
+template <class In, class Out> int launch_append(const AppendArgs &a, int sms, cudaStream_t stream)
+{
+    constexpr int kValues = sizeof(In) == 2 ? 8 : 4;
+    const int slots = a.batch.sequences * a.batch.queries, width = a.heads + 2 * a.kv.kv_heads;
+    const int at_once = kAppendThreads / (a.kv.dim / 2 / kValues), passes = (width + at_once - 1) / at_once;
+    // few slots: their heads over several CTAs (one decode step of five beams: three CTAs a slot)
+    const int share = slots >= 2 * sms ? 1 : passes < 64 ? passes : 64;
+    const int vectors = reinterpret_cast<uintptr_t>(a.qkv) % 16 == 0 && a.ld % (16 / static_cast<int>(sizeof(In))) == 0;
+    const dim3 grid(slots, share);
+    if (a.kv.dim == 64) return launch_dependent(append_kernel<In, Out, 64>, grid, kAppendThreads, stream, a, vectors);
+    return launch_dependent(append_kernel<In, Out, 128>, grid, kAppendThreads, stream, a, vectors);
 }
 } // namespace
 
-int launch_paged_append(const AppendArgs &a, cudaStream_t stream)
+int launch_paged_append(const AppendArgs &a, int sms, cudaStream_t stream)
 {
-    const int slots = a.batch.sequences * a.batch.queries;
-    if (a.qkv_bf16)
-    {
-        if (a.kv.bf16) append_kernel<__nv_bfloat16, __nv_bfloat16><<<slots, 256, 0, stream>>>(a);
-        else append_kernel<__nv_bfloat16, float><<<slots, 256, 0, stream>>>(a);
-    }
-    else if (a.kv.bf16) append_kernel<float, __nv_bfloat16><<<slots, 256, 0, stream>>>(a);
-    else append_kernel<float, float><<<slots, 256, 0, stream>>>(a);
-    return cudaGetLastError();
+    if (a.qkv_bf16) return a.kv.bf16 ? launch_append<__nv_bfloat16, __nv_bfloat16>(a, sms, stream) : launch_append<__nv_bfloat16, float>(a, sms, stream);
+    return a.kv.bf16 ? launch_append<float, __nv_bfloat16>(a, sms, stream) : launch_append<float, float>(a, sms, stream);
 }
 
 int launch_beam_reorder(const ReorderArgs &a, int sms, cudaStream_t stream)
 {
-    const int share = (sms * 4 + a.groups - 1) / a.groups;
-    reorder_kernel<<<dim3(a.groups, share), 256, 0, stream>>>(a, a.kv.bf16 ? 2 : 4);
-    return cudaGetLastError();
+    // eight CTAs of eight warps per SM, shared by the groups
+    const int share = (sms * 8 + a.groups - 1) / a.groups;
+    return launch_dependent(reorder_kernel, dim3(a.groups, share), kCopyWarps * 32, stream, a, a.kv.bf16 ? 1 : 2);
 }
 } // namespace ernie_b200
