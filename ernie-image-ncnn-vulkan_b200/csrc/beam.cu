@@ -1,52 +1,57 @@
 // Beam selection: of each group's beams x vocabulary continuations the best `beams`, by
 // score + logit - log sum exp(logits).
 //
-// The logits are read once. Within a row the order of the totals is the order of the logits, so a CTA that
-// owns a stretch of a row needs only the stretch's maximum m, its sum of exp(x - m) and its `beams` largest
-// logits; a second kernel joins the stretches of each row (lse = m + log sum s_c exp(m_c - m), in 64 bits)
-// and merges the rows' sorted lists. The bound is the logits' traffic: a thread holds 32 logits of a tile and
-// has the next tile's loads in flight meanwhile, keeps its own maximum and sum, and the CTA's threads meet
-// once per tile to ask whether any logit beats the list, which after the first tile is rare.
+// The logits are read once. Within a row the order of the totals is the order of the logits, so whoever owns a
+// stretch of a row needs only the sum of its exponentials and its `beams` largest logits. A stretch belongs to
+// a warp, which never waits for another one: a lane holds eight 16-byte vectors of a tile and has the next
+// tile's in flight meanwhile (the bound is the logits' traffic), keeps its own reference and sum, and the
+// warp's list of the best lies sorted across its lanes, one each. Of a tile only what beats the list's last
+// entry is looked at one by one, which after a few tiles is rare. (Eight warps with one list met several times
+// a tile and took 157 us for 64 x 8 rows of 131072 logits; warps by themselves: see below.)
+// A second kernel joins the stretches of each row and merges the rows' lists.
+//
+// Sums: a lane's reference is c = x L rounded, for its largest logit x so far and L = log2(e) rounded, and its
+// sum that of 2^(x L - c), one FMA and one exponential each. With S and C joined in 64 bits the logarithm of
+// the row's sum is (C + log2 S) / L: the roundings of c and, to first order, of L cancel.
 #include "decode.h"
 #include "ptx.cuh"
+#include <climits>
 
 namespace ernie_b200
 {
 namespace
 {
-constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kMaxChunks = 64;   // stretches of a row: two lists per lane of the joining warp
+constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int kVectors = 8;        // 16-byte vectors of a tile that a lane holds
+constexpr int kMaxStretches = 64;  // of a row: two lists per lane of the joining warp
 constexpr int kListEntries = 4096; // of a group's lists in the joining CTA's shared memory
-constexpr int kCandidates = 512; // of a tile, before the exact ranking
-constexpr int kTilesAhead = 4;   // tiles of a stretch where there are plenty
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct Plan
 {
-    int per_thread; // logits of a tile that a thread holds
-    int chunks, tiles_per_chunk;
+    int stretches, tiles; // of a row, of a stretch
 };
 
-// Large tiles (8192 logits) when they give every SM two CTAs, smaller ones otherwise; with many tiles a CTA
-// takes four in a row, so that three of four loads are covered by work.
-Plan plan_of(long long rows, int vocab, int beams, int sms)
+// Up to 16 warps per SM work at a time; `skew` logits of a row's first vector may lie before the row.
+Plan plan_of(long long rows, int vocab, int skew, int beams, bool bf16, int sms)
 {
-    Plan p;
-    const long long span = static_cast<long long>(vocab) + 8; // a row may begin inside a vector
-    for (p.per_thread = 32; p.per_thread > 8; p.per_thread /= 2)
-        if (rows * ((span + p.per_thread * kThreads - 1) / (p.per_thread * kThreads)) >= 2 * sms) break;
-    const long long tile = static_cast<long long>(p.per_thread) * kThreads, tiles = (span + tile - 1) / tile;
+    const long long tile = 32 * kVectors * (bf16 ? 8 : 4), tiles = (static_cast<long long>(vocab) + skew + tile - 1) / tile;
     long long most = kListEntries / (beams * beams);
-    most = most < kMaxChunks ? most : kMaxChunks;
-    p.tiles_per_chunk = static_cast<int>((tiles + most - 1) / most);
-    if (p.tiles_per_chunk < kTilesAhead && rows * tiles >= 2ll * sms * 2 * kTilesAhead) p.tiles_per_chunk = kTilesAhead;
-    p.chunks = static_cast<int>((tiles + p.tiles_per_chunk - 1) / p.tiles_per_chunk);
+    if (most > kMaxStretches) most = kMaxStretches;
+    if (most > tiles) most = tiles;
+    // no more stretches than fill the SMs four times over: a stretch's first tiles cost several times a later one's
+    const long long enough = (64ll * sms + rows - 1) / rows;
+    if (most > enough) most = enough;
+    Plan p;
+    p.tiles = static_cast<int>((tiles + most - 1) / most);
+    p.stretches = static_cast<int>((tiles + p.tiles - 1) / p.tiles);
     return p;
 }
 
-// What a stretch leaves behind: [rows][chunks] of each.
+// What a stretch leaves behind: [rows][stretches] of each.
 struct Parts
 {
-    float *top, *sum;  // sum is NaN where the stretch holds a NaN or a +inf
+    float *reference, *sum; // sum is NaN where the stretch holds a NaN or a +inf
     float *value;      // [beams] logits, descending, equal ones by token; -inf past the last
     int *token;
 };
@@ -55,10 +60,10 @@ size_t rounded(size_t bytes) { return (bytes + 15) / 16 * 16; }
 
 Parts parts_of(void *workspace, long long rows, int beams, const Plan &p)
 {
-    const size_t n = static_cast<size_t>(rows) * p.chunks;
+    const size_t n = static_cast<size_t>(rows) * p.stretches;
     char *at = static_cast<char *>(workspace);
     Parts parts;
-    parts.top = reinterpret_cast<float *>(at);
+    parts.reference = reinterpret_cast<float *>(at);
     parts.sum = reinterpret_cast<float *>(at += rounded(n * 4));
     parts.value = reinterpret_cast<float *>(at += rounded(n * 4));
     parts.token = reinterpret_cast<int *>(at += rounded(n * beams * 4));
@@ -73,240 +78,177 @@ __device__ __forceinline__ bool row_offers(const BeamSelectArgs &a, long long ro
     return !a.finished[row] && isfinite(a.scores[row]);
 }
 
+// Sixteen bytes of logits.
 template <class T> struct Vector;
 template <> struct Vector<float>
 {
     static constexpr int kSize = 4;
-    static __device__ __forceinline__ void load(const float *p, float *v)
+    static __device__ __forceinline__ float get(const uint4 &x, int i)
     {
-        const float4 x = __ldcs(reinterpret_cast<const float4 *>(p));
-        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
+        return __uint_as_float(i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w);
     }
-    static __device__ __forceinline__ float one(const float *p) { return *p; }
 };
 template <> struct Vector<__nv_bfloat16>
 {
     static constexpr int kSize = 8;
-    static __device__ __forceinline__ void load(const __nv_bfloat16 *p, float *v)
+    static __device__ __forceinline__ float get(const uint4 &x, int i)
     {
-        const uint4 x = __ldcs(reinterpret_cast<const uint4 *>(p));
-        const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-        {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+        const unsigned w = i < 2 ? x.x : i < 4 ? x.y : i < 6 ? x.z : x.w;
+        return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
     }
-    static __device__ __forceinline__ float one(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 };
 
-// A thread's logits of the tile that starts at `base` (an index of the row, on a 16-byte boundary).
-template <class T, int E> __device__ __forceinline__ void load_tile(const T *x, long long base, int vocab, float (&v)[E])
+// The lane's vectors of the tile that starts at `base` (an index of the row, on a 16-byte boundary); -inf
+// outside the row.
+template <class T> __device__ __forceinline__ void load_tile(const T *x, long long base, int vocab, int lane, uint4 (&v)[kVectors])
 {
     constexpr int V = Vector<T>::kSize;
 #pragma unroll
-    for (int j = 0; j < E / V; ++j)
+    for (int j = 0; j < kVectors; ++j)
     {
-        const long long at = base + static_cast<long long>(j * kThreads + threadIdx.x) * V;
-        if (at >= 0 && at + V <= vocab) Vector<T>::load(x + at, v + j * V);
+        const long long at = base + (j * 32 + lane) * V;
+        if (at >= 0 && at + V <= vocab) v[j] = __ldcs(reinterpret_cast<const uint4 *>(x + at));
         else
+        {
+            unsigned w[4] = {};
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[j * V + e] = at + e >= 0 && at + e < vocab ? Vector<T>::one(x + at + e) : -INFINITY;
+            for (int e = 0; e < V; ++e)
+            {
+                const bool inside = at + e >= 0 && at + e < vocab;
+                if constexpr (V == 4) w[e] = inside ? __float_as_uint(x[at + e]) : 0xff800000u;
+                else w[e / 2] |= (inside ? static_cast<unsigned>(__bfloat16_as_ushort(x[at + e])) : 0xff80u) << (16 * (e & 1));
+            }
+            v[j] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
     }
 }
 
-template <class T, int E> __global__ void __launch_bounds__(kThreads, 2) stretch_kernel(BeamSelectArgs a, Plan plan, Parts parts)
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <class T> __global__ void __launch_bounds__(kThreads, 4) stretch_kernel(const __grid_constant__ BeamSelectArgs a, Plan plan, Parts parts)
 {
     constexpr int V = Vector<T>::kSize;
-    __shared__ float warp_value[kWarps], list_value[kMaxBeams], cand_value[kCandidates];
-    __shared__ float warp_sum[kWarps];
-    __shared__ int list_token[kMaxBeams], cand_token[kCandidates], found;
+    constexpr unsigned full = 0xffffffffu;
     grid_dependency_wait();
     grid_dependents_launch();
-    const long long row = blockIdx.x / plan.chunks;
-    const int chunk = static_cast<int>(blockIdx.x - row * plan.chunks);
-    if (!row_offers(a, row)) return;
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, k = a.beams;
+    const int lane = threadIdx.x % 32, k = a.beams;
+    const long long out = static_cast<long long>(blockIdx.x) * kWarps + threadIdx.x / 32, row = out / plan.stretches;
+    if (row >= static_cast<long long>(a.groups) * k || !row_offers(a, row)) return;
     const T *x = static_cast<const T *>(a.logits) + row * a.ld;
-    // vectors start at 16-byte boundaries: index 0 of the row is element `shift` of the first one
-    const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
-    long long base = static_cast<long long>(chunk) * plan.tiles_per_chunk * (E * kThreads) - shift;
-    const long long end = min(static_cast<long long>(a.vocab), base + static_cast<long long>(plan.tiles_per_chunk) * (E * kThreads));
-    if (tid < kMaxBeams)
+    // vectors start at 16-byte boundaries: index 0 of the row is element `skew` of the first one
+    const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+    constexpr int kTileSize = 32 * kVectors * V;
+    long long base = (out - row * plan.stretches) * plan.tiles * kTileSize - skew;
+    const long long end = min(static_cast<long long>(a.vocab), base + static_cast<long long>(plan.tiles) * kTileSize);
+    float c = -INFINITY, sum = 0.f, top = -INFINITY; // the lane's reference, sum and largest logit
+    float value = -INFINITY, last_value = -INFINITY; // the list: lane i holds the i-th best; its last entry
+    int token = INT_MAX, last_token = INT_MAX;
+    uint4 next[kVectors];
+    if (base < end) load_tile<T>(x, base, a.vocab, lane, next);
+    for (bool first = true; base < end; base += kTileSize, first = false)
     {
-        list_value[tid] = -INFINITY;
-        list_token[tid] = -1;
-    }
-    if (tid == 0) found = 0;
-    auto token_at = [&](int e) { return static_cast<int>(base + static_cast<long long>((e / V) * kThreads + tid) * V + e % V); };
-    float top = -INFINITY, sum = 0.f; // the thread's own
-    bool bad = false;
-    float bound = -INFINITY; // the list's last entry
-    float next[E];
-    load_tile<T, E>(x, base, a.vocab, next);
-    __syncthreads();
-    for (bool first = true; base < end; base += E * kThreads, first = false)
-    {
-        float v[E];
+        uint4 v[kVectors];
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = next[e];
-        if (base + E * kThreads < end) load_tile<T, E>(x, base + E * kThreads, a.vocab, next);
-        float mine = -INFINITY;
+        for (int j = 0; j < kVectors; ++j) v[j] = next[j];
+        if (base + kTileSize < end) load_tile<T>(x, base + kTileSize, a.vocab, lane, next);
+        float mine[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < E; ++e)
+        for (int j = 0; j < kVectors; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) mine[e & 3] = fmaxf(mine[e & 3], Vector<T>::get(v[j], e));
+        const float best = fmaxf(fmaxf(mine[0], mine[1]), fmaxf(mine[2], mine[3]));
+        if (best > top)
         {
-            mine = fmaxf(mine, v[e]);
-            bad |= !(v[e] < INFINITY);
-        }
-        if (mine > top)
-        {
-            sum *= __expf(top - mine); // 0 while nothing has been seen
-            top = mine;
+            const float raised = best * kLog2e;
+            sum *= exp2_fast(c - raised); // 0 while nothing has been seen
+            c = raised;
+            top = best;
         }
         if (top > -INFINITY)
         {
             float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int e = 0; e < E; ++e) s[e & 3] += __expf(v[e] - top);
+            for (int j = 0; j < kVectors; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e) s[e & 3] += exp2_fast(fmaf(Vector<T>::get(v[j], e), kLog2e, -c));
             sum += (s[0] + s[1]) + (s[2] + s[3]);
         }
-        // Later tokens have to beat the list's last one; the first tile finds its own bound: of a warp's lane
-        // maxima in descending order the k-th bounds the warp's k-th largest logit from below.
-        bool wanted = mine > bound;
+        else
+        {
+            // nothing but -inf, or NaN, which the maximum passes over
+#pragma unroll
+            for (int j = 0; j < kVectors; ++j)
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (Vector<T>::get(v[j], e) != Vector<T>::get(v[j], e)) sum = NAN;
+        }
+        // In the first tile the lanes' maxima bound the k-th largest logit from below: the k-th of them, in
+        // descending order. Later tokens have to beat the list's last one.
+        float bound = last_value;
         if (first)
         {
-            float sorted = mine;
+            float sorted = best;
 #pragma unroll
             for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
                 for (int step = size / 2; step > 0; step /= 2)
                 {
-                    const float other = __shfl_xor_sync(0xffffffffu, sorted, step);
+                    const float other = __shfl_xor_sync(full, sorted, step);
                     const bool high = ((lane & step) == 0) == ((lane & size) == 0);
                     sorted = high ? fmaxf(sorted, other) : fminf(sorted, other);
                 }
-            sorted = __shfl_sync(0xffffffffu, sorted, k - 1);
-            if (lane == 0) warp_value[warp] = sorted;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) bound = fmaxf(bound, warp_value[w]);
-            wanted = mine >= bound && mine > -INFINITY;
+            bound = __shfl_sync(full, sorted, k - 1);
         }
-        if (!__syncthreads_or(wanted)) continue;
-        if (wanted)
-        {
+        if (!__any_sync(full, first ? best >= bound && best > -INFINITY : best > bound)) continue;
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if ((first ? v[e] >= bound : v[e] > bound) && v[e] > -INFINITY)
-                {
-                    const int n = atomicAdd(&found, 1);
-                    if (n < kCandidates)
-                    {
-                        cand_value[n] = v[e];
-                        cand_token[n] = token_at(e);
-                    }
-                }
-        }
-        if (!first && tid < k && list_value[tid] > -INFINITY)
-        {
-            const int n = atomicAdd(&found, 1);
-            if (n < kCandidates)
+        for (int j = 0; j < kVectors; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e)
             {
-                cand_value[n] = list_value[tid];
-                cand_token[n] = list_token[tid];
+                const float mine_value = Vector<T>::get(v[j], e);
+                unsigned found = __ballot_sync(full, mine_value >= bound && mine_value > -INFINITY);
+                if (!found) continue;
+                const int mine_token = static_cast<int>(base + (j * 32 + lane) * V + e);
+                found = __ballot_sync(full, mine_value >= bound && mine_value > -INFINITY && better(mine_value, mine_token, last_value, last_token));
+                while (found)
+                {
+                    const int from = __ffs(found) - 1;
+                    found &= found - 1;
+                    const float new_value = __shfl_sync(full, mine_value, from);
+                    const int new_token = __shfl_sync(full, mine_token, from);
+                    // the entries before it are a prefix of the lanes
+                    const int place = __popc(__ballot_sync(full, better(value, token, new_value, new_token)));
+                    const float moved_value = __shfl_up_sync(full, value, 1);
+                    const int moved_token = __shfl_up_sync(full, token, 1);
+                    if (lane == place) value = new_value, token = new_token;
+                    else if (lane > place) value = moved_value, token = moved_token;
+                    last_value = __shfl_sync(full, value, k - 1);
+                    last_token = __shfl_sync(full, token, k - 1);
+                }
+                bound = fmaxf(bound, last_value);
             }
-        }
-        __syncthreads();
-        const int n = found;
-        if (n <= kCandidates)
-        {
-            if (tid < k) list_value[tid] = -INFINITY, list_token[tid] = -1;
-            __syncthreads();
-            for (int c = tid; c < n; c += kThreads)
-            {
-                const float cv = cand_value[c];
-                const int ci = cand_token[c];
-                int rank = 0;
-                for (int o = 0; o < n; ++o) rank += better(cand_value[o], cand_token[o], cv, ci);
-                if (rank < k)
-                {
-                    list_value[rank] = cv;
-                    list_token[rank] = ci;
-                }
-            }
-        }
-        else
-        {
-            // many equal logits at the bound: the list entry by entry, each the best one after the last
-            const float old_value = tid < k ? list_value[tid] : -INFINITY;
-            const int old_token = tid < k ? list_token[tid] : -1;
-            float last_value = INFINITY;
-            int last_token = -1;
-            for (int r = 0; r < k; ++r)
-            {
-                float bv = -INFINITY;
-                int bi = INT32_MAX;
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (better(last_value, last_token, v[e], token_at(e)) && better(v[e], token_at(e), bv, bi)) bv = v[e], bi = token_at(e);
-                if (better(last_value, last_token, old_value, old_token) && better(old_value, old_token, bv, bi) && old_token >= 0)
-                    bv = old_value, bi = old_token;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1)
-                {
-                    const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-                    const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-                    if (better(ov, oi, bv, bi)) bv = ov, bi = oi;
-                }
-                __syncthreads();
-                if (lane == 0)
-                {
-                    cand_value[warp] = bv;
-                    cand_token[warp] = bi;
-                }
-                __syncthreads();
-                for (int w = 0; w < kWarps; ++w)
-                    if (better(cand_value[w], cand_token[w], bv, bi)) bv = cand_value[w], bi = cand_token[w];
-                last_value = bv;
-                last_token = bi;
-                if (tid == 0)
-                {
-                    list_value[r] = bv;
-                    list_token[r] = bv > -INFINITY ? bi : -1;
-                }
-            }
-        }
-        __syncthreads();
-        bound = list_value[k - 1];
-        if (tid == 0) found = 0;
     }
-    // the threads' maxima and sums
-    float most = top;
+    // the lanes' references and sums
+    float reference = c;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if (lane == 0) warp_value[warp] = most;
-    const bool poisoned = __syncthreads_or(bad);
-    most = warp_value[0];
+    for (int o = 16; o > 0; o >>= 1) reference = fmaxf(reference, __shfl_xor_sync(full, reference, o));
+    if (top > -INFINITY) sum *= exp2_fast(c - reference); // (NaN where both are infinite: poisoned)
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) most = fmaxf(most, warp_value[w]);
-    sum = top > -INFINITY ? sum * __expf(top - most) : 0.f;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) warp_sum[warp] = sum;
-    __syncthreads();
-    const size_t out = blockIdx.x;
-    if (tid == 0)
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(full, sum, o);
+    if (lane == 0)
     {
-        float s = 0.f;
-        for (int w = 0; w < kWarps; ++w) s += warp_sum[w];
-        parts.top[out] = most;
-        parts.sum[out] = poisoned ? NAN : s;
+        parts.reference[out] = reference;
+        parts.sum[out] = sum;
     }
-    if (tid < k)
+    if (lane < k)
     {
-        parts.value[out * k + tid] = list_value[tid];
-        parts.token[out * k + tid] = list_token[tid];
+        parts.value[out * k + lane] = value;
+        parts.token[out * k + lane] = token;
     }
 }
 
@@ -346,7 +288,7 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
     else if (offers)
     {
         // the lists into shared memory, the statistics into registers, all at once
-        const int entries = plan.chunks * k;
+        const int entries = plan.stretches * k;
         float *values = entry_value + warp * entries;
         int *tokens = entry_token + warp * entries;
         for (int e = lane; e < entries; e += 32)
@@ -354,28 +296,28 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
             values[e] = parts.value[row * entries + e];
             tokens[e] = parts.token[row * entries + e];
         }
-        float part_top[2], part_sum[2];
+        float part_reference[2], part_sum[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
         {
             const int c = lane + 32 * h;
-            part_top[h] = c < plan.chunks ? parts.top[row * plan.chunks + c] : -INFINITY;
-            part_sum[h] = c < plan.chunks ? parts.sum[row * plan.chunks + c] : 0.f;
+            part_reference[h] = c < plan.stretches ? parts.reference[row * plan.stretches + c] : -INFINITY;
+            part_sum[h] = c < plan.stretches ? parts.sum[row * plan.stretches + c] : 0.f;
         }
         __syncwarp();
-        float top = fmaxf(part_top[0], part_top[1]);
+        float reference = fmaxf(part_reference[0], part_reference[1]);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(full, top, o));
+        for (int o = 16; o > 0; o >>= 1) reference = fmaxf(reference, __shfl_xor_sync(full, reference, o));
         double sum = 0.0;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
         {
             if (part_sum[h] != part_sum[h]) sum = NAN;
-            else if (part_top[h] > -INFINITY) sum += static_cast<double>(part_sum[h]) * exp(static_cast<double>(part_top[h]) - top);
+            else if (part_reference[h] > -INFINITY) sum += static_cast<double>(part_sum[h]) * exp2(static_cast<double>(part_reference[h]) - reference);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(full, sum, o);
-        const double lse = static_cast<double>(top) + log(sum);
+        const double lse = (static_cast<double>(reference) + log2(sum)) / static_cast<double>(kLog2e);
         if (isfinite(lse))
         {
             // lane's lists: stretches lane and lane + 32, each with the place of its next entry
@@ -388,7 +330,7 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
                 for (int h = 0; h < 2; ++h)
                 {
                     const int c = lane + 32 * h;
-                    if (c >= plan.chunks || at[h] >= k) continue;
+                    if (c >= plan.stretches || at[h] >= k) continue;
                     const float v = values[c * k + at[h]];
                     const int i = tokens[c * k + at[h]];
                     if (v > -INFINITY && better(v, i, bv, bi)) bv = v, bi = i, from = h;
@@ -441,30 +383,39 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
     }
 }
 
-template <class T> cudaError_t launch_stretches(const BeamSelectArgs &a, const Plan &p, const Parts &parts, unsigned ctas, cudaStream_t stream)
+size_t parts_bytes(long long rows, int beams, const Plan &p)
 {
-    if (p.per_thread == 32) return launch_dependent(stretch_kernel<T, 32>, ctas, kThreads, stream, a, p, parts);
-    if (p.per_thread == 16) return launch_dependent(stretch_kernel<T, 16>, ctas, kThreads, stream, a, p, parts);
-    return launch_dependent(stretch_kernel<T, 8>, ctas, kThreads, stream, a, p, parts);
+    const size_t n = static_cast<size_t>(rows) * p.stretches;
+    return 2 * rounded(n * 4) + 2 * rounded(n * beams * 4);
 }
 } // namespace
 
 size_t beam_select_workspace(int groups, int beams, int vocab, int sms)
 {
+    // whatever the logits' type and alignment turn out to be
     const long long rows = static_cast<long long>(groups) * beams;
-    const Plan p = plan_of(rows, vocab, beams, sms);
-    const size_t n = static_cast<size_t>(rows) * p.chunks;
-    return 2 * rounded(n * 4) + 2 * rounded(n * beams * 4);
+    size_t most = 0;
+    for (const bool bf16 : {false, true})
+        for (const int skew : {0, bf16 ? 7 : 3})
+        {
+            const size_t bytes = parts_bytes(rows, beams, plan_of(rows, vocab, skew, beams, bf16, sms));
+            if (bytes > most) most = bytes;
+        }
+    return most;
 }
 
 int launch_beam_select(const BeamSelectArgs &a, int sms, cudaStream_t stream)
 {
     const long long rows = static_cast<long long>(a.groups) * a.beams;
-    const Plan p = plan_of(rows, a.vocab, a.beams, sms);
-    if (rows * p.chunks > INT32_MAX) return cudaErrorInvalidValue;
+    const int vector = a.bf16 ? 8 : 4;
+    const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && (rows == 1 || a.ld % vector == 0);
+    const Plan p = plan_of(rows, a.vocab, aligned ? 0 : vector - 1, a.beams, a.bf16, sms);
+    const long long ctas = (rows * p.stretches + kWarps - 1) / kWarps;
+    if (ctas > INT32_MAX) return cudaErrorInvalidValue;
     const Parts parts = parts_of(a.workspace, rows, a.beams, p);
-    const unsigned ctas = static_cast<unsigned>(rows * p.chunks);
-    const cudaError_t e = a.bf16 ? launch_stretches<__nv_bfloat16>(a, p, parts, ctas, stream) : launch_stretches<float>(a, p, parts, ctas, stream);
+    const unsigned grid = static_cast<unsigned>(ctas);
+    const cudaError_t e = a.bf16 ? launch_dependent(stretch_kernel<__nv_bfloat16>, grid, kThreads, stream, a, p, parts)
+                                 : launch_dependent(stretch_kernel<float>, grid, kThreads, stream, a, p, parts);
     if (e != cudaSuccess) return e;
     return launch_dependent(merge_kernel, a.groups, 32 * a.beams, stream, a, p, parts);
 }

@@ -7,83 +7,77 @@ namespace ernie_b200
 {
 namespace
 {
-template <class T> __device__ __forceinline__ float to_float(T v);
-template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-// Four or eight consecutive values in FP32.
-template <class T, int N> __device__ __forceinline__ void load_values(const T *p, bool vectors, float (&v)[N])
+// Four consecutive values, as they come: 16 bytes of FP32, 8 of BF16.
+template <class T> struct Four;
+template <> struct Four<float>
 {
-    if (!vectors)
+    float4 x;
+    __device__ __forceinline__ void load(const float *p, bool vectors)
     {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = to_float(p[i]);
+        if (vectors) x = __ldcs(reinterpret_cast<const float4 *>(p));
+        else x = make_float4(p[0], p[1], p[2], p[3]);
     }
-    else if constexpr (sizeof(T) == 4)
+    __device__ __forceinline__ float4 get() const { return x; }
+};
+template <> struct Four<__nv_bfloat16>
+{
+    uint2 x;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p, bool vectors)
     {
-#pragma unroll
-        for (int i = 0; i < N; i += 4)
-        {
-            const float4 x = __ldcs(reinterpret_cast<const float4 *>(p + i));
-            v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
-        }
+        const unsigned short *q = reinterpret_cast<const unsigned short *>(p);
+        if (vectors) x = __ldcs(reinterpret_cast<const uint2 *>(p));
+        else x = make_uint2(q[0] | static_cast<unsigned>(q[1]) << 16, q[2] | static_cast<unsigned>(q[3]) << 16);
     }
-    else
+    __device__ __forceinline__ float4 get() const
     {
-        static_assert(sizeof(T) == 4 || N == 8, "a 16-byte vector");
-        const uint4 x = __ldcs(reinterpret_cast<const uint4 *>(p));
-        const unsigned w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int i = 0; i < N / 2; ++i)
-        {
-            v[2 * i] = __uint_as_float(w[i] << 16);
-            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
+        return make_float4(__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u), __uint_as_float(x.y << 16), __uint_as_float(x.y & 0xffff0000u));
     }
+};
+
+__device__ __forceinline__ void store_four(float *p, float4 v) { *reinterpret_cast<float4 *>(p) = v; }
+__device__ __forceinline__ void store_four(__nv_bfloat16 *p, float4 v)
+{
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    *reinterpret_cast<uint2 *>(p) = make_uint2(*reinterpret_cast<const unsigned *>(&a), *reinterpret_cast<const unsigned *>(&b));
 }
 
-template <int N> __device__ __forceinline__ void store_values(float *p, const float (&v)[N])
+// x c - y s and y c + x s without contraction
+__device__ __forceinline__ float4 turn_low(float4 x, float4 y, float4 c, float4 s)
 {
-#pragma unroll
-    for (int i = 0; i < N; i += 4) *reinterpret_cast<float4 *>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+    return make_float4(__fsub_rn(__fmul_rn(x.x, c.x), __fmul_rn(y.x, s.x)), __fsub_rn(__fmul_rn(x.y, c.y), __fmul_rn(y.y, s.y)),
+                       __fsub_rn(__fmul_rn(x.z, c.z), __fmul_rn(y.z, s.z)), __fsub_rn(__fmul_rn(x.w, c.w), __fmul_rn(y.w, s.w)));
 }
-template <int N> __device__ __forceinline__ void store_values(__nv_bfloat16 *p, const float (&v)[N])
+__device__ __forceinline__ float4 turn_high(float4 x, float4 y, float4 c, float4 s)
 {
-    unsigned w[N / 2];
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i)
-    {
-        const __nv_bfloat162 x = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const unsigned *>(&x);
-    }
-    if constexpr (N == 8) *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    else *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+    return make_float4(__fadd_rn(__fmul_rn(y.x, c.x), __fmul_rn(x.x, s.x)), __fadd_rn(__fmul_rn(y.y, c.y), __fmul_rn(x.y, s.y)),
+                       __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(x.z, s.z)), __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(x.w, s.w)));
 }
 
 constexpr int kAppendThreads = 256;
 
-// A CTA per slot (a token, or nothing) and share of its heads. A thread holds N dims of a head's lower half
-// and their partners in the upper one (16 bytes of the projection each) of every head of its row of threads,
-// with one read of their cos and sin; the first heads' loads are issued before the token's place is known.
-// The bound is the traffic: projection in, queries, keys and values out.
-template <class In, class Out, int D> __global__ void __launch_bounds__(kAppendThreads) append_kernel(const __grid_constant__ AppendArgs a, int vectors)
+// A CTA per slot (a token, or nothing) and share of its heads. A thread holds four dims of a head's lower half
+// and their partners in the upper one, of every head of its row of threads, with one read of their cos and sin;
+// the first heads' loads are issued before the token's place is known. The bound is the traffic: projection in,
+// queries, keys and values out. (Eight dims to a thread of a BF16 projection: 114 registers, a quarter of the
+// warps, 140 us for 16000 tokens of 48 heads; this way see below.)
+template <class In, class Out, int D> __global__ void __launch_bounds__(kAppendThreads, 4) append_kernel(const __grid_constant__ AppendArgs a, int vectors)
 {
-    constexpr int N = sizeof(In) == 2 ? 8 : 4, kHalf = D / 2, kLanes = kHalf / N, kHeads = kAppendThreads / kLanes;
+    constexpr int kHalf = D / 2, kLanes = kHalf / 4, kHeads = kAppendThreads / kLanes;
     constexpr int kAhead = 3; // heads of a thread whose loads are in flight together
     grid_dependency_wait();
     grid_dependents_launch();
     const int slot = blockIdx.x, s = slot / a.batch.queries, i = slot - s * a.batch.queries;
-    const int d = (threadIdx.x % kLanes) * N, first = blockIdx.y * kHeads + threadIdx.x / kLanes, step = gridDim.y * kHeads;
+    const int d = (threadIdx.x % kLanes) * 4, first = blockIdx.y * kHeads + threadIdx.x / kLanes, step = gridDim.y * kHeads;
     const int rotated = a.heads + a.kv.kv_heads, width = rotated + a.kv.kv_heads;
     const In *x = static_cast<const In *>(a.qkv) + static_cast<size_t>(slot) * a.ld + d;
-    float lo[kAhead][N], hi[kAhead][N];
+    Four<In> lo[kAhead], hi[kAhead];
     auto fetch = [&](int head) {
 #pragma unroll
         for (int t = 0; t < kAhead; ++t)
         {
             if (head + t * step >= width) break;
-            load_values<In, N>(x + (head + t * step) * D, vectors, lo[t]);
-            load_values<In, N>(x + (head + t * step) * D + kHalf, vectors, hi[t]);
+            lo[t].load(x + (head + t * step) * D, vectors);
+            hi[t].load(x + (head + t * step) * D + kHalf, vectors);
         }
     };
     if (first < width) fetch(first);
@@ -97,16 +91,9 @@ template <class In, class Out, int D> __global__ void __launch_bounds__(kAppendT
         return;
     }
     int page = place >= 0 ? a.batch.tables[static_cast<size_t>(s) * a.batch.max_pages + (place >> a.kv.page_shift)] : -1;
-    float cos_lo[N], cos_hi[N], sin_lo[N], sin_hi[N];
-    const size_t angle = static_cast<size_t>(position) * D + d;
-#pragma unroll
-    for (int e = 0; e < N; e += 4)
-    {
-        *reinterpret_cast<float4 *>(cos_lo + e) = *reinterpret_cast<const float4 *>(a.cos + angle + e);
-        *reinterpret_cast<float4 *>(cos_hi + e) = *reinterpret_cast<const float4 *>(a.cos + angle + kHalf + e);
-        *reinterpret_cast<float4 *>(sin_lo + e) = *reinterpret_cast<const float4 *>(a.sin + angle + e);
-        *reinterpret_cast<float4 *>(sin_hi + e) = *reinterpret_cast<const float4 *>(a.sin + angle + kHalf + e);
-    }
+    const float *cos = a.cos + static_cast<size_t>(position) * D + d, *sin = a.sin + static_cast<size_t>(position) * D + d;
+    const float4 cos_lo = *reinterpret_cast<const float4 *>(cos), cos_hi = *reinterpret_cast<const float4 *>(cos + kHalf);
+    const float4 sin_lo = *reinterpret_cast<const float4 *>(sin), sin_hi = *reinterpret_cast<const float4 *>(sin + kHalf);
     if (place >= 0 && (page < 0 || page >= a.kv.pages))
     {
         report_range(a.batch.error_flag);
@@ -120,16 +107,7 @@ template <class In, class Out, int D> __global__ void __launch_bounds__(kAppendT
         {
             const int h = head + t * step;
             if (h >= width) break;
-            if (h < rotated)
-            {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                {
-                    const float low = lo[t][e], high = hi[t][e];
-                    lo[t][e] = __fsub_rn(__fmul_rn(low, cos_lo[e]), __fmul_rn(high, sin_lo[e]));
-                    hi[t][e] = __fadd_rn(__fmul_rn(high, cos_hi[e]), __fmul_rn(low, sin_hi[e]));
-                }
-            }
+            const float4 low = lo[t].get(), high = hi[t].get();
             Out *dst;
             if (h < a.heads) dst = static_cast<Out *>(a.q_out) + (static_cast<size_t>(slot) * a.heads + h) * D;
             else
@@ -140,8 +118,8 @@ template <class In, class Out, int D> __global__ void __launch_bounds__(kAppendT
                                    (place & ((1 << a.kv.page_shift) - 1));
                 dst = static_cast<Out *>(h < rotated ? a.kv.k : a.kv.v) + row * D;
             }
-            store_values<N>(dst + d, lo[t]);
-            store_values<N>(dst + d + kHalf, hi[t]);
+            store_four(dst + d, h < rotated ? turn_low(low, high, cos_lo, sin_lo) : low);
+            store_four(dst + d + kHalf, h < rotated ? turn_high(low, high, cos_hi, sin_hi) : high);
         }
     }
 }
@@ -283,12 +261,11 @@ __global__ void __launch_bounds__(kCopyWarps * 32) reorder_kernel(const __grid_c
 
 template <class In, class Out> int launch_append(const AppendArgs &a, int sms, cudaStream_t stream)
 {
-    constexpr int kValues = sizeof(In) == 2 ? 8 : 4;
     const int slots = a.batch.sequences * a.batch.queries, width = a.heads + 2 * a.kv.kv_heads;
-    const int at_once = kAppendThreads / (a.kv.dim / 2 / kValues), passes = (width + at_once - 1) / at_once;
+    const int at_once = kAppendThreads / (a.kv.dim / 8), passes = (width + at_once - 1) / at_once;
     // few slots: their heads over several CTAs (one decode step of five beams: three CTAs a slot)
     const int share = slots >= 2 * sms ? 1 : passes < 64 ? passes : 64;
-    const int vectors = reinterpret_cast<uintptr_t>(a.qkv) % 16 == 0 && a.ld % (16 / static_cast<int>(sizeof(In))) == 0;
+    const int vectors = reinterpret_cast<uintptr_t>(a.qkv) % (4 * sizeof(In)) == 0 && a.ld % 4 == 0;
     const dim3 grid(slots, share);
     if (a.kv.dim == 64) return launch_dependent(append_kernel<In, Out, 64>, grid, kAppendThreads, stream, a, vectors);
     return launch_dependent(append_kernel<In, Out, 128>, grid, kAppendThreads, stream, a, vectors);
