@@ -6,8 +6,10 @@
 // a warp, which never waits for another one: a lane holds eight 16-byte vectors of a tile and has the next
 // tile's in flight meanwhile (the bound is the logits' traffic), keeps its own reference and sum, and the
 // warp's list of the best lies sorted across its lanes, one each. Of a tile only what beats the list's last
-// entry is looked at one by one, which after a few tiles is rare. (Eight warps with one list met several times
-// a tile and took 157 us for 64 x 8 rows of 131072 logits; warps by themselves: see below.)
+// entry is looked at one by one, which after a few tiles is rare; so stretches are as long as keeps every warp
+// busy. (64 x 8 rows of 131072 logits, 268 MB: 157 us with eight warps on one list that meet several times a
+// tile, 78 us with four times as many stretches, 76 to 87 us with warps that read each other's lists for a
+// higher bound.)
 // A second kernel joins the stretches of each row and merges the rows' lists.
 //
 // Sums: a lane's reference is c = x L rounded, for its largest logit x so far and L = log2(e) rounded, and its
@@ -15,16 +17,19 @@
 // the row's sum is (C + log2 S) / L: the roundings of c and, to first order, of L cancel.
 #include "decode.h"
 #include "ptx.cuh"
+#include <cfloat>
 #include <climits>
 
 namespace ernie_b200
 {
 namespace
 {
-constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kVectors = 8;        // 16-byte vectors of a tile that a lane holds
 constexpr int kMaxStretches = 64;  // of a row: two lists per lane of the joining warp
 constexpr int kListEntries = 4096; // of a group's lists in the joining CTA's shared memory
+constexpr int kRing = 3;           // tiles of a warp in shared memory: one in work, two in flight
+constexpr int kRingBytes = kWarps * kRing * kVectors * 32 * 16;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Plan
@@ -32,19 +37,22 @@ struct Plan
     int stretches, tiles; // of a row, of a stretch
 };
 
-// Up to 16 warps per SM work at a time; `skew` logits of a row's first vector may lie before the row.
+// Up to 16 warps per SM work at a time; `skew` logits of a row's first vector may lie before the row. A row is
+// cut so that the rounds of warps times a stretch's tiles are fewest, a stretch's start counted as six tiles.
 Plan plan_of(long long rows, int vocab, int skew, int beams, bool bf16, int sms)
 {
     const long long tile = 32 * kVectors * (bf16 ? 8 : 4), tiles = (static_cast<long long>(vocab) + skew + tile - 1) / tile;
-    long long most = kListEntries / (beams * beams);
+    long long most = kListEntries / (beams * beams), best = LLONG_MAX;
     if (most > kMaxStretches) most = kMaxStretches;
-    if (most > tiles) most = tiles;
-    // no more stretches than fill the SMs four times over: a stretch's first tiles cost several times a later one's
-    const long long enough = (64ll * sms + rows - 1) / rows;
-    if (most > enough) most = enough;
-    Plan p;
-    p.tiles = static_cast<int>((tiles + most - 1) / most);
-    p.stretches = static_cast<int>((tiles + p.tiles - 1) / p.tiles);
+    Plan p = {1, 1};
+    for (long long s = 1; s <= most && s <= tiles; ++s)
+    {
+        const long long each = (tiles + s - 1) / s, rounds = (rows * s + 16 * sms - 1) / (16 * sms), cost = rounds * (each + 6);
+        if (cost >= best) continue;
+        best = cost;
+        p.tiles = static_cast<int>(each);
+        p.stretches = static_cast<int>((tiles + each - 1) / each);
+    }
     return p;
 }
 
@@ -87,6 +95,7 @@ template <> struct Vector<float>
     {
         return __uint_as_float(i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w);
     }
+    static __device__ __forceinline__ float value(float v) { return v; }
 };
 template <> struct Vector<__nv_bfloat16>
 {
@@ -96,18 +105,21 @@ template <> struct Vector<__nv_bfloat16>
         const unsigned w = i < 2 ? x.x : i < 4 ? x.y : i < 6 ? x.z : x.w;
         return __uint_as_float(i & 1 ? w & 0xffff0000u : w << 16);
     }
+    static __device__ __forceinline__ float value(__nv_bfloat16 v) { return __bfloat162float(v); }
 };
 
-// The lane's vectors of the tile that starts at `base` (an index of the row, on a 16-byte boundary); -inf
-// outside the row.
-template <class T> __device__ __forceinline__ void load_tile(const T *x, long long base, int vocab, int lane, uint4 (&v)[kVectors])
+// Copies the lane's vectors of the tile that starts at `base` (an index of the row, on a 16-byte boundary) to
+// `ring`, where only this lane reads them; -inf outside the row. The copies run on until waited for.
+template <class T> __device__ __forceinline__ void fill_tile(const T *x, long long base, int vocab, int lane, uint4 *ring)
 {
     constexpr int V = Vector<T>::kSize;
 #pragma unroll
     for (int j = 0; j < kVectors; ++j)
     {
         const long long at = base + (j * 32 + lane) * V;
-        if (at >= 0 && at + V <= vocab) v[j] = __ldcs(reinterpret_cast<const uint4 *>(x + at));
+        uint4 *slot = ring + j * 32 + lane;
+        if (at >= 0 && at + V <= vocab)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slot)), "l"(x + at) : "memory");
         else
         {
             unsigned w[4] = {};
@@ -118,9 +130,27 @@ template <class T> __device__ __forceinline__ void load_tile(const T *x, long lo
                 if constexpr (V == 4) w[e] = inside ? __float_as_uint(x[at + e]) : 0xff800000u;
                 else w[e / 2] |= (inside ? static_cast<unsigned>(__bfloat16_as_ushort(x[at + e])) : 0xff80u) << (16 * (e & 1));
             }
-            v[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            *slot = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
+}
+__device__ __forceinline__ void close_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the newest kRing - 2 groups of copies have arrived.
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory"); }
+
+// FP32 bits in an order of unsigned integers (the two zeros equal), and back.
+__device__ __forceinline__ unsigned ordered(float v)
+{
+    const unsigned u = __float_as_uint(v + 0.f);
+    return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(unsigned u) { return __uint_as_float(u ^ ((u >> 31) ? 0x80000000u : 0xffffffffu)); }
+
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 __device__ __forceinline__ float exp2_fast(float x)
@@ -130,14 +160,14 @@ __device__ __forceinline__ float exp2_fast(float x)
     return y;
 }
 
-template <class T> __global__ void __launch_bounds__(kThreads, 4) stretch_kernel(const __grid_constant__ BeamSelectArgs a, Plan plan, Parts parts)
+template <class T> __global__ void __launch_bounds__(kThreads, 2) stretch_kernel(const __grid_constant__ BeamSelectArgs a, Plan plan, Parts parts)
 {
     constexpr int V = Vector<T>::kSize;
     constexpr unsigned full = 0xffffffffu;
     grid_dependency_wait();
     grid_dependents_launch();
-    const int lane = threadIdx.x % 32, k = a.beams;
-    const long long out = static_cast<long long>(blockIdx.x) * kWarps + threadIdx.x / 32, row = out / plan.stretches;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, k = a.beams;
+    const long long out = static_cast<long long>(blockIdx.x) * kWarps + warp, row = out / plan.stretches;
     if (row >= static_cast<long long>(a.groups) * k || !row_offers(a, row)) return;
     const T *x = static_cast<const T *>(a.logits) + row * a.ld;
     // vectors start at 16-byte boundaries: index 0 of the row is element `skew` of the first one
@@ -147,21 +177,34 @@ template <class T> __global__ void __launch_bounds__(kThreads, 4) stretch_kernel
     const long long end = min(static_cast<long long>(a.vocab), base + static_cast<long long>(plan.tiles) * kTileSize);
     float c = -INFINITY, sum = 0.f, top = -INFINITY; // the lane's reference, sum and largest logit
     float value = -INFINITY, last_value = -INFINITY; // the list: lane i holds the i-th best; its last entry
-    int token = INT_MAX, last_token = INT_MAX;
-    uint4 next[kVectors];
-    if (base < end) load_tile<T>(x, base, a.vocab, lane, next);
-    for (bool first = true; base < end; base += kTileSize, first = false)
+    int token = INT_MAX;
+    bool listed = false; // whether the list has its beginning
+    extern __shared__ uint4 ring_memory[];
+    uint4 *ring = ring_memory + warp * (kRing * kVectors * 32);
+#pragma unroll
+    for (int t = 0; t < kRing - 1; ++t)
     {
+        if (base + t * kTileSize < end) fill_tile<T>(x, base + t * kTileSize, a.vocab, lane, ring + t * (kVectors * 32));
+        close_copies();
+    }
+    int slot = 0;
+    for (; base < end; base += kTileSize, slot = slot == kRing - 1 ? 0 : slot + 1)
+    {
+        wait_copies();
+        __syncwarp(); // any lane may look at another's logits from here on
         uint4 v[kVectors];
 #pragma unroll
-        for (int j = 0; j < kVectors; ++j) v[j] = next[j];
-        if (base + kTileSize < end) load_tile<T>(x, base + kTileSize, a.vocab, lane, next);
+        for (int j = 0; j < kVectors; ++j) v[j] = ring[slot * (kVectors * 32) + j * 32 + lane];
+        // the tile before this one has left its slot
+        const int free = slot == 0 ? kRing - 1 : slot - 1;
+        if (base + (kRing - 1) * kTileSize < end) fill_tile<T>(x, base + (kRing - 1) * kTileSize, a.vocab, lane, ring + free * (kVectors * 32));
+        close_copies();
         float mine[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int j = 0; j < kVectors; ++j)
 #pragma unroll
-            for (int e = 0; e < V; ++e) mine[e & 3] = fmaxf(mine[e & 3], Vector<T>::get(v[j], e));
-        const float best = fmaxf(fmaxf(mine[0], mine[1]), fmaxf(mine[2], mine[3]));
+            for (int e = 0; e < V; e += 2) mine[(e / 2) & 3] = max3(mine[(e / 2) & 3], Vector<T>::get(v[j], e), Vector<T>::get(v[j], e + 1));
+        const float best = fmaxf(max3(mine[0], mine[1], mine[2]), mine[3]);
         if (best > top)
         {
             const float raised = best * kLog2e;
@@ -187,51 +230,74 @@ template <class T> __global__ void __launch_bounds__(kThreads, 4) stretch_kernel
                 for (int e = 0; e < V; ++e)
                     if (Vector<T>::get(v[j], e) != Vector<T>::get(v[j], e)) sum = NAN;
         }
-        // In the first tile the lanes' maxima bound the k-th largest logit from below: the k-th of them, in
-        // descending order. Later tokens have to beat the list's last one.
-        float bound = last_value;
+        // The first tile: the lanes' largest logits, sorted, are the list's beginning, and the k-th of them bounds
+        // the k-th largest of all from below. Later tokens have to beat the list's last one.
+        float limit = last_value > -INFINITY ? from_ordered(ordered(last_value) + 1) : -FLT_MAX;
+        if (!__any_sync(full, best >= limit)) continue;
+        int best_place = 0; // of the lane's largest logit, the first of equal ones
+#pragma unroll
+        for (int j = kVectors - 1; j >= 0; --j)
+#pragma unroll
+            for (int e = V - 1; e >= 0; --e)
+                if (Vector<T>::get(v[j], e) == best) best_place = j * 32 * V + e;
+        const int best_token = static_cast<int>(base + lane * V + best_place);
+        const bool first = !listed;
         if (first)
         {
-            float sorted = best;
+            listed = true;
+            value = best;
+            token = best > -INFINITY ? best_token : INT_MAX;
 #pragma unroll
             for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
                 for (int step = size / 2; step > 0; step /= 2)
                 {
-                    const float other = __shfl_xor_sync(full, sorted, step);
+                    const float other_value = __shfl_xor_sync(full, value, step);
+                    const int other_token = __shfl_xor_sync(full, token, step);
                     const bool high = ((lane & step) == 0) == ((lane & size) == 0);
-                    sorted = high ? fmaxf(sorted, other) : fminf(sorted, other);
+                    if (high == better(other_value, other_token, value, token)) value = other_value, token = other_token;
                 }
-            bound = __shfl_sync(full, sorted, k - 1);
+            limit = fmaxf(limit, __shfl_sync(full, value, k - 1));
         }
-        if (!__any_sync(full, first ? best >= bound && best > -INFINITY : best > bound)) continue;
+        int count = 0;
 #pragma unroll
         for (int j = 0; j < kVectors; ++j)
 #pragma unroll
-            for (int e = 0; e < V; ++e)
+            for (int e = 0; e < V; ++e) count += Vector<T>::get(v[j], e) >= limit;
+        auto insert = [&](float new_value, int new_token) {
+            // the entries before it are a prefix of the lanes
+            const int place = __popc(__ballot_sync(full, better(value, token, new_value, new_token)));
+            const float moved_value = __shfl_up_sync(full, value, 1);
+            const int moved_token = __shfl_up_sync(full, token, 1);
+            if (lane == place) value = new_value, token = new_token;
+            else if (lane > place) value = moved_value, token = moved_token;
+        };
+        if (!first)
+            for (unsigned holders = __ballot_sync(full, count == 1); holders; holders &= holders - 1)
             {
-                const float mine_value = Vector<T>::get(v[j], e);
-                unsigned found = __ballot_sync(full, mine_value >= bound && mine_value > -INFINITY);
-                if (!found) continue;
-                const int mine_token = static_cast<int>(base + (j * 32 + lane) * V + e);
-                found = __ballot_sync(full, mine_value >= bound && mine_value > -INFINITY && better(mine_value, mine_token, last_value, last_token));
-                while (found)
-                {
-                    const int from = __ffs(found) - 1;
-                    found &= found - 1;
-                    const float new_value = __shfl_sync(full, mine_value, from);
-                    const int new_token = __shfl_sync(full, mine_token, from);
-                    // the entries before it are a prefix of the lanes
-                    const int place = __popc(__ballot_sync(full, better(value, token, new_value, new_token)));
-                    const float moved_value = __shfl_up_sync(full, value, 1);
-                    const int moved_token = __shfl_up_sync(full, token, 1);
-                    if (lane == place) value = new_value, token = new_token;
-                    else if (lane > place) value = moved_value, token = moved_token;
-                    last_value = __shfl_sync(full, value, k - 1);
-                    last_token = __shfl_sync(full, token, k - 1);
-                }
-                bound = fmaxf(bound, last_value);
+                const int from = __ffs(holders) - 1;
+                insert(__shfl_sync(full, best, from), __shfl_sync(full, best_token, from));
             }
+        // lanes that hold several: the warp looks through such a lane's logits together
+        for (unsigned holders = __ballot_sync(full, count > 1); holders; holders &= holders - 1)
+        {
+            const int from = __ffs(holders) - 1, held = first ? __shfl_sync(full, best_token, from) : -1;
+#pragma unroll 1
+            for (int i = lane; i < kVectors * V; i += 32)
+            {
+                const int j = i / V, e = i % V;
+                const float x = Vector<T>::value(reinterpret_cast<const T *>(ring + slot * (kVectors * 32) + j * 32 + from)[e]);
+                const int x_token = static_cast<int>(base + (j * 32 + from) * V + e);
+                for (unsigned found = __ballot_sync(full, x >= limit && x_token != held); found; found &= found - 1)
+                {
+                    const int one = __ffs(found) - 1;
+                    const float new_value = __shfl_sync(full, x, one);
+                    const int new_token = __shfl_sync(full, x_token, one);
+                    if (__any_sync(full, lane == k - 1 && better(new_value, new_token, value, token))) insert(new_value, new_token);
+                }
+            }
+        }
+        last_value = __shfl_sync(full, value, k - 1);
     }
     // the lanes' references and sums
     float reference = c;
@@ -250,13 +316,6 @@ template <class T> __global__ void __launch_bounds__(kThreads, 4) stretch_kernel
         parts.value[out * k + lane] = value;
         parts.token[out * k + lane] = token;
     }
-}
-
-// FP32 bits in an order of unsigned integers (the two zeros equal).
-__device__ __forceinline__ unsigned ordered(float v)
-{
-    const unsigned u = __float_as_uint(v + 0.f);
-    return u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
 }
 
 // One CTA per group, a warp per beam: the beam's list from its stretches' lists, then one warp merges the
@@ -313,7 +372,7 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
         for (int h = 0; h < 2; ++h)
         {
             if (part_sum[h] != part_sum[h]) sum = NAN;
-            else if (part_reference[h] > -INFINITY) sum += static_cast<double>(part_sum[h]) * exp2(static_cast<double>(part_reference[h]) - reference);
+            else if (part_reference[h] > -INFINITY) sum += static_cast<double>(part_sum[h]) * exp2f(part_reference[h] - reference);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(full, sum, o);
@@ -351,18 +410,17 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
     __syncthreads();
     if (warp != 0) return;
     int at = 0, parent = -1, chosen = -1, ended = 1;
-    float value = -INFINITY;
+    float result = -INFINITY;
     for (int r = 0; r < k; ++r)
     {
-        double best = lane < k && at < k ? total[lane][at] : -INFINITY;
-        int who = lane;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-        {
-            const double other = __shfl_xor_sync(full, best, o);
-            const int other_who = __shfl_xor_sync(full, who, o);
-            if (other > best || (other == best && other_who < who)) best = other, who = other_who;
-        }
+        // the largest head, as an ordered integer in two halves; of equal ones the lowest beam's
+        const double mine = lane < k && at < k ? total[lane][at] : -INFINITY;
+        const long long raw = __double_as_longlong(mine + 0.0);
+        const unsigned long long key = static_cast<unsigned long long>(raw) ^ (raw < 0 ? ~0ull : 1ull << 63);
+        const unsigned high = static_cast<unsigned>(key >> 32), most_high = __reduce_max_sync(full, high);
+        const unsigned low = high == most_high ? static_cast<unsigned>(key) : 0u, most_low = __reduce_max_sync(full, low);
+        const int who = __ffs(__ballot_sync(full, high == most_high && static_cast<unsigned>(key) == most_low)) - 1;
+        const double best = __shfl_sync(full, mine, who);
         if (best == -INFINITY) break;
         const int taken = __shfl_sync(full, at, who);
         if (lane == who) ++at;
@@ -370,7 +428,7 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
         {
             parent = who;
             chosen = token[who][taken];
-            value = static_cast<float>(best);
+            result = static_cast<float>(best);
             ended = done[who] || (a.end_token >= 0 && chosen == a.end_token);
         }
     }
@@ -378,7 +436,7 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
     {
         a.parents[base + lane] = parent;
         a.tokens[base + lane] = chosen;
-        a.new_scores[base + lane] = value;
+        a.new_scores[base + lane] = result;
         a.new_finished[base + lane] = ended;
     }
 }
@@ -404,6 +462,15 @@ size_t beam_select_workspace(int groups, int beams, int vocab, int sms)
     return most;
 }
 
+int prepare_beam_kernels()
+{
+    cudaError_t e = cudaFuncSetAttribute(stretch_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(stretch_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    // the SMs' split between shared memory and L1 stays as it is between the two kernels
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(merge_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    return e;
+}
+
 int launch_beam_select(const BeamSelectArgs &a, int sms, cudaStream_t stream)
 {
     const long long rows = static_cast<long long>(a.groups) * a.beams;
@@ -414,9 +481,9 @@ int launch_beam_select(const BeamSelectArgs &a, int sms, cudaStream_t stream)
     if (ctas > INT32_MAX) return cudaErrorInvalidValue;
     const Parts parts = parts_of(a.workspace, rows, a.beams, p);
     const unsigned grid = static_cast<unsigned>(ctas);
-    const cudaError_t e = a.bf16 ? launch_dependent(stretch_kernel<__nv_bfloat16>, grid, kThreads, stream, a, p, parts)
-                                 : launch_dependent(stretch_kernel<float>, grid, kThreads, stream, a, p, parts);
+    const cudaError_t e = a.bf16 ? launch_dependent(stretch_kernel<__nv_bfloat16>, grid, kThreads, kRingBytes, stream, a, p, parts)
+                                 : launch_dependent(stretch_kernel<float>, grid, kThreads, kRingBytes, stream, a, p, parts);
     if (e != cudaSuccess) return e;
-    return launch_dependent(merge_kernel, a.groups, 32 * a.beams, stream, a, p, parts);
+    return launch_dependent(merge_kernel, a.groups, 32 * a.beams, 0, stream, a, p, parts);
 }
 } // namespace ernie_b200

@@ -250,6 +250,7 @@ extern "C" int ernie_cuda_context_create(int device, ernie_cuda_context **out)
     if (e == cudaSuccess) e = static_cast<cudaError_t>(prepare_flash_f32_kernels());
     if (e == cudaSuccess) e = static_cast<cudaError_t>(prepare_conv_kernels());
     if (e == cudaSuccess) e = static_cast<cudaError_t>(prepare_prefix_attention_kernels());
+    if (e == cudaSuccess) e = static_cast<cudaError_t>(prepare_beam_kernels());
     if (e != cudaSuccess)
     {
         ernie_cuda_context_destroy(ctx);

@@ -29,7 +29,7 @@ struct PagedBatch
 // A kernel that waits for the one before it by itself (griddepcontrol.wait), so that its launch and set-up
 // overlap that one's end.
 template <class... Params, class... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, Args &&...args)
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream, Args &&...args)
 {
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -37,6 +37,7 @@ cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, c
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
+    cfg.dynamicSmemBytes = shared;
     cfg.stream = stream;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
@@ -145,5 +146,6 @@ struct BeamSelectArgs
     void *workspace = nullptr;
 };
 size_t beam_select_workspace(int groups, int beams, int vocab, int sms);
+int prepare_beam_kernels();
 int launch_beam_select(const BeamSelectArgs &args, int sms, cudaStream_t stream);
 } // namespace ernie_b200
