@@ -53,82 +53,77 @@ __device__ __forceinline__ float4 turn_high(float4 x, float4 y, float4 c, float4
                        __fadd_rn(__fmul_rn(y.z, c.z), __fmul_rn(x.z, s.z)), __fadd_rn(__fmul_rn(y.w, c.w), __fmul_rn(x.w, s.w)));
 }
 
-constexpr int kAppendThreads = 256;
-template <class In> constexpr int kAppendCtas = sizeof(In) == 2 ? 4 : 3; // of an SM: two slots' loads in registers
+constexpr int kAppendThreads = 128;
+constexpr int kAppendAhead = 6; // heads of a thread whose loads are in flight together
+template <class In> constexpr int kAppendCtas = sizeof(In) == 2 ? 8 : 5; // of an SM
 
-// CTAs take slots (a token, or nothing) in turn, or a share of a slot's heads. A thread holds four dims of a
-// head's lower half and their partners in the upper one, of every head of its row of threads, with one read of
-// their cos and sin; the next slot's loads are in flight meanwhile. The bound is the traffic: projection in,
-// queries, keys and values out. (16000 tokens of 48 heads from BF16 to BF16, 410 MB: 140 us with eight dims to
-// a thread at 114 registers, 94 us with four and one slot per CTA.)
-template <class In, class Out, int D> __global__ void __launch_bounds__(kAppendThreads, kAppendCtas<In>) append_kernel(const __grid_constant__ AppendArgs a, int vectors)
+// A CTA per slot (a token, or nothing) and share of its heads. A thread holds four dims of a head's lower half
+// and their partners in the upper one, of every head of its row of threads, with one read of their cos and sin;
+// the first heads' loads are issued before the token's place is known. The bound is the traffic: projection in,
+// queries, keys and values out. A slot is a chain of some 3 us (lengths, page and angles, stores) around 24 KB,
+// so an SM needs many slots at a time: small CTAs with six heads to a thread. (16000 tokens of 48 heads from
+// BF16 to BF16, 410 MB: 140 us with eight dims to a thread at 114 registers, 94 us with 256 threads and three
+// heads each, 96 us with these walking over the slots and the next one's loads in flight.)
+template <class In, class Out, int D>
+__global__ void __launch_bounds__(kAppendThreads, kAppendCtas<In>) append_kernel(const __grid_constant__ AppendArgs a, int vectors)
 {
     constexpr int kHalf = D / 2, kLanes = kHalf / 4, kHeads = kAppendThreads / kLanes;
-    constexpr int kAhead = 3; // heads of a thread whose loads are in flight together
     grid_dependency_wait();
     grid_dependents_launch();
-    const int slots = a.batch.sequences * a.batch.queries;
+    const int slot = blockIdx.x, s = slot / a.batch.queries, i = slot - s * a.batch.queries;
     const int d = (threadIdx.x % kLanes) * 4, first = blockIdx.y * kHeads + threadIdx.x / kLanes, step = gridDim.y * kHeads;
     const int rotated = a.heads + a.kv.kv_heads, width = rotated + a.kv.kv_heads;
-    auto fetch = [&](int slot, int head, Four<In>(&lo)[kAhead], Four<In>(&hi)[kAhead]) {
-        const In *x = static_cast<const In *>(a.qkv) + static_cast<size_t>(slot) * a.ld + d;
+    const In *x = static_cast<const In *>(a.qkv) + static_cast<size_t>(slot) * a.ld + d;
+    Four<In> lo[kAppendAhead], hi[kAppendAhead];
+    auto fetch = [&](int head) {
 #pragma unroll
-        for (int t = 0; t < kAhead; ++t)
-        {
-            if (head + t * step >= width) break;
-            lo[t].load(x + (head + t * step) * D, vectors);
-            hi[t].load(x + (head + t * step) * D + kHalf, vectors);
-        }
-    };
-    Four<In> next_lo[kAhead], next_hi[kAhead];
-    if (first < width) fetch(blockIdx.x, first, next_lo, next_hi);
-    for (int slot = blockIdx.x; slot < slots; slot += gridDim.x)
-    {
-        Four<In> lo[kAhead], hi[kAhead];
-#pragma unroll
-        for (int t = 0; t < kAhead; ++t) lo[t] = next_lo[t], hi[t] = next_hi[t];
-        if (slot + static_cast<int>(gridDim.x) < slots && first < width) fetch(slot + gridDim.x, first, next_lo, next_hi);
-        const int s = slot / a.batch.queries, i = slot - s * a.batch.queries;
-        const SequenceView view = sequence_view(a.batch, a.kv.page_shift, s);
-        if (i >= view.count) continue;
-        const int place = view.len - view.count + i; // in the sequence's own pages
-        const int position = view.prefix_len + place;
-        if (position < 0 || position >= a.rope_rows)
-        {
-            report_range(a.batch.error_flag);
-            continue;
-        }
-        int page = place >= 0 ? a.batch.tables[static_cast<size_t>(s) * a.batch.max_pages + (place >> a.kv.page_shift)] : -1;
-        const float *cos = a.cos + static_cast<size_t>(position) * D + d, *sin = a.sin + static_cast<size_t>(position) * D + d;
-        const float4 cos_lo = *reinterpret_cast<const float4 *>(cos), cos_hi = *reinterpret_cast<const float4 *>(cos + kHalf);
-        const float4 sin_lo = *reinterpret_cast<const float4 *>(sin), sin_hi = *reinterpret_cast<const float4 *>(sin + kHalf);
-        if (place >= 0 && (page < 0 || page >= a.kv.pages))
-        {
-            report_range(a.batch.error_flag);
-            page = -1;
-        }
-        for (int head = first; head < width; head += kAhead * step)
-        {
-            if (head != first) fetch(slot, head, lo, hi);
-#pragma unroll
-            for (int t = 0; t < kAhead; ++t)
+        for (int t = 0; t < kAppendAhead; ++t)
+            if (head + t * step < width)
             {
-                const int h = head + t * step;
-                if (h >= width) break;
-                const float4 low = lo[t].get(), high = hi[t].get();
-                Out *dst;
-                if (h < a.heads) dst = static_cast<Out *>(a.q_out) + (static_cast<size_t>(slot) * a.heads + h) * D;
-                else
-                {
-                    if (page < 0) continue;
-                    const int kv_head = h - (h < rotated ? a.heads : rotated);
-                    const size_t row = ((static_cast<size_t>(page) * a.kv.kv_heads + kv_head) << a.kv.page_shift) +
-                                       (place & ((1 << a.kv.page_shift) - 1));
-                    dst = static_cast<Out *>(h < rotated ? a.kv.k : a.kv.v) + row * D;
-                }
-                store_four(dst + d, h < rotated ? turn_low(low, high, cos_lo, sin_lo) : low);
-                store_four(dst + d + kHalf, h < rotated ? turn_high(low, high, cos_hi, sin_hi) : high);
+                lo[t].load(x + (head + t * step) * D, vectors);
+                hi[t].load(x + (head + t * step) * D + kHalf, vectors);
             }
+    };
+    fetch(first);
+    const SequenceView view = sequence_view(a.batch, a.kv.page_shift, s);
+    if (i >= view.count) return;
+    const int place = view.len - view.count + i; // in the sequence's own pages
+    const int position = view.prefix_len + place;
+    if (position < 0 || position >= a.rope_rows)
+    {
+        report_range(a.batch.error_flag);
+        return;
+    }
+    int page = place >= 0 ? a.batch.tables[static_cast<size_t>(s) * a.batch.max_pages + (place >> a.kv.page_shift)] : -1;
+    const float *cos = a.cos + static_cast<size_t>(position) * D + d, *sin = a.sin + static_cast<size_t>(position) * D + d;
+    const float4 cos_lo = *reinterpret_cast<const float4 *>(cos), cos_hi = *reinterpret_cast<const float4 *>(cos + kHalf);
+    const float4 sin_lo = *reinterpret_cast<const float4 *>(sin), sin_hi = *reinterpret_cast<const float4 *>(sin + kHalf);
+    if (place >= 0 && (page < 0 || page >= a.kv.pages))
+    {
+        report_range(a.batch.error_flag);
+        page = -1;
+    }
+    for (int head = first; head < width; head += kAppendAhead * step)
+    {
+        if (head != first) fetch(head);
+#pragma unroll
+        for (int t = 0; t < kAppendAhead; ++t)
+        {
+            const int h = head + t * step;
+            if (h >= width) break;
+            const float4 low = lo[t].get(), high = hi[t].get();
+            Out *dst;
+            if (h < a.heads) dst = static_cast<Out *>(a.q_out) + (static_cast<size_t>(slot) * a.heads + h) * D;
+            else
+            {
+                if (page < 0) continue;
+                const int kv_head = h - (h < rotated ? a.heads : rotated);
+                const size_t row = ((static_cast<size_t>(page) * a.kv.kv_heads + kv_head) << a.kv.page_shift) +
+                                   (place & ((1 << a.kv.page_shift) - 1));
+                dst = static_cast<Out *>(h < rotated ? a.kv.k : a.kv.v) + row * D;
+            }
+            store_four(dst + d, h < rotated ? turn_low(low, high, cos_lo, sin_lo) : low);
+            store_four(dst + d + kHalf, h < rotated ? turn_high(low, high, cos_hi, sin_hi) : high);
         }
     }
 }
@@ -272,11 +267,10 @@ template <class In, class Out> int launch_append(const AppendArgs &a, int sms, c
 {
     const int slots = a.batch.sequences * a.batch.queries, width = a.heads + 2 * a.kv.kv_heads;
     const int at_once = kAppendThreads / (a.kv.dim / 8), passes = (width + at_once - 1) / at_once;
-    // few slots: their heads over several CTAs (one decode step of five beams: three CTAs a slot)
-    const int share = slots >= 2 * sms ? 1 : passes < 64 ? passes : 64;
+    // few slots: their heads over several CTAs (one decode step of five beams: six CTAs a slot)
+    const int share = slots >= 4 * sms ? 1 : passes < 64 ? passes : 64;
     const int vectors = reinterpret_cast<uintptr_t>(a.qkv) % (4 * sizeof(In)) == 0 && a.ld % 4 == 0;
-    const int most = kAppendCtas<In> * sms;
-    const dim3 grid(slots < most ? slots : most, share);
+    const dim3 grid(slots, share);
     if (a.kv.dim == 64) return launch_dependent(append_kernel<In, Out, 64>, grid, kAppendThreads, 0, stream, a, vectors);
     return launch_dependent(append_kernel<In, Out, 128>, grid, kAppendThreads, 0, stream, a, vectors);
 }
