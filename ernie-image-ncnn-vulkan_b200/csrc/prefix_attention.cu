@@ -1299,31 +1299,38 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------- the join
-// A warp per row: the weights of its parts (a lane each), then the weighted sum of their values.
+// R rows per warp (consecutive rows of q and out): 32 / R lanes work out a row's weights, eight parts at a
+// time, and all 32 its weighted sum of values, A parts' loads in flight together. Few rows: one per warp with
+// eight loads ahead, since a row may have many parts. Many: four per warp, so that they are all on the SMs at
+// once with their places worked out before the attention ends (16384 rows one by one took three rounds, 10 us).
 constexpr int kJoinWarps = 8;
 
-template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ AttendArgs p)
+template <class T, int D, int R, int A>
+__global__ void __launch_bounds__(kJoinWarps * 32, R == 1 ? 1 : 4) join_kernel(const __grid_constant__ AttendArgs p)
 {
-    constexpr int N = D / 32; // values of a lane
+    constexpr int N = D / 32, kLanes = 32 / R, kBatch = 8; // values of a lane; lanes of a row; parts weighed together
+    static_assert(kLanes >= kBatch && kBatch % A == 0, "parts of a batch");
     const unsigned full = 0xffffffffu;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, first_row = (blockIdx.x * kJoinWarps + threadIdx.x / 32) * R;
     const PagedBatch &b = p.a.batch;
-    const int at = blockIdx.x * kJoinWarps + threadIdx.x / 32; // row of q and out
-    // The lengths are older than the kernel before this one, which waited for them before it let this one start.
-    bool row = at < b.sequences * b.queries * p.a.heads;
-    const int slot = row ? divide(at, p.by_heads) : 0, head = at - slot * p.a.heads, s = divide(slot, p.by_queries), i = slot - s * b.queries;
+    const int rows = b.sequences * b.queries * p.a.heads;
+    // The lane's row. The lengths are older than the kernel before this one, which waited for them before it let
+    // this one start.
+    const int at = first_row + lane / kLanes;
+    const int slot = at < rows ? divide(at, p.by_heads) : 0, head = at < rows ? at - slot * p.a.heads : 0;
+    const int s = divide(slot, p.by_queries), i = slot - s * b.queries;
     const int kv_head = divide(head, p.by_share), group = divide(slot, p.by_group);
     SequenceView view;
     view.prefix_len = b.max_prefix_pages ? b.prefix_lens[group] : 0;
     static_cast<OwnView &>(view) = own_view(b, p.a.kv.page_shift, s);
     if (b.max_prefix_pages) view.prefix_len = clamped_length(view.prefix_len, b.max_prefix_pages, p.a.kv.page_shift, b.error_flag);
-    row = row && i < view.count;
+    const bool wanted = at < rows && i < view.count;
     int item[2] = {-1, -1}, within[2] = {0, 0};
 #pragma unroll
     for (int which = 0; which < 2; ++which)
     {
         const List &l = p.list[which];
-        if (which == 0 ? view.prefix_len == 0 : view.len - view.count + i + 1 <= 0) continue;
+        if (!wanted || (which == 0 ? view.prefix_len == 0 : view.len - view.count + i + 1 <= 0)) continue;
         const int owner = which == 0 ? group : s;
         const int r = (which == 0 ? slot - owner * l.slots : i) * p.share + head - kv_head * p.share, block = r >> l.block_shift;
         item[which] = (owner * l.blocks + block) * p.a.kv.kv_heads + kv_head;
@@ -1331,86 +1338,113 @@ template <class T, int D> __global__ void __launch_bounds__(kJoinWarps * 32) joi
     }
     grid_dependency_wait();
     grid_dependents_launch();
-    if (!row) return;
-    int parts[2] = {0, 0};
-    size_t first[2] = {0, 0}; // row of the first part's statistics
+    if (first_row >= rows) return;
+    int parts[2] = {0, 0}, first[2] = {0, 0}; // of the lane's row, and the first part's place
 #pragma unroll
     for (int which = 0; which < 2; ++which)
     {
         if (item[which] < 0) continue;
         const int2 meta = p.list[which].meta[item[which]];
         parts[which] = meta.y - meta.x + 1;
-        first[which] = static_cast<size_t>(item[which] + meta.x) * p.list[which].part_rows + within[which];
+        first[which] = item[which] + meta.x;
     }
-    const int total = parts[0] + parts[1];
-    auto row_at = [&](int j, const List *&l) {
-        const bool shared = j < parts[0];
-        l = &p.list[shared ? 0 : 1];
-        return (shared ? first[0] : first[1]) + static_cast<size_t>(shared ? j : j - parts[0]) * l->part_rows;
-    };
-    constexpr int kAhead = 8; // parts whose values are fetched together, before their weights are known
-    float top = -INFINITY, sum = 0.f, o[N] = {};
-    for (int base = 0; base < total; base += kAhead)
+    const int total = parts[0] + parts[1], most_parts = __reduce_max_sync(full, total);
+    float top = -INFINITY, sum = 0.f, o[R][N] = {};
+    for (int base = 0; base < most_parts; base += kBatch)
     {
-        const int here = min(kAhead, total - base);
-        const List *l;
+        const int j = base + lane % kLanes;
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (lane < here)
+        if (lane % kLanes < kBatch && j < total)
         {
-            const size_t r = row_at(base + lane, l);
-            ml = l->ml[r];
+            const int which = j < parts[0] ? 0 : 1;
+            const List &l = p.list[which];
+            ml = l.ml[static_cast<size_t>(which ? first[1] + j - parts[0] : first[0] + j) * l.part_rows + (which ? within[1] : within[0])];
         }
-        float x[kAhead][N];
+        float weight = 0.f, before = 1.f;
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
+        for (int k0 = 0; k0 < kBatch; k0 += A)
         {
-            if (k >= here) break;
-            const size_t r = row_at(base + k, l);
-            const float *src = l->o + r * D + lane * N;
-            if constexpr (N == 4)
+            if (base + k0 >= most_parts) break;
+            float x[R][A][N];
+#pragma unroll
+            for (int r = 0; r < R; ++r)
             {
-                const float4 t = *reinterpret_cast<const float4 *>(src);
-                x[k][0] = t.x, x[k][1] = t.y, x[k][2] = t.z, x[k][3] = t.w;
+                const int parts0 = __shfl_sync(full, parts[0], r * kLanes), total_r = __shfl_sync(full, total, r * kLanes);
+                const int first0 = __shfl_sync(full, first[0], r * kLanes), first1 = __shfl_sync(full, first[1], r * kLanes);
+                const int within0 = __shfl_sync(full, within[0], r * kLanes), within1 = __shfl_sync(full, within[1], r * kLanes);
+#pragma unroll
+                for (int k = 0; k < A; ++k)
+                {
+                    const int jj = base + k0 + k;
+                    const bool shared = jj < parts0;
+                    const List &l = p.list[shared ? 0 : 1];
+                    const float *src = l.o + (static_cast<size_t>(shared ? first0 + jj : first1 + jj - parts0) * l.part_rows + (shared ? within0 : within1)) * D + lane * N;
+#pragma unroll
+                    for (int d = 0; d < N; ++d) x[r][k][d] = 0.f;
+                    if (jj < total_r)
+                    {
+                        if constexpr (N == 4)
+                        {
+                            const float4 t = *reinterpret_cast<const float4 *>(src);
+                            x[r][k][0] = t.x, x[r][k][1] = t.y, x[r][k][2] = t.z, x[r][k][3] = t.w;
+                        }
+                        else
+                        {
+                            const float2 t = *reinterpret_cast<const float2 *>(src);
+                            x[r][k][0] = t.x, x[r][k][1] = t.y;
+                        }
+                    }
+                }
             }
-            else
+            if (k0 == 0) // the batch's weights, while the values are on their way
             {
-                const float2 t = *reinterpret_cast<const float2 *>(src);
-                x[k][0] = t.x, x[k][1] = t.y;
+                float most = ml.x;
+#pragma unroll
+                for (int step = kLanes / 2; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor_sync(full, most, step));
+                most = fmaxf(most, top);
+                before = top == most ? 1.f : exp2_fast(top - most);
+                weight = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - most);
+                float part_sum = weight * ml.y;
+#pragma unroll
+                for (int step = kLanes / 2; step > 0; step >>= 1) part_sum += __shfl_xor_sync(full, part_sum, step);
+                sum = sum * before + part_sum;
+                top = most;
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+                {
+                    const float f = __shfl_sync(full, before, r * kLanes);
+#pragma unroll
+                    for (int d = 0; d < N; ++d) o[r][d] *= f;
+                }
             }
-        }
-        float most = ml.x;
 #pragma unroll
-        for (int step = kAhead / 2; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor_sync(full, most, step));
-        most = fmaxf(__shfl_sync(full, most, 0), top);
-        const float before = top == most ? 1.f : exp2_fast(top - most);
-        const float weight = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - most);
-        float part_sum = weight * ml.y;
+            for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int step = kAhead / 2; step > 0; step >>= 1) part_sum += __shfl_xor_sync(full, part_sum, step);
-        sum = sum * before + __shfl_sync(full, part_sum, 0);
-        top = most;
+                for (int k = 0; k < A; ++k)
+                {
+                    const float f = __shfl_sync(full, weight, r * kLanes + k0 + k);
 #pragma unroll
-        for (int d = 0; d < N; ++d) o[d] *= before;
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-        {
-            const float f = __shfl_sync(full, weight, k);
-            if (k >= here) break;
-#pragma unroll
-            for (int d = 0; d < N; ++d) o[d] = fmaf(f, x[k][d], o[d]);
+                    for (int d = 0; d < N; ++d) o[r][d] = fmaf(f, x[r][k][d], o[r][d]);
+                }
         }
     }
     const float inverse = sum > 0.f ? 1.f / sum : 0.f;
-    T *dst = static_cast<T *>(p.a.out) + static_cast<size_t>(at) * D + lane * N;
-    if constexpr (sizeof(T) == 4)
+#pragma unroll
+    for (int r = 0; r < R; ++r)
     {
-        if constexpr (N == 4) *reinterpret_cast<float4 *>(dst) = make_float4(o[0] * inverse, o[1] * inverse, o[2] * inverse, o[3] * inverse);
-        else *reinterpret_cast<float2 *>(dst) = make_float2(o[0] * inverse, o[1] * inverse);
+        const float f = __shfl_sync(full, inverse, r * kLanes);
+        if (!__shfl_sync(full, static_cast<int>(wanted), r * kLanes)) continue;
+        T *dst = static_cast<T *>(p.a.out) + static_cast<size_t>(first_row + r) * D + lane * N;
+        if constexpr (sizeof(T) == 4)
+        {
+            if constexpr (N == 4) *reinterpret_cast<float4 *>(dst) = make_float4(o[r][0] * f, o[r][1] * f, o[r][2] * f, o[r][3] * f);
+            else *reinterpret_cast<float2 *>(dst) = make_float2(o[r][0] * f, o[r][1] * f);
+        }
+        else if constexpr (N == 4)
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[r][0] * f, o[r][1] * f), pack2(o[r][2] * f, o[r][3] * f));
+        else
+            *reinterpret_cast<uint32_t *>(dst) = pack2(o[r][0] * f, o[r][1] * f);
     }
-    else if constexpr (N == 4)
-        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack2(o[0] * inverse, o[1] * inverse), pack2(o[2] * inverse, o[3] * inverse));
-    else
-        *reinterpret_cast<uint32_t *>(dst) = pack2(o[0] * inverse, o[1] * inverse);
 }
 
 // ---------------------------------------------------------------- host
@@ -1495,23 +1529,13 @@ template <class T, int D> int launch(const PrefixAttentionArgs &a, int sms, cuda
     if (p.granule > Layout<T, D>::kSlotKeys) p.granule = Layout<T, D>::kSlotKeys;
     CUtensorMap map_k, map_v;
     if (!map_pool(&map_k, a.kv.k, a.kv, p.granule) || !map_pool(&map_v, a.kv.v, a.kv, p.granule)) return cudaErrorInvalidValue;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cfg.gridDim = dim3(sms);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Layout<T, D>::kSmemBytes;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, attend_kernel<T, D>, map_k, map_v, p);
+    const cudaError_t e = launch_dependent(attend_kernel<T, D>, sms, kThreads, Layout<T, D>::kSmemBytes, stream, map_k, map_v, p);
     if (e != cudaSuccess) return e;
     const long long rows = static_cast<long long>(a.batch.sequences) * a.batch.queries * a.heads;
-    cfg.gridDim = dim3(static_cast<unsigned>((rows + kJoinWarps - 1) / kJoinWarps));
-    cfg.blockDim = dim3(kJoinWarps * 32);
-    cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p);
+    const bool many = rows > 32ll * sms; // one row per warp fills the SMs once up to here
+    const long long per_cta = kJoinWarps * (many ? 4 : 1);
+    const dim3 grid(static_cast<unsigned>((rows + per_cta - 1) / per_cta));
+    return launch_dependent(many ? join_kernel<T, D, 4, 2> : join_kernel<T, D, 1, 8>, grid, kJoinWarps * 32, 0, stream, p);
 }
 
 template <class T, int D> cudaError_t prepare()
@@ -1524,7 +1548,8 @@ template <class T, int D> cudaError_t prepare()
     static_assert(Layout<T, D>::kSmemBytes <= 232448, "shared memory of a CTA");
     // the join keeps the SMs' split between shared memory and L1: changing it between the two kernels of every
     // call drains the SMs
-    const cudaError_t c = cudaFuncSetAttribute(join_kernel<T, D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    cudaError_t c = cudaFuncSetAttribute(join_kernel<T, D, 1, 8>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (c == cudaSuccess) c = cudaFuncSetAttribute(join_kernel<T, D, 4, 2>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (c != cudaSuccess) return c;
     return cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<T, D>::kSmemBytes);
 }
