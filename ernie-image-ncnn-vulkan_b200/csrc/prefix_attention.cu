@@ -106,6 +106,14 @@ __device__ __forceinline__ float exp2_fast(float x)
     return y;
 }
 
+// The same, kept in its place among waits and arrivals.
+__device__ __forceinline__ float exp2_here(float x)
+{
+    float y;
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c)
 {
     float d;
@@ -897,6 +905,9 @@ __device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan 
 // K and V tiles are loaded in the order K0 K1 V0 K2 V1 K3 V2 ..., in which they are also used: load i goes to
 // tile i % 3 once load i - 3 has been used, which is a whole unit ahead of its own use for K and V alike
 // (with two buffers for K and one for V, V came 0.6 us late in every unit).
+// The two tiles of rows take turns at the exponentials, each with the SM's 16 per clock to itself, and have an
+// issuing warp of their own, so that neither waits for the other's scores or weights: in step they would
+// compete for the exponentials and then leave them idle together.
 template <int D> struct TileSmem
 {
     using L = Layout<__nv_bfloat16, D>;
@@ -915,8 +926,14 @@ template <int D> struct TileSmem
     __device__ uint32_t p_full(int g) const { return bars + 8u * (12 + g); }
     __device__ uint32_t pv_done(int g) const { return bars + 8u * (14 + g); }
     __device__ uint32_t done() const { return bars + 8u * 16; }
-    __device__ uint32_t tmem_slot() const { return bars + 8u * 17; }
-    static constexpr int kBarriers = 17;
+    __device__ uint32_t turn(int g) const { return bars + 8u * (17 + g); }
+    __device__ uint32_t tmem_slot() const { return bars + 8u * 19; }
+    static constexpr int kBarriers = 19;
+    // both issuers empty a K/V tile; the four softmax warps of a tile of rows arrive together
+    static __device__ uint32_t arrivals(int barrier)
+    {
+        return barrier < 3 ? 1 : barrier < 6 ? 2 : barrier < 8 ? 4 : barrier < 10 ? 1 : barrier < 14 ? 4 : barrier < 16 ? 1 : barrier == 16 ? 8 : 4;
+    }
 };
 
 // Descriptor of V [key][dim] as the second operand (dims x keys, dims contiguous): 128-byte rows of 64 dims,
@@ -982,14 +999,17 @@ __device__ __forceinline__ void tile_produce(const AttendArgs &p, int which, Wal
     if (!ok && lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
 }
 
-template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs &p, int which, Walk w, const TileSmem<D> &sm, uint32_t tmem)
+// The products of tile g of rows, by one thread.
+template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs &p, int which, Walk w, const TileSmem<D> &sm, uint32_t tmem, int g)
 {
     const List &l = p.list[which];
     constexpr uint32_t score_desc = idesc_bf16(128, 128);
     constexpr uint32_t value_idesc = idesc_bf16(128, D) | (1u << 16); // second operand with contiguous dims
-    unsigned n = 0, seen[2] = {0, 0}, parts[2] = {0, 0}; // units; units and parts of each tile of rows
+    unsigned n = 0, seen = 0, parts = 0; // units; units and parts of this tile of rows
     bool ok = true;
-    auto issue_s = [&](int g, unsigned unit) {
+    auto arrived = [&](unsigned load) { return ok = ok && mbar_wait(sm.full(load), sm.round(load)); };
+    auto issue_s = [&](unsigned unit) {
+        tc_fence_after();
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
         {
@@ -998,45 +1018,40 @@ template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs 
             umma_bf16(tmem + g * 128, ad, bd, score_desc, i > 0 ? 1u : 0u);
         }
         umma_commit(sm.s_full(g));
+        umma_commit(sm.empty(sm.k_load(unit)));
     };
     Part part;
     while (ok && next_part(p, which, w, part))
     {
-        const int groups = min(l.block, l.rows - part.block * l.block) > kTile ? 2 : 1;
-        for (int g = 0; g < groups && ok; ++g) ok = mbar_wait(sm.q_full(g), parts[g]++ & 1u);
-        if (ok) ok = mbar_wait(sm.full(sm.k_load(n)), sm.round(sm.k_load(n)));
-        if (!ok) break;
-        tc_fence_after();
-        for (int g = 0; g < groups; ++g) issue_s(g, n);
-        umma_commit(sm.empty(sm.k_load(n)));
-        for (int u = 0; u < part.units && ok; ++u, ++n)
+        if (min(l.block, l.rows - part.block * l.block) <= g * kTile)
+        {
+            // no rows in this tile: the other one's K and V pass by
+            for (int u = 0; u < part.units; ++u, ++n)
+            {
+                if (arrived(sm.k_load(n))) mbar_arrive(sm.empty(sm.k_load(n)));
+                if (arrived(sm.v_load(n))) mbar_arrive(sm.empty(sm.v_load(n)));
+            }
+            continue;
+        }
+        ok = mbar_wait(sm.q_full(g), parts++ & 1u);
+        if (arrived(sm.k_load(n))) issue_s(n);
+        for (int u = 0; u < part.units && ok; ++u, ++n, ++seen)
         {
             if (u + 1 < part.units)
             {
-                if (!(ok = mbar_wait(sm.full(sm.k_load(n + 1)), sm.round(sm.k_load(n + 1))))) break;
-                for (int g = 0; g < groups; ++g)
-                {
-                    if (!(ok = mbar_wait(sm.s_free(g), seen[g] & 1u))) break;
-                    tc_fence_after();
-                    issue_s(g, n + 1);
-                }
-                if (!ok) break;
-                umma_commit(sm.empty(sm.k_load(n + 1)));
+                if (!arrived(sm.k_load(n + 1)) || !(ok = mbar_wait(sm.s_free(g), seen & 1u))) break;
+                issue_s(n + 1);
             }
-            if (!(ok = mbar_wait(sm.full(sm.v_load(n)), sm.round(sm.v_load(n))))) break;
-            for (int g = 0; g < groups; ++g)
-            {
-                if (!(ok = mbar_wait(sm.p_full(g), seen[g]++ & 1u))) break;
-                tc_fence_after();
+            if (!arrived(sm.v_load(n)) || !(ok = mbar_wait(sm.p_full(g), seen & 1u))) break;
+            tc_fence_after();
 #pragma unroll
-                for (int i = 0; i < kTile / 16; ++i)
-                {
-                    const uint64_t ad = smem_desc_sw128(sm.p(g) + (i >> 2) * (kTile * 128)) + 2u * (i & 3);
-                    umma_bf16(tmem + 256 + g * 128, ad, value_desc(sm.kv(sm.v_load(n)) + i * 2048), value_idesc, (u > 0 || i > 0) ? 1u : 0u);
-                }
-                umma_commit(sm.pv_done(g));
+            for (int i = 0; i < kTile / 16; ++i)
+            {
+                const uint64_t ad = smem_desc_sw128(sm.p(g) + (i >> 2) * (kTile * 128)) + 2u * (i & 3);
+                umma_bf16(tmem + 256 + g * 128, ad, value_desc(sm.kv(sm.v_load(n)) + i * 2048), value_idesc, (u > 0 || i > 0) ? 1u : 0u);
             }
-            if (ok) umma_commit(sm.empty(sm.v_load(n)));
+            umma_commit(sm.pv_done(g));
+            umma_commit(sm.empty(sm.v_load(n)));
         }
     }
     if (!ok) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
@@ -1049,7 +1064,7 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Wal
     const int warp = threadIdx.x / 32 - 4, lane = threadIdx.x & 31, g = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quarter * 32) << 16), s_at = lanes + g * 128, o_at = lanes + 256 + g * 128;
     const float c = p.scale;
-    unsigned seen = 0; // units of this tile of rows
+    unsigned seen = 0, turns = 0; // units of this tile of rows; of them with the other tile at work too
     bool ok = true;
     unsigned n = 0; // units of the CTA
     Part part;
@@ -1106,14 +1121,16 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Wal
 #pragma unroll
             for (int k = 8; k < 128; k += 2) mx[(k >> 1) & 7] = max3(mx[(k >> 1) & 7], x[k], x[k + 1]);
             const float top = fmaxf(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], max3(mx[5], mx[6], mx[7])));
-            if (u > 0)
-            {
-                if (!(ok = warp_wait(sm.pv_done(g), (seen - 1) & 1u))) break;
-                tc_fence_after();
-            }
+            // PV_g of the last unit still reads P_g and adds to O_g: a rescale waits for it, otherwise the weights
+            // are worked out meanwhile and only their stores wait (waiting before the exponentials: 2.05 us per
+            // unit of two tiles)
+            bool waited = u == 0;
             if (u == 0) m = top;
             else if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) // NaN while neither is finite: no
             {
+                if (!(ok = warp_wait(sm.pv_done(g), (seen - 1) & 1u))) break;
+                tc_fence_after();
+                waited = true;
                 const float raised = fmaxf(m, top), alpha = raised == m ? 1.f : exp2_fast((m - raised) * c);
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i)
@@ -1131,21 +1148,32 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Wal
             const float offset = m == -INFINITY ? 0.f : -m * c;
             const float2 scale2 = make_float2(c, c), offset2 = make_float2(offset, offset);
             float2 part_sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+            uint32_t packed[64];
+            const bool both = rows > kTile;
+            if (both && !(ok = warp_wait(sm.turn(g), (turns & 1u) ^ (g ? 0u : 1u)))) break;
 #pragma unroll
-            for (int k8 = 0; k8 < 128; k8 += 8)
+            for (int k = 0; k < 128; k += 2)
             {
-                uint32_t packed[4];
-#pragma unroll
-                for (int t = 0; t < 8; t += 2)
-                {
-                    const float2 arg = __ffma2_rn(make_float2(x[k8 + t], x[k8 + t + 1]), scale2, offset2);
-                    const float e0 = exp2_fast(arg.x), e1 = exp2_fast(arg.y);
-                    part_sum[t >> 1] = __fadd2_rn(part_sum[t >> 1], make_float2(e0, e1));
-                    packed[t >> 1] = pack2(e0, e1);
-                }
-                const int chunk = (k8 & 63) >> 3;
-                st_shared_v4(sm.p(g) + (k8 >> 6) * (kTile * 128) + r * 128 + ((chunk ^ (r & 7)) << 4), packed[0], packed[1], packed[2], packed[3]);
+                const float2 arg = __ffma2_rn(make_float2(x[k], x[k + 1]), scale2, offset2);
+                const float e0 = exp2_here(arg.x), e1 = exp2_here(arg.y);
+                part_sum[(k >> 1) & 3] = __fadd2_rn(part_sum[(k >> 1) & 3], make_float2(e0, e1));
+                packed[k >> 1] = pack2(e0, e1);
             }
+            if (both)
+            {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sm.turn(1 - g));
+                ++turns;
+            }
+            if (!waited)
+            {
+                if (!(ok = warp_wait(sm.pv_done(g), (seen - 1) & 1u))) break;
+                tc_fence_after();
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                st_shared_v4(sm.p(g) + (i >> 3) * (kTile * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4), packed[4 * i], packed[4 * i + 1],
+                             packed[4 * i + 2], packed[4 * i + 3]);
             const float2 s4 = __fadd2_rn(__fadd2_rn(part_sum[0], part_sum[1]), __fadd2_rn(part_sum[2], part_sum[3]));
             sum += s4.x + s4.y;
             // values past the item's last key may be anything, NaN too: zeros, by both tiles' threads alike
@@ -1227,11 +1255,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     static_assert(2 * kWorkers * L::kRing + TileSmem<D>::kBarriers <= kThreads, "a thread per barrier");
     static_assert(2 * kWorkers * L::kRing * 8 + TileSmem<D>::kBarriers * 8 + 8 <= 1152, "barriers");
     {
-        // both ways' barriers: the softmax warps of a tile of rows arrive on three kinds, all of them on the last
+        // both ways' barriers
         const int t = threadIdx.x - 2 * kWorkers * L::kRing;
         if (t < 0) mbar_init(bars + 8 * threadIdx.x, 1);
         else if (t < TileSmem<D>::kBarriers)
-            mbar_init(sm.bars + 8 * t, t == 16 ? 8 : (t >= 6 && t < 8) || (t >= 10 && t < 14) ? 4 : 1);
+            mbar_init(sm.bars + 8 * t, TileSmem<D>::arrivals(t));
         fence_barrier_init();
         if (threadIdx.x == kThreads - 1)
         {
@@ -1261,11 +1289,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             {
                 const Walk w = walk_of(p, plan, shared, 0);
                 if (warp == 0) tile_produce<D>(p, plan.which, w, &map_k, &map_v, sm);
-                else if (warp == 1)
+                else if (warp <= 2)
                 {
                     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(base_ptr + (sm.tmem_slot() - base));
-                    if ((threadIdx.x & 31) == 0) tile_multiply<D>(p, plan.which, w, sm, tmem);
+                    if ((threadIdx.x & 31) == 0) tile_multiply<D>(p, plan.which, w, sm, tmem, warp - 1);
                     __syncwarp();
+                    if (warp == 2) return;
                     if (!warp_wait(sm.done(), 0) && (threadIdx.x & 31) == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
                     tc_fence_after();
                     tmem_dealloc(tmem, 512);
