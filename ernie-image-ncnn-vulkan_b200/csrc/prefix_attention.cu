@@ -87,11 +87,11 @@ struct AttendArgs
 
 template <class T, int D> struct Layout
 {
-    static constexpr int kSlotKeys = sizeof(T) == 2 ? 16 : 8;                     // a K/V slot: one step of a streaming warp
-    static constexpr int kColumns = D * static_cast<int>(sizeof(T)) / 128;        // 128-byte column blocks of a row
-    static constexpr int kSlotHalf = kSlotKeys * D * static_cast<int>(sizeof(T)); // K or V of a slot
-    static constexpr int kRing = D == 128 ? 3 : 7;                                // slots of a warp
-    static constexpr int kStreamBytes = kWorkers * kRing * 2 * kSlotHalf;
+    static constexpr int kSlotKeys = sizeof(T) == 2 ? 16 : 8;                      // one step of a streaming warp
+    static constexpr int kColumns = D * static_cast<int>(sizeof(T)) / 128;         // 128-byte column blocks of a row
+    static constexpr int kSlotBytes = kSlotKeys * D * static_cast<int>(sizeof(T)); // a slot: a step's K or its V
+    static constexpr int kRing = D == 128 ? 7 : 11;                                // slots of a warp
+    static constexpr int kStreamBytes = kWorkers * kRing * kSlotBytes;
     static constexpr int kTileBytes = kTile * D * 2;       // a Q, K or V tile
     static constexpr int kWeightBytes = kTile * kTile * 2; // a P tile
     static constexpr int kTileModeBytes = 5 * kTileBytes + 2 * kWeightBytes;
@@ -162,6 +162,19 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Whether the phase with the given parity has completed, without waiting (try_wait may suspend the thread).
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity)
+{
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(done)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
+    return done != 0;
 }
 
 // A whole warp's bounded wait, with one answer for all its lanes.
@@ -426,7 +439,8 @@ __device__ __forceinline__ int pool_row(const AttendArgs &p, int which, const Pa
 }
 
 // ---------------------------------------------------------------- stream
-// A slot holds K and V of kSlotKeys keys, 128-byte rows in swizzled column blocks.
+// A slot holds K or V of kSlotKeys keys, 128-byte rows in swizzled column blocks. A warp's ring takes K and V of
+// a step in turn, so that K's slot is free again once the scores are done.
 
 // BF16: a warp's 16 rows in mma.sync fragments: rows lane/4 and lane/4 + 8; a lane's columns are
 // 2 (lane % 4) and the next of every eight.
@@ -498,80 +512,81 @@ template <class T, int D> struct Ring
 {
     using L = Layout<T, D>;
     uint32_t slots, bars; // of the CTA
-    __device__ uint32_t slot(int worker, unsigned n) const { return slots + (worker * L::kRing + n % L::kRing) * (2 * L::kSlotHalf); }
+    __device__ uint32_t slot(int worker, unsigned n) const { return slots + (worker * L::kRing + n % L::kRing) * L::kSlotBytes; }
     __device__ uint32_t full(int worker, unsigned n) const { return bars + 8 * (worker * L::kRing + n % L::kRing); }
     __device__ uint32_t empty(int worker, unsigned n) const { return full(worker, n) + 8 * kWorkers * L::kRing; }
     static __device__ uint32_t round(unsigned n) { return (n / L::kRing) & 1u; }
 };
 
-// Slots of a part.
-template <class T, int D> __device__ __forceinline__ int slots_of(const Part &part, int unit_shift)
+// Steps of a part.
+template <class T, int D> __device__ __forceinline__ int steps_of_part(const Part &part, int unit_shift)
 {
     constexpr int keys = Layout<T, D>::kSlotKeys;
     const int end = min(static_cast<long long>(part.item.keys), static_cast<long long>(part.first_unit + part.units) << unit_shift);
     return (end - (part.first_unit << unit_shift) + keys - 1) / keys;
 }
 
-// Four producer warps, each feeding two workers with 16 lanes: a lane issues one box of every slot.
+// Four producer warps, each feeding two workers: eight lanes for a worker's K and eight for its V, which run ahead
+// by themselves; a lane issues one box of every slot of theirs.
 template <class T, int D>
 __device__ __forceinline__ void stream_produce(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const CUtensorMap *map_k,
                                                const CUtensorMap *map_v, const Ring<T, D> &ring)
 {
     using L = Layout<T, D>;
-    const int lane = threadIdx.x & 31, sub = lane & 15, worker = (threadIdx.x / 32) * 2 + (lane >> 4), shift = p.list[plan.which].unit_shift;
-    const unsigned half_mask = 0xffffu << (lane & 16);
+    const int lane = threadIdx.x & 31, sub = lane & 7, leader = lane & 24, worker = (threadIdx.x / 32) * 2 + (lane >> 4);
+    const int shift = p.list[plan.which].unit_shift;
+    const unsigned mine = 0xffu << leader;
+    const CUtensorMap *map = lane & 8 ? map_v : map_k;
+    const bool fine = p.granule < L::kSlotKeys; // two boxes of eight keys to a column block
+    const int granule = fine ? sub & 1 : 0, column = fine ? sub >> 1 : sub, granule_shift = fine ? 3 : 31 - __clz(L::kSlotKeys);
+    const bool has_box = column < L::kColumns;
+    const int first_column = column * (128 / static_cast<int>(sizeof(T)));
+    const uint32_t into = column * (L::kSlotKeys * 128) + granule * (8 * 128);
     Walk w = walk_of(p, plan, shared, worker);
-    const int granules = L::kSlotKeys / p.granule;
-    const int granule = sub % granules, column = (sub / granules) % L::kColumns, value = sub / (granules * L::kColumns);
-    const bool has_box = value < 2;
-    const uint32_t box_bytes = p.granule * 128;
-    const uint32_t into = (value ? L::kSlotHalf : 0) + column * (L::kSlotKeys * 128) + granule * box_bytes;
-    const CUtensorMap *map = value ? map_v : map_k;
-    unsigned n = 0; // slots so far
+    unsigned n = (lane & 8) >> 3; // the next slot: even ones K's, odd ones V's
     int left = 0, key = 0, row = 0;
     bool bad = false;
     Part part;
     bool more = next_part(p, plan.which, w, part);
     if (more)
     {
-        left = slots_of<T, D>(part, shift);
+        left = steps_of_part<T, D>(part, shift);
         key = part.first_unit << shift;
-        row = has_box ? pool_row(p, plan.which, part, key + granule * p.granule, bad) : 0;
+        row = has_box ? pool_row(p, plan.which, part, key + granule * 8, bad) : 0;
     }
     long long since = clock64();
     while (__any_sync(0xffffffffu, more))
     {
-        const bool free = __shfl_sync(0xffffffffu, static_cast<int>(mbar_try_wait(ring.empty(worker, n), ring.round(n) ^ 1u)), lane & 16);
-        // neither ring has room: out of the workers' issue slots for a while (a slot lasts several times as long)
-        if (!__any_sync(0xffffffffu, more && free)) __nanosleep(64);
+        const bool free = __shfl_sync(0xffffffffu, static_cast<int>(mbar_test(ring.empty(worker, n), ring.round(n) ^ 1u)), leader);
+        // no ring has room: out of the workers' issue slots for a while (a step lasts several times as long)
+        if (!__any_sync(0xffffffffu, more && free)) __nanosleep(32);
         if (more && free)
         {
-            const int kept = min(granules, (part.item.keys - key + p.granule - 1) / p.granule); // granules with keys
-            if (sub == 0) mbar_arrive_expect_tx(ring.full(worker, n), kept * L::kColumns * 2 * box_bytes);
-            __syncwarp(half_mask);
-            if (has_box && granule < kept)
-                tma_load_2d(ring.slot(worker, n) + into, map, ring.full(worker, n), column * (128 / static_cast<int>(sizeof(T))), row);
-            ++n;
+            const int kept = min(L::kSlotKeys >> granule_shift, (part.item.keys - key + (1 << granule_shift) - 1) >> granule_shift); // granules with keys
+            if (lane == leader) mbar_arrive_expect_tx(ring.full(worker, n), (kept * L::kColumns * 128) << granule_shift);
+            __syncwarp(mine);
+            if (has_box && granule < kept) tma_load_2d(ring.slot(worker, n) + into, map, ring.full(worker, n), first_column, row);
+            n += 2;
             key += L::kSlotKeys;
             if (--left == 0)
             {
                 more = next_part(p, plan.which, w, part);
                 if (more)
                 {
-                    left = slots_of<T, D>(part, shift);
+                    left = steps_of_part<T, D>(part, shift);
                     key = part.first_unit << shift;
                 }
             }
-            if (more && has_box) row = pool_row(p, plan.which, part, key + granule * p.granule, bad);
+            if (more && has_box) row = pool_row(p, plan.which, part, key + granule * 8, bad);
             since = clock64();
         }
         else if (more && clock64() - since > kWaitLimitCycles)
         {
-            if (sub == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+            if (lane == leader) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
             more = false;
         }
         __syncwarp();
-        more = __shfl_sync(0xffffffffu, static_cast<int>(more), lane & 16);
+        more = __shfl_sync(0xffffffffu, static_cast<int>(more), leader);
     }
     if (bad) report_range(p.a.batch.error_flag);
 }
@@ -585,7 +600,7 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
     const List &l = p.list[plan.which];
     const int worker = threadIdx.x / 32 - 4, lane = threadIdx.x & 31, r0 = lane >> 2, r1 = r0 + 8;
     Walk w = walk_of(p, plan, shared, worker);
-    unsigned n = 0; // slots so far
+    unsigned n = 0; // slots so far: K and V of a step in turn
     Part part;
     while (next_part(p, plan.which, w, part))
     {
@@ -600,18 +615,20 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
         for (int i = 0; i < D / 8; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-        const int slots = slots_of<T, D>(part, l.unit_shift);
+        const int steps = steps_of_part<T, D>(part, l.unit_shift);
         int key0 = part.first_unit << l.unit_shift;
-        for (int u = 0; u < slots; ++u, ++n, key0 += L::kSlotKeys)
+        for (int u = 0; u < steps; ++u, n += 2, key0 += L::kSlotKeys)
         {
             if (!warp_wait(ring.full(worker, n), ring.round(n)))
             {
                 if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
                 return;
             }
-            const uint32_t k = ring.slot(worker, n);
+            const bool v_there = mbar_test(ring.full(worker, n + 1), ring.round(n + 1));
             float s[R::kTiles][4] = {};
-            x.scores(k, lane, s);
+            x.scores(ring.slot(worker, n), lane, s);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ring.empty(worker, n));
             if (key0 + L::kSlotKeys > all_see)
             {
 #pragma unroll
@@ -662,9 +679,14 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
                 l0 += s[t][0] + s[t][1];
                 l1 += s[t][2] + s[t][3];
             }
-            x.weigh(k + L::kSlotHalf, lane, s, part.item.keys - key0, o);
+            if (!__all_sync(0xffffffffu, v_there) && !warp_wait(ring.full(worker, n + 1), ring.round(n + 1)))
+            {
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                return;
+            }
+            x.weigh(ring.slot(worker, n + 1), lane, s, part.item.keys - key0, o);
             __syncwarp();
-            if (lane == 0) mbar_arrive(ring.empty(worker, n));
+            if (lane == 0) mbar_arrive(ring.empty(worker, n + 1));
         }
         // a lane's sums cover its columns only
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
@@ -690,7 +712,7 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
 }
 
 // FP32: R rows of a warp, in two halves of 16 lanes; a lane holds every sixteenth group of four dims of the
-// queries and values of its half's rows, two rows to a packed FMA. A step takes four keys: partial scores of
+// queries and values of its half's rows, two dims to a packed FMA. A step takes four keys: partial scores of
 // all rows, then a scatter of their sums over the 16 lanes (key lane/4 % 4 and a quarter of the rows each),
 // the weights there, and their way back by shuffles. Shared memory and shuffles deliver a value per lane and
 // cycle, so a value of K or V has to serve many rows: with eight rows to a lane a slot of eight keys takes
@@ -699,7 +721,7 @@ template <int D, int R>
 __device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const Ring<float, D> &ring)
 {
     using L = Layout<float, D>;
-    constexpr int kSlotKeys = L::kSlotKeys, kKeys = 4, kRows = R / 2, kPairs = kRows / 2, kGroups = D / 64, kDims = 4 * kGroups;
+    constexpr int kSlotKeys = L::kSlotKeys, kKeys = 4, kRows = R / 2, kGroups = D / 64, kPairs = 2 * kGroups;
     constexpr int kHeld = kRows >= 4 ? kRows / 4 : 1; // rows whose weights a lane works out
     const List &l = p.list[plan.which];
     const int worker = threadIdx.x / 32 - 4, lane = threadIdx.x & 31, half = lane & 16, share = lane & 15, first_row = half ? kRows : 0;
@@ -707,12 +729,12 @@ __device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan 
     // the lane of key 0 that holds a row
     auto holder = [&](int row) { return half + (kRows >= 4 ? row / kHeld : row * 2); };
     Walk w = walk_of(p, plan, shared, worker);
-    unsigned n = 0; // slots so far
+    unsigned n = 0; // slots so far: K and V of a step in turn
     Part part;
     while (next_part(p, plan.which, w, part))
     {
         if (lane == 0) write_meta(l, w, part);
-        float2 q[kPairs][kDims], o[kPairs][kDims];
+        float2 q[kRows][kPairs], o[kRows][kPairs]; // two neighbouring dims each
         int all_see = INT_MAX;
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
@@ -724,9 +746,8 @@ __device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan 
             for (int j = 0; j < kGroups; ++j)
             {
                 const float4 x = row.keys ? query[j * 16] : make_float4(0.f, 0.f, 0.f, 0.f);
-                const float y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) (i & 1 ? q[i / 2][4 * j + e].y : q[i / 2][4 * j + e].x) = y[e];
+                q[i][2 * j] = make_float2(x.x, x.y);
+                q[i][2 * j + 1] = make_float2(x.z, x.w);
             }
         }
         all_see = __reduce_min_sync(0xffffffffu, all_see);
@@ -740,55 +761,58 @@ __device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan 
             c[i] = sum[i] = 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < kPairs; ++i)
+        for (int i = 0; i < kRows; ++i)
 #pragma unroll
-            for (int d = 0; d < kDims; ++d) o[i][d] = make_float2(0.f, 0.f);
-        const int slots = slots_of<float, D>(part, l.unit_shift);
+            for (int d = 0; d < kPairs; ++d) o[i][d] = make_float2(0.f, 0.f);
+        const int steps = steps_of_part<float, D>(part, l.unit_shift);
         int key0 = part.first_unit << l.unit_shift;
-        for (int u = 0; u < slots; ++u, ++n)
+        for (int u = 0; u < steps; ++u, n += 2)
         {
             if (!warp_wait(ring.full(worker, n), ring.round(n)))
             {
                 if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
                 return;
             }
+            bool v_there = mbar_test(ring.full(worker, n + 1), ring.round(n + 1));
+#pragma unroll
             for (int first = 0; first < kSlotKeys; first += kKeys, key0 += kKeys)
             {
                 const int valid = part.item.keys - key0; // what lies past the last key may be anything, NaN too
                 if (valid <= 0) continue;
-                const uint32_t k = ring.slot(worker, n), v = k + L::kSlotHalf;
-                // dims 64 j + 4 share .. + 3 of the step's key i: column block, then the key's row, swizzled
-                auto at = [&](int j, int i) {
-                    const int chunk = 16 * j + share, key = first + i;
-                    return (chunk >> 3) * (kSlotKeys * 128) + key * 128 + (((chunk & 7) ^ key) << 4);
-                };
-                float2 s2[kKeys][kPairs];
-#pragma unroll
-                for (int i = 0; i < kKeys; ++i)
-                {
-#pragma unroll
-                    for (int r = 0; r < kPairs; ++r) s2[i][r] = make_float2(0.f, 0.f);
-#pragma unroll
-                    for (int j = 0; j < kGroups; ++j)
-                    {
-                        const float4 x = ld_shared_v4(k + at(j, i));
-                        const float y[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int r = 0; r < kPairs; ++r) s2[i][r] = __ffma2_rn(q[r][4 * j + e], make_float2(y[e], y[e]), s2[i][r]);
-                    }
-                }
-                // sums over the half's lanes, scattered: value i * kRows + row
+                const uint32_t k = ring.slot(worker, n), v = ring.slot(worker, n + 1);
+                // dims 64 j + 4 share .. + 3 of the step's key i: column block, the key's row and its swizzle in one
+                // exclusive or (slots are 1024-byte aligned)
+                const uint32_t lane_part = (share >> 3) * (kSlotKeys * 128) + ((share & 7) << 4);
+                auto at = [&](uint32_t slot, int j, int i) { return ((slot + lane_part) ^ ((first + i) * 144)) + j * (2 * kSlotKeys * 128); };
+                // partial sums over the lane's dims, value i * kRows + row; two keys at a time, for the registers
                 float s[kKeys * kRows];
 #pragma unroll
-                for (int i = 0; i < kKeys; ++i)
+                for (int i = 0; i < kKeys; i += 2)
+                {
+                    float2 s2[2][kRows];
 #pragma unroll
-                    for (int r = 0; r < kPairs; ++r)
+                    for (int e = 0; e < 2; ++e)
                     {
-                        s[i * kRows + 2 * r] = s2[i][r].x;
-                        s[i * kRows + 2 * r + 1] = s2[i][r].y;
+#pragma unroll
+                        for (int r = 0; r < kRows; ++r) s2[e][r] = make_float2(0.f, 0.f);
+#pragma unroll
+                        for (int j = 0; j < kGroups; ++j)
+                        {
+                            const float4 x = ld_shared_v4(at(k, j, i + e));
+#pragma unroll
+                            for (int r = 0; r < kRows; ++r)
+                            {
+                                s2[e][r] = __ffma2_rn(q[r][2 * j], make_float2(x.x, x.y), s2[e][r]);
+                                s2[e][r] = __ffma2_rn(q[r][2 * j + 1], make_float2(x.z, x.w), s2[e][r]);
+                            }
+                        }
                     }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int r = 0; r < kRows; ++r) s[(i + e) * kRows + r] = s2[e][r].x + s2[e][r].y;
+                }
+                // their sums over the half's lanes, scattered
                 int values = kKeys * kRows;
 #pragma unroll
                 for (int step = 8; step > 0; step /= 2)
@@ -833,12 +857,11 @@ __device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan 
                         sum[i] *= f[i];
                     }
 #pragma unroll
-                    for (int r = 0; r < kPairs; ++r)
+                    for (int r = 0; r < kRows; ++r)
                     {
-                        const float f0 = __shfl_sync(0xffffffffu, f[2 * r % kHeld], holder(2 * r));
-                        const float f1 = __shfl_sync(0xffffffffu, f[(2 * r + 1) % kHeld], holder(2 * r + 1));
+                        const float g = __shfl_sync(0xffffffffu, f[r % kHeld], holder(r));
 #pragma unroll
-                        for (int d = 0; d < kDims; ++d) o[r][d] = make_float2(o[r][d].x * f0, o[r][d].y * f1);
+                        for (int d = 0; d < kPairs; ++d) o[r][d] = make_float2(o[r][d].x * g, o[r][d].y * g);
                     }
                 }
 #pragma unroll
@@ -847,31 +870,37 @@ __device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan 
                     s[i] = exp2_fast(fmaf(s[i], p.scale, c[i]));
                     sum[i] += s[i];
                 }
+                if (!__all_sync(0xffffffffu, v_there))
+                {
+                    if (!warp_wait(ring.full(worker, n + 1), ring.round(n + 1)))
+                    {
+                        if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                        return;
+                    }
+                    v_there = true;
+                }
 #pragma unroll
                 for (int i = 0; i < kKeys; ++i)
                 {
-                    float2 weight[kPairs];
+                    float weight[kRows];
 #pragma unroll
-                    for (int r = 0; r < kPairs; ++r)
-                    {
-                        weight[r].x = __shfl_sync(0xffffffffu, s[2 * r % kHeld], holder(2 * r) + 4 * i);
-                        weight[r].y = __shfl_sync(0xffffffffu, s[(2 * r + 1) % kHeld], holder(2 * r + 1) + 4 * i);
-                    }
+                    for (int r = 0; r < kRows; ++r) weight[r] = __shfl_sync(0xffffffffu, s[r % kHeld], holder(r) + 4 * i);
                     if (i >= valid) break;
 #pragma unroll
                     for (int j = 0; j < kGroups; ++j)
                     {
-                        const float4 x = ld_shared_v4(v + at(j, i));
-                        const float y[4] = {x.x, x.y, x.z, x.w};
+                        const float4 x = ld_shared_v4(at(v, j, i));
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-#pragma unroll
-                            for (int r = 0; r < kPairs; ++r) o[r][4 * j + e] = __ffma2_rn(weight[r], make_float2(y[e], y[e]), o[r][4 * j + e]);
+                        for (int r = 0; r < kRows; ++r)
+                        {
+                            o[r][2 * j] = __ffma2_rn(make_float2(weight[r], weight[r]), make_float2(x.x, x.y), o[r][2 * j]);
+                            o[r][2 * j + 1] = __ffma2_rn(make_float2(weight[r], weight[r]), make_float2(x.z, x.w), o[r][2 * j + 1]);
+                        }
                     }
                 }
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(ring.empty(worker, n));
+            if (lane < 2) mbar_arrive(ring.empty(worker, n + lane));
         }
         const int rows = min(l.block, l.rows - part.block * l.block); // of the item
         const size_t place = static_cast<size_t>(part.place) * l.part_rows;
@@ -891,8 +920,7 @@ __device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan 
 #pragma unroll
             for (int j = 0; j < kGroups; ++j)
             {
-                const float2 *x = &o[i / 2][4 * j];
-                dst[j * 16] = i & 1 ? make_float4(x[0].y, x[1].y, x[2].y, x[3].y) : make_float4(x[0].x, x[1].x, x[2].x, x[3].x);
+                dst[j * 16] = make_float4(o[i][2 * j].x, o[i][2 * j].y, o[i][2 * j + 1].x, o[i][2 * j + 1].y);
             }
         }
     }
@@ -1247,13 +1275,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t *base_ptr = smem_raw + (base - raw);
     const uint32_t bars = base + L::kBody;
-    PlanShared &shared = *reinterpret_cast<PlanShared *>(base_ptr + L::kBody + 1152);
-    static_assert(sizeof(PlanShared) <= 2048 - 1152, "plan");
+    PlanShared &shared = *reinterpret_cast<PlanShared *>(base_ptr + L::kBody + 1776);
+    static_assert(sizeof(PlanShared) <= 2048 - 1776, "plan");
     const int warp = threadIdx.x / 32;
     const TileSmem<D> sm{base, bars + 2 * kWorkers * L::kRing * 8};
     const Ring<T, D> ring{base, bars};
     static_assert(2 * kWorkers * L::kRing + TileSmem<D>::kBarriers <= kThreads, "a thread per barrier");
-    static_assert(2 * kWorkers * L::kRing * 8 + TileSmem<D>::kBarriers * 8 + 8 <= 1152, "barriers");
+    static_assert(2 * kWorkers * L::kRing * 8 + TileSmem<D>::kBarriers * 8 + 8 <= 1776, "barriers");
     {
         // both ways' barriers
         const int t = threadIdx.x - 2 * kWorkers * L::kRing;

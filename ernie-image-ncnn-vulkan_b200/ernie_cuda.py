@@ -288,10 +288,11 @@ class Buffer:
 
 
 def device_pointer(a):
-    """Address of device memory: a Buffer, an address, None, or an array with data_ptr() (a torch tensor)."""
-    if a is None or isinstance(a, int):
-        return a
-    return a.ptr if isinstance(a, Buffer) else a.data_ptr()
+    """Address of device memory: an array with data_ptr() (a torch tensor), a Buffer, an address or None."""
+    try:
+        return a.data_ptr()
+    except AttributeError:
+        return a.ptr if isinstance(a, Buffer) else a
 
 
 class PagedKv:
