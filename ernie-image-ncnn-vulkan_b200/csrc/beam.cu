@@ -14,7 +14,11 @@
 //
 // Sums: a lane's reference is c = x L rounded, for its largest logit x so far and L = log2(e) rounded, and its
 // sum that of 2^(x L - c), one FMA and one exponential each. With S and C joined in 64 bits the logarithm of
-// the row's sum is (C + log2 S) / L: the roundings of c and, to first order, of L cancel.
+// the row's sum is (C + log2 S) / L: the roundings of c and, to first order, of L cancel. That needs x L - c to be
+// small, which the rounding of c itself exceeds for huge x; so c is kept within +-2^20, where it is off by 2^-4 at
+// most. Any c serves as long as nothing over- or underflows, so a lane that holds masked logits only (the type's
+// lowest value) adds its zeros to the row's sum as it should; a row whose common reference is at the limit, be it
+// masked as a whole or of logits near a million, is summed up again relative to its largest logit.
 #include "decode.h"
 #include "ptx.cuh"
 #include <cfloat>
@@ -31,6 +35,7 @@ constexpr int kListEntries = 4096; // of a group's lists in the joining CTA's sh
 constexpr int kRing = 3;           // tiles of a warp in shared memory: one in work, two in flight
 constexpr int kRingBytes = kWarps * kRing * kVectors * 32 * 16;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kSteady = 1048576.f; // the references' limit
 
 struct Plan
 {
@@ -207,7 +212,7 @@ template <class T> __global__ void __launch_bounds__(kThreads, 2) stretch_kernel
         const float best = fmaxf(max3(mine[0], mine[1], mine[2]), mine[3]);
         if (best > top)
         {
-            const float raised = best * kLog2e;
+            const float raised = fminf(fmaxf(best * kLog2e, -kSteady), kSteady);
             sum *= exp2_fast(c - raised); // 0 while nothing has been seen
             c = raised;
             top = best;
@@ -318,6 +323,31 @@ template <class T> __global__ void __launch_bounds__(kThreads, 2) stretch_kernel
     }
 }
 
+// By a warp: the largest logit of the stretches' lists, and the sum of exp(logit - top) over the row.
+__device__ __forceinline__ float row_top(const float *values, int stretches, int beams)
+{
+    float top = -INFINITY;
+    for (int c = threadIdx.x % 32; c < stretches; c += 32) top = fmaxf(top, values[c * beams]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top;
+}
+__device__ __noinline__ double row_sum(const BeamSelectArgs &a, long long row, float top)
+{
+    double sum = 0.0;
+#pragma unroll 8
+    for (int t = threadIdx.x % 32; t < a.vocab; t += 32)
+    {
+        const long long at = row * a.ld + t;
+        const float x = a.bf16 ? __uint_as_float(static_cast<unsigned>(static_cast<const unsigned short *>(a.logits)[at]) << 16)
+                               : static_cast<const float *>(a.logits)[at];
+        sum += exp2f((x - top) * kLog2e);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return sum;
+}
+
 // One CTA per group, a warp per beam: the beam's list from its stretches' lists, then one warp merges the
 // beams' lists (lane = beam).
 __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
@@ -376,8 +406,15 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(full, sum, o);
-        const double lse = (static_cast<double>(reference) + log2(sum)) / static_cast<double>(kLog2e);
-        if (isfinite(lse))
+        // the logarithm of the row's sum is base + log_sum
+        double base = 0.0, log_sum = (static_cast<double>(reference) + log2(sum)) / static_cast<double>(kLog2e);
+        if (!(fabsf(reference) < kSteady) && sum == sum)
+        {
+            const float top = row_top(values, plan.stretches, k);
+            base = top;
+            log_sum = isfinite(top) ? log(row_sum(a, row, top)) : NAN; // only -inf, or a +inf
+        }
+        if (isfinite(log_sum))
         {
             // lane's lists: stretches lane and lane + 32, each with the place of its next entry
             int at[2] = {0, 0};
@@ -401,7 +438,7 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
                 const float v = __shfl_sync(full, bv, __ffs(__ballot_sync(full, bi == best)) - 1);
                 if (lane == 0)
                 {
-                    total[warp][r] = static_cast<double>(score) + (static_cast<double>(v) - lse);
+                    total[warp][r] = static_cast<double>(score) + ((static_cast<double>(v) - base) - log_sum);
                     token[warp][r] = best;
                 }
             }

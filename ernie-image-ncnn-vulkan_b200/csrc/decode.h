@@ -129,6 +129,8 @@ struct PrefixAttentionArgs
     void *workspace = nullptr;
 };
 size_t prefix_attention_workspace(const PagedLayer &kv, const PagedBatch &batch, int heads, int sms);
+// Whether the kernel's 32-bit counts of work can hold the longest lengths that the tables allow.
+bool prefix_attention_countable(const PagedLayer &kv, const PagedBatch &batch, int heads);
 int launch_prefix_attention(const PrefixAttentionArgs &args, int sms, cudaStream_t stream);
 int prepare_prefix_attention_kernels();
 

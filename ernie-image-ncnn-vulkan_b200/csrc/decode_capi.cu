@@ -28,6 +28,15 @@ int check_precision(int precision)
     return ERNIE_CUDA_OK;
 }
 
+// What a call writes may not lie in the cache that it works on.
+int check_outside(const ernie_cuda_paged_kv *kv, const PagedLayer &layer, const void *p, size_t bytes)
+{
+    const size_t pool = layer.layer_elements() * (layer.bf16 ? 2 : 4) * kv->layers;
+    if (overlap(kv->k, pool, p, bytes) || overlap(kv->v, pool, p, bytes))
+        return fail(ERNIE_CUDA_ERROR, "A result or the workspace overlaps the paged cache");
+    return ERNIE_CUDA_OK;
+}
+
 int check_kv(const ernie_cuda_paged_kv *kv, int layer, PagedLayer &out)
 {
     if (!kv || !kv->k || !kv->v) return fail(ERNIE_CUDA_ERROR, "null argument");
@@ -95,6 +104,13 @@ int check_rows(const PagedBatch &b, int heads)
     return ERNIE_CUDA_OK;
 }
 
+int check_work(const PagedBatch &b, const PagedLayer &kv, int heads)
+{
+    if (!prefix_attention_countable(kv, b, heads))
+        return fail(ERNIE_CUDA_ERROR, "The batch's tables hold too many tokens for one attention call");
+    return ERNIE_CUDA_OK;
+}
+
 // A position or length past 2^31 - 1 tokens cannot be addressed by the 32-bit lengths.
 int check_tokens(const PagedBatch &b, const PagedLayer &kv)
 {
@@ -133,6 +149,7 @@ extern "C" int ernie_cuda_paged_append(ernie_cuda_context *ctx, const ernie_cuda
     const size_t slots = static_cast<size_t>(a.batch.sequences) * a.batch.queries;
     if (overlap(qkv, ((slots - 1) * ld + width) * element, q_out, slots * heads * a.kv.dim * (a.kv.bf16 ? 2 : 4)))
         return fail(ERNIE_CUDA_ERROR, "The queries may not overlap the projection");
+    ERNIE_TRY(check_outside(kv, a.kv, q_out, slots * heads * a.kv.dim * (a.kv.bf16 ? 2 : 4)));
     if (!ctx) return fail(ERNIE_CUDA_ERROR, "null context");
     a.qkv = qkv;
     a.qkv_bf16 = precision == ERNIE_PRECISION_BF16;
@@ -159,6 +176,7 @@ extern "C" int ernie_cuda_prefix_attention_workspace(ernie_cuda_context *ctx, co
     ERNIE_TRY(check_tokens(b, layer));
     ERNIE_TRY(check_heads(heads, layer));
     ERNIE_TRY(check_rows(b, heads));
+    ERNIE_TRY(check_work(b, layer, heads));
     if (!ctx) return fail(ERNIE_CUDA_ERROR, "null context");
     *bytes = prefix_attention_workspace(layer, b, heads, ctx->num_sms);
     return ERNIE_CUDA_OK;
@@ -174,12 +192,15 @@ extern "C" int ernie_cuda_prefix_attention(ernie_cuda_context *ctx, const ernie_
     ERNIE_TRY(check_tokens(a.batch, a.kv));
     ERNIE_TRY(check_heads(heads, a.kv));
     ERNIE_TRY(check_rows(a.batch, heads));
+    ERNIE_TRY(check_work(a.batch, a.kv, heads));
     if (!q || !out || !workspace) return fail(ERNIE_CUDA_ERROR, "null argument");
     if (!aligned(q, 16) || !aligned(out, 16) || !aligned(workspace, 16))
         return fail(ERNIE_CUDA_ERROR, "Queries, output and workspace must be 16-byte aligned");
     const size_t bytes = static_cast<size_t>(a.batch.sequences) * a.batch.queries * heads * a.kv.dim * (a.kv.bf16 ? 2 : 4);
     if (overlap(q, bytes, out, bytes) || overlap(workspace, workspace_bytes, out, bytes) || overlap(workspace, workspace_bytes, q, bytes))
         return fail(ERNIE_CUDA_ERROR, "Queries, output and workspace may not overlap");
+    ERNIE_TRY(check_outside(kv, a.kv, out, bytes));
+    ERNIE_TRY(check_outside(kv, a.kv, workspace, workspace_bytes));
     if (!ctx) return fail(ERNIE_CUDA_ERROR, "null context");
     if (workspace_bytes < prefix_attention_workspace(a.kv, a.batch, heads, ctx->num_sms))
         return fail(ERNIE_CUDA_ERROR, "The attention's workspace is too small");
@@ -217,6 +238,20 @@ extern "C" int ernie_cuda_beam_select(ernie_cuda_context *ctx, const void *logit
         !aligned(parents, 4) || !aligned(tokens, 4) || !aligned(new_scores, 4) || !aligned(new_finished, 4) ||
         !aligned(workspace, 16))
         return fail(ERNIE_CUDA_ERROR, "Beam selection's arrays are not aligned to their elements, or its workspace to 16 bytes");
+    {
+        // every output and the workspace lie apart from all else, but for the new state in place of the old one
+        const size_t list = static_cast<size_t>(groups) * beams * 4, element = precision == ERNIE_PRECISION_BF16 ? 2 : 4;
+        const size_t table = ((static_cast<size_t>(groups) * beams - 1) * ld + vocab) * element;
+        const void *arrays[8] = {parents, tokens, new_scores, new_finished, workspace, scores, finished, logits};
+        const size_t sizes[8] = {list, list, list, list, workspace_bytes, list, list, table};
+        for (int i = 0; i < 5; ++i)
+            for (int j = i + 1; j < 8; ++j)
+            {
+                const bool in_place = (i == 2 && j == 5) || (i == 3 && j == 6);
+                if (!(in_place && arrays[i] == arrays[j]) && overlap(arrays[i], sizes[i], arrays[j], sizes[j]))
+                    return fail(ERNIE_CUDA_ERROR, "Beam selection's arrays overlap");
+            }
+    }
     if (!ctx) return fail(ERNIE_CUDA_ERROR, "null context");
     if (workspace_bytes < beam_select_workspace(groups, beams, vocab, ctx->num_sms))
         return fail(ERNIE_CUDA_ERROR, "The selection's workspace is too small");
@@ -247,7 +282,8 @@ extern "C" int ernie_cuda_beam_reorder(ernie_cuda_context *ctx, const ernie_cuda
     ERNIE_TRY(check_kv(kv, 0, a.kv));
     ERNIE_TRY(check_beams(groups, beams, 1));
     if (!parents || !tables || !lens || !new_tables || !new_lens) return fail(ERNIE_CUDA_ERROR, "null argument");
-    if (max_pages < 1 || (static_cast<long long>(max_pages) << a.kv.page_shift) > INT32_MAX)
+    if (max_pages < 1 || (static_cast<long long>(max_pages) << a.kv.page_shift) > INT32_MAX ||
+        static_cast<long long>(max_pages) * beams > INT32_MAX)
         return fail(ERNIE_CUDA_ERROR, "Invalid page table width");
     if (!aligned(parents, 4) || !aligned(tables, 4) || !aligned(lens, 4) || !aligned(new_tables, 4) || !aligned(new_lens, 4))
         return fail(ERNIE_CUDA_ERROR, "Tables, lengths and parents must be 4-byte aligned");
@@ -258,6 +294,8 @@ extern "C" int ernie_cuda_beam_reorder(ernie_cuda_context *ctx, const ernie_cuda
         if (overlap(in[i], in_bytes[i], new_tables, table) || overlap(in[i], in_bytes[i], new_lens, list))
             return fail(ERNIE_CUDA_ERROR, "The new tables and lengths may not overlap the old ones or the parents");
     if (overlap(new_tables, table, new_lens, list)) return fail(ERNIE_CUDA_ERROR, "The new tables and lengths overlap");
+    ERNIE_TRY(check_outside(kv, a.kv, new_tables, table));
+    ERNIE_TRY(check_outside(kv, a.kv, new_lens, list));
     if (!ctx) return fail(ERNIE_CUDA_ERROR, "null context");
     a.layers = kv->layers;
     a.groups = groups;

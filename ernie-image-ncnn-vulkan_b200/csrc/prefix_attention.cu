@@ -1548,19 +1548,6 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
     return at;
 }
 
-// The plan counts steps in 32 bits.
-bool countable(const PagedLayer &kv, const AttendArgs &p, const PagedBatch &b)
-{
-    double units = 0;
-    for (int i = 0; i < 2; ++i)
-    {
-        const List &l = p.list[i];
-        const double keys = static_cast<double>(i == 0 ? b.max_prefix_pages : b.max_pages) * (1 << kv.page_shift);
-        units += (keys / (1 << l.unit_shift) + 1 + l.lead) * l.owners * l.blocks * kv.kv_heads;
-    }
-    return units < 1e9;
-}
-
 bool map_pool(CUtensorMap *map, const void *pool, const PagedLayer &kv, int granule)
 {
     const auto encode = tensor_map_encoder();
@@ -1580,7 +1567,6 @@ template <class T, int D> int launch(const PrefixAttentionArgs &a, int sms, cuda
     AttendArgs p;
     p.a = a;
     lay_out(a.kv, a.batch, a.heads, sms, a.workspace, p);
-    if (!countable(a.kv, p, a.batch)) return cudaErrorInvalidValue;
     p.scale = 1.4426950408889634f / sqrtf(static_cast<float>(D));
     p.granule = 1 << a.kv.page_shift;
     if (p.granule > Layout<T, D>::kSlotKeys) p.granule = Layout<T, D>::kSlotKeys;
@@ -1616,6 +1602,20 @@ size_t prefix_attention_workspace(const PagedLayer &kv, const PagedBatch &batch,
 {
     AttendArgs p;
     return lay_out(kv, batch, heads, sms, nullptr, p);
+}
+
+bool prefix_attention_countable(const PagedLayer &kv, const PagedBatch &batch, int heads)
+{
+    AttendArgs p;
+    lay_out(kv, batch, heads, 1, nullptr, p);
+    double steps = 0;
+    for (int i = 0; i < 2; ++i)
+    {
+        const List &l = p.list[i];
+        const double keys = static_cast<double>(i == 0 ? batch.max_prefix_pages : batch.max_pages) * (1 << kv.page_shift);
+        steps += (keys / (1 << l.unit_shift) + 1 + l.lead) * l.owners * l.blocks * kv.kv_heads;
+    }
+    return steps < 1e9;
 }
 
 int prepare_prefix_attention_kernels()

@@ -102,10 +102,10 @@ def select(logits, scores, finished, end_token):
             top = x.max()
             if np.isnan(x).any() or not np.isfinite(top):
                 continue
-            lse = top + np.log(np.exp(x - top).sum())
+            log_sum = np.log(np.exp(x - top).sum())
             for rank, t in enumerate(np.lexsort((np.arange(vocab), -x))[:beams]):
                 if np.isfinite(x[t]):
-                    offers.append((-(score + (x[t] - lse)), b, rank, int(t)))
+                    offers.append((-(score + ((x[t] - top) - log_sum)), b, rank, int(t)))
         offers.sort(key=lambda o: o[:3])
         for i, (total, b, _, t) in enumerate(offers[:beams]):
             parents[g, i], tokens[g, i], totals[g, i] = b, t, -total

@@ -151,6 +151,42 @@ def test_reorder_refusals(change, words):
     refused(lambda: reorder(**change), words)
 
 
+def test_results_inside_the_cache_are_refused():
+    pool = 2 * 40 * 8 * 16 * 128 * 2  # bytes of K, and of V
+    for at in (K, V + 16, K + pool - 16, V + pool - 16):
+        refused(lambda: append(q_out=at), "overlaps the paged cache")
+        refused(lambda: attend(out=at), "overlaps the paged cache")
+        refused(lambda: attend(workspace=at), "overlaps the paged cache")
+        refused(lambda: reorder(new_tables=at), "overlaps the paged cache")
+        refused(lambda: reorder(new_lens=at), "overlaps the paged cache")
+    for at in (K + pool, V + pool):
+        refused(lambda: append(q_out=at), "null context")
+        refused(lambda: attend(out=at), "null context")
+
+
+@pytest.mark.parametrize("change", [
+    dict(tokens=TABLES + 44), dict(new_scores=TABLES), dict(new_finished=COUNTS + 8), dict(workspace=OUT),
+    dict(parents=WORK + 4096), dict(new_scores=K + 4), dict(new_finished=V - 4), dict(new_scores=V), dict(tokens=K),
+    dict(tokens=Q + 4 * 11999), dict(workspace=Q - 16)])
+def test_select_overlaps_are_refused(change):
+    refused(lambda: select(**change), "overlap")
+
+
+def test_select_takes_the_new_state_in_place():
+    refused(lambda: select(new_scores=K, new_finished=V), "null context")
+    refused(lambda: select(tokens=Q + 4 * 12000), "null context")
+
+
+def test_batches_past_the_counters_are_refused():
+    for call in (attend, lambda **c: CTX.prefix_attention_workspace(kv(), c["batch_"], c.get("heads", 32))):
+        refused(lambda: call(batch_=batch(sequences=1 << 20, queries=4, groups=1), heads=1024), "query rows")
+        refused(lambda: call(batch_=batch(sequences=1 << 16, queries=1, max_pages=1 << 16)), "too many tokens")
+        refused(lambda: call(batch_=batch(sequences=1 << 10, queries=1, groups=1 << 10, max_prefix_pages=1 << 18)),
+                "too many tokens")
+    refused(lambda: attend(kv(layers=65537)), "cache shape")
+    refused(lambda: reorder(beams=32, max_pages=1 << 26), "table width")
+
+
 def test_null_descriptions():
     lib = ec.lib()
     n = ctypes.c_size_t(7)

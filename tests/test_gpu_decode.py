@@ -251,6 +251,28 @@ def test_attention(ctx, dev, case, precision):
     holds(*attention_case(ctx, dev, rng, *case, precision, layers=2, layer=1))
 
 
+LARGE = [
+    # groups, per group, queries, prefix, suffix, heads, kv heads, dim, page
+    (1, 200, 1, 300, 40, 32, 8, 128, 16),    # 6400 rows: four to a warp of the join
+    (2, 130, 1, 700, 30, 48, 4, 64, 16),
+    (1, 1, 40, 2000, 2000, 128, 1, 128, 64),  # rows of more than eight parts
+    (1, 500, 1, 40, 20, 4, 2, 64, 8),        # more sequences than a CTA has threads
+    (450, 2, 1, 30, 10, 4, 2, 64, 8),        # and groups
+]
+
+
+@pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("case", LARGE, ids=str)
+def test_attention_of_large_batches(ctx, dev, case, precision):
+    """Some of the sequences idle (no new token) and some empty."""
+    rng = np.random.default_rng(sum(case) + precision)
+    n = case[0] * case[1]
+    lens, counts = rng.integers(0, case[4] + 1, n), np.full(n, case[2])
+    counts[rng.random(n) < 0.2] = 0
+    lens[0], counts[0] = max(case[4], case[2]), case[2]
+    holds(*attention_case(ctx, dev, rng, *case, precision, lens=lens, counts=counts))
+
+
 @pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("lens,counts,prefix", [
     ([0, 0, 0, 0], [0, 0, 0, 0], [50, 50]),      # an idle batch
@@ -498,6 +520,32 @@ def test_select_of_rows_that_offer_nothing(ctx, dev):
         got = run_select(ctx, dev, logits, scores, finished, 7, ec.FP32, alias=alias)
         same_selection(got, logits, scores, finished, 7)
     assert (got[0][1] == -1).all() and (got[1][1] == -1).all() and (got[3][1] == 1).all() and np.isneginf(got[2][1]).all()
+
+
+@pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("vocab", [700, 30011])
+def test_select_of_masked_rows_and_extreme_logits(ctx, dev, vocab, precision):
+    """Masks of the type's lowest value over nearly all of a row or the whole of it, and logits so large that
+    neighbouring ones lie far apart: the sums of exponentials hold relative to the row's largest logit."""
+    rng = np.random.default_rng(vocab)
+    lowest = -3.3895313892515355e38 if precision == ec.BF16 else float(np.finfo(np.float32).min)
+    beams = 4
+    logits = values(rng, (10, beams, vocab), precision, 3.0)
+    logits[0] = np.where(np.arange(vocab) == 333, logits[0], np.float32(lowest))  # one token left
+    logits[1, :, 5:] = lowest                                                     # five left, in one lane's stretch
+    logits[2] = lowest                                                            # none: all are equally good
+    logits[3] = np.where(rng.random((beams, vocab)) < 0.99, np.float32(lowest), logits[3])
+    for group, middle in ((4, 1e6), (5, -1e6), (6, 3e9), (7, -3e9), (8, 1e38), (9, -1e38)):
+        logits[group] = middle
+        logits[group, :, 11:vocab:97] = middle * (1 + 2.0 ** -5 * np.sign(middle))  # exact multiples apart
+    logits = o.bf16_to_f32(bf16_bits(logits).reshape(-1)).reshape(logits.shape) if precision == ec.BF16 else logits
+    scores = (-1.0 - 0.37 * np.arange(beams, dtype=np.float32))[None].repeat(10, 0)
+    # one beam at a time, so that no order hangs on how different rows round
+    for beam in range(beams):
+        one = np.where(np.arange(beams) == beam, scores, np.float32(-np.inf))
+        got = run_select(ctx, dev, logits, one, np.zeros((10, beams)), -1, precision, pad=3)
+        same_selection(got, logits, one, np.zeros((10, beams)), -1)
+        assert (got[0] == beam).all()
 
 
 def test_select_first_step_of_identical_beams(ctx, dev):
