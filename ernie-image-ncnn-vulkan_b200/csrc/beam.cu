@@ -235,10 +235,12 @@ template <class T> __global__ void __launch_bounds__(kThreads, 2) stretch_kernel
                 for (int e = 0; e < V; ++e)
                     if (Vector<T>::get(v[j], e) != Vector<T>::get(v[j], e)) sum = NAN;
         }
-        // The first tile: the lanes' largest logits, sorted, are the list's beginning, and the k-th of them bounds
-        // the k-th largest of all from below. Later tokens have to beat the list's last one.
+        // Tokens have to beat the list's last one. The first tile's lanes' largest logits, sorted, are the list's
+        // beginning; there, and where more than k lanes have a candidate (logits that rise along the row), the k-th
+        // of them bounds the k-th largest of the tile from below.
         float limit = last_value > -INFINITY ? from_ordered(ordered(last_value) + 1) : -FLT_MAX;
-        if (!__any_sync(full, best >= limit)) continue;
+        const unsigned hopeful = __ballot_sync(full, best >= limit);
+        if (!hopeful) continue;
         int best_place = 0; // of the lane's largest logit, the first of equal ones
 #pragma unroll
         for (int j = kVectors - 1; j >= 0; --j)
@@ -247,22 +249,27 @@ template <class T> __global__ void __launch_bounds__(kThreads, 2) stretch_kernel
                 if (Vector<T>::get(v[j], e) == best) best_place = j * 32 * V + e;
         const int best_token = static_cast<int>(base + lane * V + best_place);
         const bool first = !listed;
-        if (first)
+        if (first || __popc(hopeful) > k)
         {
-            listed = true;
-            value = best;
-            token = best > -INFINITY ? best_token : INT_MAX;
+            float sorted_value = best;
+            int sorted_token = best > -INFINITY ? best_token : INT_MAX;
 #pragma unroll
             for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
                 for (int step = size / 2; step > 0; step /= 2)
                 {
-                    const float other_value = __shfl_xor_sync(full, value, step);
-                    const int other_token = __shfl_xor_sync(full, token, step);
+                    const float other_value = __shfl_xor_sync(full, sorted_value, step);
+                    const int other_token = __shfl_xor_sync(full, sorted_token, step);
                     const bool high = ((lane & step) == 0) == ((lane & size) == 0);
-                    if (high == better(other_value, other_token, value, token)) value = other_value, token = other_token;
+                    if (high == better(other_value, other_token, sorted_value, sorted_token)) sorted_value = other_value, sorted_token = other_token;
                 }
-            limit = fmaxf(limit, __shfl_sync(full, value, k - 1));
+            limit = fmaxf(limit, __shfl_sync(full, sorted_value, k - 1));
+            if (first)
+            {
+                listed = true;
+                value = sorted_value;
+                token = sorted_token;
+            }
         }
         int count = 0;
 #pragma unroll
@@ -293,7 +300,8 @@ template <class T> __global__ void __launch_bounds__(kThreads, 2) stretch_kernel
                 const int j = i / V, e = i % V;
                 const float x = Vector<T>::value(reinterpret_cast<const T *>(ring + slot * (kVectors * 32) + j * 32 + from)[e]);
                 const int x_token = static_cast<int>(base + (j * 32 + from) * V + e);
-                for (unsigned found = __ballot_sync(full, x >= limit && x_token != held); found; found &= found - 1)
+                const bool beats = better(x, x_token, __shfl_sync(full, value, k - 1), __shfl_sync(full, token, k - 1));
+                for (unsigned found = __ballot_sync(full, x >= limit && x_token != held && beats); found; found &= found - 1)
                 {
                     const int one = __ffs(found) - 1;
                     const float new_value = __shfl_sync(full, x, one);
@@ -308,7 +316,7 @@ template <class T> __global__ void __launch_bounds__(kThreads, 2) stretch_kernel
     float reference = c;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) reference = fmaxf(reference, __shfl_xor_sync(full, reference, o));
-    if (top > -INFINITY) sum *= exp2_fast(c - reference); // (NaN where both are infinite: poisoned)
+    if (top > -INFINITY) sum *= exp2_fast(c - reference); // (an infinite sum stands at the limit, by a factor of one)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(full, sum, o);
     if (lane == 0)
