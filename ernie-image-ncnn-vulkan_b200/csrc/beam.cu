@@ -7,9 +7,9 @@
 // tile's in flight meanwhile (the bound is the logits' traffic), keeps its own reference and sum, and the
 // warp's list of the best lies sorted across its lanes, one each. Of a tile only what beats the list's last
 // entry is looked at one by one, which after a few tiles is rare; so stretches are as long as keeps every warp
-// busy. (64 x 8 rows of 131072 logits, 268 MB: 157 us with eight warps on one list that meet several times a
-// tile, 78 us with four times as many stretches, 76 to 87 us with warps that read each other's lists for a
-// higher bound.)
+// busy. (64 x 8 rows of 131072 logits, 268 MB: 60 us, 4.5 TB/s; 157 us with eight warps on one list that meet
+// several times a tile, 78 us with four times as many stretches, 76 to 87 us with warps that read each other's
+// lists for a higher bound. 64 rows of random, falling, equal and rising logits: 20, 19, 22 and 39 us.)
 // A second kernel joins the stretches of each row and merges the rows' lists.
 //
 // Sums: a lane's reference is c = x L rounded, for its largest logit x so far and L = log2(e) rounded, and its

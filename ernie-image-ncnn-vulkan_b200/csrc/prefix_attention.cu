@@ -9,8 +9,8 @@
 //   own     (sequence, block of rows, K/V head): a sequence's rows against its own tokens.
 // A row is a query head of a slot: the heads/kv_heads query heads that share a K/V head are rows of one item.
 // An item's keys are cut into units, and each list's units are dealt out evenly, in order, to that list's
-// workers (a fixed cost of every item counted in), so that an item may span several workers and a worker several items; an item's share of a worker
-// is a part. Along the order both the item and the worker only ever step up, so item + worker numbers the
+// workers (a fixed cost of every item counted in), so that an item may span several workers and a worker
+// several items; an item's share of a worker is a part. Along the order both the item and the worker only ever step up, so item + worker numbers the
 // parts without gaps or clashes, and an item's parts lie side by side. The lists share the CTAs by their
 // estimated cost. All of this is worked out on the device, by every CTA for itself, from the lengths of this
 // very call.
@@ -18,10 +18,16 @@
 // A list is worked on in one of two ways, chosen on the host by the rows of an item:
 //   stream  few rows, or an FP32 cache. A worker is a warp: 16 rows and its own TMA ring of K/V slots. The
 //           bound is the K/V traffic, and eight independent warps per SM hide each other's latencies without
-//           ever meeting. BF16 uses mma.sync m16n8 tiles, FP32 packed FMAs (three products of TF32 parts on
-//           the tensor cores took 2.4 times as long and lost two bits).
+//           ever meeting (an SM streams 60 to 65 GB/s of a BF16 cache, 100 of them the memory's 6.3 TB/s). BF16
+//           uses mma.sync m16n8 tiles, FP32 packed FMAs (three products of TF32 parts on the tensor cores took
+//           2.4 times as long and lost two bits).
 //   tile    many rows of a BF16 cache. A worker is a CTA: 256 rows (two tiles of 128) share each K/V tile on
-//           the tensor cores (tcgen05.mma, accumulators in TMEM), one row per softmax thread.
+//           the tensor cores (tcgen05.mma, accumulators in TMEM), one row per softmax thread. A unit of 256
+//           rows and 128 keys takes about 3350 cycles. Shared memory's 128 bytes per cycle bound it: four
+//           products that read 64 KB each, 64 KB of weights stored, 64 KB of keys and values loaded, 3072
+//           cycles (the exponentials alone would take 2048).
+// 256 sequences of 1024 own tokens behind 16384 shared ones (32 query heads over 8, BF16) take 165 to 175 us,
+// 12 groups of 8 with 300 behind 1800 in FP32 116 us.
 // A second kernel joins the parts of each row.
 #include "decode.h"
 #include "ptx.cuh"
@@ -715,8 +721,9 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
 // queries and values of its half's rows, two dims to a packed FMA. A step takes four keys: partial scores of
 // all rows, then a scatter of their sums over the 16 lanes (key lane/4 % 4 and a quarter of the rows each),
 // the weights there, and their way back by shuffles. Shared memory and shuffles deliver a value per lane and
-// cycle, so a value of K or V has to serve many rows: with eight rows to a lane a slot of eight keys takes
-// about 250 of those cycles, below its 350 cycles of the memory's rate (one row to a lane: 1024).
+// cycle, so a value of K or V has to serve many rows: eight rows to a lane take 250 of those cycles for a slot of
+// eight keys, one row to a lane 1024. The issue of 75 million warp instructions then is 67 of the 116 us that 12
+// groups of 8 sequences take (254 MB; sums over single dims: 144 us; rows paired in the packed FMAs: 141 us).
 template <int D, int R>
 __device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const Ring<float, D> &ring)
 {
@@ -1150,8 +1157,7 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Wal
             for (int k = 8; k < 128; k += 2) mx[(k >> 1) & 7] = max3(mx[(k >> 1) & 7], x[k], x[k + 1]);
             const float top = fmaxf(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], max3(mx[5], mx[6], mx[7])));
             // PV_g of the last unit still reads P_g and adds to O_g: a rescale waits for it, otherwise the weights
-            // are worked out meanwhile and only their stores wait (waiting before the exponentials: 2.05 us per
-            // unit of two tiles)
+            // are worked out meanwhile and only their stores wait
             bool waited = u == 0;
             if (u == 0) m = top;
             else if (__any_sync(0xffffffffu, (top - m) * c > 8.f)) // NaN while neither is finite: no
@@ -1505,7 +1511,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32, R == 1 ? 1 : 4) join_kernel(c
 }
 
 // ---------------------------------------------------------------- host
-constexpr int kTileRows = 32; // more rows than this go to the tensor cores' tiles
+// More rows of an owner and K/V head than this go to the tensor cores' tiles. With 8 K/V heads of 128 (one group
+// behind 2048 tokens / eight such groups / one behind 16384), in us, streamed and in tiles: 24 rows 23 / 23 / 35 and
+// 17 / 34 / 29; 40 rows 22 / 29 / 37 and 17 / 34 / 29; 80 rows 20 / 50 / 45 and 17 / 41 / 30; 200 rows 25 / 105 / 91
+// and 20 / 61 / 37.
+constexpr int kTileRows = 32;
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
