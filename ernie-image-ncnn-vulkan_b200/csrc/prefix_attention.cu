@@ -15,6 +15,10 @@
 // estimated cost. All of this is worked out on the device, by every CTA for itself, from the lengths of this
 // very call.
 //
+// Where a ragged batch's group has more slots than one block holds, the rows of its prefix items are those of its
+// tokens instead of its slots, found through the sums of the sequences' counts: 64 sequences of which one brings
+// 32 new tokens and the others one each go over the prefix with 95 tokens, not with 2048 slots.
+//
 // A list is worked on in one of two ways, chosen on the host by the rows of an item:
 //   stream  few rows, or an FP32 cache. A worker is a warp: 16 rows and its own TMA ring of K/V slots. The
 //           bound is the K/V traffic, and eight independent warps per SM hide each other's latencies without
@@ -89,6 +93,12 @@ struct AttendArgs
     Divisor by_share, by_queries, by_heads, by_group; // query heads of a K/V head, slots of a sequence, query heads, slots of a group
     float scale;  // log2(e) / sqrt(D)
     int granule;  // keys of a TMA box
+    int per;      // sequences of a group
+    int *earlier; // [sequences + 1]: tokens of the sequences before one
+};
+// kTokens: the prefix items' rows are those of the tokens, otherwise those of the slots.
+template <bool kTokens> struct Args : AttendArgs
+{
 };
 
 template <class T, int D> struct Layout
@@ -193,22 +203,31 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity)
 struct Keys
 {
     int keys; // that the rows of an item see at most
+    int rows; // of a group and K/V head, if they are its tokens'
     OwnView own;
 };
 
-__device__ __forceinline__ Keys item_keys(const AttendArgs &p, int which, int owner, int block)
+template <bool X> __device__ __forceinline__ Keys item_keys(const Args<X> &p, int which, int owner, int block)
 {
     const PagedBatch &b = p.a.batch;
-    Keys k = {0, {0, 0}};
+    Keys k = {0, 0, {0, 0}};
     if (which == 0)
     {
+        if constexpr (X) k.rows = (p.earlier[(owner + 1) * p.per] - p.earlier[owner * p.per]) * p.share;
         k.keys = clamped_length(b.prefix_lens[owner], b.max_prefix_pages, p.a.kv.page_shift, b.error_flag);
+        if constexpr (X)
+            if (block << p.list[0].block_shift >= k.rows) k.keys = 0;
         return k;
     }
     k.own = own_view(b, p.a.kv.page_shift, owner);
     const int first = block << p.list[1].block_shift, rows = min(first + p.list[1].block, k.own.count * p.share);
     if (rows > first) k.keys = max(0, k.own.len - k.own.count + divide(rows - 1, p.by_share) + 1);
     return k;
+}
+
+template <bool X> __device__ __forceinline__ int rows_of(const Args<X> &p, int which, const Keys &item)
+{
+    return X && which == 0 ? item.rows : p.list[which].rows;
 }
 
 __device__ __forceinline__ int units_of(const List &l, int keys)
@@ -256,7 +275,7 @@ struct Part
 };
 
 // The next part of the walk; false at its end. All threads of a worker take the same steps.
-__device__ __forceinline__ bool next_part(const AttendArgs &p, int which, Walk &w, Part &part)
+template <bool X> __device__ __forceinline__ bool next_part(const Args<X> &p, int which, Walk &w, Part &part)
 {
     const List &l = p.list[which];
     while (w.at < w.end && w.owner < l.owners) // (the owners run out first only if the lengths change under the call)
@@ -302,7 +321,7 @@ __device__ __forceinline__ void write_meta(const List &l, const Walk &w, const P
 }
 
 // The walk of worker `local` of the CTA (tile: 0, the CTA itself).
-__device__ __forceinline__ Walk walk_of(const AttendArgs &p, const Plan &plan, const PlanShared &s, int local)
+template <bool X> __device__ __forceinline__ Walk walk_of(const Args<X> &p, const Plan &plan, const PlanShared &s, int local)
 {
     const List &l = p.list[plan.which];
     Walk w = {local * plan.ctas + plan.cta, 0, 0, 0, 0, 0, 0}; // neighbours in the order go to different SMs
@@ -327,31 +346,66 @@ __device__ __forceinline__ Walk walk_of(const AttendArgs &p, const Plan &plan, c
     return w;
 }
 
+__device__ __forceinline__ int scan_warp(int x)
+{
+#pragma unroll
+    for (int step = 1; step < 32; step *= 2)
+    {
+        const int other = __shfl_up_sync(0xffffffffu, x, step);
+        if (threadIdx.x % 32 >= step) x += other;
+    }
+    return x;
+}
+
+// All threads: sums up to and including the thread's own.
+__device__ __forceinline__ int scan_block(int x, int *warp_sum)
+{
+    const int warp = threadIdx.x / 32;
+    int scan = scan_warp(x);
+    if (threadIdx.x % 32 == 31) warp_sum[warp] = scan;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kThreads / 32; ++j)
+        if (j < warp) scan += warp_sum[j];
+    return scan;
+}
+
 // All threads: the lists' steps, dealt out.
-__device__ __forceinline__ Plan make_plan(const AttendArgs &p, PlanShared &s)
+template <bool X> __device__ __forceinline__ Plan make_plan(const Args<X> &p, PlanShared &s)
 {
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, heads = p.a.kv.kv_heads;
     int mine[2], before[2], chunk[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int n = 0; n < 2; ++n)
     {
+        const int i = X ? 1 - n : n;
         const List &l = p.list[i];
         chunk[i] = l.owners <= kThreads ? 1 : (l.owners + kThreads - 1) / kThreads;
-        int sum = 0;
-        for (int o = tid * chunk[i]; o < min(l.owners, (tid + 1) * chunk[i]); ++o)
+        const int first = tid * chunk[i], end = min(l.owners, first + chunk[i]);
+        int sum = 0, tokens = 0;
+        for (int o = first; o < end; ++o)
+        {
             for (int b = 0; b < l.blocks; ++b) sum += steps_of(l, item_keys(p, i, o, b).keys);
+            if (X && i == 1) tokens += own_view(p.a.batch, p.a.kv.page_shift, o).count;
+        }
         mine[i] = sum * heads;
+        if (X && i == 1)
+        {
+            // every CTA writes the same sums, and reads its own
+            int at = scan_block(tokens, s.warp_sum[0]) - tokens;
+            for (int o = first; o < end; ++o)
+            {
+                p.earlier[o] = at;
+                at += own_view(p.a.batch, p.a.kv.page_shift, o).count;
+                if (o == l.owners - 1) p.earlier[l.owners] = at;
+            }
+            __syncthreads();
+        }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
     {
-        int scan = mine[i];
-#pragma unroll
-        for (int step = 1; step < 32; step *= 2)
-        {
-            const int other = __shfl_up_sync(0xffffffffu, scan, step);
-            if (lane >= step) scan += other;
-        }
+        const int scan = scan_warp(mine[i]);
         before[i] = scan - mine[i];
         if (lane == 31) s.warp_sum[i][warp] = scan;
     }
@@ -404,15 +458,30 @@ struct Row
     int keys;  // that the row sees of the item's; 0 without a token
 };
 
-__device__ __forceinline__ Row row_of(const AttendArgs &p, int which, const Part &part, int row)
+template <bool X> __device__ __forceinline__ Row row_of(const Args<X> &p, int which, const Part &part, int row)
 {
     const PagedBatch &b = p.a.batch;
     const List &l = p.list[which];
     const int r = (part.block << l.block_shift) + row;
     Row out = {0, 0};
-    if (row >= l.block || r >= l.rows) return out;
-    const int at = divide(r, p.by_share), head = part.head * p.share + r - at * p.share, slot = part.owner * l.slots + at;
-    if (which == 0)
+    if (row >= l.block || r >= rows_of(p, which, part.item)) return out;
+    const int at = divide(r, p.by_share), head = part.head * p.share + r - at * p.share;
+    int slot = part.owner * l.slots + at;
+    if (X && which == 0)
+    {
+        // the last sequence with no more than `token` tokens before it holds that one
+        int s = part.owner * p.per, more = p.per;
+        const int token = p.earlier[s] + at;
+        while (more > 1)
+        {
+            const int half = more >> 1;
+            if (p.earlier[s + half] <= token) s += half, more -= half;
+            else more = half;
+        }
+        slot = s * b.queries + token - p.earlier[s];
+        out.keys = part.item.keys;
+    }
+    else if (which == 0)
     {
         const int s = divide(slot, p.by_queries);
         if (b.counts && slot - s * b.queries >= b.counts[s]) return out;
@@ -429,7 +498,7 @@ __device__ __forceinline__ Row row_of(const AttendArgs &p, int which, const Part
 
 // First row of the pool that holds key `key` of the part's item, or the row past the end (TMA reads zeros
 // there) for a key past the item's or a bad page, which `bad` remembers: nothing here waits for the table.
-__device__ __forceinline__ int pool_row(const AttendArgs &p, int which, const Part &part, int key, bool &bad)
+template <bool X> __device__ __forceinline__ int pool_row(const Args<X> &p, int which, const Part &part, int key, bool &bad)
 {
     const PagedLayer &kv = p.a.kv;
     const int outside = (kv.pages * kv.kv_heads) << kv.page_shift;
@@ -534,8 +603,8 @@ template <class T, int D> __device__ __forceinline__ int steps_of_part(const Par
 
 // Four producer warps, each feeding two workers: eight lanes for a worker's K and eight for its V, which run ahead
 // by themselves; a lane issues one box of every slot of theirs.
-template <class T, int D>
-__device__ __forceinline__ void stream_produce(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const CUtensorMap *map_k,
+template <class T, int D, bool X>
+__device__ __forceinline__ void stream_produce(const Args<X> &p, const Plan &plan, const PlanShared &shared, const CUtensorMap *map_k,
                                                const CUtensorMap *map_v, const Ring<T, D> &ring)
 {
     using L = Layout<T, D>;
@@ -597,8 +666,8 @@ __device__ __forceinline__ void stream_produce(const AttendArgs &p, const Plan &
     if (bad) report_range(p.a.batch.error_flag);
 }
 
-template <int D>
-__device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const Ring<__nv_bfloat16, D> &ring)
+template <int D, bool X>
+__device__ __forceinline__ void stream_work(const Args<X> &p, const Plan &plan, const PlanShared &shared, const Ring<__nv_bfloat16, D> &ring)
 {
     using T = __nv_bfloat16;
     using L = Layout<T, D>;
@@ -699,7 +768,7 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        const int rows = min(l.block, l.rows - part.block * l.block); // of the item
+        const int rows = min(l.block, rows_of(p, plan.which, part.item) - part.block * l.block); // of the item
         const size_t place = static_cast<size_t>(part.place) * l.part_rows;
         float *dst = l.o + place * D + 2 * (lane & 3);
         float2 *ml = l.ml + place;
@@ -724,8 +793,8 @@ __device__ __forceinline__ void stream_work(const AttendArgs &p, const Plan &pla
 // cycle, so a value of K or V has to serve many rows: eight rows to a lane take 250 of those cycles for a slot of
 // eight keys, one row to a lane 1024. The issue of 75 million warp instructions then is 67 of the 116 us that 12
 // groups of 8 sequences take (254 MB; sums over single dims: 144 us; rows paired in the packed FMAs: 141 us).
-template <int D, int R>
-__device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan &plan, const PlanShared &shared, const Ring<float, D> &ring)
+template <int D, int R, bool X>
+__device__ __forceinline__ void stream_work_f32(const Args<X> &p, const Plan &plan, const PlanShared &shared, const Ring<float, D> &ring)
 {
     using L = Layout<float, D>;
     constexpr int kSlotKeys = L::kSlotKeys, kKeys = 4, kRows = R / 2, kGroups = D / 64, kPairs = 2 * kGroups;
@@ -909,7 +978,7 @@ __device__ __forceinline__ void stream_work_f32(const AttendArgs &p, const Plan 
             __syncwarp();
             if (lane < 2) mbar_arrive(ring.empty(worker, n + lane));
         }
-        const int rows = min(l.block, l.rows - part.block * l.block); // of the item
+        const int rows = min(l.block, rows_of(p, plan.which, part.item) - part.block * l.block); // of the item
         const size_t place = static_cast<size_t>(part.place) * l.part_rows;
 #pragma unroll
         for (int i = 0; i < kHeld; ++i)
@@ -985,8 +1054,8 @@ __device__ __forceinline__ uint64_t value_desc(uint32_t addr)
 }
 
 // The K and V tiles of the CTA's units; a lane per box.
-template <int D>
-__device__ __forceinline__ void tile_produce(const AttendArgs &p, int which, Walk w, const CUtensorMap *map_k, const CUtensorMap *map_v,
+template <int D, bool X>
+__device__ __forceinline__ void tile_produce(const Args<X> &p, int which, Walk w, const CUtensorMap *map_k, const CUtensorMap *map_v,
                                              const TileSmem<D> &sm)
 {
     using L = Layout<__nv_bfloat16, D>;
@@ -1035,7 +1104,7 @@ __device__ __forceinline__ void tile_produce(const AttendArgs &p, int which, Wal
 }
 
 // The products of tile g of rows, by one thread.
-template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs &p, int which, Walk w, const TileSmem<D> &sm, uint32_t tmem, int g)
+template <int D, bool X> __device__ __forceinline__ void tile_multiply(const Args<X> &p, int which, Walk w, const TileSmem<D> &sm, uint32_t tmem, int g)
 {
     const List &l = p.list[which];
     constexpr uint32_t score_desc = idesc_bf16(128, 128);
@@ -1058,7 +1127,7 @@ template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs 
     Part part;
     while (ok && next_part(p, which, w, part))
     {
-        if (min(l.block, l.rows - part.block * l.block) <= g * kTile)
+        if (min(l.block, rows_of(p, which, part.item) - part.block * l.block) <= g * kTile)
         {
             // no rows in this tile: the other one's K and V pass by
             for (int u = 0; u < part.units; ++u, ++n)
@@ -1092,8 +1161,8 @@ template <int D> __device__ __forceinline__ void tile_multiply(const AttendArgs 
     if (!ok) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
 }
 
-template <int D>
-__device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Walk w, const TileSmem<D> &sm, uint32_t tmem)
+template <int D, bool X>
+__device__ __forceinline__ void tile_softmax(const Args<X> &p, int which, Walk w, const TileSmem<D> &sm, uint32_t tmem)
 {
     const List &l = p.list[which];
     const int warp = threadIdx.x / 32 - 4, lane = threadIdx.x & 31, g = warp >> 2, quarter = warp & 3, r = quarter * 32 + lane;
@@ -1106,7 +1175,7 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Wal
     while (next_part(p, which, w, part))
     {
         if (warp == 0 && lane == 0) write_meta(l, w, part);
-        const int rows = min(l.block, l.rows - part.block * l.block);
+        const int rows = min(l.block, rows_of(p, which, part.item) - part.block * l.block);
         if (g * kTile >= rows)
         {
             n += part.units;
@@ -1272,9 +1341,9 @@ __device__ __forceinline__ void tile_softmax(const AttendArgs &p, int which, Wal
 }
 
 // ---------------------------------------------------------------- the kernel
-template <class T, int D>
+template <class T, int D, bool X>
 __global__ void __launch_bounds__(kThreads, 1)
-    attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ AttendArgs p)
+    attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ Args<X> p)
 {
     using L = Layout<T, D>;
     extern __shared__ uint8_t smem_raw[];
@@ -1368,8 +1437,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 // once with their places worked out before the attention ends (16384 rows one by one took three rounds, 10 us).
 constexpr int kJoinWarps = 8;
 
-template <class T, int D, int R, int A>
-__global__ void __launch_bounds__(kJoinWarps * 32, R == 1 ? 1 : 4) join_kernel(const __grid_constant__ AttendArgs p)
+template <class T, int D, int R, int A, bool X>
+__global__ void __launch_bounds__(kJoinWarps * 32, R == 1 ? 1 : 4) join_kernel(const __grid_constant__ Args<X> p)
 {
     constexpr int N = D / 32, kLanes = 32 / R, kBatch = 8; // values of a lane; lanes of a row; parts weighed together
     static_assert(kLanes >= kBatch && kBatch % A == 0, "parts of a batch");
@@ -1389,18 +1458,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32, R == 1 ? 1 : 4) join_kernel(c
     if (b.max_prefix_pages) view.prefix_len = clamped_length(view.prefix_len, b.max_prefix_pages, p.a.kv.page_shift, b.error_flag);
     const bool wanted = at < rows && i < view.count;
     int item[2] = {-1, -1}, within[2] = {0, 0};
+    if constexpr (X) // the sums of the counts are the attention's
+    {
+        grid_dependency_wait();
+        grid_dependents_launch();
+    }
+    const int before = X ? p.earlier[s] - p.earlier[group * p.per] : slot - group * p.list[0].slots - i;
 #pragma unroll
     for (int which = 0; which < 2; ++which)
     {
         const List &l = p.list[which];
         if (!wanted || (which == 0 ? view.prefix_len == 0 : view.len - view.count + i + 1 <= 0)) continue;
         const int owner = which == 0 ? group : s;
-        const int r = (which == 0 ? slot - owner * l.slots : i) * p.share + head - kv_head * p.share, block = r >> l.block_shift;
+        const int r = (which == 0 ? before + i : i) * p.share + head - kv_head * p.share, block = r >> l.block_shift;
         item[which] = (owner * l.blocks + block) * p.a.kv.kv_heads + kv_head;
         within[which] = r - block * l.block;
     }
-    grid_dependency_wait();
-    grid_dependents_launch();
+    if constexpr (!X)
+    {
+        grid_dependency_wait();
+        grid_dependents_launch();
+    }
     if (first_row >= rows) return;
     int parts[2] = {0, 0}, first[2] = {0, 0}; // of the lane's row, and the first part's place
 #pragma unroll
@@ -1423,7 +1501,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, R == 1 ? 1 : 4) join_kernel(c
             const List &l = p.list[which];
             ml = l.ml[static_cast<size_t>(which ? first[1] + j - parts[0] : first[0] + j) * l.part_rows + (which ? within[1] : within[0])];
         }
-        float weight = 0.f, before = 1.f;
+        float weight = 0.f, rescale = 1.f;
 #pragma unroll
         for (int k0 = 0; k0 < kBatch; k0 += A)
         {
@@ -1465,17 +1543,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32, R == 1 ? 1 : 4) join_kernel(c
 #pragma unroll
                 for (int step = kLanes / 2; step > 0; step >>= 1) most = fmaxf(most, __shfl_xor_sync(full, most, step));
                 most = fmaxf(most, top);
-                before = top == most ? 1.f : exp2_fast(top - most);
+                rescale = top == most ? 1.f : exp2_fast(top - most);
                 weight = ml.x == -INFINITY ? 0.f : exp2_fast(ml.x - most);
                 float part_sum = weight * ml.y;
 #pragma unroll
                 for (int step = kLanes / 2; step > 0; step >>= 1) part_sum += __shfl_xor_sync(full, part_sum, step);
-                sum = sum * before + part_sum;
+                sum = sum * rescale + part_sum;
                 top = most;
 #pragma unroll
                 for (int r = 0; r < R; ++r)
                 {
-                    const float f = __shfl_sync(full, before, r * kLanes);
+                    const float f = __shfl_sync(full, rescale, r * kLanes);
 #pragma unroll
                     for (int d = 0; d < N; ++d) o[r][d] *= f;
                 }
@@ -1519,6 +1597,12 @@ constexpr int kTileRows = 32;
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
+// Within one block, slots without a token cost nothing. With one slot to a sequence they are taken to be rare: 256 such
+// sequences behind 8192 tokens take 79 us by slots and 85 by tokens (idle every other one: 57). With 32 slots and 64
+// sequences behind 4096 tokens, by slots 184 us whatever the counts; by tokens 65 with one sequence of 32 and the
+// others of one, 192 with all of 32; 16 sequences of 0 to 32 behind 2000: 47 and 38.
+bool by_tokens(const AttendArgs &p, const PagedBatch &b) { return b.counts && b.queries > 1 && p.list[0].owners && p.list[0].blocks > 1; }
+
 // Lays out the lists and the workspace; returns its size.
 size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, void *workspace, AttendArgs &p)
 {
@@ -1555,6 +1639,13 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
         l.meta = reinterpret_cast<int2 *>(base + at);
         at += rounded(items * sizeof(int2));
     }
+    p.per = b.sequences / b.groups;
+    p.earlier = nullptr;
+    if (by_tokens(p, b))
+    {
+        p.earlier = reinterpret_cast<int *>(base + at);
+        at += rounded((static_cast<size_t>(b.sequences) + 1) * sizeof(int));
+    }
     return at;
 }
 
@@ -1572,6 +1663,19 @@ bool map_pool(CUtensorMap *map, const void *pool, const PagedLayer &kv, int gran
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <class T, int D, bool X> int launch(const AttendArgs &args, const CUtensorMap &map_k, const CUtensorMap &map_v, cudaStream_t stream)
+{
+    Args<X> p;
+    static_cast<AttendArgs &>(p) = args;
+    const cudaError_t e = launch_dependent(attend_kernel<T, D, X>, p.ctas, kThreads, Layout<T, D>::kSmemBytes, stream, map_k, map_v, p);
+    if (e != cudaSuccess) return e;
+    const long long rows = static_cast<long long>(p.a.batch.sequences) * p.a.batch.queries * p.a.heads;
+    const bool many = rows > 32ll * p.ctas; // one row per warp fills the SMs once up to here
+    const long long per_cta = kJoinWarps * (many ? 4 : 1);
+    const dim3 grid(static_cast<unsigned>((rows + per_cta - 1) / per_cta));
+    return launch_dependent(many ? join_kernel<T, D, 4, 2, X> : join_kernel<T, D, 1, 8, X>, grid, kJoinWarps * 32, 0, stream, p);
+}
+
 template <class T, int D> int launch(const PrefixAttentionArgs &a, int sms, cudaStream_t stream)
 {
     AttendArgs p;
@@ -1582,29 +1686,29 @@ template <class T, int D> int launch(const PrefixAttentionArgs &a, int sms, cuda
     if (p.granule > Layout<T, D>::kSlotKeys) p.granule = Layout<T, D>::kSlotKeys;
     CUtensorMap map_k, map_v;
     if (!map_pool(&map_k, a.kv.k, a.kv, p.granule) || !map_pool(&map_v, a.kv.v, a.kv, p.granule)) return cudaErrorInvalidValue;
-    const cudaError_t e = launch_dependent(attend_kernel<T, D>, sms, kThreads, Layout<T, D>::kSmemBytes, stream, map_k, map_v, p);
-    if (e != cudaSuccess) return e;
-    const long long rows = static_cast<long long>(a.batch.sequences) * a.batch.queries * a.heads;
-    const bool many = rows > 32ll * sms; // one row per warp fills the SMs once up to here
-    const long long per_cta = kJoinWarps * (many ? 4 : 1);
-    const dim3 grid(static_cast<unsigned>((rows + per_cta - 1) / per_cta));
-    return launch_dependent(many ? join_kernel<T, D, 4, 2> : join_kernel<T, D, 1, 8>, grid, kJoinWarps * 32, 0, stream, p);
+    return p.earlier ? launch<T, D, true>(p, map_k, map_v, stream) : launch<T, D, false>(p, map_k, map_v, stream);
 }
 
-template <class T, int D> cudaError_t prepare()
+template <class T, int D, bool X> cudaError_t prepare()
 {
     cudaFuncAttributes attr;
-    const cudaError_t e = cudaFuncGetAttributes(&attr, attend_kernel<T, D>);
+    const cudaError_t e = cudaFuncGetAttributes(&attr, attend_kernel<T, D, X>);
     if (e != cudaSuccess) return e;
     // the register split needs this many registers per thread at launch
     if (attr.numRegs < kMinLaunchRegs) return cudaErrorInvalidConfiguration;
     static_assert(Layout<T, D>::kSmemBytes <= 232448, "shared memory of a CTA");
     // the join keeps the SMs' split between shared memory and L1: changing it between the two kernels of every
     // call drains the SMs
-    cudaError_t c = cudaFuncSetAttribute(join_kernel<T, D, 1, 8>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (c == cudaSuccess) c = cudaFuncSetAttribute(join_kernel<T, D, 4, 2>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    cudaError_t c = cudaFuncSetAttribute(join_kernel<T, D, 1, 8, X>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (c == cudaSuccess) c = cudaFuncSetAttribute(join_kernel<T, D, 4, 2, X>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (c != cudaSuccess) return c;
-    return cudaFuncSetAttribute(attend_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<T, D>::kSmemBytes);
+    return cudaFuncSetAttribute(attend_kernel<T, D, X>, cudaFuncAttributeMaxDynamicSharedMemorySize, Layout<T, D>::kSmemBytes);
+}
+
+template <class T, int D> cudaError_t prepare()
+{
+    const cudaError_t e = prepare<T, D, false>();
+    return e == cudaSuccess ? prepare<T, D, true>() : e;
 }
 } // namespace
 

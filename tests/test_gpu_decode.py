@@ -274,6 +274,34 @@ def test_attention_of_large_batches(ctx, dev, case, precision):
 
 
 @pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("groups,per,queries,kind", [
+    (1, 64, 32, "one long"), (3, 9, 20, "one long"), (2, 12, 33, "random"), (2, 300, 3, "random"), (5, 1, 150, "random"),
+    (2, 40, 8, "last"), (3, 30, 8, "one group idle"), (2, 20, 24, "out of range")])
+def test_attention_of_mixed_batches(ctx, dev, groups, per, queries, kind, precision):
+    """Sequences with one new token beside ones with many or none: the rows that share a prefix are the tokens'."""
+    rng = np.random.default_rng(groups + per + queries)
+    n = groups * per
+    counts = {"one long": np.where(np.arange(n) % per == per // 2, queries, 1), "random": rng.integers(0, queries + 1, n),
+              "last": np.where(np.arange(n) == n - 1, queries, 0), "one group idle": np.where(np.arange(n) // per == 1, 0, queries),
+              "out of range": rng.integers(0, queries + 1, n)}[kind]
+    lens = counts + rng.integers(0, 50, n)
+    prefix = rng.integers(1, 400, groups)
+    case = (groups, per, queries, 0, 0, 8, 1, 128, 16, precision)
+    if kind != "out of range":
+        holds(*attention_case(ctx, dev, rng, *case, counts=counts, lens=lens, prefix_lens=prefix))
+        return
+    counts[3], counts[per] = -2, queries + 5  # clamped to none and to all
+    with pytest.raises(ec.CudaError, match="status 41"):
+        attention_case(ctx, dev, rng, *case, counts=counts, lens=np.maximum(lens, 0), prefix_lens=prefix)
+    counts[3], counts[per] = 0, queries
+    fine = Device(ctx)
+    got, want, limit = attention_case(ctx, fine, np.random.default_rng(groups + per + queries + 1), *case, counts=counts, lens=np.maximum(lens, 0),
+                                      prefix_lens=prefix)
+    fine.free()
+    holds(got, want, limit)
+
+
+@pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("lens,counts,prefix", [
     ([0, 0, 0, 0], [0, 0, 0, 0], [50, 50]),      # an idle batch
     ([0, 5, 128, 1], [1, 3, 3, 1], [0, 40]),     # more new tokens than the sequence holds: rows that see nothing
