@@ -290,9 +290,12 @@ class Buffer:
 def device_pointer(a):
     """Address of device memory: an array with data_ptr() (a torch tensor), a Buffer, an address or None."""
     try:
-        return a.data_ptr()
+        address = a.data_ptr()
     except AttributeError:
         return a.ptr if isinstance(a, Buffer) else a
+    if not a.is_cuda:
+        raise ValueError("the array is not in device memory")
+    return address
 
 
 class PagedKv:
@@ -311,6 +314,8 @@ class PagedBatch:
     def __init__(self, sequences, queries, tables, max_pages, lens, counts=None, groups=1, prefix_tables=None,
                  max_prefix_pages=0, prefix_lens=None):
         self.arrays = (tables, lens, counts, prefix_tables, prefix_lens)
+        if any(hasattr(a, "element_size") and (a.element_size() != 4 or not a.is_contiguous()) for a in self.arrays):
+            raise ValueError("tables, lengths and counts are contiguous arrays of 32-bit integers")
         self.fields = PagedBatchFields(sequences, queries, device_pointer(tables), max_pages, device_pointer(lens),
                                        device_pointer(counts), groups, device_pointer(prefix_tables), max_prefix_pages,
                                        device_pointer(prefix_lens))

@@ -421,7 +421,7 @@ typedef struct
    `position` of cos/sin [rope_rows][head_dim] FP32 and rounded once to the cache's type; keys and
    values go to the token's page, queries to q_out [sequences*queries][heads][head_dim]. Slots without a
    token and everything else in the cache stay as they were. A position outside 0..rope_rows-1 stores
-   nothing and reports status 41. q_out may not overlap qkv. */
+   nothing and reports status 41. q_out may overlap neither qkv nor the cache. */
 int ernie_cuda_paged_append(ernie_cuda_context *ctx, const ernie_cuda_paged_kv *kv, int layer,
                             const ernie_cuda_paged_batch *batch, const void *qkv, int precision, int64_t ld, int heads,
                             const float *cos, const float *sin, int rope_rows, void *q_out);
@@ -429,11 +429,13 @@ int ernie_cuda_paged_append(ernie_cuda_context *ctx, const ernie_cuda_paged_kv *
 /* out = softmax(q k^T / sqrt(head_dim)) v for every slot that holds a token, over its group's prefix and
    its own sequence's tokens up to and including itself; heads/kv_heads query heads share a K/V head. q
    and out [sequences*queries][heads][head_dim] in the cache's type, 16-byte aligned, not overlapping.
-   The prefix is read once for all the rows of its group. Scores, softmax statistics and sums are FP32;
-   with a BF16 cache the weights are rounded to BF16 for the second product. Slots without a token stay
+   The prefix is read for all the rows of its group together (a ragged batch's rows are those of its tokens;
+   a batch whose slots are all filled is faster without counts). Scores, softmax statistics and sums are
+   FP32, for scores below 2^30; with a BF16 cache the weights are rounded to BF16 for the second product. Slots without a token stay
    as they were; a row that sees no key at all (a token before its sequence's begin, lens < counts,
    without a prefix) gives zeros. What lies past a sequence's last token is never used; a non-finite
-   value of an appended token may reach every row of its sequence in the same call.
+   value of an appended token may reach every row of its sequence in the same call. The tables may span
+   about 10^9 blocks of 32 tokens times K/V heads in all. out and the workspace may not overlap the cache.
    The workspace is scratch of at least ..._workspace bytes (16-byte aligned); it holds nothing between
    calls, and calls that may run at the same time need one each. */
 int ernie_cuda_prefix_attention_workspace(ernie_cuda_context *ctx, const ernie_cuda_paged_kv *kv,
@@ -451,8 +453,9 @@ int ernie_cuda_prefix_attention(ernie_cuda_context *ctx, const ernie_cuda_paged_
    finite (-inf is the usual start of all beams but the first).
    Out, best first: parents (the beam within the group), tokens, new_scores (the total rounded to FP32),
    new_finished (its parent was, or its token is end_token; a negative end_token ends none). Places
-   without a continuation left get parent -1, token -1, score -inf, finished 1. The outputs may be the
-   inputs of the same name. The workspace as for ernie_cuda_prefix_attention. */
+   without a continuation left get parent -1, token -1, score -inf, finished 1. Of the outputs new_scores
+   may be scores and new_finished may be finished; no other arrays overlap. Masks of the type's lowest
+   value are logits like any other. The workspace as for ernie_cuda_prefix_attention. */
 int ernie_cuda_beam_select_workspace(ernie_cuda_context *ctx, int groups, int beams, int vocab, size_t *bytes);
 int ernie_cuda_beam_select(ernie_cuda_context *ctx, const void *logits, int precision, int64_t ld, int groups, int beams,
                            int vocab, int end_token, const float *scores, const int32_t *finished, int32_t *parents,
@@ -467,7 +470,7 @@ int ernie_cuda_beam_select(ernie_cuda_context *ctx, const void *logits, int prec
    tokens are copied there in every layer. So pages only change hands within a group, every page keeps
    one owner, and only duplicated beams cost copies. Every row of a group needs as many good pages as its
    group's longest sequence uses (a bad one is not written: status 41). new_tables and new_lens get the
-   new rows and may not overlap tables, lens or each other; the prefix pages take no part. */
+   new rows and may not overlap the inputs, the cache or each other; the prefix pages take no part. */
 int ernie_cuda_beam_reorder(ernie_cuda_context *ctx, const ernie_cuda_paged_kv *kv, int groups, int beams,
                             const int32_t *parents, const int32_t *tables, int max_pages, const int32_t *lens,
                             int32_t *new_tables, int32_t *new_lens);

@@ -187,6 +187,16 @@ def test_batches_past_the_counters_are_refused():
     refused(lambda: reorder(beams=32, max_pages=1 << 26), "table width")
 
 
+def test_arrays_on_the_host_and_wide_integers_are_refused():
+    torch = pytest.importorskip("torch")
+    with pytest.raises(ValueError, match="device memory"):
+        append(q_out=torch.zeros(4))
+    with pytest.raises(ValueError, match="32-bit"):
+        batch(lens=torch.zeros(6, dtype=torch.int64))
+    with pytest.raises(ValueError, match="32-bit"):
+        batch(tables=torch.zeros(4, 6, dtype=torch.int32).t())
+
+
 def test_null_descriptions():
     lib = ec.lib()
     n = ctypes.c_size_t(7)
