@@ -7,9 +7,9 @@
 // tile's in flight meanwhile (the bound is the logits' traffic), keeps its own reference and sum, and the
 // warp's list of the best lies sorted across its lanes, one each. Of a tile only what beats the list's last
 // entry is looked at one by one, which after a few tiles is rare; so stretches are as long as keeps every warp
-// busy. (64 x 8 rows of 131072 logits, 268 MB: 60 us, 4.5 TB/s; 157 us with eight warps on one list that meet
+// busy. (64 x 8 rows of 131072 logits, 268 MB: 58 us, 4.6 TB/s; 157 us with eight warps on one list that meet
 // several times a tile, 78 us with four times as many stretches, 76 to 87 us with warps that read each other's
-// lists for a higher bound. 64 rows of random, falling, equal and rising logits: 20, 19, 22 and 39 us.)
+// lists for a higher bound. 64 rows of random, falling, equal and rising logits: 18, 16, 18 and 35 us.)
 // A second kernel joins the stretches of each row and merges the rows' lists.
 //
 // Sums: a lane's reference is c = x L rounded, for its largest logit x so far and L = log2(e) rounded, and its
@@ -28,12 +28,11 @@ namespace ernie_b200
 {
 namespace
 {
-constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kVectors = 8;        // 16-byte vectors of a tile that a lane holds
 constexpr int kMaxStretches = 64;  // of a row: two lists per lane of the joining warp
 constexpr int kListEntries = 4096; // of a group's lists in the joining CTA's shared memory
 constexpr int kRing = 3;           // tiles of a warp in shared memory: one in work, two in flight
-constexpr int kRingBytes = kWarps * kRing * kVectors * 32 * 16;
+constexpr int kResident = 16; // warps per SM
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSteady = 1048576.f; // the references' limit
 
@@ -42,7 +41,7 @@ struct Plan
     int stretches, tiles; // of a row, of a stretch
 };
 
-// Up to 16 warps per SM work at a time; `skew` logits of a row's first vector may lie before the row. A row is
+// Up to kResident warps per SM work at a time; `skew` logits of a row's first vector may lie before the row. A row is
 // cut so that the rounds of warps times a stretch's tiles are fewest, a stretch's start counted as six tiles.
 Plan plan_of(long long rows, int vocab, int skew, int beams, bool bf16, int sms)
 {
@@ -52,7 +51,7 @@ Plan plan_of(long long rows, int vocab, int skew, int beams, bool bf16, int sms)
     Plan p = {1, 1};
     for (long long s = 1; s <= most && s <= tiles; ++s)
     {
-        const long long each = (tiles + s - 1) / s, rounds = (rows * s + 16 * sms - 1) / (16 * sms), cost = rounds * (each + 6);
+        const long long each = (tiles + s - 1) / s, rounds = (rows * s + kResident * sms - 1) / (kResident * sms), cost = rounds * (each + 6);
         if (cost >= best) continue;
         best = cost;
         p.tiles = static_cast<int>(each);
@@ -165,15 +164,16 @@ __device__ __forceinline__ float exp2_fast(float x)
     return y;
 }
 
-template <class T> __global__ void __launch_bounds__(kThreads, 2) stretch_kernel(const __grid_constant__ BeamSelectArgs a, Plan plan, Parts parts)
+// A CTA is one warp, so that the SMs' shares of the stretches differ by one (256 threads: 60.3 for 59.0 us).
+template <class T> __global__ void __launch_bounds__(32, kResident) stretch_kernel(const __grid_constant__ BeamSelectArgs a, Plan plan, Parts parts)
 {
     constexpr int V = Vector<T>::kSize;
     constexpr unsigned full = 0xffffffffu;
     grid_dependency_wait();
     grid_dependents_launch();
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, k = a.beams;
-    const long long out = static_cast<long long>(blockIdx.x) * kWarps + warp, row = out / plan.stretches;
-    if (row >= static_cast<long long>(a.groups) * k || !row_offers(a, row)) return;
+    const int lane = threadIdx.x, k = a.beams;
+    const long long out = blockIdx.x, row = out / plan.stretches;
+    if (!row_offers(a, row)) return;
     const T *x = static_cast<const T *>(a.logits) + row * a.ld;
     // vectors start at 16-byte boundaries: index 0 of the row is element `skew` of the first one
     const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
@@ -184,8 +184,7 @@ template <class T> __global__ void __launch_bounds__(kThreads, 2) stretch_kernel
     float value = -INFINITY, last_value = -INFINITY; // the list: lane i holds the i-th best; its last entry
     int token = INT_MAX;
     bool listed = false; // whether the list has its beginning
-    extern __shared__ uint4 ring_memory[];
-    uint4 *ring = ring_memory + warp * (kRing * kVectors * 32);
+    __shared__ uint4 ring[kRing * kVectors * 32];
 #pragma unroll
     for (int t = 0; t < kRing - 1; ++t)
     {
@@ -356,12 +355,12 @@ __device__ __noinline__ double row_sum(const BeamSelectArgs &a, long long row, f
     return sum;
 }
 
-// One CTA per group, a warp per beam: the beam's list from its stretches' lists, then one warp merges the
-// beams' lists (lane = beam).
+// One CTA per group, a warp per beam: the beam's list from its stretches' lists, then each continuation's place
+// among all the beams'.
 __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
 {
     __shared__ double total[kMaxBeams][kMaxBeams];
-    __shared__ int token[kMaxBeams][kMaxBeams], done[kMaxBeams];
+    __shared__ int token[kMaxBeams][kMaxBeams], count[kMaxBeams];
     __shared__ float entry_value[kListEntries];
     __shared__ int entry_token[kListEntries];
     const unsigned full = 0xffffffffu;
@@ -373,7 +372,6 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
     grid_dependents_launch();
     if (lane < k) total[warp][lane] = -INFINITY;
     __syncwarp();
-    if (lane == 0) done[warp] = finished;
     if (finished)
     {
         if (lane == 0 && isfinite(score))
@@ -453,36 +451,38 @@ __global__ void merge_kernel(BeamSelectArgs a, Plan plan, Parts parts)
         }
     }
     __syncthreads();
-    if (warp != 0) return;
-    int at = 0, parent = -1, chosen = -1, ended = 1;
-    float result = -INFINITY;
-    for (int r = 0; r < k; ++r)
+    // A continuation's place is the number of better ones: those before it in its beam's list, and of every other beam
+    // the first few. Nothing past the last place is followed.
+    const double mine = lane < k ? total[warp][lane] : -INFINITY;
+    const int offered = __popc(__ballot_sync(full, mine > -INFINITY));
+    if (lane == 0) count[warp] = offered;
+    if (lane < offered)
     {
-        // the largest head, as an ordered integer in two halves; of equal ones the lowest beam's
-        const double mine = lane < k && at < k ? total[lane][at] : -INFINITY;
-        const long long raw = __double_as_longlong(mine + 0.0);
-        const unsigned long long key = static_cast<unsigned long long>(raw) ^ (raw < 0 ? ~0ull : 1ull << 63);
-        const unsigned high = static_cast<unsigned>(key >> 32), most_high = __reduce_max_sync(full, high);
-        const unsigned low = high == most_high ? static_cast<unsigned>(key) : 0u, most_low = __reduce_max_sync(full, low);
-        const int who = __ffs(__ballot_sync(full, high == most_high && static_cast<unsigned>(key) == most_low)) - 1;
-        const double best = __shfl_sync(full, mine, who);
-        if (best == -INFINITY) break;
-        const int taken = __shfl_sync(full, at, who);
-        if (lane == who) ++at;
-        if (lane == r)
+        int place = lane;
+        for (int b = 0; b < k; ++b)
+            for (int j = 0; b != warp && j < k && place < k; ++j, ++place)
+            {
+                const double other = total[b][j];
+                if (!(other > mine || (other == mine && b < warp && other > -INFINITY))) break;
+            }
+        if (place < k)
         {
-            parent = who;
-            chosen = token[who][taken];
-            result = static_cast<float>(best);
-            ended = done[who] || (a.end_token >= 0 && chosen == a.end_token);
+            const int chosen = token[warp][lane];
+            a.parents[base + place] = warp;
+            a.tokens[base + place] = chosen;
+            a.new_scores[base + place] = static_cast<float>(mine);
+            a.new_finished[base + place] = finished || (a.end_token >= 0 && chosen == a.end_token);
         }
     }
-    if (lane < k)
+    __syncthreads();
+    if (warp != 0) return;
+    const int every = __reduce_add_sync(full, lane < k ? count[lane] : 0);
+    if (lane < k && lane >= every)
     {
-        a.parents[base + lane] = parent;
-        a.tokens[base + lane] = chosen;
-        a.new_scores[base + lane] = result;
-        a.new_finished[base + lane] = ended;
+        a.parents[base + lane] = -1;
+        a.tokens[base + lane] = -1;
+        a.new_scores[base + lane] = -INFINITY;
+        a.new_finished[base + lane] = 1;
     }
 }
 
@@ -509,10 +509,10 @@ size_t beam_select_workspace(int groups, int beams, int vocab, int sms)
 
 int prepare_beam_kernels()
 {
-    cudaError_t e = cudaFuncSetAttribute(stretch_kernel<float>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(stretch_kernel<__nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
     // the SMs' split between shared memory and L1 stays as it is between the two kernels
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(merge_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    cudaError_t e = cudaFuncSetAttribute(merge_kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(stretch_kernel<float>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(stretch_kernel<__nv_bfloat16>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     return e;
 }
 
@@ -522,12 +522,12 @@ int launch_beam_select(const BeamSelectArgs &a, int sms, cudaStream_t stream)
     const int vector = a.bf16 ? 8 : 4;
     const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && (rows == 1 || a.ld % vector == 0);
     const Plan p = plan_of(rows, a.vocab, aligned ? 0 : vector - 1, a.beams, a.bf16, sms);
-    const long long ctas = (rows * p.stretches + kWarps - 1) / kWarps;
+    const long long ctas = rows * p.stretches;
     if (ctas > INT32_MAX) return cudaErrorInvalidValue;
     const Parts parts = parts_of(a.workspace, rows, a.beams, p);
     const unsigned grid = static_cast<unsigned>(ctas);
-    const cudaError_t e = a.bf16 ? launch_dependent(stretch_kernel<__nv_bfloat16>, grid, kThreads, kRingBytes, stream, a, p, parts)
-                                 : launch_dependent(stretch_kernel<float>, grid, kThreads, kRingBytes, stream, a, p, parts);
+    const cudaError_t e = a.bf16 ? launch_dependent(stretch_kernel<__nv_bfloat16>, grid, 32, 0, stream, a, p, parts)
+                                 : launch_dependent(stretch_kernel<float>, grid, 32, 0, stream, a, p, parts);
     if (e != cudaSuccess) return e;
     return launch_dependent(merge_kernel, a.groups, 32 * a.beams, 0, stream, a, p, parts);
 }
