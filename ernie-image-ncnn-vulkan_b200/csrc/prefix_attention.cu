@@ -30,8 +30,8 @@
 //           rows and 128 keys takes about 3350 cycles. Shared memory's 128 bytes per cycle bound it: four
 //           products that read 64 KB each, 64 KB of weights stored, 64 KB of keys and values loaded, 3072
 //           cycles (the exponentials alone would take 2048).
-// 256 sequences of 1024 own tokens behind 16384 shared ones (32 query heads over 8, BF16) take 165 to 175 us,
-// 12 groups of 8 with 300 behind 1800 in FP32 116 us.
+// 256 sequences of 1024 own tokens behind 16384 shared ones (32 query heads over 8, BF16) take 147 to 164 us,
+// 12 groups of 8 with 300 behind 1800 in FP32 115 us.
 // A second kernel joins the parts of each row.
 #include "decode.h"
 #include "ptx.cuh"
@@ -46,8 +46,9 @@ namespace
 constexpr int kThreads = 384; // three warpgroups: control, and twice four working warps
 constexpr int kWorkers = 8;   // streaming warps of a CTA
 constexpr int kTile = 128;    // rows and keys of a tile
-// As for the block attention: 128 x 88 + 256 x 208 registers are the launch's 384 x 168.
-constexpr int kRegsControl = 88, kRegsWork = 208, kMinLaunchRegs = 168;
+// 128 x 72 + 256 x 216 registers are the launch's 384 x 168 (with 88 and 208 the tiles' unit loop spills: 16 sequences of
+// 16 to 32 rows behind 2000 tokens 44.4 us for 42.3, 256 behind 16384 159 for 148).
+constexpr int kRegsControl = 72, kRegsWork = 216, kMinLaunchRegs = 168;
 static_assert(128 * kRegsControl + 256 * kRegsWork <= kThreads * kMinLaunchRegs, "register split");
 constexpr int kErrAttendTimeout = 42;
 
@@ -1190,38 +1191,97 @@ __device__ __forceinline__ void tile_softmax(const Args<X> &p, int which, Walk w
     unsigned seen = 0, turns = 0; // units of this tile of rows; of them with the other tile at work too
     bool ok = true;
     unsigned n = 0; // units of the CTA
+    constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes; // of a row of queries, 16 bytes per lane
     Part part;
-    while (next_part(p, which, w, part))
-    {
-        if (warp == 0 && lane == 0) write_meta(l, w, part);
-        const int rows = min(l.block, rows_of(p, which, part.item) - part.block * l.block);
-        if (g * kTile >= rows)
+    Row row;
+    int rows; // of the part's item
+    // the next part with rows in this tile, and its queries: the warp's 32 rows on their way to the tile
+    auto advance = [&]() {
+        while (next_part(p, which, w, part))
         {
-            n += part.units;
-            continue;
-        }
-        const Row row = row_of(p, which, part, g * kTile + r);
-        // the tile of queries: the warp's 32 rows, 16 bytes per lane, D/8 lanes per row
-        {
-            constexpr int kLanes = D / 8, kRowsAtOnce = 32 / kLanes;
-            const int chunk = lane % kLanes;
-            const uint4 *q = static_cast<const uint4 *>(p.a.q) + chunk;
-            uint4 x[32 / kRowsAtOnce];
-#pragma unroll
-            for (int i = 0; i < 32 / kRowsAtOnce; ++i)
-                x[i] = q[static_cast<size_t>(__shfl_sync(0xffffffffu, row.query, i * kRowsAtOnce + lane / kLanes)) * kLanes];
-#pragma unroll
-            for (int i = 0; i < 32 / kRowsAtOnce; ++i)
+            if (warp == 0 && lane == 0) write_meta(l, w, part);
+            rows = min(l.block, rows_of(p, which, part.item) - part.block * l.block);
+            if (g * kTile < rows)
             {
-                const int from = i * kRowsAtOnce + lane / kLanes, at = quarter * 32 + from;
-                if (!__shfl_sync(0xffffffffu, row.keys, from)) x[i] = make_uint4(0, 0, 0, 0);
-                st_shared_v4(sm.q(g) + (chunk >> 3) * (kTile * 128) + at * 128 + (((chunk & 7) ^ (at & 7)) << 4), x[i].x, x[i].y, x[i].z, x[i].w);
+                row = row_of(p, which, part, g * kTile + r);
+                const int chunk = lane % kLanes;
+                const uint4 *q = static_cast<const uint4 *>(p.a.q) + chunk;
+#pragma unroll
+                for (int i = 0; i < 32 / kRowsAtOnce; ++i)
+                {
+                    const int from = i * kRowsAtOnce + lane / kLanes, at = quarter * 32 + from;
+                    const int query = __shfl_sync(0xffffffffu, row.query, from), keys = __shfl_sync(0xffffffffu, row.keys, from);
+                    const uint32_t dst = sm.q(g) + (chunk >> 3) * (kTile * 128) + at * 128 + (((chunk & 7) ^ (at & 7)) << 4);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(q + static_cast<size_t>(query) * kLanes), "r"(keys ? 16 : 0)
+                                 : "memory"); // zeros for a row without a token
+                }
+                return true;
             }
+            n += part.units;
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sm.q_full(g));
-        float m = -INFINITY, sum = 0.f;
+        return false;
+    };
+    // The next part's queries are fetched while the last product runs, and are in place before the last part's results
+    // leave, so that its first scores are computed meanwhile.
+    const int at = g * kTile + r;
+    int done_rows = 0;                // of the part before
+    size_t place = 0;                 // of its results
+    float m = -INFINITY, sum = 0.f;
+    for (bool first = true;; first = false)
+    {
+        const bool have = ok && advance();
+        if (!first)
+        {
+            if (ok) ok = warp_wait(sm.pv_done(g), (seen - 1) & 1u);
+            if (!ok)
+            {
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                break;
+            }
+            tc_fence_after();
+        }
+        if (have)
+        {
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sm.q_full(g));
+        }
+        if (!first)
+        {
+            if (at < done_rows) l.ml[place + at] = make_float2(m * c, sum);
+            // a warp's 32 rows through its quarter of the P tile, 64 columns at a time, so that a store is whole
+            // rows: 16-byte chunk j of row i sits at chunk j ^ (i & 15)
+            const uint32_t stage = sm.p(g) + quarter * 8192;
+            float *dst = l.o + (place + g * kTile + quarter * 32) * D;
+#pragma unroll
+            for (int h = 0; h < D / 64; ++h)
+            {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                {
+                    float o[32];
+                    tmem_load_32(o_at + h * 64 + i * 32, o);
+#pragma unroll
+                    for (int t = 0; t < 8; ++t)
+                        st_shared_v4(stage + lane * 256 + (((i * 8 + t) ^ (lane & 15)) << 4), __float_as_uint(o[4 * t]), __float_as_uint(o[4 * t + 1]),
+                                     __float_as_uint(o[4 * t + 2]), __float_as_uint(o[4 * t + 3]));
+                }
+                __syncwarp();
+#pragma unroll 8
+                for (int i = 0; i < 32; i += 2)
+                {
+                    const int from = i + (lane >> 4);
+                    const float4 v = ld_shared_v4(stage + from * 256 + (((lane & 15) ^ (from & 15)) << 4));
+                    if (g * kTile + quarter * 32 + from < done_rows) *reinterpret_cast<float4 *>(dst + from * D + h * 64 + (lane & 15) * 4) = v;
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+        }
+        if (!have) break;
+        m = -INFINITY;
+        sum = 0.f;
         for (int u = 0; u < part.units && ok; ++u, ++seen)
         {
             if (!(ok = warp_wait(sm.s_full(g), seen & 1u))) break;
@@ -1315,44 +1375,8 @@ __device__ __forceinline__ void tile_softmax(const Args<X> &p, int which, Walk w
             if (lane == 0) mbar_arrive(sm.p_full(g));
         }
         n += part.units;
-        if (ok) ok = warp_wait(sm.pv_done(g), (seen - 1) & 1u);
-        if (!ok)
-        {
-            if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
-            break;
-        }
-        tc_fence_after();
-        const int at = g * kTile + r;
-        const size_t place = static_cast<size_t>(part.place) * l.part_rows;
-        if (at < rows) l.ml[place + at] = make_float2(m * c, sum);
-        // a warp's 32 rows through its quarter of the P tile, 64 columns at a time, so that a store is whole
-        // rows: 16-byte chunk j of row i sits at chunk j ^ (i & 15)
-        const uint32_t stage = sm.p(g) + quarter * 8192;
-        float *dst = l.o + (place + g * kTile + quarter * 32) * D;
-#pragma unroll
-        for (int h = 0; h < D / 64; ++h)
-        {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-            {
-                float o[32];
-                tmem_load_32(o_at + h * 64 + i * 32, o);
-#pragma unroll
-                for (int t = 0; t < 8; ++t)
-                    st_shared_v4(stage + lane * 256 + (((i * 8 + t) ^ (lane & 15)) << 4), __float_as_uint(o[4 * t]), __float_as_uint(o[4 * t + 1]),
-                                 __float_as_uint(o[4 * t + 2]), __float_as_uint(o[4 * t + 3]));
-            }
-            __syncwarp();
-#pragma unroll 8
-            for (int i = 0; i < 32; i += 2)
-            {
-                const int from = i + (lane >> 4);
-                const float4 v = ld_shared_v4(stage + from * 256 + (((lane & 15) ^ (from & 15)) << 4));
-                if (g * kTile + quarter * 32 + from < rows) *reinterpret_cast<float4 *>(dst + from * D + h * 64 + (lane & 15) * 4) = v;
-            }
-            __syncwarp();
-        }
-        tc_fence_before();
+        done_rows = rows;
+        place = static_cast<size_t>(part.place) * l.part_rows;
     }
     tc_fence_before();
     __syncwarp();
