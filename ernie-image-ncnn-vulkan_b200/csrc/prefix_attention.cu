@@ -816,7 +816,7 @@ template <int D, int R, bool X>
 __device__ __forceinline__ void stream_work_f32(const Args<X> &p, const Plan &plan, const PlanShared &shared, const Ring<float, D> &ring)
 {
     using L = Layout<float, D>;
-    constexpr int kSlotKeys = L::kSlotKeys, kKeys = 4, kRows = R / 2, kGroups = D / 64, kPairs = 2 * kGroups;
+    constexpr int kSlotKeys = L::kSlotKeys, kKeys = 4, kSteps = kSlotKeys / kKeys, kRows = R / 2, kGroups = D / 64, kPairs = 2 * kGroups;
     constexpr int kHeld = kRows >= 4 ? kRows / 4 : 1; // rows whose weights a lane works out
     const List &l = p.list[plan.which];
     const int worker = threadIdx.x / 32 - 4, lane = threadIdx.x & 31, half = lane & 16, share = lane & 15, first_row = half ? kRows : 0;
@@ -868,17 +868,17 @@ __device__ __forceinline__ void stream_work_f32(const Args<X> &p, const Plan &pl
                 if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
                 return;
             }
-            bool v_there = mbar_test(ring.full(worker, n + 1), ring.round(n + 1));
+            const bool v_there = mbar_test(ring.full(worker, n + 1), ring.round(n + 1));
+            const int valid = part.item.keys - key0; // what lies past the last key may be anything, NaN too
+            const uint32_t k = ring.slot(worker, n), v = ring.slot(worker, n + 1);
+            // dims 64 j + 4 share .. + 3 of key i of the slot: column block, the key's row and its swizzle in one
+            // exclusive or (slots are 1024-byte aligned)
+            const uint32_t lane_part = (share >> 3) * (kSlotKeys * 128) + ((share & 7) << 4);
+            auto at = [&](uint32_t slot, int j, int i) { return ((slot + lane_part) ^ (i * 144)) + j * (2 * kSlotKeys * 128); };
+            float w8[kSteps][kHeld]; // scores, then weights: of key 4 t + my_key
 #pragma unroll
-            for (int first = 0; first < kSlotKeys; first += kKeys, key0 += kKeys)
+            for (int t = 0; t < kSteps; ++t)
             {
-                const int valid = part.item.keys - key0; // what lies past the last key may be anything, NaN too
-                if (valid <= 0) continue;
-                const uint32_t k = ring.slot(worker, n), v = ring.slot(worker, n + 1);
-                // dims 64 j + 4 share .. + 3 of the step's key i: column block, the key's row and its swizzle in one
-                // exclusive or (slots are 1024-byte aligned)
-                const uint32_t lane_part = (share >> 3) * (kSlotKeys * 128) + ((share & 7) << 4);
-                auto at = [&](uint32_t slot, int j, int i) { return ((slot + lane_part) ^ ((first + i) * 144)) + j * (2 * kSlotKeys * 128); };
                 // partial sums over the lane's dims, value i * kRows + row; two keys at a time, for the registers
                 float s[kKeys * kRows];
 #pragma unroll
@@ -893,7 +893,7 @@ __device__ __forceinline__ void stream_work_f32(const Args<X> &p, const Plan &pl
 #pragma unroll
                         for (int j = 0; j < kGroups; ++j)
                         {
-                            const float4 x = ld_shared_v4(at(k, j, i + e));
+                            const float4 x = ld_shared_v4(at(k, j, t * kKeys + i + e));
 #pragma unroll
                             for (int r = 0; r < kRows; ++r)
                             {
@@ -927,73 +927,77 @@ __device__ __forceinline__ void stream_work_f32(const Args<X> &p, const Plan &pl
                     else
                         s[0] += __shfl_xor_sync(0xffffffffu, s[0], step);
                 }
-                if (key0 + kKeys > all_see)
-                {
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i) w8[t][i] = s[i];
+            }
+            if (key0 + kSlotKeys > all_see)
+            {
+#pragma unroll
+                for (int t = 0; t < kSteps; ++t)
 #pragma unroll
                     for (int i = 0; i < kHeld; ++i)
-                        if (key0 + my_key >= seen[i]) s[i] = -INFINITY;
-                }
-                bool raise = false;
+                        if (key0 + t * kKeys + my_key >= seen[i]) w8[t][i] = -INFINITY;
+            }
+            bool raise = false;
 #pragma unroll
-                for (int i = 0; i < kHeld; ++i) raise |= (s[i] - m[i]) * p.scale > 8.f;
-                // the maximum is raised only when a score passes it by 2^8, as for BF16
-                if (__any_sync(0xffffffffu, raise))
-                {
-                    float f[kHeld];
-#pragma unroll
-                    for (int i = 0; i < kHeld; ++i)
-                    {
-                        float top = fmaxf(s[i], __shfl_xor_sync(0xffffffffu, s[i], 4));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                        top = fmaxf(top, m[i]);
-                        f[i] = top == m[i] ? 1.f : exp2_fast((m[i] - top) * p.scale);
-                        m[i] = top;
-                        c[i] = top == -INFINITY ? 0.f : -top * p.scale;
-                        sum[i] *= f[i];
-                    }
-#pragma unroll
-                    for (int r = 0; r < kRows; ++r)
-                    {
-                        const float g = __shfl_sync(0xffffffffu, f[r % kHeld], holder(r));
-#pragma unroll
-                        for (int d = 0; d < kPairs; ++d) o[r][d] = make_float2(o[r][d].x * g, o[r][d].y * g);
-                    }
-                }
+            for (int i = 0; i < kHeld; ++i) raise |= (fmaxf(w8[0][i], w8[1][i]) - m[i]) * p.scale > 8.f;
+            // the maximum is raised only when a score passes it by 2^8, as for BF16
+            if (__any_sync(0xffffffffu, raise))
+            {
+                float f[kHeld];
 #pragma unroll
                 for (int i = 0; i < kHeld; ++i)
                 {
-                    s[i] = exp2_fast(fmaf(s[i], p.scale, c[i]));
-                    sum[i] += s[i];
-                }
-                if (!__all_sync(0xffffffffu, v_there))
-                {
-                    if (!warp_wait(ring.full(worker, n + 1), ring.round(n + 1)))
-                    {
-                        if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
-                        return;
-                    }
-                    v_there = true;
+                    float top = fmaxf(w8[0][i], w8[1][i]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, m[i]);
+                    f[i] = top == m[i] ? 1.f : exp2_fast((m[i] - top) * p.scale);
+                    m[i] = top;
+                    c[i] = top == -INFINITY ? 0.f : -top * p.scale;
+                    sum[i] *= f[i];
                 }
 #pragma unroll
-                for (int i = 0; i < kKeys; ++i)
+                for (int r = 0; r < kRows; ++r)
                 {
-                    float weight[kRows];
+                    const float g = __shfl_sync(0xffffffffu, f[r % kHeld], holder(r));
 #pragma unroll
-                    for (int r = 0; r < kRows; ++r) weight[r] = __shfl_sync(0xffffffffu, s[r % kHeld], holder(r) + 4 * i);
-                    if (i >= valid) break;
+                    for (int d = 0; d < kPairs; ++d) o[r][d] = make_float2(o[r][d].x * g, o[r][d].y * g);
+                }
+            }
 #pragma unroll
-                    for (int j = 0; j < kGroups; ++j)
+            for (int t = 0; t < kSteps; ++t)
+#pragma unroll
+                for (int i = 0; i < kHeld; ++i)
+                {
+                    w8[t][i] = exp2_fast(fmaf(w8[t][i], p.scale, c[i]));
+                    sum[i] += w8[t][i];
+                }
+            if (!__all_sync(0xffffffffu, v_there) && !warp_wait(ring.full(worker, n + 1), ring.round(n + 1)))
+            {
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < kSlotKeys; ++i)
+            {
+                float weight[kRows];
+#pragma unroll
+                for (int r = 0; r < kRows; ++r) weight[r] = __shfl_sync(0xffffffffu, w8[i / kKeys][r % kHeld], holder(r) + 4 * (i % kKeys));
+                if (i >= valid) break;
+#pragma unroll
+                for (int j = 0; j < kGroups; ++j)
+                {
+                    const float4 x = ld_shared_v4(at(v, j, i));
+#pragma unroll
+                    for (int r = 0; r < kRows; ++r)
                     {
-                        const float4 x = ld_shared_v4(at(v, j, i));
-#pragma unroll
-                        for (int r = 0; r < kRows; ++r)
-                        {
-                            o[r][2 * j] = __ffma2_rn(make_float2(weight[r], weight[r]), make_float2(x.x, x.y), o[r][2 * j]);
-                            o[r][2 * j + 1] = __ffma2_rn(make_float2(weight[r], weight[r]), make_float2(x.z, x.w), o[r][2 * j + 1]);
-                        }
+                        o[r][2 * j] = __ffma2_rn(make_float2(weight[r], weight[r]), make_float2(x.x, x.y), o[r][2 * j]);
+                        o[r][2 * j + 1] = __ffma2_rn(make_float2(weight[r], weight[r]), make_float2(x.z, x.w), o[r][2 * j + 1]);
                     }
                 }
             }
+            key0 += kSlotKeys;
             __syncwarp();
             if (lane < 2) mbar_arrive(ring.empty(worker, n + lane));
         }
