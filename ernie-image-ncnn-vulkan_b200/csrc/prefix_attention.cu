@@ -10,10 +10,10 @@
 // A row is a query head of a slot: the heads/kv_heads query heads that share a K/V head are rows of one item.
 // An item's keys are cut into units, and each list's units are dealt out evenly, in order, to that list's
 // workers (a fixed cost of every item counted in), so that an item may span several workers and a worker
-// several items; an item's share of a worker is a part. Along the order both the item and the worker only ever step up, so item + worker numbers the
-// parts without gaps or clashes, and an item's parts lie side by side. The lists share the CTAs by their
-// estimated cost. All of this is worked out on the device, by every CTA for itself, from the lengths of this
-// very call.
+// several items; an item's share of a worker is a part. Along the order both the item and the worker only ever
+// step up, so item + worker numbers the parts without gaps or clashes, and an item's parts lie side by side. The
+// lists share the CTAs by their estimated cost. All of this is worked out on the device, by every CTA for itself,
+// from the lengths of this very call.
 //
 // Where a ragged batch's group has more slots than one block holds, the rows of its prefix items are those of its
 // tokens instead of its slots, found through the sums of the sequences' counts: 64 sequences of which one brings
@@ -31,7 +31,7 @@
 //           products that read 64 KB each, 64 KB of weights stored, 64 KB of keys and values loaded, 3072
 //           cycles (the exponentials alone would take 2048).
 // 256 sequences of 1024 own tokens behind 16384 shared ones (32 query heads over 8, BF16) take 147 to 164 us,
-// 12 groups of 8 with 300 behind 1800 in FP32 115 us.
+// 12 groups of 8 with 300 behind 1800 in FP32 103 us.
 // A second kernel joins the parts of each row.
 #include "decode.h"
 #include "ptx.cuh"
@@ -808,10 +808,11 @@ __device__ __forceinline__ void stream_work(const Args<X> &p, const Plan &plan, 
 // FP32: R rows of a warp, in two halves of 16 lanes; a lane holds every sixteenth group of four dims of the
 // queries and values of its half's rows, two dims to a packed FMA. A step takes four keys: partial scores of
 // all rows, then a scatter of their sums over the 16 lanes (key lane/4 % 4 and a quarter of the rows each),
-// the weights there, and their way back by shuffles. Shared memory and shuffles deliver a value per lane and
-// cycle, so a value of K or V has to serve many rows: eight rows to a lane take 250 of those cycles for a slot of
-// eight keys, one row to a lane 1024. The issue of 75 million warp instructions then is 67 of the 116 us that 12
-// groups of 8 sequences take (254 MB; sums over single dims: 144 us; rows paired in the packed FMAs: 141 us).
+// the weights of a slot's eight keys there, and their way back by shuffles. Shared memory and shuffles deliver a
+// value per lane and cycle, so a value of K or V has to serve many rows: eight rows to a lane take 250 of those
+// cycles for a slot, one row to a lane 1024. What bounds it then is latency, with two warps to a scheduler: of the
+// 103 us that 12 groups of 8 sequences take (254 MB) the FMA pipe works 36 (sums over single dims: 144 us; rows
+// paired in the packed FMAs: 141 us; a round of weights for every four keys: 115 us).
 template <int D, int R, bool X>
 __device__ __forceinline__ void stream_work_f32(const Args<X> &p, const Plan &plan, const PlanShared &shared, const Ring<float, D> &ring)
 {
@@ -1674,9 +1675,10 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
         l.part_rows = l.rows < l.block ? l.rows : l.block;
         l.unit_shift = l.tile ? 7 : 5;
         // nanoseconds of an SM: a tile's unit with one and with two tiles of rows; a streamed unit as fast as an SM
-        // takes them when the memory is not the limit
+        // takes them when the memory is not the limit. An item's fixed cost: queries in, partial results out (streamed
+        // items at three units: 64 sequences behind 4096 tokens 26.6 us for 25.2, FP32 groups 108 for 103)
         l.cost = l.tile ? (l.rows > kTile ? 1900 : 1100) : (kv.bf16 ? 180 : l.rows > 8 ? 850 : l.rows > 4 ? 500 : 350) * kv.dim / 128;
-        l.lead = l.tile ? (l.rows > kTile ? 4 : 6) : 3;
+        l.lead = l.tile ? (l.rows > kTile ? 4 : 6) : 1;
         const size_t items = static_cast<size_t>(l.owners) * l.blocks * kv.kv_heads;
         const size_t parts = l.owners ? items + ctas * (l.tile ? 1 : kWorkers) : 0;
         l.o = reinterpret_cast<float *>(base + at);
