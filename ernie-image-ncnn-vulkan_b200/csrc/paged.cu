@@ -268,8 +268,9 @@ template <class In, class Out> int launch_append(const AppendArgs &a, int sms, c
 {
     const int slots = a.batch.sequences * a.batch.queries, width = a.heads + 2 * a.kv.kv_heads;
     const int at_once = kAppendThreads / (a.kv.dim / 8), passes = (width + at_once - 1) / at_once;
-    // few slots: their heads over several CTAs (one decode step of five beams: six CTAs a slot)
-    const int share = slots >= 4 * sms ? 1 : passes < 64 ? passes : 64;
+    // few slots: their heads over several CTAs (48 heads of 128: six). 100 slots 5.0 us, whole ones 5.2; 300 slots
+    // 5.2 and 5.1; 600 slots 8.5 and 5.2
+    const int share = slots >= 2 * sms ? 1 : passes < 64 ? passes : 64;
     const int vectors = reinterpret_cast<uintptr_t>(a.qkv) % (4 * sizeof(In)) == 0 && a.ld % 4 == 0;
     const dim3 grid(slots, share);
     if (a.kv.dim == 64) return launch_dependent(append_kernel<In, Out, 64>, grid, kAppendThreads, 0, stream, a, vectors);
