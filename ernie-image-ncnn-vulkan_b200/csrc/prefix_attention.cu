@@ -28,7 +28,7 @@
 //   tile    many rows of a BF16 cache. A worker is a CTA: 256 rows (two tiles of 128) share each K/V tile on
 //           the tensor cores (tcgen05.mma, accumulators in TMEM), one row per softmax thread. A unit of 256
 //           rows and 128 keys takes about 3350 cycles. Shared memory's 128 bytes per cycle bound it: four
-//           products that read 64 KB each, 64 KB of weights stored, 64 KB of keys and values loaded, 3072
+//           products that read 64 KB each, 64 KB of weights stored, 64 KB of keys and values loaded, 3070
 //           cycles (the exponentials alone would take 2048).
 // 256 sequences of 1024 own tokens behind 16384 shared ones (32 query heads over 8, BF16) take 147 to 164 us,
 // 12 groups of 8 with 300 behind 1800 in FP32 103 us.
