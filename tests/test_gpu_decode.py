@@ -314,6 +314,26 @@ def test_attention_lengths(ctx, dev, lens, counts, prefix, precision):
                           prefix_lens=prefix))
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_attention_of_random_shapes(ctx, dev, seed):
+    """Any head layout, page, batch and raggedness; the largest of the 24 has some 20000 rows."""
+    rng = np.random.default_rng(4000 + seed)
+    kv_heads, share = int(rng.choice([1, 2, 3, 4, 8])), int(rng.choice([1, 2, 3, 4, 5, 7, 8, 16]))
+    dim, page = int(rng.choice([64, 128])), int(rng.choice([8, 16, 32, 64, 128]))
+    groups, per = int(rng.choice([1, 2, 3, 5])), int(np.exp(rng.uniform(0, np.log(70))))
+    queries, prefix, suffix = (int(np.exp(rng.uniform(0, np.log(most)))) for most in (60, 3000, 600))
+    while groups * per * queries * kv_heads * share > 20000:
+        per, queries = max(1, per // 2), max(1, queries // 2)
+    n, ragged = groups * per, {}
+    if seed % 3 == 1:
+        ragged["counts"] = np.full(n, queries)
+    if seed % 3 == 2:
+        ragged["counts"] = np.where(rng.random(n) < 0.3, queries, rng.integers(0, 2, n))
+        ragged["lens"] = rng.integers(0, suffix + queries, n)
+    holds(*attention_case(ctx, dev, rng, groups, per, queries, prefix, suffix, kv_heads * share, kv_heads, dim, page,
+                          ec.BF16 if seed % 2 else ec.FP32, **ragged))
+
+
 @pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
 def test_attention_without_a_prefix(ctx, dev, precision):
     rng = np.random.default_rng(9)
