@@ -47,7 +47,7 @@ constexpr int kThreads = 384; // three warpgroups: control, and twice four worki
 constexpr int kWorkers = 8;   // streaming warps of a CTA
 constexpr int kTile = 128;    // rows and keys of a tile
 // 128 x 72 + 256 x 216 registers are the launch's 384 x 168 (with 88 and 208 the tiles' unit loop spills: 16 sequences of
-// 16 to 32 rows behind 2000 tokens 44.4 us for 42.3, 256 behind 16384 159 for 148).
+// 16 to 32 rows behind 2000 tokens 44.7 us for 42.3, 256 behind 16384 165 for 158).
 constexpr int kRegsControl = 72, kRegsWork = 216, kMinLaunchRegs = 168;
 static_assert(128 * kRegsControl + 256 * kRegsWork <= kThreads * kMinLaunchRegs, "register split");
 constexpr int kErrAttendTimeout = 42;
@@ -1638,18 +1638,22 @@ __global__ void __launch_bounds__(kJoinWarps * 32, R == 1 ? 1 : 4) join_kernel(c
 
 // ---------------------------------------------------------------- host
 // More rows of an owner and K/V head than this go to the tensor cores' tiles. With 8 K/V heads of 128 (one group
-// behind 2048 tokens / eight such groups / one behind 16384), in us, streamed and in tiles: 24 rows 23 / 23 / 35 and
-// 17 / 34 / 29; 40 rows 22 / 29 / 37 and 17 / 34 / 29; 80 rows 20 / 50 / 45 and 17 / 41 / 30; 200 rows 25 / 105 / 91
-// and 20 / 61 / 37.
+// behind 2048 tokens / eight such groups / one behind 16384), in us, streamed and in tiles: 24 rows 22 / 22 / 34 and
+// 17 / 33 / 29; 40 rows 23 / 26 / 36 and 17 / 34 / 29; 80 rows 21 / 45 / 44 and 18 / 38 / 30; 200 rows 24 / 91 / 86
+// and 20 / 55 / 38.
 constexpr int kTileRows = 32;
 
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
-// Within one block, slots without a token cost nothing. With one slot to a sequence they are taken to be rare: 256 such
-// sequences behind 8192 tokens take 79 us by slots and 85 by tokens (idle every other one: 57). With 32 slots and 64
-// sequences behind 4096 tokens, by slots 184 us whatever the counts; by tokens 65 with one sequence of 32 and the
-// others of one, 192 with all of 32; 16 sequences of 0 to 32 behind 2000: 47 and 38.
-bool by_tokens(const AttendArgs &p, const PagedBatch &b) { return b.counts && b.queries > 1 && p.list[0].owners && p.list[0].blocks > 1; }
+// Within one block, slots without a token cost nothing. The sums take 1 to 4 us of a call whose slots are all filled: 64
+// sequences of 32 slots behind 4096 tokens 172 us by slots and 176 by tokens; with one slot each, 256 behind 8192 77 and
+// 77, five behind 300 11.5 and 12.8, 12 groups of eight (FP32) 103 and 105. They save what is empty: of the 64 one with 32
+// tokens and the others with one each 179 and 58, 16 of 0 to 32 tokens behind 2000 46 and 37, every other one of the 256
+// idle 74 and 46. So sequences of one slot go by slots while a group has few rows.
+bool by_tokens(const AttendArgs &p, const PagedBatch &b)
+{
+    return b.counts && p.list[0].owners && p.list[0].blocks > 1 && (b.queries > 1 || p.list[0].rows > 256);
+}
 
 // Lays out the lists and the workspace; returns its size.
 size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, void *workspace, AttendArgs &p)

@@ -276,7 +276,7 @@ def test_attention_of_large_batches(ctx, dev, case, precision):
 @pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("groups,per,queries,kind", [
     (1, 64, 32, "one long"), (3, 9, 20, "one long"), (2, 12, 33, "random"), (2, 300, 3, "random"), (5, 1, 150, "random"),
-    (2, 40, 8, "last"), (3, 30, 8, "one group idle"), (2, 20, 24, "out of range")])
+    (2, 40, 8, "last"), (3, 30, 8, "one group idle"), (2, 20, 24, "out of range"), (2, 70, 1, "random")])
 def test_attention_of_mixed_batches(ctx, dev, groups, per, queries, kind, precision):
     """Sequences with one new token beside ones with many or none: the rows that share a prefix are the tokens'."""
     rng = np.random.default_rng(groups + per + queries)
