@@ -33,6 +33,7 @@
 // 256 sequences of 1024 own tokens behind 16384 shared ones (32 query heads over 8, BF16) take 147 to 164 us,
 // 12 groups of 8 with 300 behind 1800 in FP32 103 us.
 // A second kernel joins the parts of each row.
+#include "attend_layout.h"
 #include "decode.h"
 #include "ptx.cuh"
 #include <cudaTypedefs.h>
@@ -46,6 +47,7 @@ namespace
 constexpr int kThreads = 384; // three warpgroups: control, and twice four working warps
 constexpr int kWorkers = 8;   // streaming warps of a CTA
 constexpr int kTile = 128;    // rows and keys of a tile
+static_assert(kTile == kWeightRows, "weights' tile");
 // 128 x 72 + 256 x 216 registers are the launch's 384 x 168 (with 88 and 208 the tiles' unit loop spills: 16 sequences of
 // 16 to 32 rows behind 2000 tokens 44.7 us for 42.3, 256 behind 16384 165 for 158).
 constexpr int kRegsControl = 72, kRegsWork = 216, kMinLaunchRegs = 168;
@@ -1255,9 +1257,7 @@ __device__ __forceinline__ void tile_softmax(const Args<X> &p, int which, Walk w
         if (!first)
         {
             if (at < done_rows) l.ml[place + at] = make_float2(m * c, sum);
-            // a warp's 32 rows through its quarter of the P tile, 64 columns at a time, so that a store is whole
-            // rows: 16-byte chunk j of row i sits at chunk j ^ (i & 15)
-            const uint32_t stage = sm.p(g) + quarter * 8192;
+            // a warp's 32 rows through their own places in the P tile, 64 columns at a time, so that a store is whole rows
             float *dst = l.o + (place + g * kTile + quarter * 32) * D;
 #pragma unroll
             for (int h = 0; h < D / 64; ++h)
@@ -1269,7 +1269,7 @@ __device__ __forceinline__ void tile_softmax(const Args<X> &p, int which, Walk w
                     tmem_load_32(o_at + h * 64 + i * 32, o);
 #pragma unroll
                     for (int t = 0; t < 8; ++t)
-                        st_shared_v4(stage + lane * 256 + (((i * 8 + t) ^ (lane & 15)) << 4), __float_as_uint(o[4 * t]), __float_as_uint(o[4 * t + 1]),
+                        st_shared_v4(sm.p(g) + weight_chunk(r, i * 8 + t), __float_as_uint(o[4 * t]), __float_as_uint(o[4 * t + 1]),
                                      __float_as_uint(o[4 * t + 2]), __float_as_uint(o[4 * t + 3]));
                 }
                 __syncwarp();
@@ -1277,7 +1277,7 @@ __device__ __forceinline__ void tile_softmax(const Args<X> &p, int which, Walk w
                 for (int i = 0; i < 32; i += 2)
                 {
                     const int from = i + (lane >> 4);
-                    const float4 v = ld_shared_v4(stage + from * 256 + (((lane & 15) ^ (from & 15)) << 4));
+                    const float4 v = ld_shared_v4(sm.p(g) + weight_chunk(quarter * 32 + from, lane & 15));
                     if (g * kTile + quarter * 32 + from < done_rows) *reinterpret_cast<float4 *>(dst + from * D + h * 64 + (lane & 15) * 4) = v;
                 }
                 __syncwarp();
@@ -1359,8 +1359,7 @@ __device__ __forceinline__ void tile_softmax(const Args<X> &p, int which, Walk w
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                st_shared_v4(sm.p(g) + (i >> 3) * (kTile * 128) + r * 128 + (((i & 7) ^ (r & 7)) << 4), packed[4 * i], packed[4 * i + 1],
-                             packed[4 * i + 2], packed[4 * i + 3]);
+                st_shared_v4(sm.p(g) + weight_chunk(r, i), packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
             const float2 s4 = __fadd2_rn(__fadd2_rn(part_sum[0], part_sum[1]), __fadd2_rn(part_sum[2], part_sum[3]));
             sum += s4.x + s4.y;
             // values past the item's last key may be anything, NaN too: zeros, by both tiles' threads alike

@@ -2,6 +2,8 @@
 before the context is looked at, so a call with good arguments and no context is refused for the context alone), and
 the oracle's own definitions against direct ones."""
 import ctypes
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -204,6 +206,15 @@ def test_null_descriptions():
     assert lib.ernie_cuda_prefix_attention_workspace(None, kv().c, batch().c, 32, None) == ec.ERROR
     assert lib.ernie_cuda_beam_select_workspace(None, 1, 1, 1, None) == ec.ERROR
     assert lib.ernie_cuda_beam_reorder(None, None, 1, 1, None, None, 1, None, None, None) == ec.ERROR
+
+
+def test_warps_of_a_tile_share_no_bytes(tmp_path):
+    """Compiles the attention's layout header by itself and looks at every byte that a softmax warp touches."""
+    here, exe = os.path.dirname(os.path.abspath(__file__)), str(tmp_path / "layout")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I" + os.path.join(os.path.dirname(ec.LIB_PATH), "csrc"),
+                    os.path.join(here, "cpp", "test_attend_layout.cpp"), "-o", exe], check=True, capture_output=True, text=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "attention layout passed" in r.stdout, r.stderr + r.stdout
 
 
 # ------------------------------------------------------------------ the oracle

@@ -361,6 +361,29 @@ def test_attention_repeats_bit_for_bit_and_ignores_its_scratch(ctx, dev, queries
     assert np.array_equal(got, again)
 
 
+@pytest.mark.parametrize("groups,per,queries,heads,kv_heads,dim,page", [
+    (1, 300, 40, 2, 2, 128, 16),   # 40 rows: two of a tile's four warps store nothing
+    (1, 160, 25, 8, 2, 64, 8),     # 100 rows
+    (4, 25, 33, 8, 2, 128, 32),    # 132 rows: the second tile has four
+    (2, 40, 70, 6, 2, 128, 64),    # 210 rows
+    (120, 5, 9, 4, 2, 128, 16)])   # many short prefixes
+def test_attention_of_many_short_parts_repeats(ctx, dev, groups, per, queries, heads, kv_heads, dim, page):
+    """Several parts on every CTA and tile of rows, each of one to three key tiles: a part's results leave while the
+    next part's weights come in. Right once, then the same bits 200 times."""
+    rng = np.random.default_rng(groups + per + queries)
+    holds(*attention_case(ctx, dev, rng, groups, per, queries, 300, 300, heads, kv_heads, dim, page, ec.BF16,
+                          prefix_lens=rng.integers(1, 300, groups)))
+    (layers, pages), tables, prefix_tables = dev.shapes["k"][0][:2], dev.shapes["t"][0], dev.shapes["pt"][0]
+    b = dev.buffers
+    kv = ec.PagedKv(b["k"], b["v"], layers, pages, page, kv_heads, dim, ec.BF16)
+    batch = ec.PagedBatch(groups * per, queries, b["t"], tables[1], b["n"], b["c"], groups, b["pt"], prefix_tables[1], b["pl"])
+    first = dev.raw("out").copy()
+    for _ in range(200):
+        ctx.prefix_attention(kv, 0, batch, b["q"], heads, b["out"], b["work"], b["work"].nbytes)
+        ctx.synchronize()
+        assert np.array_equal(dev.raw("out"), first)
+
+
 @pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("per", [2, 40])
 def test_attention_of_bad_pages(ctx, dev, per, precision):
