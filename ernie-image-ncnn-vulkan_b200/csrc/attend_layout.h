@@ -28,4 +28,16 @@ constexpr bool weight_chunks_are_apart()
     return true;
 }
 static_assert(weight_chunks_are_apart(), "chunks of the weights' tile");
+
+// The parts of an item that the workers `first` to `last` left behind, at places item + first and on; a list has places
+// for items + workers of them. None where the two numbers cannot be workers: they come from the workspace, which holds
+// anything if a worker gave up before it reached the item.
+struct PartRange
+{
+    int first, count;
+};
+constexpr PartRange parts_between(int first, int last, int workers)
+{
+    return first < 0 || last < first || last >= workers ? PartRange{0, 0} : PartRange{first, last - first + 1};
+}
 } // namespace ernie_b200

@@ -285,6 +285,8 @@ extern "C" int ernie_cuda_context_synchronize(ernie_cuda_context *ctx)
         cudaMemset(ctx->error_flag, 0, sizeof(int));
         if (flag == ERNIE_CUDA_STATUS_PAGED_RANGE)
             return fail(ERNIE_CUDA_ERROR, "A page, length, position or parent is out of range (status 41)");
+        if (flag == ERNIE_CUDA_STATUS_ATTENTION_UNFINISHED)
+            return fail(ERNIE_CUDA_ERROR, "The attention did not finish: a device-side wait timed out (status 42)");
         return fail(ERNIE_CUDA_ERROR, "Device-side wait timed out (status " + std::to_string(flag) + ")");
     }
     return ERNIE_CUDA_OK;

@@ -7,7 +7,7 @@
 
 namespace ernie_b200
 {
-constexpr int kErrPagedRange = 41;
+constexpr int kErrPagedRange = 41, kErrAttendUnfinished = 42;
 
 // K and V of one layer: [pages][kv_heads][page_size][dim] of T.
 struct PagedLayer

@@ -8,6 +8,8 @@
 using namespace ernie_b200;
 using namespace ernie_b200::capi;
 
+static_assert(kErrPagedRange == ERNIE_CUDA_STATUS_PAGED_RANGE && kErrAttendUnfinished == ERNIE_CUDA_STATUS_ATTENTION_UNFINISHED, "statuses");
+
 namespace
 {
 constexpr long long kMaxSlots = 1 << 24; // sequences * queries

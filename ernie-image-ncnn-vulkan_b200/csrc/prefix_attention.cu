@@ -52,7 +52,6 @@ static_assert(kTile == kWeightRows, "weights' tile");
 // 16 to 32 rows behind 2000 tokens 44.7 us for 42.3, 256 behind 16384 165 for 158).
 constexpr int kRegsControl = 72, kRegsWork = 216, kMinLaunchRegs = 168;
 static_assert(128 * kRegsControl + 256 * kRegsWork <= kThreads * kMinLaunchRegs, "register split");
-constexpr int kErrAttendTimeout = 42;
 
 // Division of numbers below 2^31 by a divisor that the host knows: n / d = (hi32(n m) + n) >> shift.
 struct Divisor
@@ -82,6 +81,7 @@ struct List
     int unit_shift; // log2 of a unit's keys
     int lead;       // an item's fixed cost, in units
     int cost;       // of a unit on an SM, relative
+    int workers;    // that the list may be dealt out to
     float *o;       // [items + workers][part_rows][D]
     float2 *ml;     // [items + workers][part_rows]
     int2 *meta;     // [items]: the workers of the first and the last part
@@ -678,7 +678,7 @@ __device__ __forceinline__ void stream_produce(const Args<X> &p, const Plan &pla
         }
         else if (more && clock64() - since > kWaitLimitCycles)
         {
-            if (lane == leader) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+            if (lane == leader) atomicExch(p.a.batch.error_flag, kErrAttendUnfinished);
             more = false;
         }
         __syncwarp();
@@ -717,7 +717,7 @@ __device__ __forceinline__ void stream_work(const Args<X> &p, const Plan &plan, 
         {
             if (!warp_wait(ring.full(worker, n), ring.round(n)))
             {
-                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendUnfinished);
                 return;
             }
             const bool v_there = mbar_test(ring.full(worker, n + 1), ring.round(n + 1));
@@ -777,7 +777,7 @@ __device__ __forceinline__ void stream_work(const Args<X> &p, const Plan &plan, 
             }
             if (!__all_sync(0xffffffffu, v_there) && !warp_wait(ring.full(worker, n + 1), ring.round(n + 1)))
             {
-                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendUnfinished);
                 return;
             }
             x.weigh(ring.slot(worker, n + 1), lane, s, part.item.keys - key0, o);
@@ -868,7 +868,7 @@ __device__ __forceinline__ void stream_work_f32(const Args<X> &p, const Plan &pl
         {
             if (!warp_wait(ring.full(worker, n), ring.round(n)))
             {
-                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendUnfinished);
                 return;
             }
             const bool v_there = mbar_test(ring.full(worker, n + 1), ring.round(n + 1));
@@ -978,7 +978,7 @@ __device__ __forceinline__ void stream_work_f32(const Args<X> &p, const Plan &pl
                 }
             if (!__all_sync(0xffffffffu, v_there) && !warp_wait(ring.full(worker, n + 1), ring.round(n + 1)))
             {
-                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendUnfinished);
                 return;
             }
 #pragma unroll
@@ -1127,7 +1127,7 @@ __device__ __forceinline__ void tile_produce(const Args<X> &p, int which, Walk w
         have_next = have_after;
     }
     if (bad) report_range(p.a.batch.error_flag);
-    if (!ok && lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+    if (!ok && lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendUnfinished);
 }
 
 // The products of tile g of rows, by one thread.
@@ -1185,7 +1185,7 @@ template <int D, bool X> __device__ __forceinline__ void tile_multiply(const Arg
             umma_commit(sm.empty(sm.v_load(n)));
         }
     }
-    if (!ok) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+    if (!ok) atomicExch(p.a.batch.error_flag, kErrAttendUnfinished);
 }
 
 template <int D, bool X>
@@ -1242,7 +1242,7 @@ __device__ __forceinline__ void tile_softmax(const Args<X> &p, int which, Walk w
             if (ok) ok = warp_wait(sm.pv_done(g), (seen - 1) & 1u);
             if (!ok)
             {
-                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                if (lane == 0) atomicExch(p.a.batch.error_flag, kErrAttendUnfinished);
                 break;
             }
             tc_fence_after();
@@ -1445,7 +1445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if ((threadIdx.x & 31) == 0) tile_multiply<D>(p, plan.which, w, sm, tmem, warp - 1);
                     __syncwarp();
                     if (warp == 2) return;
-                    if (!warp_wait(sm.done(), 0) && (threadIdx.x & 31) == 0) atomicExch(p.a.batch.error_flag, kErrAttendTimeout);
+                    if (!warp_wait(sm.done(), 0) && (threadIdx.x & 31) == 0) atomicExch(p.a.batch.error_flag, kErrAttendUnfinished);
                     tc_fence_after();
                     tmem_dealloc(tmem, 512);
                 }
@@ -1533,8 +1533,10 @@ __global__ void __launch_bounds__(kJoinWarps * 32, R == 1 ? 1 : 4) join_kernel(c
     {
         if (item[which] < 0) continue;
         const int2 meta = p.list[which].meta[item[which]];
-        parts[which] = meta.y - meta.x + 1;
-        first[which] = item[which] + meta.x;
+        const PartRange range = parts_between(meta.x, meta.y, p.list[which].workers);
+        if (range.count == 0) atomicExch(b.error_flag, kErrAttendUnfinished); // a worker gave up
+        parts[which] = range.count;
+        first[which] = item[which] + range.first;
     }
     const int total = parts[0] + parts[1], most_parts = __reduce_max_sync(full, total);
     float top = -INFINITY, sum = 0.f, o[R][N] = {};
@@ -1683,7 +1685,8 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
         l.cost = l.tile ? (l.rows > kTile ? 1900 : 1100) : (kv.bf16 ? 180 : l.rows > 8 ? 850 : l.rows > 4 ? 500 : 350) * kv.dim / 128;
         l.lead = l.tile ? (l.rows > kTile ? 4 : 6) : 1;
         const size_t items = static_cast<size_t>(l.owners) * l.blocks * kv.kv_heads;
-        const size_t parts = l.owners ? items + ctas * (l.tile ? 1 : kWorkers) : 0;
+        l.workers = ctas * (l.tile ? 1 : kWorkers);
+        const size_t parts = l.owners ? items + l.workers : 0;
         l.o = reinterpret_cast<float *>(base + at);
         at += rounded(parts * l.part_rows * kv.dim * sizeof(float));
         l.ml = reinterpret_cast<float2 *>(base + at);

@@ -389,6 +389,9 @@ int ernie_cuda_pe_logits(ernie_cuda_pe_session *session, const float *hidden, fl
    keys count as zeros and nothing is stored there, and the next ernie_cuda_context_synchronize reports
    status 41. Two sequences that store into the same page in one call race. */
 #define ERNIE_CUDA_STATUS_PAGED_RANGE 41
+/* One of the attention's bounded waits ran out (some two seconds): the call ended, its results are not to be used.
+   Lengths, counts and tables may not change while a call runs. */
+#define ERNIE_CUDA_STATUS_ATTENTION_UNFINISHED 42
 
 typedef struct
 {

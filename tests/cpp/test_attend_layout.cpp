@@ -1,7 +1,9 @@
 // Which bytes of the weights' tile each softmax warp of the shared-prefix attention touches (no GPU): a warp stores its
 // 32 rows' weights, and between two parts its rows' results, and no barrier stands between one warp's results and
-// another's next weights, so the warps' bytes may not meet.
+// another's next weights, so the warps' bytes may not meet. And where the join looks for an item's parts, whatever the
+// workspace holds in their workers' place.
 #include "attend_layout.h"
+#include <climits>
 #include <cstdio>
 #include <vector>
 
@@ -43,10 +45,27 @@ template <class Place> int clashes(Place results)
     }
     return found;
 }
+
+// The join reads places item + first .. + count - 1 of items + workers.
+bool parts_stay_inside()
+{
+    const int anything[] = {INT_MIN, INT_MIN + 1, -1, 0, 1, 2, 7, 8, 9, 147, 148, 149, 1183, 1184, 1185, 0x3f800000, 0x7f7fffff, INT_MAX - 1, INT_MAX};
+    for (int workers : {1, 2, 8, 148, 1184})
+        for (int first : anything)
+            for (int last : anything)
+            {
+                const PartRange r = parts_between(first, last, workers);
+                const bool real = 0 <= first && first <= last && last < workers;
+                if (r.count < 0 || r.first < 0 || r.first > workers - r.count) return false;
+                if (real ? r.first != first || r.count != last - first + 1 : r.count != 0) return false;
+            }
+    return true;
+}
 } // namespace
 
 int main()
 {
+    if (!parts_stay_inside()) return std::fprintf(stderr, "an item's parts lie outside the list\n"), 1;
     const auto all = [] {
         std::vector<char> sum(kTileBytes, 0);
         for (int warp = 0; warp < 4; ++warp)
