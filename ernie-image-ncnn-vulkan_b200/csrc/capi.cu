@@ -310,6 +310,13 @@ extern "C" int ernie_cuda_context_sm_count(ernie_cuda_context *ctx, int *sms)
     return ERNIE_CUDA_OK;
 }
 
+extern "C" int ernie_cuda_context_stream(ernie_cuda_context *ctx, void **stream)
+{
+    if (!ctx || !stream) return fail(ERNIE_CUDA_ERROR, "null argument");
+    *stream = ctx->stream;
+    return ERNIE_CUDA_OK;
+}
+
 extern "C" int ernie_cuda_malloc(ernie_cuda_context *ctx, size_t bytes, void **dev)
 {
     if (!ctx || !dev) return fail(ERNIE_CUDA_ERROR, "null argument");

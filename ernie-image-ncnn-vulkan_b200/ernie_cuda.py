@@ -80,6 +80,7 @@ SIGNATURES = {
     "ernie_cuda_context_synchronize": (I, [P]),
     "ernie_cuda_context_memory": (I, [P, ctypes.POINTER(U64), ctypes.POINTER(U64)]),
     "ernie_cuda_context_sm_count": (I, [P, ctypes.POINTER(I)]),
+    "ernie_cuda_context_stream": (I, [P, ctypes.POINTER(P)]),
     "ernie_cuda_malloc": (I, [P, SZ, ctypes.POINTER(P)]),
     "ernie_cuda_free": (I, [P, P]),
     "ernie_cuda_upload": (I, [P, P, P, SZ]),
@@ -349,6 +350,14 @@ class Context:
         check(lib().ernie_cuda_context_sm_count(self.handle, ctypes.byref(n)))
         return n.value
 
+    @property
+    def stream(self):
+        """Address of the context's CUDA stream. In torch, torch.cuda.ExternalStream(ctx.stream): work that makes a
+        call's inputs or uses its results runs under it, or waits for it and it for them (Stream.wait_stream)."""
+        s = P()
+        check(lib().ernie_cuda_context_stream(self.handle, ctypes.byref(s)))
+        return s.value
+
     def memory(self):
         f, t = U64(0), U64(0)
         check(lib().ernie_cuda_context_memory(self.handle, ctypes.byref(f), ctypes.byref(t)))
@@ -444,7 +453,8 @@ class Context:
         return res
 
     # batched decoding: device arrays in and out (a Buffer, an address or a torch tensor), enqueued on the
-    # context's stream; arrays written on another stream have to be ready, and stay alive until the work is done
+    # context's stream (`stream`), which other streams' work has to be ordered with; arrays stay alive until the
+    # work is done
     def paged_append(self, kv, layer, batch, qkv, precision, ld, heads, cos, sin, rope_rows, q_out):
         check(lib().ernie_cuda_paged_append(self.handle, kv.c, layer, batch.c, device_pointer(qkv), precision, ld, heads,
                                             device_pointer(cos), device_pointer(sin), rope_rows, device_pointer(q_out)))

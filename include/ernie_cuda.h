@@ -99,6 +99,12 @@ int ernie_cuda_context_synchronize(ernie_cuda_context *ctx);
 /* Device budget reader (replaces the Vulkan budget reader, src/weight_placement.cpp:75-97). */
 int ernie_cuda_context_memory(ernie_cuda_context *ctx, uint64_t *free_bytes, uint64_t *total_bytes);
 int ernie_cuda_context_sm_count(ernie_cuda_context *ctx, int *sms);
+/* The context's stream (a cudaStream_t, valid until the context is destroyed), on which every call that takes device
+   pointers enqueues. It does not wait for other streams, the default one included, nor they for it: work that makes a
+   call's inputs or uses its results goes on this stream too, or is ordered with it by events (cudaEventRecord on the
+   one, cudaStreamWaitEvent on the other). It may be captured into a graph as long as no session runs on the context
+   meanwhile. */
+int ernie_cuda_context_stream(ernie_cuda_context *ctx, void **stream);
 int ernie_cuda_malloc(ernie_cuda_context *ctx, size_t bytes, void **dev);
 int ernie_cuda_free(ernie_cuda_context *ctx, void *dev);
 int ernie_cuda_upload(ernie_cuda_context *ctx, void *dev, const void *host, size_t bytes);
@@ -373,8 +379,9 @@ int ernie_cuda_pe_logits(ernie_cuda_pe_session *session, const float *hidden, fl
    Operators for decoding many sequences at once over a paged K/V cache (no counterpart in the reference,
    whose PeSession runs one sequence over one dense cache): the beams of a prompt, or a batch behind one
    chat template. All pointers are device memory on the context's device; every call enqueues on the
-   context's stream and returns. Lengths and tables are read on the device when the call runs, so the
-   caller may fill them by earlier work of the same stream.
+   context's stream (ernie_cuda_context_stream) and returns. Lengths and tables are read on the device when
+   the call runs, so the caller may fill them by earlier work of the same stream; work on another stream
+   has to be ordered with it.
 
    The cache of one layer is K and V [pages][kv_heads][page_size][head_dim] each, `layers` of them one
    after the other. A batch is `sequences` rows of `queries` new-token slots each. Sequence s holds

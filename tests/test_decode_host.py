@@ -199,6 +199,11 @@ def test_arrays_on_the_host_and_wide_integers_are_refused():
         batch(tables=torch.zeros(4, 6, dtype=torch.int32).t())
 
 
+def test_the_stream_needs_a_context():
+    out = ctypes.c_void_p(5)
+    assert ec.lib().ernie_cuda_context_stream(None, ctypes.byref(out)) == ec.ERROR and out.value == 5
+
+
 def test_null_descriptions():
     lib = ec.lib()
     n = ctypes.c_size_t(7)

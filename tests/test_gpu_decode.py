@@ -811,3 +811,148 @@ def test_two_contexts_at_once(ctx, dev):
         other.synchronize()
         d2.free()
         other.close()
+
+
+# ------------------------------------------------------------------ beside other streams, and in graphs
+class Step:
+    """One step of a batch of beams on torch tensors: append, attend, select, reorder."""
+
+    def __init__(self, ctx, torch, seed, workspace=None):
+        rng = np.random.default_rng(seed)
+        self.ctx, self.torch = ctx, torch
+        self.groups, self.beams, self.heads, self.kv_heads, self.dim, self.page, self.vocab = 2, 6, 8, 2, 128, 16, 3000
+        n, own, shared = self.groups * self.beams, 3, 20
+        put = lambda x: torch.from_numpy(np.ascontiguousarray(x)).cuda()
+        order = rng.permutation(n * own + self.groups * shared).astype(np.int32)
+        shape = (1, len(order), self.kv_heads, self.page, self.dim)
+        self.k, self.v = (put(values(rng, shape, ec.FP32)).bfloat16() for _ in range(2))
+        self.tables, self.prefix = put(order[:n * own].reshape(n, own)), put(order[n * own:].reshape(self.groups, shared))
+        self.lens, self.prefix_lens = put(rng.integers(1, 40, n).astype(np.int32)), put(np.array([320, 211], np.int32))
+        angle = np.arange(400)[:, None] * np.concatenate([10.0 ** -np.linspace(0, 3, self.dim // 2)] * 2)
+        self.cos, self.sin = put(np.cos(angle).astype(np.float32)), put(np.sin(angle).astype(np.float32))
+        self.width = (self.heads + 2 * self.kv_heads) * self.dim
+        self.x = put(values(rng, (n, self.width), ec.FP32))
+        self.q = torch.zeros(n, self.heads, self.dim, device="cuda", dtype=torch.bfloat16)
+        self.out = torch.zeros_like(self.q)
+        self.logits = put(values(rng, (n, self.vocab), ec.FP32, 3.0))
+        self.scores = put(-rng.random((self.groups, self.beams)).astype(np.float32))
+        ints = lambda *s: torch.zeros(*s, device="cuda", dtype=torch.int32)
+        self.finished, self.parents, self.tokens = (ints(self.groups, self.beams) for _ in range(3))
+        self.new_finished, self.new_scores = ints(self.groups, self.beams), torch.zeros(self.groups, self.beams, device="cuda")
+        self.new_tables, self.new_lens = ints(n, own), ints(n)
+        self.kv = ec.PagedKv(self.k, self.v, 1, len(order), self.page, self.kv_heads, self.dim, ec.BF16)
+        self.batch = ec.PagedBatch(n, 1, self.tables, own, self.lens, None, self.groups, self.prefix, shared, self.prefix_lens)
+        size = max(ctx.prefix_attention_workspace(self.kv, self.batch, self.heads), ctx.beam_select_workspace(self.groups, self.beams, self.vocab))
+        self.work = torch.zeros(size, device="cuda", dtype=torch.uint8) if workspace is None else workspace
+
+    def run(self):
+        c, w = self.ctx, self.work
+        c.paged_append(self.kv, 0, self.batch, self.x, ec.FP32, self.width, self.heads, self.cos, self.sin, 400, self.q)
+        c.prefix_attention(self.kv, 0, self.batch, self.q, self.heads, self.out, w, w.numel())
+        c.beam_select(self.logits, ec.FP32, self.vocab, self.groups, self.beams, self.vocab, 7, self.scores, self.finished,
+                      self.parents, self.tokens, self.new_scores, self.new_finished, w, w.numel())
+        c.beam_reorder(self.kv, self.groups, self.beams, self.parents, self.tables, self.tables.shape[1], self.lens,
+                       self.new_tables, self.new_lens)
+
+    def results(self):
+        return [t.clone() for t in (self.q, self.out, self.k, self.v, self.parents, self.tokens, self.new_scores, self.new_finished,
+                                    self.new_tables, self.new_lens)]
+
+
+def test_steps_ordered_with_another_stream(ctx):
+    """A producer and a consumer on torch's stream, each step's inputs written late, without the host waiting anywhere."""
+    torch = pytest.importorskip("torch")
+    library = torch.cuda.ExternalStream(ctx.stream)
+    steps = [Step(ctx, torch, seed) for seed in range(6)]
+    torch.cuda.synchronize()
+    want = []
+    for s in steps:
+        kept = [t.clone() for t in (s.k, s.v)]
+        torch.cuda.synchronize()
+        s.run()
+        ctx.synchronize()
+        want.append(s.results())
+        for t, old in zip((s.k, s.v), kept):
+            t.copy_(old)
+        s.inputs = [t.clone() for t in (s.x, s.lens, s.logits)]
+        for t in (s.x, s.logits):
+            t.fill_(float("nan"))
+        s.lens.zero_()
+        for t in (s.q, s.out, s.parents, s.tokens, s.new_scores, s.new_finished, s.new_tables, s.new_lens):
+            t.zero_()
+    torch.cuda.synchronize()
+    mine = torch.cuda.Stream()
+    got = []
+    with torch.cuda.stream(mine):
+        for s in steps:
+            torch.cuda._sleep(3_000_000)  # the inputs come a millisecond late
+            for t, new in zip((s.x, s.lens, s.logits), s.inputs):
+                t.copy_(new)
+            library.wait_stream(mine)
+            s.run()
+            mine.wait_stream(library)
+            got.append(s.results())
+    mine.synchronize()
+    ctx.synchronize()
+    for one, other in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(one, other))
+
+
+def test_steps_under_the_contexts_stream(ctx):
+    """torch's work on the context's own stream needs no events."""
+    torch = pytest.importorskip("torch")
+    s = Step(ctx, torch, 40)
+    kept = [t.clone() for t in (s.k, s.v, s.x, s.logits)]
+    torch.cuda.synchronize()
+    s.run()
+    ctx.synchronize()
+    want = s.results()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.ExternalStream(ctx.stream)):
+        torch.cuda._sleep(3_000_000)
+        for t, old in zip((s.k, s.v, s.x, s.logits), kept):
+            t.copy_(old)
+        s.out.zero_()
+        s.run()
+        got = s.results()
+    ctx.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_steps_in_graphs_that_share_a_workspace(ctx):
+    """Two captured steps with one scratch, replayed in turn on one stream with lengths, logits and projections that change
+    between the replays, against the same steps called eagerly."""
+    torch = pytest.importorskip("torch")
+    library = torch.cuda.ExternalStream(ctx.stream)
+    first = Step(ctx, torch, 50)
+    steps = [first, Step(ctx, torch, 51, first.work)]
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in steps]
+    for s, graph in zip(steps, graphs):
+        with torch.cuda.graph(graph, stream=library):
+            s.run()
+    ctx.synchronize()
+    rng = np.random.default_rng(52)
+    for turn in range(5):
+        lens = torch.from_numpy(rng.integers(1, 48, 12).astype(np.int32)).cuda()
+        for s, graph in zip(steps, graphs):
+            s.lens.copy_(lens)
+            s.x.mul_(-0.75)
+            s.logits.copy_(s.logits.roll(turn + 1, 1))
+        kept = [[t.clone() for t in (s.k, s.v)] for s in steps]
+        torch.cuda.synchronize()
+        for s in steps:
+            s.run()
+        ctx.synchronize()
+        want = [s.results() for s in steps]
+        for s, (k, v) in zip(steps, kept):
+            s.k.copy_(k), s.v.copy_(v), s.out.zero_(), s.parents.zero_(), s.new_tables.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(library):
+            for graph in graphs:
+                graph.replay()
+        ctx.synchronize()
+        for s, result in zip(steps, want):
+            assert all(torch.equal(a, b) for a, b in zip(s.results(), result)), turn
+        torch.cuda.synchronize()
+    del graphs
