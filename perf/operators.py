@@ -5,6 +5,10 @@ of the beams' cached state.
 Each case has a plain form (elementary torch operations in 32 bits, 64 where a selection hangs on the last bits)
 and the library's own call; `own` chooses between them. `exact` restates the definitions in 64 bits.
 
+The library's calls enqueue on its context's stream. With `own` torch's work runs on that stream too, from the first
+`prepare` on, so that inputs, calls and what uses the results are in one order; a caller who runs torch on another stream
+is ordered with it by events. Either way a pass is over for torch's current stream when the calls are.
+
 The cache of one layer is K and V [pages][kv_heads][page_size][head_dim]. A sequence's tokens lie in the pages of
 its table row; the sequences of a group share the prefix in the group's own pages, which comes before their
 tokens."""
@@ -17,17 +21,22 @@ import torch
 own = False
 
 _context = None
+_stream = _context_stream = None  # the context's, for torch and as an address
 
 
 def _library():
-    """The library's binding and one context for the process."""
-    global _context
+    """The library's binding and one context for the process, whose stream becomes torch's current one."""
+    global _context, _stream, _context_stream
     package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ernie-image-ncnn-vulkan_b200")
     if package not in sys.path:
         sys.path.insert(0, package)
     import ernie_cuda
     if _context is None:
         _context = ernie_cuda.Context(torch.cuda.current_device())
+        _context_stream = _context.stream
+        _stream = torch.cuda.ExternalStream(_context_stream)
+        _stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(_stream)
     return ernie_cuda, _context
 
 
@@ -301,7 +310,15 @@ def _handles(c, s):
 def run(s):
     op = s["case"]["op"]
     if own:
-        return {"append": _own_append, "attend": _own_attend, "select": _own_select, "reorder": _own_reorder}[op](s)
+        call = {"append": _own_append, "attend": _own_attend, "select": _own_select, "reorder": _own_reorder}[op]
+        # (torch.cuda.current_stream() would take as long as a small call)
+        if torch._C._cuda_getCurrentRawStream(_context.device) == _context_stream:
+            return call(s)
+        current = torch.cuda.current_stream()
+        _stream.wait_stream(current)
+        out = call(s)
+        current.wait_stream(_stream)
+        return out
     return {"append": _plain_append, "attend": _plain_attend, "select": _plain_select, "reorder": _plain_reorder}[op](s)
 
 
