@@ -288,15 +288,59 @@ class Buffer:
             self.ptr = None
 
 
-def device_pointer(a):
-    """Address of device memory: an array with data_ptr() (a torch tensor), a Buffer, an address or None."""
+class ArrayKind:
+    """What a device array holds. `dtype` is torch's, known from the first tensor on; None: anything."""
+    __slots__ = ("name", "size", "text", "dtype")
+
+    def __init__(self, name, size, text):
+        self.name, self.size, self.text, self.dtype = name, size, text, name and "not known yet"
+
+
+NUMBERS = {BF16: ArrayKind("torch.bfloat16", 2, "BF16 numbers"), FP32: ArrayKind("torch.float32", 4, "FP32 numbers")}
+FLOATS, INTEGERS, BYTES = NUMBERS[FP32], ArrayKind("torch.int32", 4, "32-bit integers"), ArrayKind(None, 1, "bytes")
+
+
+def device_array(what, a, kind, count, ctx=None, rows=None):
+    """Address of `count` elements of device memory: a torch tensor's, a Buffer's, an address or None. A tensor has to
+    hold them in one piece, or as `rows` (rows, width, row stride) of a two-dimensional one; a tensor or Buffer of
+    another kind, too small or on another device than the context's is refused, an address is taken as it is. (An
+    unknown precision has no kind: the library refuses the call.)"""
+    if type(a) is int or a is None:
+        return a
+    if kind is None:
+        kind, count = BYTES, 0
+    if isinstance(a, Buffer):
+        if a.nbytes >= count * kind.size and (ctx is None or a.ctx.device == ctx.device):
+            return a.ptr
+        raise ValueError(f"{what}: {count} {kind.text} are needed on the context's device, the buffer has {a.nbytes} bytes")
+    # (the usual case in as few steps as there are things to ask: a small call is bound by the host)
     try:
-        address = a.data_ptr()
+        dtype, device = a.dtype, a.get_device()
     except AttributeError:
-        return a.ptr if isinstance(a, Buffer) else a
-    if not a.is_cuda:
-        raise ValueError("the array is not in device memory")
-    return address
+        return a
+    if (dtype is kind.dtype or kind.dtype is None) and device >= 0 and (ctx is None or device == ctx.device):
+        if a.nbytes >= count * kind.size and a.is_contiguous():
+            return a.data_ptr()
+        if rows and a.dim() == 2 and a.shape[0] >= rows[0] and a.shape[1] >= rows[1] and a.stride() == (rows[2], 1):
+            return a.data_ptr()
+    elif kind.dtype == "not known yet" and str(dtype) == kind.name:
+        kind.dtype = dtype
+        return device_array(what, a, kind, count, ctx, rows)
+    raise ValueError(f"{what}: {count} contiguous {kind.text} are needed in device memory of the context's device, got "
+                     f"{tuple(a.shape)} of {dtype} on {a.device} with strides {tuple(a.stride())}")
+
+
+def device_of(arrays):
+    """The one device of the tensors and Buffers among `arrays`; None if there are only addresses."""
+    found = {a.get_device() if hasattr(a, "data_ptr") else a.ctx.device for a in arrays if hasattr(a, "data_ptr") or isinstance(a, Buffer)}
+    if len(found) > 1:
+        raise ValueError(f"arrays on different devices: {sorted(found)}")
+    return found.pop() if found else None
+
+
+def same_device(ctx, cache, batch=None):
+    if (cache is not None and cache != ctx.device) or (batch is not None and batch != ctx.device):
+        raise ValueError(f"the cache or the batch is on device {cache if cache != ctx.device else batch}, the context on {ctx.device}")
 
 
 class PagedKv:
@@ -304,8 +348,11 @@ class PagedKv:
 
     def __init__(self, k, v, layers, pages, page_size, kv_heads, head_dim, precision):
         self.arrays = (k, v)
-        self.fields = PagedKvFields(device_pointer(k), device_pointer(v), precision, layers, pages, page_size, kv_heads,
-                                    head_dim)
+        kind, count = NUMBERS.get(precision), layers * pages * page_size * kv_heads * head_dim
+        self.fields = PagedKvFields(device_array("k", k, kind, count), device_array("v", v, kind, count), precision, layers,
+                                    pages, page_size, kv_heads, head_dim)
+        self.device = device_of(self.arrays)
+        self.kind, self.dim, self.kv_heads = kind, head_dim, kv_heads
         self.c = ctypes.c_void_p(ctypes.addressof(self.fields))
 
 
@@ -315,11 +362,13 @@ class PagedBatch:
     def __init__(self, sequences, queries, tables, max_pages, lens, counts=None, groups=1, prefix_tables=None,
                  max_prefix_pages=0, prefix_lens=None):
         self.arrays = (tables, lens, counts, prefix_tables, prefix_lens)
-        if any(hasattr(a, "element_size") and (a.element_size() != 4 or not a.is_contiguous()) for a in self.arrays):
-            raise ValueError("tables, lengths and counts are contiguous arrays of 32-bit integers")
-        self.fields = PagedBatchFields(sequences, queries, device_pointer(tables), max_pages, device_pointer(lens),
-                                       device_pointer(counts), groups, device_pointer(prefix_tables), max_prefix_pages,
-                                       device_pointer(prefix_lens))
+        self.fields = PagedBatchFields(sequences, queries, device_array("tables", tables, INTEGERS, sequences * max_pages), max_pages,
+                                       device_array("lens", lens, INTEGERS, sequences),
+                                       device_array("counts", counts, INTEGERS, sequences), groups,
+                                       device_array("prefix_tables", prefix_tables, INTEGERS, groups * max_prefix_pages),
+                                       max_prefix_pages, device_array("prefix_lens", prefix_lens, INTEGERS, groups))
+        self.device = device_of(self.arrays)
+        self.slots = sequences * queries
         self.c = ctypes.c_void_p(ctypes.addressof(self.fields))
 
 
@@ -456,8 +505,16 @@ class Context:
     # context's stream (`stream`), which other streams' work has to be ordered with; arrays stay alive until the
     # work is done
     def paged_append(self, kv, layer, batch, qkv, precision, ld, heads, cos, sin, rope_rows, q_out):
-        check(lib().ernie_cuda_paged_append(self.handle, kv.c, layer, batch.c, device_pointer(qkv), precision, ld, heads,
-                                            device_pointer(cos), device_pointer(sin), rope_rows, device_pointer(q_out)))
+        same_device(self, kv.device, batch.device)
+        slots, dim = batch.slots, kv.dim
+        width, angles = (heads + 2 * kv.kv_heads) * dim, rope_rows * dim
+        rc = (_lib or lib()).ernie_cuda_paged_append(
+            self.handle, kv.c, layer, batch.c,
+            device_array("qkv", qkv, NUMBERS.get(precision), (slots - 1) * ld + width, self, (slots, width, ld)), precision, ld, heads,
+            device_array("cos", cos, FLOATS, angles, self), device_array("sin", sin, FLOATS, angles, self), rope_rows,
+            device_array("q_out", q_out, kv.kind, slots * heads * dim, self))
+        if rc:
+            check(rc)
 
     def prefix_attention_workspace(self, kv, batch, heads):
         n = SZ(0)
@@ -465,8 +522,13 @@ class Context:
         return n.value
 
     def prefix_attention(self, kv, layer, batch, q, heads, out, workspace, workspace_bytes):
-        check(lib().ernie_cuda_prefix_attention(self.handle, kv.c, layer, batch.c, device_pointer(q), heads,
-                                                device_pointer(out), device_pointer(workspace), workspace_bytes))
+        same_device(self, kv.device, batch.device)
+        kind, count = kv.kind, batch.slots * heads * kv.dim
+        rc = (_lib or lib()).ernie_cuda_prefix_attention(
+            self.handle, kv.c, layer, batch.c, device_array("q", q, kind, count, self), heads, device_array("out", out, kind, count, self),
+            device_array("workspace", workspace, BYTES, workspace_bytes, self), workspace_bytes)
+        if rc:
+            check(rc)
 
     def beam_select_workspace(self, groups, beams, vocab):
         n = SZ(0)
@@ -475,15 +537,27 @@ class Context:
 
     def beam_select(self, logits, precision, ld, groups, beams, vocab, end_token, scores, finished, parents, tokens,
                     new_scores, new_finished, workspace, workspace_bytes):
-        check(lib().ernie_cuda_beam_select(self.handle, device_pointer(logits), precision, ld, groups, beams, vocab,
-                                           end_token, device_pointer(scores), device_pointer(finished),
-                                           device_pointer(parents), device_pointer(tokens), device_pointer(new_scores),
-                                           device_pointer(new_finished), device_pointer(workspace), workspace_bytes))
+        n = groups * beams
+        rc = (_lib or lib()).ernie_cuda_beam_select(
+            self.handle, device_array("logits", logits, NUMBERS.get(precision), (n - 1) * ld + vocab, self, (n, vocab, ld)), precision,
+            ld, groups, beams, vocab, end_token, device_array("scores", scores, FLOATS, n, self),
+            device_array("finished", finished, INTEGERS, n, self), device_array("parents", parents, INTEGERS, n, self),
+            device_array("tokens", tokens, INTEGERS, n, self), device_array("new_scores", new_scores, FLOATS, n, self),
+            device_array("new_finished", new_finished, INTEGERS, n, self),
+            device_array("workspace", workspace, BYTES, workspace_bytes, self), workspace_bytes)
+        if rc:
+            check(rc)
 
     def beam_reorder(self, kv, groups, beams, parents, tables, max_pages, lens, new_tables, new_lens):
-        check(lib().ernie_cuda_beam_reorder(self.handle, kv.c, groups, beams, device_pointer(parents),
-                                            device_pointer(tables), max_pages, device_pointer(lens),
-                                            device_pointer(new_tables), device_pointer(new_lens)))
+        same_device(self, kv.device)
+        n = groups * beams
+        rc = (_lib or lib()).ernie_cuda_beam_reorder(
+            self.handle, kv.c, groups, beams, device_array("parents", parents, INTEGERS, n, self),
+            device_array("tables", tables, INTEGERS, n * max_pages, self), max_pages, device_array("lens", lens, INTEGERS, n, self),
+            device_array("new_tables", new_tables, INTEGERS, n * max_pages, self),
+            device_array("new_lens", new_lens, INTEGERS, n, self))
+        if rc:
+            check(rc)
 
     def euler_step(self, sample, prediction, delta):
         sample = np.ascontiguousarray(sample, np.float32)

@@ -199,6 +199,105 @@ def test_arrays_on_the_host_and_wide_integers_are_refused():
         batch(tables=torch.zeros(4, 6, dtype=torch.int32).t())
 
 
+class OnDevice:
+    """Stands for a torch tensor in device memory: its kind, shape and strides, at an address that no call follows."""
+
+    def __init__(self, torch, address, *shape, dtype="int32", device=0, stride=None):
+        self.address, self.device_index, self.is_cuda = address, device, True
+        self.meta = torch.empty(shape, dtype=getattr(torch, dtype), device="meta")
+        if stride:
+            self.meta = torch.empty_strided(shape, stride, dtype=getattr(torch, dtype), device="meta")
+
+    def data_ptr(self):
+        return self.address
+
+    def get_device(self):
+        return self.device_index
+
+    def __getattr__(self, name):
+        return getattr(self.meta, name)
+
+
+class FirstDevice(NoContext):
+    device = 0
+
+
+def test_tensors_of_the_right_kind_pass_and_others_are_refused():
+    """Every array of every call: another type, too few elements, gaps between them, another device."""
+    torch = pytest.importorskip("torch")
+    first = FirstDevice()
+    n, q, h, k, d = 6, 2, 32, 8, 128
+    pool = (2, 40, k, 16, d)
+    good = dict(
+        cache=dict(k=(K, pool, "bfloat16"), v=(V, pool, "bfloat16")),
+        batch=dict(tables=(TABLES, (n, 4), "int32"), lens=(LENS, (n,), "int32"), counts=(COUNTS, (n,), "int32"),
+                   prefix_tables=(PREFIX_TABLES, (2, 5), "int32"), prefix_lens=(PREFIX_LENS, (2,), "int32")),
+        append=dict(qkv=(QKV, (n * q, (h + 2 * k) * d), "float32"), cos=(COS, (100, d), "float32"), sin=(SIN, (100, d), "float32"),
+                    q_out=(Q, (n * q, h, d), "bfloat16")),
+        attend=dict(q=(Q, (n, q, h, d), "bfloat16"), out=(OUT, (n * q, h * d), "bfloat16"), workspace=(WORK, (1 << 20,), "uint8")),
+        select=dict(logits=(Q, (3, 4, 1000), "float32"), scores=(K, (3, 4), "float32"), finished=(V, (3, 4), "int32"),
+                    parents=(TABLES, (3, 4), "int32"), tokens=(LENS, (12,), "int32"), new_scores=(COUNTS, (3, 4), "float32"),
+                    new_finished=(OUT, (3, 4), "int32"), workspace=(WORK, (1 << 20,), "uint8")),
+        reorder=dict(parents=(Q, (3, 4), "int32"), tables=(TABLES, (12, 4), "int32"), lens=(LENS, (12,), "int32"),
+                     new_tables=(OUT, (12, 4), "int32"), new_lens=(COUNTS, (12,), "int32")))
+
+    def call(where=None, name=None, change=None):
+        arrays = {}
+        for part, fields in good.items():
+            arrays[part] = {f: OnDevice(torch, at, *shape, dtype=dtype) for f, (at, shape, dtype) in fields.items()}
+        if where:
+            arrays[where][name] = change(*good[where][name])
+        cache, rows = kv(**arrays["cache"]), batch(**arrays["batch"])
+        a, t, s, r = arrays["append"], arrays["attend"], arrays["select"], arrays["reorder"]
+        return (
+            lambda: first.paged_append(cache, 0, rows, a["qkv"], ec.FP32, 48 * d, h, a["cos"], a["sin"], 100, a["q_out"]),
+            lambda: first.prefix_attention(cache, 1, rows, t["q"], h, t["out"], t["workspace"], 1 << 20),
+            lambda: first.beam_select(s["logits"], ec.FP32, 1000, 3, 4, 1000, 2, *[s[x] for x in list(s)[1:]], 1 << 20),
+            lambda: first.beam_reorder(cache, 3, 4, r["parents"], r["tables"], 4, r["lens"], r["new_tables"], r["new_lens"]))
+
+    for one in call():
+        refused(one, "null context")
+    changes = dict(
+        kind=lambda at, shape, dtype: OnDevice(torch, at, *shape, dtype={"int32": "bool", "float32": "bfloat16", "bfloat16": "float16",
+                                                                        "uint8": "uint8"}[dtype]),
+        wide=lambda at, shape, dtype: OnDevice(torch, at, *shape, dtype={"int32": "int64"}.get(dtype, "float64" if dtype != "uint8" else "uint8")),
+        same_size=lambda at, shape, dtype: OnDevice(torch, at, *shape, dtype={"int32": "float32", "float32": "int32"}.get(dtype, "int16" if dtype != "uint8" else "uint8")),
+        short=lambda at, shape, dtype: OnDevice(torch, at, *(shape[:-1] + (shape[-1] - 1,)), dtype=dtype),
+        gaps=lambda at, shape, dtype: OnDevice(torch, at, *shape, dtype=dtype,
+                                               stride=tuple(2 * x for x in torch.empty(shape, device="meta").stride())),
+        spread=lambda at, shape, dtype: OnDevice(torch, at, *shape, dtype=dtype, stride=(0,) * len(shape)),
+        elsewhere=lambda at, shape, dtype: OnDevice(torch, at, *shape, dtype=dtype, device=1),
+        host=lambda at, shape, dtype: torch.zeros((), dtype=getattr(torch, dtype)).expand(shape))
+    order = ("append", "attend", "select", "reorder")
+    for where, fields in good.items():
+        for name, (_, _, dtype) in fields.items():
+            for change, make in changes.items():
+                if dtype == "uint8" and change in ("kind", "wide", "same_size"):
+                    continue
+                with pytest.raises(ValueError, match=name if where in order else "arrays on different devices|the cache or the batch|" + name):
+                    calls = call(where, name, make)
+                    calls[order.index(where) if where in order else 0]()
+
+
+def test_rows_of_wider_tensors_and_buffers():
+    torch = pytest.importorskip("torch")
+    first, wide = FirstDevice(), 48 * 128 + 64
+    rows = lambda stride, width=48 * 128, count=12, dtype="float32": OnDevice(torch, QKV, count, width, dtype=dtype, stride=(stride, 1))
+    go = lambda qkv, ld=wide: first.paged_append(kv(), 0, batch(), qkv, ec.FP32, ld, 32, COS, SIN, 100, Q)
+    refused(lambda: go(rows(wide)), "null context")
+    refused(lambda: go(OnDevice(torch, QKV, 6, 2, wide, dtype="float32")), "null context")
+    for bad in (rows(wide + 1), rows(wide, 48 * 128 - 1), rows(wide, count=11), rows(wide, dtype="bfloat16")):
+        with pytest.raises(ValueError, match="qkv"):
+            go(bad)
+    held = ec.Buffer.__new__(ec.Buffer)
+    held.ctx, held.ptr, held.nbytes = first, Q, 12 * 32 * 128 * 2
+    attended = lambda: first.prefix_attention(kv(), 1, batch(), held, 32, OUT, WORK, 1 << 20)
+    refused(attended, "null context")
+    held.nbytes -= 1
+    with pytest.raises(ValueError, match="q: "):
+        attended()
+
+
 def test_the_stream_needs_a_context():
     out = ctypes.c_void_p(5)
     assert ec.lib().ernie_cuda_context_stream(None, ctypes.byref(out)) == ec.ERROR and out.value == 5
