@@ -14,6 +14,7 @@ namespace
 {
 constexpr long long kMaxSlots = 1 << 24; // sequences * queries
 constexpr int kMaxHeads = 1024;
+constexpr long long kMaxCount = INT32_MAX - 1024; // of what 32-bit indices count: the last one steps past the end by a tile or a CTA's threads
 
 bool aligned(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
@@ -101,8 +102,8 @@ int check_heads(int heads, const PagedLayer &kv)
 
 int check_rows(const PagedBatch &b, int heads)
 {
-    if (static_cast<long long>(b.sequences) * b.queries * heads > INT32_MAX)
-        return fail(ERNIE_CUDA_ERROR, "More than 2^31 query rows in one call");
+    if (static_cast<long long>(b.sequences) * b.queries * heads > kMaxCount)
+        return fail(ERNIE_CUDA_ERROR, "2^31 query rows in one call, or nearly");
     return ERNIE_CUDA_OK;
 }
 
@@ -113,12 +114,12 @@ int check_work(const PagedBatch &b, const PagedLayer &kv, int heads)
     return ERNIE_CUDA_OK;
 }
 
-// A position or length past 2^31 - 1 tokens cannot be addressed by the 32-bit lengths.
+// Positions and lengths are 32-bit numbers.
 int check_tokens(const PagedBatch &b, const PagedLayer &kv)
 {
     const long long own = static_cast<long long>(b.max_pages) << kv.page_shift;
     const long long shared = static_cast<long long>(b.max_prefix_pages) << kv.page_shift;
-    if (own + shared > INT32_MAX) return fail(ERNIE_CUDA_ERROR, "Tables span more than 2^31 tokens");
+    if (own + shared > kMaxCount) return fail(ERNIE_CUDA_ERROR, "Tables span 2^31 tokens, or nearly");
     return ERNIE_CUDA_OK;
 }
 
@@ -127,6 +128,7 @@ int check_beams(int groups, int beams, int vocab)
     if (groups < 1 || beams < 1 || beams > kMaxBeams || vocab < 1)
         return fail(ERNIE_CUDA_ERROR, "Beam search needs groups, 1..32 beams and a vocabulary");
     if (static_cast<long long>(groups) * beams > kMaxSlots) return fail(ERNIE_CUDA_ERROR, "Too many beams in one call");
+    if (vocab > kMaxCount) return fail(ERNIE_CUDA_ERROR, "A vocabulary of 2^31 tokens, or nearly");
     return ERNIE_CUDA_OK;
 }
 } // namespace
@@ -284,8 +286,8 @@ extern "C" int ernie_cuda_beam_reorder(ernie_cuda_context *ctx, const ernie_cuda
     ERNIE_TRY(check_kv(kv, 0, a.kv));
     ERNIE_TRY(check_beams(groups, beams, 1));
     if (!parents || !tables || !lens || !new_tables || !new_lens) return fail(ERNIE_CUDA_ERROR, "null argument");
-    if (max_pages < 1 || (static_cast<long long>(max_pages) << a.kv.page_shift) > INT32_MAX ||
-        static_cast<long long>(max_pages) * beams > INT32_MAX)
+    if (max_pages < 1 || (static_cast<long long>(max_pages) << a.kv.page_shift) > kMaxCount ||
+        static_cast<long long>(max_pages) * beams > kMaxCount)
         return fail(ERNIE_CUDA_ERROR, "Invalid page table width");
     if (!aligned(parents, 4) || !aligned(tables, 4) || !aligned(lens, 4) || !aligned(new_tables, 4) || !aligned(new_lens, 4))
         return fail(ERNIE_CUDA_ERROR, "Tables, lengths and parents must be 4-byte aligned");

@@ -189,6 +189,25 @@ def test_batches_past_the_counters_are_refused():
     refused(lambda: reorder(beams=32, max_pages=1 << 26), "table width")
 
 
+def test_counts_whose_last_step_passes_32_bits_are_refused():
+    """Indices step past their end by a tile of keys or a CTA's threads, which may not wrap around."""
+    last = 2 ** 31 - 1
+    refused(lambda: select(vocab=last, ld=last), "vocabulary of 2\\^31")
+    refused(lambda: CTX.beam_select_workspace(1, 1, last - 1023), "vocabulary of 2\\^31")
+    refused(lambda: CTX.beam_select_workspace(1, 1, last - 1024), "null context")
+    for page, beams, pages in ((8, 8, 2 ** 28 - 1), (8, 1, 2 ** 28 - 1), (128, 1, 2 ** 24 - 1)):
+        refused(lambda: reorder(kv(page_size=page, pages=4), groups=1, beams=beams, max_pages=pages, new_tables=1 << 50), "table width")
+    # 2^31 - 2048 tokens
+    refused(lambda: reorder(kv(page_size=128, pages=4), groups=1, beams=1, max_pages=2 ** 24 - 16, new_tables=1 << 50), "null context")
+    alone = dict(prefix_tables=None, max_prefix_pages=0, prefix_lens=None, groups=1, sequences=1, queries=1)
+    for call in (append, attend):
+        refused(lambda: call(batch_=batch(max_pages=2 ** 27 - 1, **alone)), "2\\^31")
+        refused(lambda: call(batch_=batch(max_pages=2 ** 27 - 64, **alone)), "2\\^31")
+        refused(lambda: call(kv(kv_heads=1), batch(max_pages=2 ** 27 - 128, **alone)), "null context")
+        refused(lambda: call(batch_=batch(max_pages=2 ** 26, max_prefix_pages=2 ** 26 - 1)), "2\\^31")
+    refused(lambda: attend(batch_=batch(sequences=(1 << 21) - 1, queries=1, groups=1), heads=1024), "query rows")
+
+
 def test_arrays_on_the_host_and_wide_integers_are_refused():
     torch = pytest.importorskip("torch")
     with pytest.raises(ValueError, match="device memory"):
