@@ -85,20 +85,23 @@ __global__ void __launch_bounds__(kAppendThreads, kAppendCtas<In>) append_kernel
             }
     };
     fetch(first);
+    const int len = a.batch.lens[s];
     const SequenceView view = sequence_view(a.batch, a.kv.page_shift, s);
     if (i >= view.count) return;
-    const int place = view.len - view.count + i; // in the sequence's own pages
-    const int position = view.prefix_len + place;
+    // in the sequence's own pages; a length past the table counts as it is here, so that no new token takes an old one's place
+    const int place = max(len, view.len) - view.count + i;
+    const bool held = place >= 0 && place < static_cast<long long>(a.batch.max_pages) << a.kv.page_shift;
+    const long long position = static_cast<long long>(view.prefix_len) + place;
     if (position < 0 || position >= a.rope_rows)
     {
         report_range(a.batch.error_flag);
         return;
     }
-    int page = place >= 0 ? a.batch.tables[static_cast<size_t>(s) * a.batch.max_pages + (place >> a.kv.page_shift)] : -1;
+    int page = held ? a.batch.tables[static_cast<size_t>(s) * a.batch.max_pages + (place >> a.kv.page_shift)] : -1;
     const float *cos = a.cos + static_cast<size_t>(position) * D + d, *sin = a.sin + static_cast<size_t>(position) * D + d;
     const float4 cos_lo = *reinterpret_cast<const float4 *>(cos), cos_hi = *reinterpret_cast<const float4 *>(cos + kHalf);
     const float4 sin_lo = *reinterpret_cast<const float4 *>(sin), sin_hi = *reinterpret_cast<const float4 *>(sin + kHalf);
-    if (place >= 0 && (page < 0 || page >= a.kv.pages))
+    if (held && (page < 0 || page >= a.kv.pages))
     {
         report_range(a.batch.error_flag);
         page = -1;

@@ -393,8 +393,8 @@ int ernie_cuda_pe_logits(ernie_cuda_pe_session *session, const float *hidden, fl
 
    A length above its table's pages, a negative one, a count outside 0..queries or a page outside
    0..pages-1 that a call has to touch is never followed: lengths and counts are clamped, a bad page's
-   keys count as zeros and nothing is stored there, and the next ernie_cuda_context_synchronize reports
-   status 41. Two sequences that store into the same page in one call race. */
+   keys count as zeros, nothing is stored there nor for a new token past its table's pages, and the next
+   ernie_cuda_context_synchronize reports status 41. Two sequences that store into the same page in one call race. */
 #define ERNIE_CUDA_STATUS_PAGED_RANGE 41
 /* One of the attention's bounded waits ran out (some two seconds): the call ended, its results are not to be used.
    Lengths, counts and tables may not change while a call runs. */

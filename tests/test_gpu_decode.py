@@ -165,6 +165,44 @@ def test_append_range_reports(ctx, dev):
     ctx.synchronize()
 
 
+@pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
+def test_append_past_the_table_keeps_the_cache(ctx, dev, precision):
+    """New tokens of a sequence whose pages are full: stored nowhere, the tokens before them stay and those that still
+    have a place get it; status 41."""
+    rng = np.random.default_rng(17)
+    n, queries, page, dim, own = 6, 3, 8, 64, 16
+    k, v = (values(rng, (1, 2 * n, 1, page, dim), precision) for _ in range(2))
+    cos, sin = rng.uniform(-1, 1, (2, 40, dim)).astype(np.float32)
+    tables = rng.permutation(2 * n).reshape(n, 2).astype(np.int32)
+    lens, counts = np.array([16, 17, 17, 18, 30, 2 ** 31 - 1], np.int32), np.array([1, 1, 3, 3, 3, 3], np.int32)
+    x, q = values(rng, (n * queries, 3 * dim), precision), values(rng, (n * queries, 1, dim), precision)
+    kv = ec.PagedKv(dev.put("k", k, precision), dev.put("v", v, precision), 1, 2 * n, page, 1, dim, precision)
+    batch = ec.PagedBatch(n, queries, dev.put("t", tables), 2, dev.put("n", lens), dev.put("c", counts))
+    ctx.paged_append(kv, 0, batch, dev.put("x", x, precision), precision, 3 * dim, 1, dev.put("cos", cos), dev.put("sin", sin), 40,
+                     dev.put("q", q, precision))
+    with pytest.raises(ec.CudaError, match="status 41"):
+        ctx.synchronize()
+    got_k, got_v, got_q = dev.get("k"), dev.get("v"), dev.get("q")
+    for s in range(n):
+        for i in range(queries):
+            place, row = int(lens[s]) - int(counts[s]) + i, s * queries + i
+            if i >= counts[s] or place >= 40:
+                assert np.array_equal(got_q[row], q[row])
+                continue
+            c, m = cos[place].astype(np.float64), sin[place].astype(np.float64)
+            for got, old, at in ((got_q[row, 0], x[row, :dim], None), (None, x[row, dim:2 * dim], got_k)):
+                y, size = od.rotate(old.astype(np.float64), c, m), np.abs(old) * np.abs(c) + np.abs(np.roll(old, dim // 2)) * np.abs(m)
+                if at is not None:
+                    if place >= own:
+                        continue
+                    page_at = tables[s, place // page]
+                    got = at[0, page_at, 0, place % page].copy()
+                    k[0, page_at, 0, place % page], v[0, page_at, 0, place % page] = got, x[row, 2 * dim:]
+                limit = 3 * U * size + (H if precision == ec.BF16 else 0.0) * (np.abs(y) + 3 * U * size)
+                assert (np.abs(got - y) <= limit).all(), (s, i)
+    assert np.array_equal(got_k, k) and np.array_equal(got_v, v), "a token was overwritten"
+
+
 # ------------------------------------------------------------------ attention
 def attention_case(ctx, dev, rng, groups, per, queries, prefix, suffix, heads, kv_heads, dim, page, precision,
                    counts=None, lens=None, prefix_lens=None, layers=1, layer=0, poison=True, scale=1.0, prefix_free=False):
