@@ -481,6 +481,63 @@ def test_attention_of_bad_pages(ctx, dev, per, precision):
     assert not run(tables, changed, 32)[1]
 
 
+@pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("per,queries", [(2, 1), (40, 1), (3, 40)])
+def test_attention_of_bad_pages_and_lengths_is_what_the_header_says(ctx, dev, per, queries, precision):
+    """A bad page's keys and values are zeros and count, a length outside its table is clamped: against the oracle on
+    such a cache, within the roundings of the type."""
+    rng = np.random.default_rng(60 + per)
+    heads, kv_heads, dim, page, own, shared = 8, 2, 128, 16, 5, 3
+    lens = rng.integers(queries, own * page + 1, per).astype(np.int32)
+    lens[0] = own * page
+    tables, pages = split_pages(rng, [own] * per + [shared])
+    tables, prefix = tables[:-1].copy(), tables[-1:, :shared].copy()
+    k, v = (values(rng, (1, pages, kv_heads, page, dim), precision) for _ in range(2))
+    q = values(rng, (per * queries, heads, dim), precision, 1.5)
+    dev.put("k", k, precision), dev.put("v", v, precision), dev.put("q", q, precision)
+    kv = ec.PagedKv(dev.buffers["k"], dev.buffers["v"], 1, pages, page, kv_heads, dim, precision)
+
+    def agrees(tables, prefix, lens, prefix_len, zeroed, lens_held, prefix_held):
+        d = Device(ctx)
+        batch = ec.PagedBatch(per, queries, d.put("t", tables), own, d.put("n", lens.astype(np.int32)), None, 1, d.put("p", prefix), shared,
+                              d.put("l", np.array([prefix_len], np.int32)))
+        size = ctx.prefix_attention_workspace(kv, batch, heads)
+        ctx.prefix_attention(kv, 0, batch, dev.buffers["q"], heads, d.put("out", q, precision), d.put("w", np.zeros(size, np.uint8)), size)
+        with pytest.raises(ec.CudaError, match="status 41"):
+            ctx.synchronize()
+        got = d.get("out").astype(np.float64)
+        d.free()
+        k0, v0 = k.copy(), v.copy()
+        k0[0, zeroed], v0[0, zeroed] = 0, 0
+        ref = q.astype(np.float64)
+        weight, spread = od.attention(k0, v0, 0, q, ref, good_tables, lens_held, [queries] * per, good_prefix, [prefix_held])
+        e = (dim + 4) * U * spread[:, :, None]
+        limit = weight * (2 * np.expm1(2 * e) + 16 * U + 2 * (int(max(lens_held)) + prefix_held + 16) * U)
+        limit = limit + H * weight + H * (np.abs(ref) + limit + H * weight) if precision == ec.BF16 else limit + U * np.abs(ref)
+        holds(got, ref, limit)
+
+    good_tables, good_prefix = tables, prefix
+    for bad in (-1, pages, 2 ** 31 - 1, -2 ** 31):
+        at = int(rng.integers(0, own))
+        changed = tables.copy()
+        changed[0, at] = bad
+        agrees(changed, prefix, lens, 40, [tables[0, at]], lens, 40)
+        changed = prefix.copy()
+        changed[0, 2] = bad
+        agrees(tables, changed, lens, 40, [prefix[0, 2]], lens, 40)
+    for prefix_len, held in ((4000, shared * page), (shared * page + 1, shared * page), (-4, 0), (-2 ** 31, 0)):
+        agrees(tables, prefix, lens, prefix_len, [], lens, held)
+    for length in (own * page + 1, 2 ** 31 - 1):
+        changed = lens.copy()
+        changed[0] = length
+        agrees(tables, prefix, changed, 33, [], lens, 33)
+    changed = lens.copy()
+    changed[-1] = -3
+    emptied = lens.copy()
+    emptied[-1] = 0
+    agrees(tables, prefix, changed, 33, [], emptied, 33)
+
+
 def test_attention_past_32_bit_offsets(ctx, dev):
     """Pages whose elements lie beyond 2^32 in the cache."""
     rng = np.random.default_rng(13)
