@@ -1051,3 +1051,45 @@ def test_steps_in_graphs_that_share_a_workspace(ctx):
             assert all(torch.equal(a, b) for a, b in zip(s.results(), result)), turn
         torch.cuda.synchronize()
     del graphs
+
+
+@pytest.mark.parametrize("copies", [False, True], ids=["after kernels", "after copies"])
+def test_a_step_forked_off_another_streams_capture(ctx, copies):
+    """A graph captured on torch's stream whose middle runs on the context's, ordered both ways by events."""
+    torch = pytest.importorskip("torch")
+    library, mine = torch.cuda.ExternalStream(ctx.stream), torch.cuda.Stream()
+    s = Step(ctx, torch, 70)
+    x, logits = s.x.clone(), s.logits.clone()
+    kept, late, out = [t.clone() for t in (s.k, s.v)], s.lens.clone(), torch.empty_like(s.out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=mine):
+        if copies:
+            s.lens.copy_(late), s.x.copy_(x), s.logits.copy_(logits)
+        else:
+            torch.add(late, 0, out=s.lens), torch.mul(x, 1.0, out=s.x), torch.mul(logits, 1.0, out=s.logits)
+        library.wait_stream(mine)
+        s.run()
+        mine.wait_stream(library)
+        torch.mul(s.out, 2.0, out=out)
+    for turn in range(4):
+        late.copy_(late % 40 + 3)
+        x.mul_(-1.25)
+        for t in (s.lens, s.out, s.parents):
+            t.zero_()
+        s.x.fill_(float("nan"))
+        for t, old in zip((s.k, s.v), kept):
+            t.copy_(old)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(mine):
+            graph.replay()
+        torch.cuda.synchronize()
+        ctx.synchronize()
+        got = s.results() + [out.clone()]
+        for t, old in zip((s.k, s.v), kept):
+            t.copy_(old)
+        torch.cuda.synchronize()
+        s.run()
+        ctx.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, s.results() + [s.out * 2.0])), turn
+    del graph
