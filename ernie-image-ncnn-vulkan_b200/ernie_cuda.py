@@ -300,11 +300,24 @@ NUMBERS = {BF16: ArrayKind("torch.bfloat16", 2, "BF16 numbers"), FP32: ArrayKind
 FLOATS, INTEGERS, BYTES = NUMBERS[FP32], ArrayKind("torch.int32", 4, "32-bit integers"), ArrayKind(None, 1, "bytes")
 
 
+def _has_rows(a, rows, width, ld):
+    """Whether a tensor's last dimension holds `width` neighbours and the others run through `rows` of them, `ld` apart."""
+    shape, stride = a.shape, a.stride()
+    if len(shape) < 2 or shape[-1] < width or stride[-1] != 1 or a.numel() // max(1, shape[-1]) < rows:
+        return False
+    step = ld
+    for n, s in zip(reversed(shape[:-1]), reversed(stride[:-1])):
+        if n != 1 and s != step:
+            return False
+        step *= n
+    return True
+
+
 def device_array(what, a, kind, count, ctx=None, rows=None):
     """Address of `count` elements of device memory: a torch tensor's, a Buffer's, an address or None. A tensor has to
-    hold them in one piece, or as `rows` (rows, width, row stride) of a two-dimensional one; a tensor or Buffer of
-    another kind, too small or on another device than the context's is refused, an address is taken as it is. (An
-    unknown precision has no kind: the library refuses the call.)"""
+    hold them in one piece, or as the `rows` (rows, width, row stride) of a wider one; a tensor or Buffer of another
+    kind, too small or on another device than the context's is refused, an address is taken as it is. (An unknown
+    precision has no kind: the library refuses the call.)"""
     if type(a) is int or a is None:
         return a
     if kind is None:
@@ -321,7 +334,7 @@ def device_array(what, a, kind, count, ctx=None, rows=None):
     if (dtype is kind.dtype or kind.dtype is None) and device >= 0 and (ctx is None or device == ctx.device):
         if a.nbytes >= count * kind.size and a.is_contiguous():
             return a.data_ptr()
-        if rows and a.dim() == 2 and a.shape[0] >= rows[0] and a.shape[1] >= rows[1] and a.stride() == (rows[2], 1):
+        if rows and _has_rows(a, *rows):
             return a.data_ptr()
     elif kind.dtype == "not known yet" and str(dtype) == kind.name:
         kind.dtype = dtype

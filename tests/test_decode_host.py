@@ -305,6 +305,14 @@ def test_rows_of_wider_tensors_and_buffers():
     go = lambda qkv, ld=wide: first.paged_append(kv(), 0, batch(), qkv, ec.FP32, ld, 32, COS, SIN, 100, Q)
     refused(lambda: go(rows(wide)), "null context")
     refused(lambda: go(OnDevice(torch, QKV, 6, 2, wide, dtype="float32")), "null context")
+    # the sequences' slots as a dimension of their own, one slot or one row of a wider tensor
+    view = lambda *shape, stride: OnDevice(torch, QKV, *shape, dtype="float32", stride=stride)
+    refused(lambda: go(view(6, 2, 48 * 128, stride=(2 * wide, wide, 1))), "null context")
+    refused(lambda: go(view(12, 1, 48 * 128, stride=(wide, 5, 1))), "null context")
+    for bad in (view(6, 2, 48 * 128, stride=(3 * wide, wide, 1)), view(6, 2, 48 * 128, stride=(wide, 6 * wide, 1)),
+                view(3, 2, 48 * 128, stride=(2 * wide, wide, 1)), view(12, 48 * 128, stride=(wide, 2)), view(12, 48 * 128, stride=(0, 1))):
+        with pytest.raises(ValueError, match="qkv"):
+            go(bad)
     for bad in (rows(wide + 1), rows(wide, 48 * 128 - 1), rows(wide, count=11), rows(wide, dtype="bfloat16")):
         with pytest.raises(ValueError, match="qkv"):
             go(bad)
