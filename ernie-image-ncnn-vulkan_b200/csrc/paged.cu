@@ -62,7 +62,7 @@ template <class In> constexpr int kAppendCtas = sizeof(In) == 2 ? 8 : 5; // of a
 // the first heads' loads are issued before the token's place is known. The bound is the traffic: projection in,
 // queries, keys and values out. A slot is a chain of some 3 us (lengths, page and angles, stores) around 24 KB,
 // so an SM needs many slots at a time: small CTAs with six heads to a thread. (16000 tokens of 48 heads from
-// BF16 to BF16, 410 MB: 80 us, 5.1 TB/s; 140 us with eight dims to a thread at 114 registers, 94 us with 256
+// BF16 to BF16, 410 MB: 80 to 84 us, 4.9 to 5.1 TB/s; 140 us with eight dims to a thread at 114 registers, 94 us with 256
 // threads and three heads each, 96 us with these walking over the slots and the next one's loads in flight.)
 template <class In, class Out, int D>
 __global__ void __launch_bounds__(kAppendThreads, kAppendCtas<In>) append_kernel(const __grid_constant__ AppendArgs a, int vectors)
@@ -200,7 +200,7 @@ __device__ __forceinline__ void copy_rows(const uint4 *k_from, uint4 *k_into, co
 // grid (groups, y): the warps of a group's CTAs share its copies, a layer's head of a page at a time; each CTA
 // works out the moves for itself, the first one writes the new rows. Sources are pages that pass to an heir,
 // targets those of childless places, so no page is both and the copies need no order. The bound is the traffic: the
-// copies of 12 groups of 4 beams over 26 layers, 479 MB read and written, take 83 us, 5.8 TB/s.
+// copies of 12 groups of 4 beams over 26 layers, 479 MB read and written, take 79 to 83 us, 5.8 to 6.1 TB/s.
 __global__ void __launch_bounds__(kCopyWarps * 32) reorder_kernel(const __grid_constant__ ReorderArgs a, int element_shift)
 {
     __shared__ GroupMoves m;

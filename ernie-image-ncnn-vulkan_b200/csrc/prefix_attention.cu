@@ -30,8 +30,8 @@
 //           rows and 128 keys takes about 3350 cycles. Shared memory's 128 bytes per cycle bound it: four
 //           products that read 64 KB each, 64 KB of weights stored, 64 KB of keys and values loaded, 3070
 //           cycles (the exponentials alone would take 2048).
-// 256 sequences of 1024 own tokens behind 16384 shared ones (32 query heads over 8, BF16) take 147 to 164 us,
-// 12 groups of 8 with 300 behind 1800 in FP32 103 us.
+// 256 sequences of 1024 own tokens behind 16384 shared ones (32 query heads over 8, BF16) take 147 to 170 us (power),
+// 64 of 512 behind 4096 30, 12 groups of 8 with 300 behind 1800 in FP32 103.
 // A second kernel joins the parts of each row.
 #include "attend_layout.h"
 #include "decode.h"
@@ -53,7 +53,8 @@ static_assert(kTile == kWeightRows, "weights' tile");
 constexpr int kRegsControl = 72, kRegsWork = 216, kMinLaunchRegs = 168;
 static_assert(128 * kRegsControl + 256 * kRegsWork <= kThreads * kMinLaunchRegs, "register split");
 
-// Division of numbers below 2^31 by a divisor that the host knows: n / d = (hi32(n m) + n) >> shift.
+// Division of numbers below 2^31 by a divisor that the host knows, n / d = (hi32(n m) + n) >> shift: Granlund and
+// Montgomery, "Division by invariant integers using multiplication", 1994.
 struct Divisor
 {
     unsigned m, shift;
@@ -813,7 +814,7 @@ __device__ __forceinline__ void stream_work(const Args<X> &p, const Plan &plan, 
 // the weights of a slot's eight keys there, and their way back by shuffles. Shared memory and shuffles deliver a
 // value per lane and cycle, so a value of K or V has to serve many rows: eight rows to a lane take 250 of those
 // cycles for a slot, one row to a lane 1024. What bounds it then is latency, with two warps to a scheduler: of the
-// 103 us that 12 groups of 8 sequences take (254 MB) the FMA pipe works 36 (sums over single dims: 144 us; rows
+// 103 us that 12 groups of 8 sequences take (254 MB) the FMA pipe works 43 (sums over single dims: 144 us; rows
 // paired in the packed FMAs: 141 us; a round of weights for every four keys: 115 us).
 template <int D, int R, bool X>
 __device__ __forceinline__ void stream_work_f32(const Args<X> &p, const Plan &plan, const PlanShared &shared, const Ring<float, D> &ring)
@@ -1681,7 +1682,7 @@ size_t lay_out(const PagedLayer &kv, const PagedBatch &b, int heads, int ctas, v
         l.unit_shift = l.tile ? 7 : 5;
         // nanoseconds of an SM: a tile's unit with one and with two tiles of rows; a streamed unit as fast as an SM
         // takes them when the memory is not the limit. An item's fixed cost: queries in, partial results out (streamed
-        // items at three units: 64 sequences behind 4096 tokens 26.6 us for 25.2, FP32 groups 108 for 103)
+        // items at three units: 64 sequences behind 4096 tokens 31.1 us for 30.1, FP32 groups 110 for 102)
         l.cost = l.tile ? (l.rows > kTile ? 1900 : 1100) : (kv.bf16 ? 180 : l.rows > 8 ? 850 : l.rows > 4 ? 500 : 350) * kv.dim / 128;
         l.lead = l.tile ? (l.rows > kTile ? 4 : 6) : 1;
         const size_t items = static_cast<size_t>(l.owners) * l.blocks * kv.kv_heads;
