@@ -538,6 +538,60 @@ def test_attention_of_bad_pages_and_lengths_is_what_the_header_says(ctx, dev, pe
     agrees(tables, prefix, changed, 33, [], emptied, 33)
 
 
+@pytest.mark.parametrize("precision", [ec.BF16, ec.FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("groups,per,queries", [(2, 3, 1), (2, 50, 1), (2, 4, 40), (1, 300, 2)])
+def test_attention_keeps_bad_values_to_their_own_rows(ctx, dev, groups, per, queries, precision):
+    """NaN and infinities in one row's query reach that row alone, those in one sequence's tokens that sequence, those
+    in a prefix its group: everything else has the same bits as before."""
+    rng = np.random.default_rng(groups + per + queries)
+    heads, kv_heads, dim, page, n = 8, 2, 128, 16, groups * per
+    lens = rng.integers(queries, 90, n).astype(np.int32)
+    holds(*attention_case(ctx, dev, rng, groups, per, queries, 300, 90, heads, kv_heads, dim, page, precision, lens=lens,
+                          counts=np.full(n, queries), prefix_lens=rng.integers(200, 300, groups), poison=False))
+    b, (layers, pages) = dev.buffers, dev.shapes["k"][0][:2]
+    own, shared = dev.shapes["t"][0][1], dev.shapes["pt"][0][1]
+    kv = ec.PagedKv(b["k"], b["v"], layers, pages, page, kv_heads, dim, precision)
+    batch = ec.PagedBatch(n, queries, b["t"], own, b["n"], b["c"], groups, b["pt"], shared, b["pl"])
+
+    def run(**changed):
+        kept = {name: dev.raw(name).copy() for name in changed}
+        for name, array in changed.items():
+            b[name].upload(array)
+        ctx.prefix_attention(kv, 0, batch, b["q"], heads, b["out"], b["work"], b["work"].nbytes)
+        ctx.synchronize()
+        for name, array in kept.items():
+            b[name].upload(array)
+        return dev.raw("out").reshape(n, queries, heads, dim).copy()
+
+    good = run()
+    tables, prefix = dev.raw("t"), dev.raw("pt")
+    for value in (np.nan, np.inf, -np.inf):
+        bits = np.float32(value).view(np.uint32) >> 16 if precision == ec.BF16 else np.float32(value)
+        slot, head = int(rng.integers(0, n * queries)), int(rng.integers(0, heads))
+        q = dev.raw("q").copy()
+        q.reshape(-1, heads, dim)[slot, head] = bits
+        got = run(q=q)
+        same = np.ones(good.shape[:3], bool)
+        same.reshape(-1, heads)[slot, head] = False
+        assert np.array_equal(got[same], good[same])
+        for name in ("k", "v"):
+            sequence = int(rng.integers(0, n))
+            pool = dev.raw(name).copy()
+            pool[0, tables[sequence, 0], 1, 0] = bits
+            got = run(**{name: pool})
+            same = np.ones(good.shape[:3], bool)
+            same[sequence, :, heads // 2:] = False
+            assert np.array_equal(got[same], good[same])
+            group = int(rng.integers(0, groups))
+            pool = dev.raw(name).copy()
+            pool[0, prefix[group, 1], 0, 3] = bits
+            got = run(**{name: pool})
+            same = np.ones(good.shape[:3], bool)
+            same[group * per:(group + 1) * per, :, :heads // 2] = False
+            assert np.array_equal(got[same], good[same])
+    assert np.array_equal(run(), good)
+
+
 def test_attention_past_32_bit_offsets(ctx, dev):
     """Pages whose elements lie beyond 2^32 in the cache."""
     rng = np.random.default_rng(13)
